@@ -52,6 +52,60 @@ FelixStatus flash_attn_bwd_launch(const half* Q, const half* K, const half* V, c
                                   uint32_t heads, uint32_t batch_size, uint32_t QKV_seqlen,
                                   cudaStream_t stream, bool causal = false);
 
+// new: the 4-bit paged cache of keys and values, its attention and its pages,
+// and token sampling (felix_c.h describes the arguments). No reference
+// counterpart: the reference has no cache and no sampling.
+enum class ElementType : int { F16 = 0, BF16 = 1, F32 = 2 };
+
+struct Kv4Cache {
+  void* pages;
+  uint64_t num_pages;
+  uint32_t page_size, kv_heads, head_dim;
+  const int32_t* table;  // [slots, width]
+  const int32_t* lens;   // [slots]
+  uint32_t slots, width;
+};
+
+// Bytes of a page; 0 where the sizes are not supported.
+size_t kv4_page_bytes(uint32_t kv_heads, uint32_t head_dim, uint32_t page_size);
+
+FelixStatus kv4_append_launch(const Kv4Cache& cache, const void* key, const void* value,
+                              ElementType type, uint32_t rows, const int64_t key_strides[3],
+                              const int64_t value_strides[3], const int32_t* counts,
+                              cudaStream_t stream);
+FelixStatus kv4_read_launch(const Kv4Cache& cache, uint32_t rows, const int32_t* counts, half* key,
+                            half* value, cudaStream_t stream);
+FelixStatus kv4_attention_launch(const Kv4Cache& cache, const void* q, ElementType type,
+                                 uint32_t heads, uint32_t rows, const int64_t q_strides[3],
+                                 const int32_t* counts, float scale, void* out, float* lse,
+                                 cudaStream_t stream);
+
+// State of a pool's pages: table [slots, width], lens [slots], refs [num_pages].
+struct Kv4Pages {
+  int32_t *table, *lens, *refs;
+};
+FelixStatus kv4_reserve_launch(const Kv4Pages& in, const int32_t* counts, uint32_t slots,
+                               uint32_t width, uint32_t num_pages, uint32_t page_size,
+                               const Kv4Pages& out, int32_t* status, cudaStream_t stream);
+FelixStatus kv4_fork_launch(void* pages, size_t page_bytes, const Kv4Pages& in,
+                            const int32_t* parents, const int32_t* children, uint32_t n,
+                            uint32_t slots, uint32_t width, uint32_t num_pages, uint32_t page_size,
+                            const Kv4Pages& out, int32_t* status, cudaStream_t stream);
+FelixStatus kv4_free_launch(const Kv4Pages& in, const int32_t* list, uint32_t n, uint32_t slots,
+                            uint32_t width, uint32_t num_pages, uint32_t page_size,
+                            const Kv4Pages& out, cudaStream_t stream);
+FelixStatus kv4_compact_launch(void* pages, size_t page_bytes, const Kv4Pages& in, uint32_t slots,
+                               uint32_t width, uint32_t num_pages, const Kv4Pages& out,
+                               cudaStream_t stream);
+FelixStatus kv4_copy_pages_launch(const void* from, uint64_t from_pages, void* to,
+                                  uint64_t to_pages, size_t page_bytes, const int32_t* src,
+                                  const int32_t* dst, uint32_t n, cudaStream_t stream);
+
+FelixStatus sample_launch(const void* logits, ElementType type, uint32_t rows, uint32_t vocab,
+                          int64_t stride, const float* uniform, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p,
+                          int32_t* tokens, float* logprobs, cudaStream_t stream);
+
 // new: reads (and clears) the device watchdog word; KERNEL_RUNTIME_ERROR when a
 // bounded wait inside a kernel gave up. Synchronises the device.
 FelixStatus check_watchdog();

@@ -201,6 +201,132 @@ int felix_topk_select(const float* data, float* out, uint32_t num_slices, uint32
                       uint32_t k, int largest, void* stream);
 
 /*
+ * 4-bit paged cache of keys and values (no reference counterpart: the
+ * reference has no cache). A pool is num_pages pages of
+ * felix_kv4_page_bytes() bytes; a page holds page_size tokens (a power of two,
+ * 16..4096) of every key/value head. Each head vector (head_dim 64 or 128) is
+ * held as x ~ base + scale * (code - 8): a code of 0..15 per value and an fp16
+ * (scale, base) per token and head, (head_dim + 8) bytes for K and V together
+ * (byte order: csrc/kv4_layout.cuh). `table` [slots][width] names the pages of
+ * each slot in order, `lens` [slots] the tokens in it, new ones included.
+ * Entries of `table` that name no page of the pool are not an error: tokens
+ * there are not written, read as zero, and attention does not see them. All
+ * arrays are on the device; pages is 16-byte aligned.
+ */
+typedef struct felix_kv4_cache {
+  void* pages;
+  uint64_t num_pages;
+  uint32_t page_size, kv_heads, head_dim;
+  const int32_t* table;
+  const int32_t* lens;
+  uint32_t slots, width;
+} felix_kv4_cache;
+
+/* Element types of the new operators' inputs. */
+#define FELIX_F16 0
+#define FELIX_BF16 1
+#define FELIX_F32 2
+
+int felix_kv4_page_bytes(uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, size_t* bytes);
+
+/*
+ * Writes new tokens into the cache: row i (0..rows-1) of slot s is token
+ * lens[s] - counts[s] + i where i < counts[s] (counts NULL: rows), other rows
+ * are left out. key, value: fp16 or bf16 [slot][head][row][head_dim] with the
+ * given element strides of slot, head and row (head_dim is contiguous). Per
+ * vector scale = fp16((max - min) / 15), base = fp16(min + 8 scale), code =
+ * clamp(rint((x - base) / scale) + 8, 0, 15). bf16 values past fp16's range are
+ * held as its largest value; a vector with an infinity or a NaN reads as NaN.
+ */
+int felix_kv4_append(const felix_kv4_cache* cache, const void* key, const void* value, int dtype,
+                     uint32_t rows, const int64_t* key_strides, const int64_t* value_strides,
+                     const int32_t* counts, void* stream);
+/*
+ * Reads the last tokens of each slot back as fp16, [slots][kv_heads][rows]
+ * [head_dim] contiguous, rows as in felix_kv4_append; rows that are no token
+ * are zero.
+ */
+int felix_kv4_read(const felix_kv4_cache* cache, uint32_t rows, const int32_t* counts, void* key,
+                   void* value, void* stream);
+/*
+ * Attention of new tokens over the cache (append them first): q, fp16 or bf16,
+ * [slot][head][row][head_dim] with the given strides; row i of slot s, with
+ * n = counts[s] (NULL: rows), sees the tokens 0 .. lens[s] - n + i. heads is a
+ * multiple of the cache's kv_heads; head h reads key/value head
+ * h / (heads / kv_heads). out [slots][heads][rows][head_dim] contiguous in q's
+ * type; lse (may be NULL) fp32 [slots][heads][rows], natural log. Rows that see
+ * nothing (i >= n, an empty slot) give zeros and lse = -inf. scale <= 0 selects
+ * 1/sqrt(head_dim). workspace: NULL = library-owned per (device, stream), else
+ * felix_kv4_attention_workspace_size() bytes, zero-filled before its first use.
+ */
+int felix_kv4_attention(const felix_kv4_cache* cache, const void* q, int dtype, uint32_t heads,
+                        uint32_t rows, const int64_t* q_strides, const int32_t* counts,
+                        float scale, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int felix_kv4_attention_workspace_size(uint32_t head_dim, size_t* bytes);
+
+/*
+ * Page operations. table [slots][width], lens [slots], refs [num_pages] (how
+ * many slots hold a page; <= 0: free); the *_out arrays are written whole and
+ * each may be its input. Free pages are given out from the lowest number up.
+ * status (reserve, fork): [0] pages that were missing (0: done; otherwise
+ * nothing was changed), [1] entries of the lists that were skipped.
+ *   reserve: lens grows by counts and each slot gets the pages for that (pages
+ *            past a slot's width count as missing).
+ *   fork:    slot children[i] becomes a copy of slot parents[i]: whole pages are
+ *            shared, a last page that is not full is copied to a fresh one.
+ *            Skipped: numbers out of range, a child that holds tokens, is its
+ *            parent or was named before.
+ *   free:    the listed slots become empty; pages that no slot holds any more
+ *            are free. Numbers out of range are ignored, repeated ones count once.
+ *   compact: pages in use move to the lowest numbers (the used pages past the
+ *            number in use fill the free ones below it, both in ascending
+ *            order), bytes included; table and refs follow.
+ */
+int felix_kv4_reserve(const int32_t* table, const int32_t* lens, const int32_t* refs,
+                      const int32_t* counts, uint32_t slots, uint32_t width, uint32_t num_pages,
+                      uint32_t page_size, int32_t* table_out, int32_t* lens_out,
+                      int32_t* refs_out, int32_t* status, void* stream);
+int felix_kv4_fork(void* pages, size_t page_bytes, const int32_t* table, const int32_t* lens,
+                   const int32_t* refs, const int32_t* parents, const int32_t* children,
+                   uint32_t n, uint32_t slots, uint32_t width, uint32_t num_pages,
+                   uint32_t page_size, int32_t* table_out, int32_t* lens_out, int32_t* refs_out,
+                   int32_t* status, void* stream);
+int felix_kv4_free(const int32_t* table, const int32_t* lens, const int32_t* refs,
+                   const int32_t* list, uint32_t n, uint32_t slots, uint32_t width,
+                   uint32_t num_pages, uint32_t page_size, int32_t* table_out, int32_t* lens_out,
+                   int32_t* refs_out, void* stream);
+int felix_kv4_compact(void* pages, size_t page_bytes, const int32_t* table, const int32_t* refs,
+                      uint32_t slots, uint32_t width, uint32_t num_pages, int32_t* table_out,
+                      int32_t* refs_out, void* stream);
+/*
+ * Copies page src[i] of one pool to page dst[i] of another (or of the same,
+ * where no page is both source and destination; dst without repeats). Numbers
+ * outside their pool are left out.
+ */
+int felix_kv4_copy_pages(const void* from, uint64_t from_pages, void* to, uint64_t to_pages,
+                         size_t page_bytes, const int32_t* src, const int32_t* dst, uint32_t n,
+                         void* stream);
+
+/*
+ * Samples a token per row of logits (FELIX_F16, FELIX_BF16 or FELIX_F32,
+ * [rows][vocab], `stride` elements between rows) from uniform[row] in [0, 1).
+ * Per-row parameters, each may be NULL: temperature (NULL: 1; <= 0: the first
+ * of the largest), top_k (NULL or <= 0: all), top_p (NULL or >= 1: all), min_p
+ * (NULL or <= 0: all). With w = exp((x - max) / T) as 31-bit fixed point and
+ * the order larger first, ties by lower index: top-k keeps the first k, top-p
+ * those with less than p of the kept mass before them, min-p those with
+ * w >= min_p, and the first always stays; the token is the first by index at
+ * which the running sum of kept mass exceeds floor(uniform * total). NaN counts
+ * as -inf. logprobs: log of the probability with which the token was drawn (0
+ * where temperature <= 0). A row with nothing above -inf: -1 and -inf.
+ */
+int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, int64_t stride,
+                 const float* uniform, const float* temperature, const int32_t* top_k,
+                 const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+                 void* stream);
+
+/*
  * Device watchdog. Every bounded wait inside the kernels records a nonzero
  * site code in a per-device status word when it gives up. Reads (and, when
  * clear != 0, resets) the word of the current device; synchronises the device.

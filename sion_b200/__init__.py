@@ -12,6 +12,16 @@ Python surface (mirrors the reference module ``sion``, python/binding.cpp:6-11):
     flash_attention_backward(Q, K, V, O, LSE, dO) -> (dQ, dK, dV)
     flash_attention_autograd(Q, K, V)   differentiable forward (torch.autograd)
 
+Decoding (no counterpart in the reference): a paged cache of keys and values in
+4 bits, attention of new tokens over it, its pages, and sampling:
+
+    kv4_append(pages, table, lens, K, V)       new tokens into the cache
+    kv4_read(pages, table, lens, rows, Hkv, D) the last tokens back as fp16
+    kv4_attention(Q, pages, table, lens, Hkv)  Q fp16/bf16 [slots,H,rows,D]
+    kv4_attention_lse(...)                     -> (O, fp32 LSE)
+    kv4_reserve / kv4_fork / kv4_free / kv4_compact / kv4_copy_pages
+    sample(logits, uniform, temperature, top_k, top_p, min_p)
+
 These come from the native module ``_sion`` (LibTorch C++), which calls the
 felix:: C++ API in ``libfelix_b200.so``. The C ABI of that library
 (include/felix_c.h) is reachable through :mod:`sion_b200.abi`. There is no
@@ -108,5 +118,86 @@ def flash_attention_autograd(query, key, value, causal: bool = False):
     return _FA_FN.apply(query, key, value, causal)
 
 
+def kv4_page_bytes(kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Bytes of a page: page_size * kv_heads * (head_dim + 8). A pool of the
+    4-bit cache is a uint8 tensor [pages, kv4_page_bytes(...)]."""
+    return _load_ext().kv4_page_bytes(kv_heads, head_dim, page_size)
+
+
+def kv4_append(pages, table, lens, key, value, counts=None):
+    """Writes new tokens into the cache: row i of key / value [slots, kv_heads,
+    rows, D] is token lens - counts + i of its slot (`lens` includes the new
+    tokens; `counts`, int32 [slots], says how many of the rows are tokens)."""
+    _load_ext().kv4_append(pages, table, lens, key, value, counts)
+
+
+def kv4_read(pages, table, lens, rows: int, kv_heads: int, head_dim: int, counts=None):
+    """(K, V), fp16 [slots, kv_heads, rows, D]: the last tokens of each slot as
+    the cache holds them; rows that are no token are zero."""
+    return _load_ext().kv4_read(pages, table, lens, rows, kv_heads, head_dim, counts)
+
+
+def kv4_attention(query, pages, table, lens, kv_heads: int, counts=None, scale: float = 0.0):
+    """Attention of the new tokens query [slots, heads, rows, D] (fp16 or bf16)
+    over the cache: row i of n sees the tokens 0 .. len - n + i. Rows that see
+    nothing give zeros. scale <= 0: 1 / sqrt(D)."""
+    return _load_ext().kv4_attention(query, pages, table, lens, kv_heads, counts, scale)
+
+
+def kv4_attention_lse(query, pages, table, lens, kv_heads: int, counts=None, scale: float = 0.0):
+    """kv4_attention returning (O, LSE), LSE fp32 [slots, heads, rows] (-inf
+    where a row sees nothing)."""
+    return _load_ext().kv4_attention_lse(query, pages, table, lens, kv_heads, counts, scale)
+
+
+def kv4_reserve(table, lens, refs, counts, page_size: int, out=None):
+    """(table, lens, refs, status) after each slot has grown by counts tokens and
+    has the pages for them, the lowest free ones first. status[0]: pages that
+    were missing; nothing changes unless it is 0. `out`: tensors to write, which
+    may be (table, lens, refs) themselves."""
+    return _load_ext().kv4_reserve(table, lens, refs, counts, page_size, out)
+
+
+def kv4_fork(pages, table, lens, refs, parents, children, page_size: int, out=None):
+    """(table, lens, refs, status) after slot children[i] (empty before) has
+    become a copy of slot parents[i]: whole pages are shared, a last page that is
+    not full is copied. status: [pages missing, pairs skipped]."""
+    return _load_ext().kv4_fork(pages, table, lens, refs, parents, children, page_size, out)
+
+
+def kv4_free(table, lens, refs, slots, page_size: int, out=None):
+    """(table, lens, refs) after the listed slots were emptied."""
+    return _load_ext().kv4_free(table, lens, refs, slots, page_size, out)
+
+
+def kv4_compact(pages, table, refs, out=None):
+    """(table, refs) after the pages in use have moved to the lowest numbers."""
+    return _load_ext().kv4_compact(pages, table, refs, out)
+
+
+def kv4_copy_pages(src_pages, dst_pages, src, dst):
+    """Copies page src[i] of one pool to page dst[i] of another."""
+    _load_ext().kv4_copy_pages(src_pages, dst_pages, src, dst)
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
+    """One token per row of logits [rows, vocab] from uniform [rows] in [0, 1):
+    (tokens int32 [rows], log-probability of each under the kept tokens).
+    temperature, top_p, min_p (fp32 [rows]) and top_k (int32 [rows]) may be
+    numbers, for all rows, or None."""
+    import torch
+
+    def rows(v, dtype):
+        if v is None or isinstance(v, torch.Tensor):
+            return v
+        return torch.full((logits.shape[0],), v, dtype=dtype, device=logits.device)
+
+    return _load_ext().sample(logits, uniform, rows(temperature, torch.float32),
+                              rows(top_k, torch.int32), rows(top_p, torch.float32),
+                              rows(min_p, torch.float32))
+
+
 __all__ = ["sgemm", "hgemm", "hgemm_nt", "gemm", "flash_attention", "flash_attention_lse",
-           "flash_attention_backward", "flash_attention_autograd", "LIB_PATH"]
+           "flash_attention_backward", "flash_attention_autograd", "kv4_page_bytes", "kv4_append",
+           "kv4_read", "kv4_attention", "kv4_attention_lse", "kv4_reserve", "kv4_fork", "kv4_free",
+           "kv4_compact", "kv4_copy_pages", "sample", "LIB_PATH"]

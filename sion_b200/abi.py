@@ -56,10 +56,37 @@ _SIGS = {
                           [C.c_int, C.c_void_p]),
     "felix_flash_attn_fwd_ex": (C.c_int, [C.c_void_p] * 5 + [C.c_uint32] * 4 +
                                 [C.c_float, C.c_int, C.c_void_p]),
+    "felix_kv4_page_bytes": (C.c_int, [C.c_uint32] * 3 + [C.POINTER(C.c_size_t)]),
+    "felix_kv4_append": (C.c_int, [C.c_void_p] * 3 + [C.c_int, C.c_uint32] + [C.c_void_p] * 4),
+    "felix_kv4_read": (C.c_int, [C.c_void_p, C.c_uint32] + [C.c_void_p] * 4),
+    "felix_kv4_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint32, C.c_uint32,
+                                      C.c_void_p, C.c_void_p, C.c_float] + [C.c_void_p] * 3 +
+                            [C.c_size_t, C.c_void_p]),
+    "felix_kv4_attention_workspace_size": (C.c_int, [C.c_uint32, C.POINTER(C.c_size_t)]),
+    "felix_kv4_reserve": (C.c_int, [C.c_void_p] * 4 + [C.c_uint32] * 4 + [C.c_void_p] * 5),
+    "felix_kv4_fork": (C.c_int, [C.c_void_p, C.c_size_t] + [C.c_void_p] * 5 + [C.c_uint32] * 5 +
+                       [C.c_void_p] * 5),
+    "felix_kv4_free": (C.c_int, [C.c_void_p] * 4 + [C.c_uint32] * 5 + [C.c_void_p] * 4),
+    "felix_kv4_compact": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p] +
+                          [C.c_uint32] * 3 + [C.c_void_p] * 3),
+    "felix_kv4_copy_pages": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_size_t,
+                                       C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "felix_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_int64] +
+                     [C.c_void_p] * 8),
     "felix_watchdog_status": (C.c_int, [C.POINTER(C.c_uint), C.c_int]),
     "felix_watchdog_probe": (C.c_int, [C.c_uint32, C.c_void_p]),
     "felix_num_sms": (C.c_int, [C.POINTER(C.c_int)]),
 }
+
+F16, BF16, F32 = 0, 1, 2
+
+
+class Kv4Cache(C.Structure):
+    """felix_kv4_cache of include/felix_c.h."""
+    _fields_ = [("pages", C.c_void_p), ("num_pages", C.c_uint64), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("table", C.c_void_p),
+                ("lens", C.c_void_p), ("slots", C.c_uint32), ("width", C.c_uint32)]
+
 
 _lib = None
 
@@ -211,6 +238,61 @@ def topk_select(data, out, k, largest=True, stream=None):
     check(lib().felix_topk_select(_ptr(data), _ptr(out), num_slices, slice_size, k,
                                   1 if largest else 0, _stream(stream)))
     return out
+
+
+def _dtype(t):
+    import torch
+    return {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}[t.dtype]
+
+
+def _strides(t):
+    return (C.c_int64 * 3)(*t.stride()[:3])
+
+
+def kv4_page_bytes(kv_heads, head_dim, page_size) -> int:
+    n = C.c_size_t(0)
+    check(lib().felix_kv4_page_bytes(kv_heads, head_dim, page_size, C.byref(n)))
+    return n.value
+
+
+def kv4_cache(pages, table, lens, page_size, kv_heads, head_dim) -> Kv4Cache:
+    """The C struct over a pool [pages, bytes], a table [slots, width] and lens [slots]."""
+    return Kv4Cache(pages.data_ptr(), pages.shape[0], page_size, kv_heads, head_dim,
+                    table.data_ptr(), lens.data_ptr(), table.shape[0], table.shape[1])
+
+
+def kv4_append(cache, key, value, counts=None, stream=None):
+    check(lib().felix_kv4_append(C.byref(cache), _ptr(key), _ptr(value), _dtype(key),
+                                 key.shape[2], _strides(key), _strides(value), _ptr(counts),
+                                 _stream(stream)))
+
+
+def kv4_read(cache, rows, key, value, counts=None, stream=None):
+    check(lib().felix_kv4_read(C.byref(cache), rows, _ptr(counts), _ptr(key), _ptr(value),
+                               _stream(stream)))
+
+
+def kv4_attention(cache, q, out, lse=None, counts=None, scale=0.0, workspace=None, stream=None):
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(lib().felix_kv4_attention(C.byref(cache), _ptr(q), _dtype(q), q.shape[1], q.shape[2],
+                                    _strides(q), _ptr(counts), float(scale), _ptr(out), _ptr(lse),
+                                    _ptr(workspace), ws_bytes, _stream(stream)))
+    return out
+
+
+def kv4_attention_workspace_size(head_dim) -> int:
+    n = C.c_size_t(0)
+    check(lib().felix_kv4_attention_workspace_size(head_dim, C.byref(n)))
+    return n.value
+
+
+def sample(logits, uniform, tokens, logprobs, temperature=None, top_k=None, top_p=None,
+           min_p=None, stream=None):
+    rows, vocab = logits.shape
+    check(lib().felix_sample(_ptr(logits), _dtype(logits), rows, vocab, logits.stride(0),
+                             _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                             _ptr(min_p), _ptr(tokens), _ptr(logprobs), _stream(stream)))
+    return tokens, logprobs
 
 
 def watchdog_status(clear=True) -> int:

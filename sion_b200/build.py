@@ -26,9 +26,10 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["felix_c.cu", "sgemm_sm100.cu", "hgemm_sm100.cu", "flash_attn_sm100.cu",
-              "topk_sm100.cu", "flash_attn_bwd_sm100.cu"]
+              "topk_sm100.cu", "flash_attn_bwd_sm100.cu", "kv4_attn_sm100.cu",
+              "kv4_cache_sm100.cu", "sample_sm100.cu"]
 CPP_SOURCES = ["felix_api.cpp"]
-HEADERS = ["sm100_ptx.cuh", "felix_internal.h"]
+HEADERS = ["sm100_ptx.cuh", "felix_internal.h", "kv4_layout.cuh"]
 
 NVCC_FLAGS = [
     "-std=c++20", "-O3", "-lineinfo",

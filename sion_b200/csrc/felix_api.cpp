@@ -230,6 +230,87 @@ FelixStatus flash_attn_bwd_launch<128>(const half* Q, const half* K, const half*
                                      QKV_seqlen, 128, 0.0f, causal ? 1 : 0, nullptr, 0, stream));
 }
 
+namespace {
+felix_kv4_cache c_cache(const Kv4Cache& c) {
+  return {c.pages, c.num_pages, c.page_size, c.kv_heads, c.head_dim,
+          c.table, c.lens,      c.slots,     c.width};
+}
+}  // namespace
+
+size_t kv4_page_bytes(uint32_t kv_heads, uint32_t head_dim, uint32_t page_size) {
+  size_t n = 0;
+  return felix_kv4_page_bytes(kv_heads, head_dim, page_size, &n) == FELIX_SUCCESS ? n : 0;
+}
+
+FelixStatus kv4_append_launch(const Kv4Cache& cache, const void* key, const void* value,
+                              ElementType type, uint32_t rows, const int64_t key_strides[3],
+                              const int64_t value_strides[3], const int32_t* counts,
+                              cudaStream_t stream) {
+  const felix_kv4_cache c = c_cache(cache);
+  return from_c(felix_kv4_append(&c, key, value, static_cast<int>(type), rows, key_strides,
+                                 value_strides, counts, stream));
+}
+
+FelixStatus kv4_read_launch(const Kv4Cache& cache, uint32_t rows, const int32_t* counts, half* key,
+                            half* value, cudaStream_t stream) {
+  const felix_kv4_cache c = c_cache(cache);
+  return from_c(felix_kv4_read(&c, rows, counts, key, value, stream));
+}
+
+FelixStatus kv4_attention_launch(const Kv4Cache& cache, const void* q, ElementType type,
+                                 uint32_t heads, uint32_t rows, const int64_t q_strides[3],
+                                 const int32_t* counts, float scale, void* out, float* lse,
+                                 cudaStream_t stream) {
+  const felix_kv4_cache c = c_cache(cache);
+  return from_c(felix_kv4_attention(&c, q, static_cast<int>(type), heads, rows, q_strides, counts,
+                                    scale, out, lse, nullptr, 0, stream));
+}
+
+FelixStatus kv4_reserve_launch(const Kv4Pages& in, const int32_t* counts, uint32_t slots,
+                               uint32_t width, uint32_t num_pages, uint32_t page_size,
+                               const Kv4Pages& out, int32_t* status, cudaStream_t stream) {
+  return from_c(felix_kv4_reserve(in.table, in.lens, in.refs, counts, slots, width, num_pages,
+                                  page_size, out.table, out.lens, out.refs, status, stream));
+}
+
+FelixStatus kv4_fork_launch(void* pages, size_t page_bytes, const Kv4Pages& in,
+                            const int32_t* parents, const int32_t* children, uint32_t n,
+                            uint32_t slots, uint32_t width, uint32_t num_pages, uint32_t page_size,
+                            const Kv4Pages& out, int32_t* status, cudaStream_t stream) {
+  return from_c(felix_kv4_fork(pages, page_bytes, in.table, in.lens, in.refs, parents, children, n,
+                               slots, width, num_pages, page_size, out.table, out.lens, out.refs,
+                               status, stream));
+}
+
+FelixStatus kv4_free_launch(const Kv4Pages& in, const int32_t* list, uint32_t n, uint32_t slots,
+                            uint32_t width, uint32_t num_pages, uint32_t page_size,
+                            const Kv4Pages& out, cudaStream_t stream) {
+  return from_c(felix_kv4_free(in.table, in.lens, in.refs, list, n, slots, width, num_pages,
+                               page_size, out.table, out.lens, out.refs, stream));
+}
+
+FelixStatus kv4_compact_launch(void* pages, size_t page_bytes, const Kv4Pages& in, uint32_t slots,
+                               uint32_t width, uint32_t num_pages, const Kv4Pages& out,
+                               cudaStream_t stream) {
+  return from_c(felix_kv4_compact(pages, page_bytes, in.table, in.refs, slots, width, num_pages,
+                                  out.table, out.refs, stream));
+}
+
+FelixStatus kv4_copy_pages_launch(const void* from, uint64_t from_pages, void* to,
+                                  uint64_t to_pages, size_t page_bytes, const int32_t* src,
+                                  const int32_t* dst, uint32_t n, cudaStream_t stream) {
+  return from_c(felix_kv4_copy_pages(from, from_pages, to, to_pages, page_bytes, src, dst, n,
+                                     stream));
+}
+
+FelixStatus sample_launch(const void* logits, ElementType type, uint32_t rows, uint32_t vocab,
+                          int64_t stride, const float* uniform, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p,
+                          int32_t* tokens, float* logprobs, cudaStream_t stream) {
+  return from_c(felix_sample(logits, static_cast<int>(type), rows, vocab, stride, uniform,
+                             temperature, top_k, top_p, min_p, tokens, logprobs, stream));
+}
+
 FelixStatus check_watchdog() {
   unsigned code = 0;
   return from_c(felix_watchdog_status(&code, 1));

@@ -7,6 +7,7 @@
 
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <string>
@@ -249,6 +250,63 @@ static int finish(FelixCode c) {
 
 using namespace felix_impl;
 
+// The entry points below may not throw (scratch is kept in a std::map).
+template <class F>
+static int guarded(F&& f) {
+  try {
+    return finish(f());
+  } catch (const std::exception& e) {
+    return api_error(e.what(), cudaErrorMemoryAllocation).type;
+  } catch (...) {
+    return api_error("unknown C++ exception", cudaErrorUnknown).type;
+  }
+}
+
+// log2 of a page size, or -1 where it is none.
+static int page_shift_of(uint32_t page_size) {
+  if (page_size < felix_kv4::kBlock || page_size > felix_kv4::kMaxPageSize ||
+      (page_size & (page_size - 1)))
+    return -1;
+  return __builtin_ctz(page_size);
+}
+
+static FelixCode view_of(const felix_kv4_cache* c, felix_kv4::CacheView* v) {
+  // arrays without elements may be null
+  if (!c || !c->pages || (!c->table && c->slots && c->width) || (!c->lens && c->slots))
+    return api_error("kv4: null cache or array");
+  if (c->head_dim != 64 && c->head_dim != 128) return api_error("kv4: head_dim must be 64 or 128");
+  const int shift = page_shift_of(c->page_size);
+  if (shift < 0) return api_error("kv4: page_size must be a power of two, 16..4096");
+  if (c->kv_heads == 0 || c->kv_heads > 65535) return api_error("kv4: kv_heads must be 1..65535");
+  if (c->num_pages == 0 || c->num_pages > 0x7fffffffull)
+    return api_error("kv4: num_pages must be 1..2^31-1");
+  if (c->slots > (1u << 24) || c->width > 0x7fffffffu / c->page_size)
+    return api_error("kv4: too many slots or pages of a slot");
+  if (reinterpret_cast<uintptr_t>(c->pages) & 15) return api_error("kv4: pages must be 16-byte aligned");
+  v->pages = static_cast<unsigned char*>(c->pages);
+  v->table = c->table;
+  v->lens = c->lens;
+  v->num_pages = c->num_pages;
+  v->page_bytes = size_t(c->page_size) * c->kv_heads * (c->head_dim + 8);
+  v->slots = c->slots;
+  v->width = c->width;
+  v->kv_heads = c->kv_heads;
+  v->page_shift = uint32_t(shift);
+  return FelixCode{FELIX_SUCCESS, cudaSuccess};
+}
+
+static FelixCode pages_op(const Kv4PagesOp& o, uint32_t page_size, void* stream) {
+  if (!o.refs || !o.refs_out || ((!o.table || !o.table_out) && o.slots && o.width))
+    return api_error("kv4: null array");
+  if (o.num_pages == 0 || o.num_pages > 0x7fffffffu)
+    return api_error("kv4: num_pages must be 1..2^31-1");
+  if (o.slots > (1u << 24) || o.n > (1u << 24) || o.width > 0x7fffffffu / page_size)
+    return api_error("kv4: too many slots, pages of a slot or list entries");
+  if (o.pages && ((reinterpret_cast<uintptr_t>(o.pages) & 15) || o.page_bytes % 16))
+    return api_error("kv4: pages must be 16-byte aligned and their size a multiple of 16");
+  return kv4_pages_launch(o, static_cast<cudaStream_t>(stream));
+}
+
 extern "C" {
 
 int felix_last_cuda_error(void) { return t_last_cuda; }
@@ -409,6 +467,161 @@ int felix_topk_select(const float* data, float* out, uint32_t num_slices, uint32
                       uint32_t k, int largest, void* stream) {
   return finish(topk_select_launch(data, out, num_slices, slice_size, k, largest != 0,
                                    static_cast<cudaStream_t>(stream)));
+}
+
+int felix_kv4_page_bytes(uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, size_t* bytes) {
+  if (head_dim != 64 && head_dim != 128) return api_error("kv4: head_dim must be 64 or 128").type;
+  if (page_shift_of(page_size) < 0)
+    return api_error("kv4: page_size must be a power of two, 16..4096").type;
+  if (bytes) *bytes = size_t(page_size) * kv_heads * (head_dim + 8);
+  return FELIX_SUCCESS;
+}
+
+int felix_kv4_append(const felix_kv4_cache* cache, const void* key, const void* value, int dtype,
+                     uint32_t rows, const int64_t* key_strides, const int64_t* value_strides,
+                     const int32_t* counts, void* stream) {
+  return guarded([&]() -> FelixCode {
+    felix_kv4::CacheView v;
+    const FelixCode rc = view_of(cache, &v);
+    if (rc.type != FELIX_SUCCESS) return rc;
+    if (dtype != FELIX_F16 && dtype != FELIX_BF16)
+      return api_error("kv4_append: key and value must be fp16 or bf16");
+    if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+    if (!key || !value || !key_strides || !value_strides) return api_error("kv4_append: null pointer");
+    return kv4_append_launch(v, cache->head_dim, key, value, dtype == FELIX_BF16, rows, key_strides,
+                             value_strides, counts, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int felix_kv4_read(const felix_kv4_cache* cache, uint32_t rows, const int32_t* counts, void* key,
+                   void* value, void* stream) {
+  return guarded([&]() -> FelixCode {
+    felix_kv4::CacheView v;
+    const FelixCode rc = view_of(cache, &v);
+    if (rc.type != FELIX_SUCCESS) return rc;
+    if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+    if (!key || !value) return api_error("kv4_read: null pointer");
+    if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15)
+      return api_error("kv4_read: outputs must be 16-byte aligned");
+    return kv4_read_launch(v, cache->head_dim, rows, counts, static_cast<__half*>(key),
+                           static_cast<__half*>(value), static_cast<cudaStream_t>(stream));
+  });
+}
+
+int felix_kv4_attention(const felix_kv4_cache* cache, const void* q, int dtype, uint32_t heads,
+                        uint32_t rows, const int64_t* q_strides, const int32_t* counts,
+                        float scale, void* out, float* lse, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  return guarded([&]() -> FelixCode {
+    felix_kv4::CacheView v;
+    const FelixCode rc = view_of(cache, &v);
+    if (rc.type != FELIX_SUCCESS) return rc;
+    if (dtype != FELIX_F16 && dtype != FELIX_BF16)
+      return api_error("kv4_attention: q must be fp16 or bf16");
+    if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+    if (!q || !q_strides || !out) return api_error("kv4_attention: null pointer");
+    if (heads == 0 || heads > 65535 || heads % v.kv_heads)
+      return api_error("kv4_attention: heads must be a multiple of kv_heads, at most 65535");
+    if (rows > 65535) return api_error("kv4_attention: at most 65535 rows");
+    return kv4_attention_launch(v, cache->head_dim, q, dtype == FELIX_BF16, heads, rows, q_strides,
+                                counts, scale, out, lse, workspace, workspace_bytes,
+                                static_cast<cudaStream_t>(stream));
+  });
+}
+
+int felix_kv4_attention_workspace_size(uint32_t head_dim, size_t* bytes) {
+  if (head_dim != 64 && head_dim != 128) return api_error("kv4: head_dim must be 64 or 128").type;
+  DeviceInfo* d = current_device_info();
+  if (!d) return launch_error(cudaGetLastError(), "no device").type;
+  if (bytes) *bytes = kv4_attention_workspace_bytes(head_dim, d->num_sms);
+  return FELIX_SUCCESS;
+}
+
+int felix_kv4_reserve(const int32_t* table, const int32_t* lens, const int32_t* refs,
+                      const int32_t* counts, uint32_t slots, uint32_t width, uint32_t num_pages,
+                      uint32_t page_size, int32_t* table_out, int32_t* lens_out,
+                      int32_t* refs_out, int32_t* status, void* stream) {
+  return guarded([&]() -> FelixCode {
+    const int shift = page_shift_of(page_size);
+    if (shift < 0) return api_error("kv4: page_size must be a power of two, 16..4096");
+    if (!status || ((!lens || !counts || !lens_out) && slots)) return api_error("kv4_reserve: null array");
+    return pages_op({Kv4PagesOp::kReserve, table, lens, refs, table_out, lens_out, refs_out, status,
+                     counts, nullptr, slots, width, num_pages, uint32_t(shift), 0, nullptr, 0},
+                    page_size, stream);
+  });
+}
+
+int felix_kv4_fork(void* pages, size_t page_bytes, const int32_t* table, const int32_t* lens,
+                   const int32_t* refs, const int32_t* parents, const int32_t* children,
+                   uint32_t n, uint32_t slots, uint32_t width, uint32_t num_pages,
+                   uint32_t page_size, int32_t* table_out, int32_t* lens_out, int32_t* refs_out,
+                   int32_t* status, void* stream) {
+  return guarded([&]() -> FelixCode {
+    const int shift = page_shift_of(page_size);
+    if (shift < 0) return api_error("kv4: page_size must be a power of two, 16..4096");
+    if (!pages || !status || ((!lens || !lens_out) && slots) || ((!parents || !children) && n))
+      return api_error("kv4_fork: null array");
+    return pages_op({Kv4PagesOp::kFork, table, lens, refs, table_out, lens_out, refs_out, status,
+                     parents, children, slots, width, num_pages, uint32_t(shift), n, pages,
+                     page_bytes},
+                    page_size, stream);
+  });
+}
+
+int felix_kv4_free(const int32_t* table, const int32_t* lens, const int32_t* refs,
+                   const int32_t* list, uint32_t n, uint32_t slots, uint32_t width,
+                   uint32_t num_pages, uint32_t page_size, int32_t* table_out, int32_t* lens_out,
+                   int32_t* refs_out, void* stream) {
+  return guarded([&]() -> FelixCode {
+    const int shift = page_shift_of(page_size);
+    if (shift < 0) return api_error("kv4: page_size must be a power of two, 16..4096");
+    if (((!lens || !lens_out) && slots) || (!list && n)) return api_error("kv4_free: null array");
+    return pages_op({Kv4PagesOp::kFree, table, lens, refs, table_out, lens_out, refs_out, nullptr,
+                     list, nullptr, slots, width, num_pages, uint32_t(shift), n, nullptr, 0},
+                    page_size, stream);
+  });
+}
+
+int felix_kv4_compact(void* pages, size_t page_bytes, const int32_t* table, const int32_t* refs,
+                      uint32_t slots, uint32_t width, uint32_t num_pages, int32_t* table_out,
+                      int32_t* refs_out, void* stream) {
+  return guarded([&]() -> FelixCode {
+    if (!pages) return api_error("kv4_compact: null array");
+    return pages_op({Kv4PagesOp::kCompact, table, nullptr, refs, table_out, nullptr, refs_out,
+                     nullptr, nullptr, nullptr, slots, width, num_pages, 4, 0, pages, page_bytes},
+                    16, stream);
+  });
+}
+
+int felix_kv4_copy_pages(const void* from, uint64_t from_pages, void* to, uint64_t to_pages,
+                         size_t page_bytes, const int32_t* src, const int32_t* dst, uint32_t n,
+                         void* stream) {
+  return guarded([&]() -> FelixCode {
+    if (n == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+    if (!from || !to || !src || !dst) return api_error("kv4_copy_pages: null pointer");
+    if (((reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) & 15) ||
+        page_bytes == 0 || page_bytes % 16)
+      return api_error("kv4_copy_pages: pools must be 16-byte aligned, pages a multiple of 16 bytes");
+    return kv4_copy_launch(from, from_pages, to, to_pages, page_bytes, src, dst, n,
+                           static_cast<cudaStream_t>(stream));
+  });
+}
+
+int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, int64_t stride,
+                 const float* uniform, const float* temperature, const int32_t* top_k,
+                 const float* top_p, const float* min_p, int32_t* tokens, float* logprobs,
+                 void* stream) {
+  return guarded([&]() -> FelixCode {
+    if (dtype != FELIX_F16 && dtype != FELIX_BF16 && dtype != FELIX_F32)
+      return api_error("sample: logits must be fp16, bf16 or fp32");
+    if (rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+    if (!logits || !uniform || !tokens || !logprobs) return api_error("sample: null pointer");
+    if (vocab == 0 || vocab > 0x7fffffffu) return api_error("sample: vocab must be 1..2^31-1");
+    if (stride < 0) return api_error("sample: stride must not be negative");
+    return sample_launch({logits, dtype, rows, vocab, stride, uniform, temperature, top_k, top_p,
+                          min_p, tokens, logprobs},
+                         static_cast<cudaStream_t>(stream));
+  });
 }
 
 int felix_watchdog_status(unsigned* code, int clear) {

@@ -10,6 +10,7 @@
 #include <cstdint>
 
 #include "../../include/felix_c.h"
+#include "kv4_layout.cuh"
 
 namespace felix_impl {
 
@@ -138,6 +139,44 @@ FelixCode flash_attn_bwd_launch(const __half* Q, const __half* K, const __half* 
 
 FelixCode topk_select_launch(const float* data, float* out, uint32_t num_slices,
                              uint32_t slice_size, uint32_t k, bool largest, cudaStream_t stream);
+
+// 4-bit paged cache (kv4_layout.cuh). Strides are of elements: slot, head, row.
+size_t kv4_attention_workspace_bytes(uint32_t head_dim, int num_sms);
+FelixCode kv4_attention_launch(const felix_kv4::CacheView& c, uint32_t head_dim, const void* q,
+                               bool bf16, uint32_t heads, uint32_t rows, const int64_t* strides,
+                               const int32_t* counts, float scale, void* out, float* lse,
+                               void* workspace, size_t ws_bytes, cudaStream_t stream);
+FelixCode kv4_append_launch(const felix_kv4::CacheView& c, uint32_t head_dim, const void* key,
+                            const void* value, bool bf16, uint32_t rows, const int64_t* ks,
+                            const int64_t* vs, const int32_t* counts, cudaStream_t stream);
+FelixCode kv4_read_launch(const felix_kv4::CacheView& c, uint32_t head_dim, uint32_t rows,
+                          const int32_t* counts, __half* key, __half* value, cudaStream_t stream);
+FelixCode kv4_copy_launch(const void* from, uint64_t from_pages, void* to, uint64_t to_pages,
+                          size_t page_bytes, const int32_t* src, const int32_t* dst, uint32_t count,
+                          cudaStream_t stream);
+struct Kv4PagesOp {
+  enum Kind { kReserve, kFork, kFree, kCompact } kind;
+  const int32_t *table, *lens, *refs;
+  int32_t *table_out, *lens_out, *refs_out, *status;
+  const int32_t *a, *b;  // counts / parents, children / slots to free
+  uint32_t slots, width, num_pages, page_shift, n;
+  void* pages;
+  size_t page_bytes;
+};
+FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream);
+
+struct SampleArgs {
+  const void* logits;
+  int dtype;  // FELIX_F16, FELIX_BF16, FELIX_F32
+  uint32_t rows, vocab;
+  int64_t stride;
+  const float *uniform, *temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  int32_t* tokens;
+  float* logprobs;
+};
+FelixCode sample_launch(const SampleArgs& a, cudaStream_t stream);
 
 FelixCode watchdog_probe_launch(uint32_t limit_us, cudaStream_t stream);
 

@@ -207,6 +207,310 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> flash_attention_backward
   return {dQ, dK, dV};
 }
 
+// ------------------------------------------------- decoding: cache and sampling
+namespace {
+using OptTensor = std::optional<torch::Tensor>;
+
+void check_i32(const torch::Tensor& t, const torch::Device& dev, int64_t dim, const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
+  TORCH_CHECK(t.dtype() == torch::kInt32, name, " must be int32");
+  TORCH_CHECK(t.dim() == dim, name, " must be ", dim, "D");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+const int32_t* i32(const torch::Tensor& t) { return t.data_ptr<int32_t>(); }
+const int32_t* counts_of(const OptTensor& counts, const torch::Tensor& lens) {
+  if (!counts) return nullptr;
+  check_i32(*counts, lens.device(), 1, "counts");
+  TORCH_CHECK(counts->size(0) == lens.size(0), "counts must have one entry per slot");
+  return i32(*counts);
+}
+
+felix::Kv4Cache cache_of(const torch::Tensor& pages, const torch::Tensor& table,
+                         const torch::Tensor& lens, int64_t kv_heads, int64_t head_dim) {
+  TORCH_CHECK(pages.is_cuda(), "pages must be CUDA tensor");
+  TORCH_CHECK(pages.dtype() == torch::kUInt8 && pages.dim() == 2 && pages.is_contiguous(),
+              "pages must be contiguous uint8 [pages, page bytes]");
+  check_i32(table, pages.device(), 2, "table");
+  check_i32(lens, pages.device(), 1, "lens");
+  TORCH_CHECK(table.size(0) == lens.size(0), "table and lens must have the same slots");
+  TORCH_CHECK(kv_heads > 0, "kv_heads must be positive");
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, "unsupported head dimension ", head_dim);
+  const int64_t token = kv_heads * (head_dim + 8);
+  TORCH_CHECK(pages.size(1) > 0 && pages.size(1) % token == 0,
+              "a page's bytes must be page_size * kv_heads * (head_dim + 8)");
+  return {pages.data_ptr(), uint64_t(pages.size(0)), uint32_t(pages.size(1) / token),
+          uint32_t(kv_heads), uint32_t(head_dim), i32(table), i32(lens), uint32_t(table.size(0)),
+          uint32_t(table.size(1))};
+}
+
+felix::ElementType half_type(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.dtype() == torch::kHalf || t.dtype() == torch::kBFloat16, name,
+              " must be float16 or bfloat16");
+  return t.dtype() == torch::kHalf ? felix::ElementType::F16 : felix::ElementType::BF16;
+}
+
+// Strides are passed on; only the innermost dimension has to be contiguous.
+torch::Tensor inner_contiguous(const torch::Tensor& t) {
+  return t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous();
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_attention_impl(
+    const torch::Tensor& query, const torch::Tensor& pages, const torch::Tensor& table,
+    const torch::Tensor& lens, int64_t kv_heads, const OptTensor& counts, double scale,
+    bool want_lse) {
+  TORCH_CHECK(query.is_cuda(), "query must be CUDA tensor");
+  TORCH_CHECK(query.dim() == 4, "query must be 4D [slots, heads, rows, D]");
+  const auto type = half_type(query, "query");
+  const auto cache = cache_of(pages, table, lens, kv_heads, query.size(3));
+  TORCH_CHECK(query.device() == pages.device(), "query must be on ", pages.device());
+  TORCH_CHECK(query.size(0) == table.size(0), "query must have one entry per slot");
+  TORCH_CHECK(query.size(1) > 0 && query.size(1) % kv_heads == 0,
+              "query's heads must be a multiple of kv_heads");
+  const int32_t* n = counts_of(counts, lens);
+  const c10::cuda::CUDAGuard guard(query.device());
+  const auto Q = inner_contiguous(query);
+  auto O = torch::empty(Q.sizes(), Q.options());
+  torch::Tensor L;
+  if (want_lse) L = torch::empty(Q.sizes().slice(0, 3), Q.options().dtype(torch::kFloat32));
+  const auto status = felix::kv4_attention_launch(
+      cache, Q.data_ptr(), type, uint32_t(Q.size(1)), uint32_t(Q.size(2)), Q.strides().data(), n,
+      float(scale), O.data_ptr(), want_lse ? L.data_ptr<float>() : nullptr,
+      at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_attention: kernel launch failed: ", status.str());
+  return {O, L};
+}
+
+// Outputs of a page operation: `out`, or new tensors of the inputs' shapes.
+std::vector<torch::Tensor> page_outputs(const std::vector<torch::Tensor>& in, const Kv4Out& out) {
+  std::vector<torch::Tensor> r;
+  if (!out) {
+    for (const auto& t : in) r.push_back(torch::empty_like(t));
+    return r;
+  }
+  TORCH_CHECK(out->size() == in.size(), "out must have ", in.size(), " tensors");
+  for (size_t i = 0; i < in.size(); ++i) {
+    const auto& t = (*out)[i];
+    check_i32(t, in[i].device(), in[i].dim(), "out");
+    TORCH_CHECK(t.sizes() == in[i].sizes(), "out must have the inputs' shapes");
+    r.push_back(t);
+  }
+  return r;
+}
+
+void check_state(const torch::Tensor& table, const torch::Tensor* lens, const torch::Tensor& refs) {
+  TORCH_CHECK(table.is_cuda(), "table must be CUDA tensor");
+  check_i32(table, table.device(), 2, "table");
+  check_i32(refs, table.device(), 1, "refs");
+  if (!lens) return;
+  check_i32(*lens, table.device(), 1, "lens");
+  TORCH_CHECK(table.size(0) == lens->size(0), "table and lens must have the same slots");
+}
+felix::Kv4Pages pages_of(const torch::Tensor& table, const torch::Tensor* lens,
+                         const torch::Tensor& refs) {
+  return {table.data_ptr<int32_t>(), lens ? lens->data_ptr<int32_t>() : nullptr,
+          refs.data_ptr<int32_t>()};
+}
+void check_pool(const torch::Tensor& pages, const torch::Tensor& refs) {
+  TORCH_CHECK(pages.device() == refs.device() && pages.dtype() == torch::kUInt8 &&
+                  pages.dim() == 2 && pages.is_contiguous(),
+              "pages must be contiguous uint8 [pages, page bytes]");
+  TORCH_CHECK(pages.size(0) == refs.size(0), "refs must have one entry per page");
+}
+uint32_t page_size_of(int64_t page_size) {
+  TORCH_CHECK(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
+              "page_size must be a power of two, 16..4096");
+  return uint32_t(page_size);
+}
+}  // namespace
+
+int64_t kv4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t page_size) {
+  TORCH_CHECK(kv_heads > 0, "kv_heads must be positive");
+  TORCH_CHECK(head_dim == 64 || head_dim == 128, "unsupported head dimension ", head_dim);
+  return int64_t(felix::kv4_page_bytes(uint32_t(kv_heads), uint32_t(head_dim),
+                                       page_size_of(page_size)));
+}
+
+void kv4_append(const torch::Tensor& pages, const torch::Tensor& table, const torch::Tensor& lens,
+                const torch::Tensor& key, const torch::Tensor& value, const OptTensor& counts) {
+  TORCH_CHECK(key.dim() == 4 && key.sizes() == value.sizes(),
+              "key and value must have the same shape [slots, kv_heads, rows, D]");
+  const auto type = half_type(key, "key");
+  TORCH_CHECK(value.dtype() == key.dtype(), "key and value must have the same dtype");
+  const auto cache = cache_of(pages, table, lens, key.size(1), key.size(3));
+  TORCH_CHECK(key.device() == pages.device() && value.device() == pages.device(),
+              "key and value must be on ", pages.device());
+  TORCH_CHECK(key.size(0) == table.size(0), "key must have one entry per slot");
+  const int32_t* n = counts_of(counts, lens);
+  const c10::cuda::CUDAGuard guard(pages.device());
+  const auto K = inner_contiguous(key), V = inner_contiguous(value);
+  const auto status = felix::kv4_append_launch(
+      cache, K.data_ptr(), V.data_ptr(), type, uint32_t(K.size(2)), K.strides().data(),
+      V.strides().data(), n, at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_append: kernel launch failed: ", status.str());
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_read(const torch::Tensor& pages,
+                                                  const torch::Tensor& table,
+                                                  const torch::Tensor& lens, int64_t rows,
+                                                  int64_t kv_heads, int64_t head_dim,
+                                                  const OptTensor& counts) {
+  TORCH_CHECK(rows >= 0 && rows <= 0x7fffffff, "rows must be 0..2^31-1");
+  const auto cache = cache_of(pages, table, lens, kv_heads, head_dim);
+  const int32_t* n = counts_of(counts, lens);
+  const c10::cuda::CUDAGuard guard(pages.device());
+  const auto opt = pages.options().dtype(torch::kHalf);
+  auto K = torch::empty({table.size(0), kv_heads, rows, head_dim}, opt);
+  auto V = torch::empty_like(K);
+  if (K.numel() == 0) return {K, V};
+  const auto status = felix::kv4_read_launch(
+      cache, uint32_t(rows), n, reinterpret_cast<half*>(K.data_ptr<at::Half>()),
+      reinterpret_cast<half*>(V.data_ptr<at::Half>()), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_read: kernel launch failed: ", status.str());
+  return {K, V};
+}
+
+torch::Tensor kv4_attention(const torch::Tensor& query, const torch::Tensor& pages,
+                            const torch::Tensor& table, const torch::Tensor& lens, int64_t kv_heads,
+                            const OptTensor& counts, double scale) {
+  return std::get<0>(
+      kv4_attention_impl(query, pages, table, lens, kv_heads, counts, scale, false));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_attention_lse(
+    const torch::Tensor& query, const torch::Tensor& pages, const torch::Tensor& table,
+    const torch::Tensor& lens, int64_t kv_heads, const OptTensor& counts, double scale) {
+  return kv4_attention_impl(query, pages, table, lens, kv_heads, counts, scale, true);
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv4_reserve(
+    const torch::Tensor& table, const torch::Tensor& lens, const torch::Tensor& refs,
+    const torch::Tensor& counts, int64_t page_size, const Kv4Out& out) {
+  check_state(table, &lens, refs);
+  const int32_t* n = counts_of(counts, lens);
+  const uint32_t size = page_size_of(page_size);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const auto o = page_outputs({table, lens, refs}, out);
+  auto report = torch::empty({2}, lens.options());
+  const auto status = felix::kv4_reserve_launch(
+      pages_of(table, &lens, refs), n, uint32_t(table.size(0)), uint32_t(table.size(1)),
+      uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]), report.data_ptr<int32_t>(),
+      at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_reserve: kernel launch failed: ", status.str());
+  return {o[0], o[1], o[2], report};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv4_fork(
+    const torch::Tensor& pages, const torch::Tensor& table, const torch::Tensor& lens,
+    const torch::Tensor& refs, const torch::Tensor& parents, const torch::Tensor& children,
+    int64_t page_size, const Kv4Out& out) {
+  check_state(table, &lens, refs);
+  check_pool(pages, refs);
+  check_i32(parents, table.device(), 1, "parents");
+  check_i32(children, table.device(), 1, "children");
+  TORCH_CHECK(parents.size(0) == children.size(0), "parents and children must have the same length");
+  const uint32_t size = page_size_of(page_size);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const auto o = page_outputs({table, lens, refs}, out);
+  auto report = torch::empty({2}, lens.options());
+  const auto status = felix::kv4_fork_launch(
+      pages.data_ptr(), size_t(pages.size(1)), pages_of(table, &lens, refs), i32(parents),
+      i32(children), uint32_t(parents.size(0)), uint32_t(table.size(0)), uint32_t(table.size(1)),
+      uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]), report.data_ptr<int32_t>(),
+      at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_fork: kernel launch failed: ", status.str());
+  return {o[0], o[1], o[2], report};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv4_free(
+    const torch::Tensor& table, const torch::Tensor& lens, const torch::Tensor& refs,
+    const torch::Tensor& slots, int64_t page_size, const Kv4Out& out) {
+  check_state(table, &lens, refs);
+  check_i32(slots, table.device(), 1, "slots");
+  const uint32_t size = page_size_of(page_size);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const auto o = page_outputs({table, lens, refs}, out);
+  const auto status = felix::kv4_free_launch(
+      pages_of(table, &lens, refs), i32(slots), uint32_t(slots.size(0)), uint32_t(table.size(0)),
+      uint32_t(table.size(1)), uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]),
+      at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_free: kernel launch failed: ", status.str());
+  return {o[0], o[1], o[2]};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_compact(const torch::Tensor& pages,
+                                                     const torch::Tensor& table,
+                                                     const torch::Tensor& refs,
+                                                     const Kv4Out& out) {
+  check_state(table, nullptr, refs);
+  check_pool(pages, refs);
+  const c10::cuda::CUDAGuard guard(table.device());
+  const auto o = page_outputs({table, refs}, out);
+  const auto status = felix::kv4_compact_launch(
+      pages.data_ptr(), size_t(pages.size(1)), pages_of(table, nullptr, refs),
+      uint32_t(table.size(0)), uint32_t(table.size(1)), uint32_t(refs.size(0)),
+      pages_of(o[0], nullptr, o[1]), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_compact: kernel launch failed: ", status.str());
+  return {o[0], o[1]};
+}
+
+void kv4_copy_pages(const torch::Tensor& src_pages, const torch::Tensor& dst_pages,
+                    const torch::Tensor& src, const torch::Tensor& dst) {
+  for (const auto* p : {&src_pages, &dst_pages})
+    TORCH_CHECK(p->is_cuda() && p->dtype() == torch::kUInt8 && p->dim() == 2 && p->is_contiguous(),
+                "pages must be contiguous uint8 [pages, page bytes] on a CUDA device");
+  TORCH_CHECK(src_pages.device() == dst_pages.device() && src_pages.size(1) == dst_pages.size(1),
+              "both pools must be on one device and have pages of the same bytes");
+  check_i32(src, dst_pages.device(), 1, "src");
+  check_i32(dst, dst_pages.device(), 1, "dst");
+  TORCH_CHECK(src.size(0) == dst.size(0), "src and dst must have the same length");
+  const c10::cuda::CUDAGuard guard(dst_pages.device());
+  const auto status = felix::kv4_copy_pages_launch(
+      src_pages.data_ptr(), uint64_t(src_pages.size(0)), dst_pages.data_ptr(),
+      uint64_t(dst_pages.size(0)), size_t(dst_pages.size(1)), i32(src), i32(dst),
+      uint32_t(src.size(0)), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "kv4_copy_pages: kernel launch failed: ", status.str());
+}
+
+std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits,
+                                                const torch::Tensor& uniform,
+                                                const OptTensor& temperature,
+                                                const OptTensor& top_k, const OptTensor& top_p,
+                                                const OptTensor& min_p) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be CUDA tensor");
+  TORCH_CHECK(logits.dim() == 2, "logits must be 2D [rows, vocab]");
+  TORCH_CHECK(logits.dtype() == torch::kFloat32 || logits.dtype() == torch::kHalf ||
+                  logits.dtype() == torch::kBFloat16,
+              "logits must be float32, float16 or bfloat16");
+  TORCH_CHECK(logits.size(1) > 0, "vocab must not be empty");
+  const int64_t rows = logits.size(0);
+  auto per_row = [&](const torch::Tensor& t, torch::ScalarType type, const char* name) {
+    TORCH_CHECK(t.device() == logits.device(), name, " must be on ", logits.device());
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == rows && t.is_contiguous(), name,
+                " must be contiguous with one entry per row");
+  };
+  auto f32 = [&](const OptTensor& t, const char* name) -> const float* {
+    if (!t) return nullptr;
+    per_row(*t, torch::kFloat32, name);
+    return t->data_ptr<float>();
+  };
+  per_row(uniform, torch::kFloat32, "uniform");
+  if (top_k) per_row(*top_k, torch::kInt32, "top_k");
+  const float *t = f32(temperature, "temperature"), *p = f32(top_p, "top_p"),
+              *m = f32(min_p, "min_p");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const auto X = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
+  auto tokens = torch::empty({rows}, X.options().dtype(torch::kInt32));
+  auto logprobs = torch::empty({rows}, X.options().dtype(torch::kFloat32));
+  const auto type = X.dtype() == torch::kFloat32 ? felix::ElementType::F32 : half_type(X, "logits");
+  const auto status = felix::sample_launch(
+      X.data_ptr(), type, uint32_t(rows), uint32_t(X.size(1)), X.stride(0),
+      uniform.data_ptr<float>(), t, top_k ? i32(*top_k) : nullptr, p, m, tokens.data_ptr<int32_t>(),
+      logprobs.data_ptr<float>(), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(status.ok(), "sample: kernel launch failed: ", status.str());
+  return {tokens, logprobs};
+}
+
 }  // namespace sion
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -232,4 +536,34 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "flash attention backward returning (dQ, dK, dV)", py::arg("query"), py::arg("key"),
         py::arg("value"), py::arg("out"), py::arg("lse"), py::arg("grad_out"),
         py::arg("causal") = false);
+  const auto none = py::none();
+  m.def("kv4_page_bytes", &sion::kv4_page_bytes, "bytes of a page of the 4-bit cache",
+        py::arg("kv_heads"), py::arg("head_dim"), py::arg("page_size"));
+  m.def("kv4_append", &sion::kv4_append, "write new tokens into the 4-bit cache", py::arg("pages"),
+        py::arg("table"), py::arg("lens"), py::arg("key"), py::arg("value"),
+        py::arg("counts") = none);
+  m.def("kv4_read", &sion::kv4_read, "the last tokens of each slot as fp16 (K, V)",
+        py::arg("pages"), py::arg("table"), py::arg("lens"), py::arg("rows"), py::arg("kv_heads"),
+        py::arg("head_dim"), py::arg("counts") = none);
+  m.def("kv4_attention", &sion::kv4_attention, "attention of new tokens over the 4-bit cache",
+        py::arg("query"), py::arg("pages"), py::arg("table"), py::arg("lens"), py::arg("kv_heads"),
+        py::arg("counts") = none, py::arg("scale") = 0.0);
+  m.def("kv4_attention_lse", &sion::kv4_attention_lse, "kv4_attention returning (O, fp32 LSE)",
+        py::arg("query"), py::arg("pages"), py::arg("table"), py::arg("lens"), py::arg("kv_heads"),
+        py::arg("counts") = none, py::arg("scale") = 0.0);
+  m.def("kv4_reserve", &sion::kv4_reserve, "pages for each slot's next tokens", py::arg("table"),
+        py::arg("lens"), py::arg("refs"), py::arg("counts"), py::arg("page_size"),
+        py::arg("out") = none);
+  m.def("kv4_fork", &sion::kv4_fork, "slots that share a parent's pages", py::arg("pages"),
+        py::arg("table"), py::arg("lens"), py::arg("refs"), py::arg("parents"),
+        py::arg("children"), py::arg("page_size"), py::arg("out") = none);
+  m.def("kv4_free", &sion::kv4_free, "empty slots", py::arg("table"), py::arg("lens"),
+        py::arg("refs"), py::arg("slots"), py::arg("page_size"), py::arg("out") = none);
+  m.def("kv4_compact", &sion::kv4_compact, "move the pages in use to the lowest numbers",
+        py::arg("pages"), py::arg("table"), py::arg("refs"), py::arg("out") = none);
+  m.def("kv4_copy_pages", &sion::kv4_copy_pages, "copy pages between pools", py::arg("src_pages"),
+        py::arg("dst_pages"), py::arg("src"), py::arg("dst"));
+  m.def("sample", &sion::sample, "one token per row of logits (tokens, log-probabilities)",
+        py::arg("logits"), py::arg("uniform"), py::arg("temperature") = none,
+        py::arg("top_k") = none, py::arg("top_p") = none, py::arg("min_p") = none);
 }
