@@ -18,6 +18,12 @@
 // that of score + exponent of scale_v), so that neither tiny nor huge values
 // lose bits, and the -8 is applied to the sum of the same rounded numbers, so
 // that the offset cancels exactly. Sums and statistics are fp32.
+//
+// The mma.sync form is used, not tcgen05: the product has 8 useful columns (one
+// group of heads), the codes reach the instruction from registers after one
+// logic operation per pair, and the kernel is bound by reading the cache and by
+// those logic operations, not by the matrix unit; tcgen05 would need the codes
+// expanded to fp16 in shared or tensor memory, four times the bytes of the cache.
 #include "felix_internal.h"
 #include "kv4_layout.cuh"
 #include "sm100_ptx.cuh"
@@ -29,8 +35,8 @@ using namespace felix_kv4;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kCentre = 8;  // blocks of a warp between two centrings of the sums
-constexpr int kTile = kBlock * kWarps;  // tokens of a tile: one block per warp
+constexpr int kStep = 2;                     // blocks that a warp takes at once
+constexpr int kStepTokens = kStep * kBlock;  // 32: one per lane
 
 struct AttnParams {
   CacheView c;
@@ -44,6 +50,8 @@ struct AttnParams {
   float scale_log2;                  // softmax scale * log2(e)
   uint32_t* counters;                // one per CTA, zero between launches
   float* partials;                   // [CTA][2][8 NT][D + 2]
+  unsigned* status;                  // watchdog word
+  bool q_vec;                        // rows of q are 16-byte aligned
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -53,6 +61,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a * b + c, c left as it is
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1,
+                                         const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]),
+        "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -66,12 +85,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 template <int W>
-struct Words;  // W 32-bit words loaded as one vector
+struct Words;  // W 32-bit words loaded as one vector from shared memory
 template <>
 struct Words<4> {
   uint32_t w[4];
   __device__ __forceinline__ void load(const unsigned char* p) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
 };
@@ -79,53 +98,26 @@ template <>
 struct Words<2> {
   uint32_t w[2];
   __device__ __forceinline__ void load(const unsigned char* p) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x, w[1] = v.y;
   }
 };
 
-// A lane's share of one block: D/32 words of K for tokens g and g + 8, of V for
-// the token pairs of both halves, and the parameters of tokens g and g + 8.
-template <int D>
-struct BlockRegs {
-  Words<D / 32> k0, k1, v0, v1;
-  uint32_t kp0, kp1, vp0, vp1;
-  bool there;
-  __device__ __forceinline__ void load(const unsigned char* p, int lane) {
-    there = p != nullptr;
-    if (!there) return;
-    constexpr int kLane = D / 8;  // bytes of a lane's vector
-    const int g = lane >> 2;
-    k0.load(p + lane * kLane);
-    k1.load(p + 4 * D + lane * kLane);
-    v0.load(p + v_codes_at(D) + lane * kLane);
-    v1.load(p + v_codes_at(D) + 4 * D + lane * kLane);
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(p + k_params_at(D));
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(p + v_params_at(D));
-    kp0 = __ldg(kp + g), kp1 = __ldg(kp + g + 8);
-    vp0 = __ldg(vp + g), vp1 = __ldg(vp + g + 8);
-  }
+// What a step's tokens bring to scores and sums, decoded once by one lane each.
+struct alignas(16) TokenParams {
+  float4 v[kStepTokens];  // exponent E of scale_v, 2^-E, scale_v 2^-E, base_v 2^-E
+  float2 k[kStepTokens];  // scale_k, base_k - 8 scale_k
 };
-
-// (scale, base) of a K token -> scale and base - 8 scale.
 __device__ __forceinline__ float2 k_params(uint32_t p) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
   return make_float2(f.x, fmaf(-8.f, f.x, f.y));
 }
-// (scale, base) of a V token: the scale's exponent E (of the smallest normal
-// where it is subnormal), 2^-E, scale * 2^-E, base * 2^-E.
-struct VParams {
-  float e, inv, mant, base;
-};
-__device__ __forceinline__ VParams v_params(uint32_t p) {
+// E is the exponent of the smallest normal where scale_v is subnormal or zero.
+__device__ __forceinline__ float4 v_params(uint32_t p) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
   const int e = max(int((p >> 10) & 31u), 1) - 15;
-  VParams r;
-  r.e = float(e);
-  r.inv = __int_as_float((127 - e) << 23);
-  r.mant = f.x * r.inv;
-  r.base = f.y * r.inv;
-  return r;
+  const float inv = __int_as_float((127 - e) << 23);
+  return make_float4(float(e), inv, f.x * inv, f.y * inv);
 }
 
 template <typename T>
@@ -141,20 +133,20 @@ __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 
-// One segment (slot, kv head, tile of rows) or a part of it: tokens
-// [tile_lo, tile_hi) * kTile. Registers of a warp after its blocks.
+// The sums of one warp over its steps of a segment (slot, kv head, tile of rows).
 template <typename T, int D, int NT>
 struct Attn {
   static constexpr int kRows = 8 * NT;
   static constexpr int kW = D / 32;       // words of a lane's vector
+  static constexpr int kLane = D / 8;     // its bytes
   uint32_t q[NT][2 * kW][2];              // operand registers of 8 query rows each
   // score = (raw * scale_k + qs * (base_k - 8 scale_k)) * f: raw sums are in units
   // of 2^-24 and of the row's power of two, and so is qs = sum(q), so that the
   // terms cancel before anything is rounded to a scale
   float f[NT][2], qs[NT][2];
   int lim[NT][2];                         // tokens that this thread's two rows see
-  float o[NT][D / 16][4], o8[NT][4];      // sums of p scale_v c, of 8 p scale_v since centre()
-  float m[NT][2], l[NT][2], b[NT][2];     // running maximum, sum of p, sum of p base_v
+  float o[NT][D / 16][4];                 // sums of p scale_v (c - 8); odd rows 16 times that
+  float m[NT][2], l[NT][2], b_[NT][2];     // running maximum, sum of p, sum of p base_v
   int low;                                // the smallest of lim
 
   __device__ __forceinline__ void load_q(const AttnParams& P, uint32_t slot, uint32_t kvh,
@@ -170,11 +162,20 @@ struct Attn {
       float top = 0.f, sum = 0.f;
       const T* src = static_cast<const T*>(P.q) + int64_t(slot) * P.qs_slot +
                      int64_t(head) * P.qs_head + int64_t(row) * P.qs_row + t * (D / 4);
+      if (live && P.q_vec) {
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) {
-        v[i] = live ? to_f<T>(src[i]) : 0.f;
-        top = fmaxf(top, fabsf(v[i]));
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 w = reinterpret_cast<const uint4*>(src)[i];
+          const T* x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[8 * i + j] = to_f<T>(x[j]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) v[i] = live ? to_f<T>(src[i]) : 0.f;
       }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(v[i]));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       // scale the row by a power of two so that its largest value is in
@@ -210,7 +211,7 @@ struct Attn {
         const int rw = int(rr / P.group);
         lim[n][c] = (rw < int(P.rows) && rw < count) ? max(len - count + rw + 1, 0) : 0;
         m[n][c] = -INFINITY;
-        l[n][c] = b[n][c] = 0.f;
+        l[n][c] = b_[n][c] = 0.f;
       }
       // rows past the last do not narrow the unmasked range
       const bool past = rt * kRows + 8 * n + 2 * t >= P.rows * P.group;
@@ -220,61 +221,96 @@ struct Attn {
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[n][j][c] = 0.f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o8[n][c] = 0.f;
     }
     low = min(low, __shfl_xor_sync(~0u, low, 1));
     low = min(low, __shfl_xor_sync(~0u, low, 2));
   }
 
-  __device__ __forceinline__ void block(const BlockRegs<D>& x, int token0, int lane) {
+  // One step: kStep blocks at `x`, of which those in `there` exist.
+  __device__ __forceinline__ void step(const unsigned char* x, TokenParams& tp, uint32_t there,
+                                       int token0, int lane) {
+    constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
+    constexpr int kB = int(block_bytes(D));
     const int g = lane >> 2;
-    const float2 ka = k_params(x.kp0), kb = k_params(x.kp1);
-    const VParams va = v_params(x.vp0), vb = v_params(x.vp1);
-    uint32_t pt[NT][2];
+    {
+      const unsigned char* p = x + (lane / 16) * kB;
+      tp.k[lane] = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[lane & 15]);
+      tp.v[lane] = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
+    }
+    __syncwarp();
+    float s[NT][kStep][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < kStep; ++b) {
+      Words<kW> k0, k1;
+      k0.load(x + b * kB + lane * kLane);
+      k1.load(x + b * kB + 4 * D + lane * kLane);
+      float s2[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[n][b][c] = s2[n][c] = 0.f;
 #pragma unroll
       for (int w = 0; w < kW; ++w) {
-        const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
-        const uint32_t a = x.k0.w[w], c = x.k1.w[w], a8 = a >> 8, c8 = c >> 8;
-        mma16816(s, a & lo, c & lo, a & hi, c & hi, q[n][2 * w][0], q[n][2 * w][1]);
-        mma16816(s, a8 & lo, c8 & lo, a8 & hi, c8 & hi, q[n][2 * w + 1][0], q[n][2 * w + 1][1]);
-      }
-      // s[0], s[1]: token g of rows 2t, 2t + 1; s[2], s[3]: token g + 8.
+        const uint32_t a = k0.w[w], c = k1.w[w], a8 = a >> 8, c8 = c >> 8;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        s[c] = fmaf(fmaf(s[c], ka.x, qs[n][c] * ka.y), f[n][c], va.e);
-        s[2 + c] = fmaf(fmaf(s[2 + c], kb.x, qs[n][c] * kb.y), f[n][c], vb.e);
-      }
-      bool on[4] = {true, true, true, true};
-      if (token0 + int(kBlock) > low) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          on[c] = token0 + g < lim[n][c];
-          on[2 + c] = token0 + g + 8 < lim[n][c];
-          if (!on[c]) s[c] = -INFINITY;
-          if (!on[2 + c]) s[2 + c] = -INFINITY;
+        for (int n = 0; n < NT; ++n) {
+          mma16816(s[n][b], a & lo, c & lo, a & hi, c & hi, q[n][2 * w][0], q[n][2 * w][1]);
+          // two chains where few others run beside them
+          mma16816(NT == 1 ? s2[n] : s[n][b], a8 & lo, c8 & lo, a8 & hi, c8 & hi,
+                   q[n][2 * w + 1][0], q[n][2 * w + 1][1]);
         }
+      }
+      if (NT == 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[0][b][c] += s2[0][c];
+    }
+    const bool all = there == (1u << kStep) - 1 && token0 + kStepTokens <= low;
+    uint32_t pt[NT][kStep][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // s[b][0], s[b][1]: token g of block b, rows 2t, 2t + 1; s[b][2], s[b][3]: token g + 8
+      float ex[kStep][2];
+#pragma unroll
+      for (int b = 0; b < kStep; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 k = tp.k[b * 16 + h * 8 + g];
+          ex[b][h] = tp.v[b * 16 + h * 8 + g].x;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            s[n][b][2 * h + c] =
+                fmaf(fmaf(s[n][b][2 * h + c], k.x, qs[n][c] * k.y), f[n][c], ex[b][h]);
+        }
+      uint32_t off = 0;  // a bit for each masked score
+      if (!all) {
+#pragma unroll
+        for (int b = 0; b < kStep; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool on = (there >> b & 1) && token0 + b * 16 + (i / 2) * 8 + g < lim[n][i & 1];
+            if (!on) s[n][b][i] = -INFINITY, off |= 1u << (4 * b + i);
+          }
       }
       // The sums are kept relative to a maximum that is only moved when a score
       // passes it by 2^8: probabilities stay below 2^9 and fp16 holds them.
-      const bool over = s[0] > m[n][0] + 8.f || s[2] > m[n][0] + 8.f || s[1] > m[n][1] + 8.f ||
-                        s[3] > m[n][1] + 8.f;
-      if (__any_sync(~0u, over)) {
+      float t0 = s[n][0][0], t1 = s[n][0][1];
+      t0 = fmaxf(t0, s[n][0][2]), t1 = fmaxf(t1, s[n][0][3]);
+#pragma unroll
+      for (int b = 1; b < kStep; ++b) {
+        t0 = fmaxf(t0, fmaxf(s[n][b][0], s[n][b][2]));
+        t1 = fmaxf(t1, fmaxf(s[n][b][1], s[n][b][3]));
+      }
+      if (__any_sync(~0u, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float top = fmaxf(m[n][c], fmaxf(s[c], s[2 + c]));
+          float top = fmaxf(m[n][c], c ? t1 : t0);
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
           const float keep = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
           m[n][c] = top;
           l[n][c] *= keep;
-          b[n][c] *= keep;
-          o8[n][c] *= keep;
-          o8[n][2 + c] *= keep;
+          b_[n][c] *= keep;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             o[n][j][c] *= keep;
@@ -282,49 +318,73 @@ struct Attn {
           }
         }
       }
-      float p[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float e = on[c] ? ex2(s[c] - m[n][c & 1]) : 0.f;
-        const VParams& v = c < 2 ? va : vb;
-        // a masked token's parameters may be anything, NaN among it
-        p[c] = on[c] ? e * v.mant : 0.f;
-        l[n][c & 1] = on[c] ? fmaf(e, v.inv, l[n][c & 1]) : l[n][c & 1];
-        b[n][c & 1] = on[c] ? fmaf(e, v.base, b[n][c & 1]) : b[n][c & 1];
+      for (int b = 0; b < kStep; ++b) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 v = tp.v[b * 16 + h * 8 + g];
+          float p[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int i = 2 * h + c;
+            const float e = ex2(s[n][b][i] - m[n][c]);
+            if (off >> (4 * b + i) & 1) {  // a masked token's parameters may be anything
+              p[c] = 0.f;
+            } else {
+              p[c] = e * v.z;
+              l[n][c] = fmaf(e, v.y, l[n][c]);
+              b_[n][c] = fmaf(e, v.w, b_[n][c]);
+            }
+          }
+          pt[n][b][h] = transpose8x8(felix_sm100::pack_half2(p[0], p[1]));
+        }
       }
-      pt[n][0] = transpose8x8(felix_sm100::pack_half2(p[0], p[1]));
-      pt[n][1] = transpose8x8(felix_sm100::pack_half2(p[2], p[3]));
-      constexpr uint32_t eight = 0x00080008u;  // 8 * 2^-24, the codes' unit
-      mma16816(o8[n], eight, eight, eight, eight, pt[n][0], pt[n][1]);
+    }
+    // -8 sum(p scale_v) of the step in the codes' unit, 16 times that for the odd
+    // rows: where the second product starts, so that it sums to what is small.
+    float start[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      constexpr uint32_t m8 = 0x80088008u, m128 = 0x80808080u;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) start[n][c] = 0.f;
+#pragma unroll
+      for (int b = 0; b < kStep; ++b)
+        mma16816(start[n], m8, m128, m8, m128, pt[n][b][0], pt[n][b][1]);
+    }
+    Words<kW> v0[kStep], v1[kStep];
+#pragma unroll
+    for (int b = 0; b < kStep; ++b) {
+      v0[b].load(x + b * kB + v_codes_at(D) + lane * kLane);
+      v1[b].load(x + b * kB + v_codes_at(D) + 4 * D + lane * kLane);
     }
 #pragma unroll
     for (int w = 0; w < kW; ++w) {
-      const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
-      const uint32_t a = x.v0.w[w], c = x.v1.w[w], a8 = a >> 8, c8 = c >> 8;
+      float r[NT][2][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma16816(o[n][2 * w], a & lo, a & hi, c & lo, c & hi, pt[n][0], pt[n][1]);
-        mma16816(o[n][2 * w + 1], a8 & lo, a8 & hi, c8 & lo, c8 & hi, pt[n][0], pt[n][1]);
-      }
-    }
-  }
-
-  // Takes the codes' offset out of the sums: o (the odd registers are of 16 code)
-  // would otherwise grow with the number of tokens, and its last bits with it,
-  // while the result is a mean. Once every kCentre blocks.
-  __device__ __forceinline__ void centre() {
+      for (int b = 0; b < kStep; ++b) {
+        const uint32_t a = v0[b].w[w], c = v1[b].w[w], a8 = a >> 8, c8 = c >> 8;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          o[n][j][c] -= o8[n][c];
-          o[n][j][2 + c] = fmaf(-16.f, o8[n][c], o[n][j][2 + c]);
+        for (int n = 0; n < NT; ++n) {
+          if (b == 0) {
+            mma16816(r[n][0], a & lo, a & hi, c & lo, c & hi, pt[n][b][0], pt[n][b][1], start[n]);
+            mma16816(r[n][1], a8 & lo, a8 & hi, c8 & lo, c8 & hi, pt[n][b][0], pt[n][b][1],
+                     start[n]);
+          } else {
+            mma16816(r[n][0], a & lo, a & hi, c & lo, c & hi, pt[n][b][0], pt[n][b][1]);
+            mma16816(r[n][1], a8 & lo, a8 & hi, c8 & lo, c8 & hi, pt[n][b][0], pt[n][b][1]);
+          }
         }
+      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o8[n][c] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          o[n][2 * w][c] += r[n][0][c];
+          o[n][2 * w + 1][c] += r[n][1][c];
+        }
     }
+    __syncwarp();  // the stage and tp are free
   }
 
   // Writes the warp's sums to shared memory: O [kRows][D] (base term included)
@@ -338,12 +398,12 @@ struct Attn {
 #pragma unroll
         for (int x = 4; x < 32; x *= 2) {
           l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
-          b[n][c] += __shfl_xor_sync(~0u, b[n][c], x);
+          b_[n][c] += __shfl_xor_sync(~0u, b_[n][c], x);
         }
         const int r = 8 * n + 2 * t + c;
         if (g == 0) sml[2 * r] = m[n][c], sml[2 * r + 1] = l[n][c];
         constexpr float u = 16777216.f;
-        const float off = b[n][c];
+        const float off = b_[n][c];
         float4* dst = reinterpret_cast<float4*>(so + r * D + g * (D / 8));
 #pragma unroll
         for (int w = 0; w < kW; ++w)
@@ -355,19 +415,62 @@ struct Attn {
   }
 };
 
-// Persistent grid. The work is a line of units (a segment's tiles of kTile
-// tokens, segment after segment; an empty slot counts as one unit), cut into
-// equal shares, one per CTA, whatever the slots' lengths. A segment that lies in
-// several shares is finished by the CTA that comes last to it, which joins the
-// parts in the order of the shares: the result does not depend on who is last.
+template <int D, int NT>
+struct Smem {
+  // stages of kStep blocks per warp: 37 to 52 KB of cache are under way per CTA, about
+  // 150 KB per SM
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kRows = 8 * NT;
+  alignas(128) unsigned char ring[kWarps][kStages][kStep * block_bytes(D)];
+  alignas(16) float o[kWarps][kRows * D];
+  TokenParams tp[kWarps];
+  uint64_t full[kWarps][kStages];
+  uint32_t there[kWarps][kStages];
+  float ml[kWarps][2 * kRows];
+  uint32_t scan[kWarps], at[2], ticket;
+  int abort;
+};
+
+// A place in a CTA's share of the work: the part [lo, hi) of a segment's steps.
+struct Place {
+  uint32_t slot, slot_at;  // slot, and the units before it
+  uint32_t tiles;          // steps of each of the slot's segments (an empty slot: one)
+  int len, reach;
+  uint32_t seg, lo, hi;
+  __device__ __forceinline__ void read(const AttnParams& P) {
+    len = slot_length(P.c, slot);
+    reach = slot_reach(P.c, slot);
+    tiles = max((reach + kStepTokens - 1) / kStepTokens, 1);
+  }
+  // unit u, at or after the current slot's first
+  __device__ __forceinline__ void open(const AttnParams& P, uint32_t u, uint32_t last) {
+    const uint32_t per_tile = P.c.kv_heads * P.row_tiles;
+    while (u >= slot_at + tiles * per_tile) {
+      slot_at += tiles * per_tile;
+      ++slot;
+      read(P);
+    }
+    seg = (u - slot_at) / tiles;
+    lo = (u - slot_at) % tiles;
+    hi = min(tiles, lo + (last - u));
+  }
+  __device__ __forceinline__ uint32_t end() const { return slot_at + seg * tiles + hi; }
+};
+
+// Persistent grid. The work is a line of units (a segment's steps of 32 tokens,
+// segment after segment; an empty slot counts as one), cut into equal shares, one
+// per CTA, whatever the slots' lengths; the warps of a CTA take its steps in turn.
+// Each warp has a ring of stages of its own in shared memory, filled by bulk
+// copies that it issues itself a few steps ahead, across segments: no barrier in
+// the loop, and the registers hold sums only. A segment that lies in several
+// shares is finished by the CTA that comes last to it, which joins the parts in a
+// fixed order: the result does not depend on who is last.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) {
-  constexpr int kRows = 8 * NT;
-  __shared__ __align__(16) float so[kWarps][kRows * D];
-  __shared__ float sml[kWarps][2 * kRows];
-  __shared__ uint32_t s_scan[kWarps];
-  __shared__ uint32_t s_at[2];
-  __shared__ uint32_t s_ticket;
+  constexpr int kRows = 8 * NT, kB = int(block_bytes(D)), kVec = kRows * D / 4;
+  using S = Smem<D, NT>;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const CacheView& c = P.c;
   const uint32_t per_tile = c.kv_heads * P.row_tiles;
@@ -375,153 +478,277 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
   // ---- this CTA's share: units before each thread's run of slots, then the slot
   const uint32_t run = (c.slots + kThreads - 1) / kThreads;
   const uint32_t s0 = min(tid * run, c.slots), s1 = min(s0 + run, c.slots);
+  auto units = [&](uint32_t s) {
+    return uint32_t(max((slot_reach(c, s) + kStepTokens - 1) / kStepTokens, 1)) * per_tile;
+  };
   uint32_t mine = 0;
-  for (uint32_t s = s0; s < s1; ++s)
-    mine += max((slot_reach(c, s) + kTile - 1) / kTile, 1) * per_tile;
+  for (uint32_t s = s0; s < s1; ++s) mine += units(s);
   uint32_t upto = mine;
 #pragma unroll
   for (int x = 1; x < 32; x *= 2) {
     const uint32_t v = __shfl_up_sync(~0u, upto, x);
     if (lane >= x) upto += v;
   }
-  if (lane == 31) s_scan[warp] = upto;
+  if (lane == 31) sm.scan[warp] = upto;
+  if (tid == 0) sm.abort = 0;
+  if (lane < S::kStages) felix_sm100::mbar_init(&sm.full[warp][lane], 1);
+  felix_sm100::fence_mbar_init();
+  felix_sm100::fence_proxy_async_smem();
   __syncthreads();
   uint32_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += s_scan[w];
-    total += s_scan[w];
+    if (w < warp) upto += sm.scan[w];
+    total += sm.scan[w];
   }
-  const uint32_t quota = (total + gridDim.x - 1) / gridDim.x;
-  const uint32_t first = blockIdx.x * quota, last = min(first + quota, total);
+  // at least one step for each warp: smaller parts cost more to join than they save
+  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, uint32_t(kWarps));
+  const uint32_t first = min(blockIdx.x * quota, total), last = min(first + quota, total);
   if (first >= last) return;
   if (first >= upto - mine && first < upto) {
     uint32_t at = upto - mine;
     for (uint32_t s = s0; s < s1; ++s) {
-      const uint32_t n = max((slot_reach(c, s) + kTile - 1) / kTile, 1) * per_tile;
+      const uint32_t n = units(s);
       if (first < at + n) {
-        s_at[0] = s, s_at[1] = at;
+        sm.at[0] = s, sm.at[1] = at;
         break;
       }
       at += n;
     }
   }
   __syncthreads();
-  uint32_t slot = s_at[0], slot_at = s_at[1];
 
-  for (uint32_t u = first; u < last;) {
-    const int len = slot_length(c, slot), reach = slot_reach(c, slot);
-    const uint32_t tiles = max((reach + kTile - 1) / kTile, 1);
-    if (u >= slot_at + tiles * per_tile) {
-      slot_at += tiles * per_tile;
-      ++slot;
-      continue;
+  Place use, get;  // the part being summed, and the one whose steps are being fetched
+  use.slot = sm.at[0], use.slot_at = sm.at[1];
+  use.read(P);
+  use.open(P, first, last);
+  get = use;
+  uint32_t get_t = get.lo + warp;
+  bool more = true;
+  // the next step to fetch: lane b looks up the page of its block b
+  int page = -1;
+  uint32_t in_page = 0;
+  auto look = [&]() {
+    while (more && get_t >= get.hi) {
+      const uint32_t u = get.end();
+      more = u < last;
+      if (more) {
+        get.open(P, u, last);
+        get_t = get.lo + warp;
+      }
     }
-    const uint32_t seg = (u - slot_at) / tiles, tile_lo = (u - slot_at) % tiles;
-    const uint32_t kvh = seg / P.row_tiles, rt = seg % P.row_tiles;
-    const uint32_t tile_hi = min(tiles, tile_lo + (last - u));
-    const int count = P.counts ? min(max(P.counts[slot], 0), int(P.rows)) : int(P.rows);
+    if (!more) return;
+    const uint32_t token = get_t * kStepTokens + lane * kBlock;
+    page = -1;
+    if (lane < kStep && int(token) < get.reach) {
+      page = c.table[size_t(get.slot) * c.width + (token >> c.page_shift)];
+      const uint32_t blocks = 1u << (c.page_shift - 4);
+      in_page = (get.seg / P.row_tiles) * blocks + ((token >> 4) & (blocks - 1));
+    }
+    get_t += kWarps;
+  };
+  auto fetch = [&](int stage) {  // issues the step that look() found
+    if (!more) return;
+    const bool ok = page >= 0 && uint64_t(page) < c.num_pages;
+    const uint32_t there = __ballot_sync(~0u, ok);
+    if (lane == 0) {
+      sm.there[warp][stage] = there;
+      felix_sm100::mbar_arrive_expect_tx(&sm.full[warp][stage], __popc(there) * kB);
+    }
+    __syncwarp();
+    if (ok)
+      felix_sm100::bulk_load_1d(&sm.ring[warp][stage][lane * kB],
+                                c.pages + size_t(page) * c.page_bytes + size_t(in_page) * kB, kB,
+                                &sm.full[warp][stage]);
+  };
+  for (int s = 0; s < S::kStages; ++s) {
+    look();
+    fetch(s);
+  }
+  look();
 
+  int stage = 0;
+  uint32_t parity = 0;
+  for (;;) {
+    const uint32_t kvh = use.seg / P.row_tiles, rt = use.seg % P.row_tiles;
+    const int count =
+        P.counts ? min(max(P.counts[use.slot], 0), int(P.rows)) : int(P.rows);
     Attn<T, D, NT> A;
-    A.load_q(P, slot, kvh, rt, len, count, lane);
-    BlockRegs<D> cur, next;
-    int token = int(tile_lo) * kTile + warp * int(kBlock);
-    const int end = min(reach, int(tile_hi) * kTile);
-    cur.load(token < end ? block_of(c, slot, token, kvh, D) : nullptr, lane);
-    for (int k = 1; token < end; token += kTile, ++k) {
-      const int then = token + kTile;
-      next.load(then < end ? block_of(c, slot, then, kvh, D) : nullptr, lane);
-      if (cur.there) A.block(cur, token, lane);
-      if (k % kCentre == 0) A.centre();
-      cur = next;
+    A.load_q(P, use.slot, kvh, rt, use.len, count, lane);
+    for (uint32_t t = use.lo + warp; t < use.hi; t += kWarps) {
+      if (felix_sm100::mbar_wait(&sm.full[warp][stage], parity, &sm.abort, P.status,
+                                 felix_sm100::kWdKv4Load)) {
+        const uint32_t there = sm.there[warp][stage];
+        if (there) A.step(sm.ring[warp][stage], sm.tp[warp], there, int(t) * kStepTokens, lane);
+      }
+      __syncwarp();
+      fetch(stage);
+      look();
+      if (++stage == S::kStages) stage = 0, parity ^= 1;
     }
-    A.centre();
-    A.park(so[warp], sml[warp], lane);
+    A.park(sm.o[warp], sm.ml[warp], lane);
     __syncthreads();
 
     // ---- join the warps; write the result, or this share's part of it
-    const bool whole = tile_lo == 0 && tile_hi == tiles;
-    const uint32_t seg_lo = slot_at + seg * tiles, seg_hi = seg_lo + tiles;
+    const bool whole = use.lo == 0 && use.hi == use.tiles;
+    const uint32_t seg_lo = use.slot_at + use.seg * use.tiles, seg_hi = seg_lo + use.tiles;
     const uint32_t c0 = seg_lo / quota, c1 = (seg_hi - 1) / quota;
-    const size_t part = size_t(kRows) * (D + 2);
-    float* mypart = P.partials + (size_t(blockIdx.x) * 2 + (tile_lo == 0 ? 1 : 0)) * part;
-    auto put = [&](int r, int d, float val, float top, float sum) {
+    constexpr size_t kPart = size_t(kRows) * (D + 2);
+    float* mypart = P.partials + (size_t(blockIdx.x) * 2 + (use.lo == 0 ? 1 : 0)) * kPart;
+    auto put = [&](int r, int d, float4 v, float top, float sum) {
       const uint32_t rr = rt * kRows + r;
       const uint32_t row = rr / P.group, head = kvh * P.group + rr % P.group;
       if (row >= P.rows) return;
-      const size_t at = (size_t(slot) * P.heads + head) * P.rows + row;
-      static_cast<T*>(P.out)[at * D + d] = from_f<T>(sum == 0.f ? 0.f : val / sum);
+      const size_t at = (size_t(use.slot) * P.heads + head) * P.rows + row;
+      const float k = sum == 0.f ? 0.f : 1.f / sum;
+      T x[4] = {from_f<T>(sum == 0.f ? 0.f : v.x * k), from_f<T>(sum == 0.f ? 0.f : v.y * k),
+                from_f<T>(sum == 0.f ? 0.f : v.z * k), from_f<T>(sum == 0.f ? 0.f : v.w * k)};
+      *reinterpret_cast<uint2*>(static_cast<T*>(P.out) + at * D + d) =
+          *reinterpret_cast<const uint2*>(x);
       if (P.lse && d == 0)
         P.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     };
-    for (int i = tid; i < kRows * D; i += kThreads) {
-      const int r = i / D, d = i % D;
-      float top = sml[0][2 * r];
+    for (int i = tid; i < kVec; i += kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float top = sm.ml[0][2 * r];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sml[w][2 * r]);
-      float val = 0.f, sum = 0.f;
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][2 * r]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        // a warp that saw nothing of the row has m = -inf, l = 0 and O = 0
-        const float k = sml[w][2 * r] == -INFINITY ? 0.f : ex2(sml[w][2 * r] - top);
-        if (k != 0.f) {
-          val = fmaf(so[w][i], k, val);
-          sum = fmaf(sml[w][2 * r + 1], k, sum);
-        } else if (sml[w][2 * r + 1] != sml[w][2 * r + 1]) {
-          val = sum = sml[w][2 * r + 1];  // NaN
-        }
+        // a warp that saw nothing of the row has l = 0 and O = 0; m = -inf with l
+        // not 0 is a warp that saw NaN only
+        const float wl = sm.ml[w][2 * r + 1], wm = sm.ml[w][2 * r];
+        if (wl == 0.f) continue;
+        const float k = wm == -INFINITY ? 1.f : ex2(wm - top);
+        const float4 x = reinterpret_cast<const float4*>(sm.o[w])[i];
+        v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y);
+        v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
+        sum = fmaf(wl, k, sum);
       }
       if (whole) {
-        put(r, d, val, top, sum);
+        put(r, d, v, top, sum);
       } else {
-        mypart[r * D + d] = val;
+        reinterpret_cast<float4*>(mypart)[i] = v;
         if (d == 0) mypart[kRows * D + 2 * r] = top, mypart[kRows * D + 2 * r + 1] = sum;
       }
     }
     if (!whole) {
       __threadfence();
       __syncthreads();
-      if (tid == 0) s_ticket = atomicAdd(P.counters + c0, 1u);
+      if (tid == 0) sm.ticket = atomicAdd(P.counters + c0, 1u);
       __syncthreads();
-      if (s_ticket == c1 - c0) {
+      if (sm.ticket == c1 - c0) {
         __threadfence();
-        for (int i = tid; i < kRows * D; i += kThreads) {
-          const int r = i / D, d = i % D;
-          float top = -INFINITY, val = 0.f, sum = 0.f;
-          for (uint32_t k = c0; k <= c1; ++k) {
-            const float* pp = P.partials + (size_t(k) * 2 + (k == c0 ? 1 : 0)) * part;
-            const float pm = __ldcg(pp + kRows * D + 2 * r), pl = __ldcg(pp + kRows * D + 2 * r + 1);
-            const float pv = __ldcg(pp + r * D + d);
-            if (pl == 0.f) continue;  // saw nothing of the row
-            const float to = fmaxf(top, pm);
-            const float ka = top == -INFINITY ? 0.f : ex2(top - to);
-            const float kb = pm == -INFINITY ? 1.f : ex2(pm - to);
-            val = val * ka + pv * kb;
-            sum = sum * ka + pl * kb;
-            top = to;
+        // each warp joins every kWarps-th part, then the warps are joined: all
+        // loads of a warp are independent of one another
+        auto part_at = [&](uint32_t k) {
+          return P.partials + (size_t(k) * 2 + (k == c0 ? 1 : 0)) * kPart;
+        };
+        for (int r = lane; r < kRows; r += 32) {
+          float top = -INFINITY, sum = 0.f;
+          for (uint32_t k = c0 + warp; k <= c1; k += kWarps)
+            top = fmaxf(top, __ldcg(part_at(k) + kRows * D + 2 * r));
+          for (uint32_t k = c0 + warp; k <= c1; k += kWarps) {
+            const float pm = __ldcg(part_at(k) + kRows * D + 2 * r);
+            const float pl = __ldcg(part_at(k) + kRows * D + 2 * r + 1);
+            if (pl != 0.f) sum = fmaf(pl, pm == -INFINITY ? 1.f : ex2(pm - top), sum);
           }
-          put(r, d, val, top, sum);
+          sm.ml[warp][2 * r] = top;
+          sm.ml[warp][2 * r + 1] = sum;
+        }
+        __syncwarp();
+        constexpr int kPer = kVec / 32;  // vectors of a lane
+        for (int j0 = 0; j0 < kPer; j0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (uint32_t k = c0 + warp; k <= c1; k += kWarps) {
+            const float* pp = part_at(k);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (j0 + j >= kPer) break;
+              const int i = (j0 + j) * 32 + lane, r = i / (D / 4);
+              const float pm = __ldcg(pp + kRows * D + 2 * r), pl = __ldcg(pp + kRows * D + 2 * r + 1);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(pp) + i);
+              const float w = pl == 0.f ? 0.f : pm == -INFINITY ? 1.f : ex2(pm - sm.ml[warp][2 * r]);
+              v[j].x = fmaf(x.x, w, v[j].x), v[j].y = fmaf(x.y, w, v[j].y);
+              v[j].z = fmaf(x.z, w, v[j].z), v[j].w = fmaf(x.w, w, v[j].w);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j0 + j < kPer)
+              reinterpret_cast<float4*>(sm.o[warp])[(j0 + j) * 32 + lane] = v[j];
+        }
+        __syncthreads();
+        for (int i = tid; i < kVec; i += kThreads) {
+          const int r = i / (D / 4), d = i % (D / 4) * 4;
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][2 * r]);
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float wl = sm.ml[w][2 * r + 1], wm = sm.ml[w][2 * r];
+            if (wl == 0.f) continue;
+            const float k = wm == -INFINITY ? 1.f : ex2(wm - top);
+            const float4 x = reinterpret_cast<const float4*>(sm.o[w])[i];
+            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y);
+            v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
+            sum = fmaf(wl, k, sum);
+          }
+          put(r, d, v, top, sum);
         }
         if (tid == 0) P.counters[c0] = 0;
       }
     }
     __syncthreads();
-    u += tile_hi - tile_lo;
+    const uint32_t u = use.end();
+    if (u >= last) break;
+    use.open(P, u, last);
   }
+  // after a wait that gave up, copies may still be under way into this CTA's
+  // shared memory: give them time to land (with a limit) before it goes to another
+  if (sm.abort)
+    for (int s = 0; s < S::kStages; ++s) {
+      const uint64_t t0 = felix_sm100::globaltimer_ns();
+      while (!felix_sm100::mbar_try_wait(felix_sm100::smem_u32(&sm.full[warp][s]), parity) &&
+             felix_sm100::globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
 }
+
+// CTAs per SM that a caller's workspace has room for.
+constexpr int kMaxPerSm = 4;
+constexpr size_t ws_bytes_for(uint32_t grid, int rows, int D) {
+  return kWsCounterBytes + size_t(grid) * 2 * rows * (D + 2) * sizeof(float);
+}
+// Tiles of 8 query rows that a warp keeps in registers: 5 of D = 64, 3 of D = 128.
+constexpr int max_nt(int D) { return D == 64 ? 5 : 3; }
 
 template <typename T, int D, int NT>
 FelixCode launch(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_bytes,
                  cudaStream_t stream) {
   static int per_sm[64];
   static PerDeviceOnce once;
+  constexpr int smem = int(sizeof(Smem<D, NT>));
   const int rc = once.run(dev->ordinal, [&] {
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-               &per_sm[dev->ordinal], kv4_attn_kernel<T, D, NT>, kThreads, 0) == cudaSuccess ? 0 : -1;
+    if (cudaFuncSetAttribute(kv4_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             smem) != cudaSuccess)
+      return -1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attn_kernel<T, D, NT>, kThreads,
+                                                      smem) != cudaSuccess || n < 1)
+      return -1;
+    per_sm[dev->ordinal] = n < kMaxPerSm ? n : kMaxPerSm;
+    return 0;
   });
   if (rc != 0) return launch_error(cudaGetLastError(), "kv4_attention: occupancy");
-  const uint32_t grid = uint32_t(dev->num_sms) * uint32_t(min(per_sm[dev->ordinal], 8));
-  const size_t need = kWsCounterBytes + size_t(grid) * 2 * 8 * NT * (D + 2) * sizeof(float);
+  const uint32_t grid = uint32_t(dev->num_sms) * uint32_t(per_sm[dev->ordinal]);
+  const size_t need = ws_bytes_for(grid, 8 * NT, D);
   if (workspace && ws_bytes < need)
     return api_error("kv4_attention: workspace smaller than felix_kv4_attention_workspace_size");
   void* ws = workspace ? workspace : library_workspace(dev, stream, need);
@@ -529,17 +756,37 @@ FelixCode launch(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_byte
   P.counters = static_cast<uint32_t*>(ws);
   P.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + kWsCounterBytes);
   P.row_tiles = (P.rows * P.group + 8 * NT - 1) / (8 * NT);
-  kv4_attn_kernel<T, D, NT><<<grid, kThreads, 0, stream>>>(P);
+  kv4_attn_kernel<T, D, NT><<<grid, kThreads, smem, stream>>>(P);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return launch_error(e, "kv4_attention");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
+// The fewest row tiles that registers allow, then as even as possible: each tile
+// of rows reads the cache again.
+template <typename T, int D>
+FelixCode launch_rows(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_bytes,
+                      cudaStream_t stream) {
+  const uint32_t eights = (P.rows * P.group + 7) / 8;
+  const uint32_t tiles = (eights + max_nt(D) - 1) / max_nt(D);
+  switch ((eights + tiles - 1) / tiles) {
+    case 1: return launch<T, D, 1>(P, dev, workspace, ws_bytes, stream);
+    case 2: return launch<T, D, 2>(P, dev, workspace, ws_bytes, stream);
+    case 3: return launch<T, D, 3>(P, dev, workspace, ws_bytes, stream);
+    default: break;
+  }
+  if constexpr (D == 64) {
+    if ((eights + tiles - 1) / tiles == 4) return launch<T, D, 4>(P, dev, workspace, ws_bytes, stream);
+    return launch<T, D, 5>(P, dev, workspace, ws_bytes, stream);
+  }
+  return api_error("kv4_attention: rows");
+}
+
 }  // namespace kv4
 
-// At most 8 CTAs per SM: what a caller's workspace must hold on any device.
 size_t kv4_attention_workspace_bytes(uint32_t head_dim, int num_sms) {
-  return kWsCounterBytes + size_t(num_sms) * 8 * 2 * 8 * 2 * (head_dim + 2) * sizeof(float);
+  return kv4::ws_bytes_for(uint32_t(num_sms) * kv4::kMaxPerSm, 8 * kv4::max_nt(int(head_dim)),
+                           int(head_dim));
 }
 
 FelixCode kv4_attention_launch(const felix_kv4::CacheView& c, uint32_t head_dim, const void* q,
@@ -559,17 +806,16 @@ FelixCode kv4_attention_launch(const felix_kv4::CacheView& c, uint32_t head_dim,
   P.rows = rows;
   P.group = heads / c.kv_heads;
   P.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(float(head_dim))) * 1.4426950408889634f;
-  const bool two = rows * P.group > 8;
-#define KV4_GO(T, D)                                                              \
-  return two ? kv4::launch<T, D, 2>(P, dev, workspace, ws_bytes, stream)          \
-             : kv4::launch<T, D, 1>(P, dev, workspace, ws_bytes, stream)
+  P.status = dev->status_word;
+  P.q_vec = ((reinterpret_cast<uintptr_t>(q) | uintptr_t(strides[0] * 2) |
+              uintptr_t(strides[1] * 2) | uintptr_t(strides[2] * 2)) & 15) == 0;
   if (bf16) {
-    if (head_dim == 128) KV4_GO(__nv_bfloat16, 128);
-    KV4_GO(__nv_bfloat16, 64);
+    if (head_dim == 128)
+      return kv4::launch_rows<__nv_bfloat16, 128>(P, dev, workspace, ws_bytes, stream);
+    return kv4::launch_rows<__nv_bfloat16, 64>(P, dev, workspace, ws_bytes, stream);
   }
-  if (head_dim == 128) KV4_GO(__half, 128);
-  KV4_GO(__half, 64);
-#undef KV4_GO
+  if (head_dim == 128) return kv4::launch_rows<__half, 128>(P, dev, workspace, ws_bytes, stream);
+  return kv4::launch_rows<__half, 64>(P, dev, workspace, ws_bytes, stream);
 }
 
 }  // namespace felix_impl

@@ -33,6 +33,7 @@ enum WatchdogSite : unsigned {
   kWdAttnCorrection = 10,
   kWdSmemAlign = 11,
   kWdTileQueue = 12,  // HGEMM dynamic tile queue (producer push or consumer pop)
+  kWdKv4Load = 14,    // 4-bit cache attention: bulk copy of a step's blocks
   kWdTopkLoad = 13,   // top-k: bulk copy of a staged slice  // dynamic shared memory not 1024-byte aligned: kernel did nothing
 };
 
