@@ -84,6 +84,37 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 numbers in a register pair, one instruction for both: here always the
+// two query rows 2t, 2t + 1 that a thread holds of a matrix instruction's result.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 un(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 template <int W>
 struct Words;  // W 32-bit words loaded as one vector from shared memory
 template <>
@@ -104,9 +135,14 @@ struct Words<2> {
 };
 
 // What a step's tokens bring to scores and sums, decoded once by one lane each.
+// Each number stands twice, as the pair that F2 operations take.
+struct alignas(16) Pair2 {
+  F2 a, b;
+};
 struct alignas(16) TokenParams {
-  float4 v[kStepTokens];  // exponent E of scale_v, 2^-E, scale_v 2^-E, base_v 2^-E
-  float2 k[kStepTokens];  // scale_k, base_k - 8 scale_k
+  Pair2 k[kStepTokens];  // scale_k; base_k - 8 scale_k
+  Pair2 e[kStepTokens];  // exponent E of scale_v; 2^-E
+  Pair2 v[kStepTokens];  // scale_v 2^-E; base_v 2^-E
 };
 __device__ __forceinline__ float2 k_params(uint32_t p) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
@@ -143,10 +179,11 @@ struct Attn {
   // score = (raw * scale_k + qs * (base_k - 8 scale_k)) * f: raw sums are in units
   // of 2^-24 and of the row's power of two, and so is qs = sum(q), so that the
   // terms cancel before anything is rounded to a scale
-  float f[NT][2], qs[NT][2];
+  F2 f[NT], qs[NT];
   int lim[NT][2];                         // tokens that this thread's two rows see
-  float o[NT][D / 16][4];                 // sums of p scale_v (c - 8); odd rows 16 times that
-  float m[NT][2], l[NT][2], b_[NT][2];     // running maximum, sum of p, sum of p base_v
+  F2 o[NT][D / 16][2];                    // sums of p scale_v (c - 8); odd rows 16 times that
+  float m[NT][2];                         // running maximum
+  F2 l[NT], b_[NT];                       // sum of p, sum of p base_v
   int low;                                // the smallest of lim
 
   __device__ __forceinline__ void load_q(const AttnParams& P, uint32_t slot, uint32_t kvh,
@@ -201,18 +238,21 @@ struct Attn {
       }
       // statistics of rows 2t and 2t + 1, which lanes 4 * (2t) and 4 * (2t + 1) hold
       const float down = __int_as_float((127 - up) << 23);
+      float fc[2], qc[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = 4 * (2 * t + c);
         const float dn = __shfl_sync(~0u, down, from), sm = __shfl_sync(~0u, sum, from);
-        f[n][c] = P.scale_log2 * dn * 16777216.f;  // raw sums are of code * 2^-24
-        qs[n][c] = sm * (1.f / 16777216.f);
+        fc[c] = P.scale_log2 * dn * 16777216.f;  // raw sums are of code * 2^-24
+        qc[c] = sm * (1.f / 16777216.f);
         const uint32_t rr = rt * kRows + 8 * n + 2 * t + c;
         const int rw = int(rr / P.group);
         lim[n][c] = (rw < int(P.rows) && rw < count) ? max(len - count + rw + 1, 0) : 0;
         m[n][c] = -INFINITY;
-        l[n][c] = b_[n][c] = 0.f;
       }
+      f[n] = f2(fc[0], fc[1]);
+      qs[n] = f2(qc[0], qc[1]);
+      l[n] = b_[n] = f2(0.f, 0.f);
       // rows past the last do not narrow the unmasked range
       const bool past = rt * kRows + 8 * n + 2 * t >= P.rows * P.group;
       if (!past) low = min(low, min(lim[n][0], rt * kRows + 8 * n + 2 * t + 1 < P.rows * P.group
@@ -220,10 +260,88 @@ struct Attn {
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[n][j][c] = 0.f;
+        for (int h = 0; h < 2; ++h) o[n][j][h] = f2(0.f, 0.f);
     }
     low = min(low, __shfl_xor_sync(~0u, low, 1));
     low = min(low, __shfl_xor_sync(~0u, low, 2));
+  }
+
+  // Scores of a step -> probabilities as operand registers `pt`, and the sums.
+  // s[n][b][h]: token 8h + g of block b, rows 2t and 2t + 1. kMask: some of the
+  // tokens are not there or not seen by every row.
+  template <bool kMask>
+  __device__ __forceinline__ void softmax(float (&s)[NT][kStep][4], const TokenParams& tp,
+                                          uint32_t there, int token0, int g,
+                                          uint32_t (&pt)[NT][kStep][2]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float2 x[kStep][2];
+      bool on[kStep][2][2];
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < kStep; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = b * 16 + h * 8 + g;
+          const Pair2 k = tp.k[i];
+          const F2 raw = f2(s[n][b][2 * h], s[n][b][2 * h + 1]);
+          x[b][h] = un(fma(fma(raw, k.a, mul(qs[n], k.b)), f[n], tp.e[i].a));
+          if (kMask) {
+            const bool in = there >> b & 1;
+            on[b][h][0] = in && token0 + i < lim[n][0];
+            on[b][h][1] = in && token0 + i < lim[n][1];
+            if (!on[b][h][0]) x[b][h].x = -INFINITY;
+            if (!on[b][h][1]) x[b][h].y = -INFINITY;
+          }
+          t0 = fmaxf(t0, x[b][h].x);
+          t1 = fmaxf(t1, x[b][h].y);
+        }
+      // The sums are kept relative to a maximum that is only moved when a score
+      // passes it by 2^8: probabilities stay below 2^9 and fp16 holds them.
+      if (__any_sync(~0u, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
+        float keep[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = fmaxf(m[n][c], c ? t1 : t0);
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          keep[c] = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
+          m[n][c] = top;
+        }
+        const F2 kk = f2(keep[0], keep[1]);
+        l[n] = mul(l[n], kk);
+        b_[n] = mul(b_[n], kk);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) o[n][j][h] = mul(o[n][j][h], kk);
+      }
+      const F2 minus = f2(-m[n][0], -m[n][1]);
+#pragma unroll
+      for (int b = 0; b < kStep; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int i = b * 16 + h * 8 + g;
+          const float2 d = un(add(f2(x[b][h].x, x[b][h].y), minus));
+          float2 e = make_float2(ex2(d.x), ex2(d.y));
+          Pair2 v = tp.v[i];
+          F2 inv = tp.e[i].b;
+          if (kMask) {  // a masked token's parameters may be anything
+            if (!on[b][h][0]) e.x = 0.f;
+            if (!on[b][h][1]) e.y = 0.f;
+            const float2 a = un(v.a), w = un(v.b), u = un(inv);
+            v.a = f2(on[b][h][0] ? a.x : 0.f, on[b][h][1] ? a.y : 0.f);
+            v.b = f2(on[b][h][0] ? w.x : 0.f, on[b][h][1] ? w.y : 0.f);
+            inv = f2(on[b][h][0] ? u.x : 0.f, on[b][h][1] ? u.y : 0.f);
+          }
+          const F2 ee = f2(e.x, e.y);
+          l[n] = fma(ee, inv, l[n]);
+          b_[n] = fma(ee, v.b, b_[n]);
+          const float2 p = un(mul(ee, v.a));
+          pt[n][b][h] = transpose8x8(felix_sm100::pack_half2(p.x, p.y));
+        }
+    }
   }
 
   // One step: kStep blocks at `x`, of which those in `there` exist.
@@ -234,122 +352,58 @@ struct Attn {
     const int g = lane >> 2;
     {
       const unsigned char* p = x + (lane / 16) * kB;
-      tp.k[lane] = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[lane & 15]);
-      tp.v[lane] = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
+      const float2 k = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[lane & 15]);
+      const float4 v = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
+      tp.k[lane] = {f2(k.x, k.x), f2(k.y, k.y)};
+      tp.e[lane] = {f2(v.x, v.x), f2(v.y, v.y)};
+      tp.v[lane] = {f2(v.z, v.z), f2(v.w, v.w)};
     }
     __syncwarp();
     float s[NT][kStep][4];
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < kStep; ++b) {
       Words<kW> k0, k1;
       k0.load(x + b * kB + lane * kLane);
       k1.load(x + b * kB + 4 * D + lane * kLane);
-      float s2[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[n][b][c] = s2[n][c] = 0.f;
+      float s2[4];  // two chains where few others run beside them
 #pragma unroll
       for (int w = 0; w < kW; ++w) {
         const uint32_t a = k0.w[w], c = k1.w[w], a8 = a >> 8, c8 = c >> 8;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma16816(s[n][b], a & lo, c & lo, a & hi, c & hi, q[n][2 * w][0], q[n][2 * w][1]);
-          // two chains where few others run beside them
-          mma16816(NT == 1 ? s2[n] : s[n][b], a8 & lo, c8 & lo, a8 & hi, c8 & hi,
-                   q[n][2 * w + 1][0], q[n][2 * w + 1][1]);
+          if (w == 0)
+            mma16816(s[n][b], a & lo, c & lo, a & hi, c & hi, q[n][0][0], q[n][0][1], zero);
+          else
+            mma16816(s[n][b], a & lo, c & lo, a & hi, c & hi, q[n][2 * w][0], q[n][2 * w][1]);
+          if (NT > 1)
+            mma16816(s[n][b], a8 & lo, c8 & lo, a8 & hi, c8 & hi, q[n][2 * w + 1][0],
+                     q[n][2 * w + 1][1]);
+          else if (w == 0)
+            mma16816(s2, a8 & lo, c8 & lo, a8 & hi, c8 & hi, q[n][1][0], q[n][1][1], zero);
+          else
+            mma16816(s2, a8 & lo, c8 & lo, a8 & hi, c8 & hi, q[n][2 * w + 1][0],
+                     q[n][2 * w + 1][1]);
         }
       }
       if (NT == 1)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[0][b][c] += s2[0][c];
+        for (int c = 0; c < 4; ++c) s[0][b][c] += s2[c];
     }
-    const bool all = there == (1u << kStep) - 1 && token0 + kStepTokens <= low;
     uint32_t pt[NT][kStep][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      // s[b][0], s[b][1]: token g of block b, rows 2t, 2t + 1; s[b][2], s[b][3]: token g + 8
-      float ex[kStep][2];
-#pragma unroll
-      for (int b = 0; b < kStep; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 k = tp.k[b * 16 + h * 8 + g];
-          ex[b][h] = tp.v[b * 16 + h * 8 + g].x;
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            s[n][b][2 * h + c] =
-                fmaf(fmaf(s[n][b][2 * h + c], k.x, qs[n][c] * k.y), f[n][c], ex[b][h]);
-        }
-      uint32_t off = 0;  // a bit for each masked score
-      if (!all) {
-#pragma unroll
-        for (int b = 0; b < kStep; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool on = (there >> b & 1) && token0 + b * 16 + (i / 2) * 8 + g < lim[n][i & 1];
-            if (!on) s[n][b][i] = -INFINITY, off |= 1u << (4 * b + i);
-          }
-      }
-      // The sums are kept relative to a maximum that is only moved when a score
-      // passes it by 2^8: probabilities stay below 2^9 and fp16 holds them.
-      float t0 = s[n][0][0], t1 = s[n][0][1];
-      t0 = fmaxf(t0, s[n][0][2]), t1 = fmaxf(t1, s[n][0][3]);
-#pragma unroll
-      for (int b = 1; b < kStep; ++b) {
-        t0 = fmaxf(t0, fmaxf(s[n][b][0], s[n][b][2]));
-        t1 = fmaxf(t1, fmaxf(s[n][b][1], s[n][b][3]));
-      }
-      if (__any_sync(~0u, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float top = fmaxf(m[n][c], c ? t1 : t0);
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-          const float keep = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
-          m[n][c] = top;
-          l[n][c] *= keep;
-          b_[n][c] *= keep;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            o[n][j][c] *= keep;
-            o[n][j][2 + c] *= keep;
-          }
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < kStep; ++b) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 v = tp.v[b * 16 + h * 8 + g];
-          float p[2];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int i = 2 * h + c;
-            const float e = ex2(s[n][b][i] - m[n][c]);
-            if (off >> (4 * b + i) & 1) {  // a masked token's parameters may be anything
-              p[c] = 0.f;
-            } else {
-              p[c] = e * v.z;
-              l[n][c] = fmaf(e, v.y, l[n][c]);
-              b_[n][c] = fmaf(e, v.w, b_[n][c]);
-            }
-          }
-          pt[n][b][h] = transpose8x8(felix_sm100::pack_half2(p[0], p[1]));
-        }
-      }
-    }
+    if (there == (1u << kStep) - 1 && token0 + kStepTokens <= low)
+      softmax<false>(s, tp, there, token0, g, pt);
+    else
+      softmax<true>(s, tp, there, token0, g, pt);
     // -8 sum(p scale_v) of the step in the codes' unit, 16 times that for the odd
     // rows: where the second product starts, so that it sums to what is small.
     float start[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       constexpr uint32_t m8 = 0x80088008u, m128 = 0x80808080u;
+      mma16816(start[n], m8, m128, m8, m128, pt[n][0][0], pt[n][0][1], zero);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) start[n][c] = 0.f;
-#pragma unroll
-      for (int b = 0; b < kStep; ++b)
+      for (int b = 1; b < kStep; ++b)
         mma16816(start[n], m8, m128, m8, m128, pt[n][b][0], pt[n][b][1]);
     }
     Words<kW> v0[kStep], v1[kStep];
@@ -379,10 +433,10 @@ struct Attn {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          o[n][2 * w][c] += r[n][0][c];
-          o[n][2 * w + 1][c] += r[n][1][c];
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            o[n][2 * w + i][h] = add(o[n][2 * w + i][h], f2(r[n][i][2 * h], r[n][i][2 * h + 1]));
     }
     __syncwarp();  // the stage and tp are free
   }
@@ -393,23 +447,27 @@ struct Attn {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      const float2 ls = un(l[n]), bs = un(b_[n]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        float lc = c ? ls.y : ls.x, off = c ? bs.y : bs.x;
 #pragma unroll
         for (int x = 4; x < 32; x *= 2) {
-          l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
-          b_[n][c] += __shfl_xor_sync(~0u, b_[n][c], x);
+          lc += __shfl_xor_sync(~0u, lc, x);
+          off += __shfl_xor_sync(~0u, off, x);
         }
         const int r = 8 * n + 2 * t + c;
-        if (g == 0) sml[2 * r] = m[n][c], sml[2 * r + 1] = l[n][c];
+        if (g == 0) sml[2 * r] = m[n][c], sml[2 * r + 1] = lc;
         constexpr float u = 16777216.f;
-        const float off = b_[n][c];
         float4* dst = reinterpret_cast<float4*>(so + r * D + g * (D / 8));
+        auto at = [&](int j, int h) {
+          const float2 v = un(o[n][j][h]);
+          return c ? v.y : v.x;
+        };
 #pragma unroll
         for (int w = 0; w < kW; ++w)
-          dst[w] = make_float4(fmaf(o[n][2 * w][c], u, off), fmaf(o[n][2 * w][2 + c], u / 16, off),
-                               fmaf(o[n][2 * w + 1][c], u, off),
-                               fmaf(o[n][2 * w + 1][2 + c], u / 16, off));
+          dst[w] = make_float4(fmaf(at(2 * w, 0), u, off), fmaf(at(2 * w, 1), u / 16, off),
+                               fmaf(at(2 * w + 1, 0), u, off), fmaf(at(2 * w + 1, 1), u / 16, off));
       }
     }
   }
@@ -431,34 +489,44 @@ struct Smem {
   int abort;
 };
 
-// A place in a CTA's share of the work: the part [lo, hi) of a segment's steps.
+// Units of a segment beyond its steps: what opening and closing it costs (q, the
+// join of the warps). Without them a share of many short segments takes longest.
+constexpr uint32_t kOpen = 12;
+
+// A place in a CTA's share of the work: the part [lo, hi) of a segment's units,
+// whose first kOpen units hold no steps.
 struct Place {
   uint32_t slot, slot_at;  // slot, and the units before it
-  uint32_t tiles;          // steps of each of the slot's segments (an empty slot: one)
+  uint32_t size;           // units of each of the slot's segments
   int len, reach;
-  uint32_t seg, lo, hi;
+  uint32_t kvh, rt, seg_at, lo, hi;
   __device__ __forceinline__ void read(const AttnParams& P) {
     len = slot_length(P.c, slot);
     reach = slot_reach(P.c, slot);
-    tiles = max((reach + kStepTokens - 1) / kStepTokens, 1);
+    size = kOpen + (reach + kStepTokens - 1) / kStepTokens;
   }
   // unit u, at or after the current slot's first
   __device__ __forceinline__ void open(const AttnParams& P, uint32_t u, uint32_t last) {
-    const uint32_t per_tile = P.c.kv_heads * P.row_tiles;
-    while (u >= slot_at + tiles * per_tile) {
-      slot_at += tiles * per_tile;
+    const uint32_t per = P.c.kv_heads * P.row_tiles;
+    while (u >= slot_at + size * per) {
+      slot_at += size * per;
       ++slot;
       read(P);
     }
-    seg = (u - slot_at) / tiles;
-    lo = (u - slot_at) % tiles;
-    hi = min(tiles, lo + (last - u));
+    const uint32_t seg = (u - slot_at) / size;
+    kvh = seg / P.row_tiles;
+    rt = seg - kvh * P.row_tiles;
+    seg_at = slot_at + seg * size;
+    lo = u - seg_at;
+    hi = min(size, lo + (last - u));
   }
-  __device__ __forceinline__ uint32_t end() const { return slot_at + seg * tiles + hi; }
+  __device__ __forceinline__ uint32_t end() const { return seg_at + hi; }
+  __device__ __forceinline__ uint32_t first_step() const { return lo > kOpen ? lo - kOpen : 0; }
+  __device__ __forceinline__ uint32_t end_step() const { return hi > kOpen ? hi - kOpen : 0; }
 };
 
-// Persistent grid. The work is a line of units (a segment's steps of 32 tokens,
-// segment after segment; an empty slot counts as one), cut into equal shares, one
+// Persistent grid. The work is a line of units (a segment's steps of 32 tokens and
+// kOpen for the segment itself, one after another), cut into equal shares, one
 // per CTA, whatever the slots' lengths; the warps of a CTA take its steps in turn.
 // Each warp has a ring of stages of its own in shared memory, filled by bulk
 // copies that it issues itself a few steps ahead, across segments: no barrier in
@@ -473,13 +541,13 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const CacheView& c = P.c;
-  const uint32_t per_tile = c.kv_heads * P.row_tiles;
+  const uint32_t per_seg = c.kv_heads * P.row_tiles;
 
   // ---- this CTA's share: units before each thread's run of slots, then the slot
   const uint32_t run = (c.slots + kThreads - 1) / kThreads;
   const uint32_t s0 = min(tid * run, c.slots), s1 = min(s0 + run, c.slots);
   auto units = [&](uint32_t s) {
-    return uint32_t(max((slot_reach(c, s) + kStepTokens - 1) / kStepTokens, 1)) * per_tile;
+    return (kOpen + uint32_t(slot_reach(c, s) + kStepTokens - 1) / kStepTokens) * per_seg;
   };
   uint32_t mine = 0;
   for (uint32_t s = s0; s < s1; ++s) mine += units(s);
@@ -501,8 +569,9 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
     if (w < warp) upto += sm.scan[w];
     total += sm.scan[w];
   }
-  // at least one step for each warp: smaller parts cost more to join than they save
-  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, uint32_t(kWarps));
+  // at least a segment's opening and one step for each warp: smaller parts cost
+  // more to join than they save
+  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, kOpen + kWarps);
   const uint32_t first = min(blockIdx.x * quota, total), last = min(first + quota, total);
   if (first >= last) return;
   if (first >= upto - mine && first < upto) {
@@ -523,18 +592,20 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
   use.read(P);
   use.open(P, first, last);
   get = use;
-  uint32_t get_t = get.lo + warp;
+  uint32_t get_t = get.first_step() + warp, get_end = get.end_step();
   bool more = true;
+  const uint32_t blocks = 1u << (c.page_shift - 4);  // of a page and head
   // the next step to fetch: lane b looks up the page of its block b
   int page = -1;
   uint32_t in_page = 0;
   auto look = [&]() {
-    while (more && get_t >= get.hi) {
+    while (more && get_t >= get_end) {
       const uint32_t u = get.end();
       more = u < last;
       if (more) {
         get.open(P, u, last);
-        get_t = get.lo + warp;
+        get_t = get.first_step() + warp;
+        get_end = get.end_step();
       }
     }
     if (!more) return;
@@ -542,8 +613,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
     page = -1;
     if (lane < kStep && int(token) < get.reach) {
       page = c.table[size_t(get.slot) * c.width + (token >> c.page_shift)];
-      const uint32_t blocks = 1u << (c.page_shift - 4);
-      in_page = (get.seg / P.row_tiles) * blocks + ((token >> 4) & (blocks - 1));
+      in_page = get.kvh * blocks + ((token >> 4) & (blocks - 1));
     }
     get_t += kWarps;
   };
@@ -570,12 +640,12 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
   int stage = 0;
   uint32_t parity = 0;
   for (;;) {
-    const uint32_t kvh = use.seg / P.row_tiles, rt = use.seg % P.row_tiles;
+    const uint32_t kvh = use.kvh, rt = use.rt;
     const int count =
         P.counts ? min(max(P.counts[use.slot], 0), int(P.rows)) : int(P.rows);
     Attn<T, D, NT> A;
     A.load_q(P, use.slot, kvh, rt, use.len, count, lane);
-    for (uint32_t t = use.lo + warp; t < use.hi; t += kWarps) {
+    for (uint32_t t = use.first_step() + warp; t < use.end_step(); t += kWarps) {
       if (felix_sm100::mbar_wait(&sm.full[warp][stage], parity, &sm.abort, P.status,
                                  felix_sm100::kWdKv4Load)) {
         const uint32_t there = sm.there[warp][stage];
@@ -590,9 +660,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
     __syncthreads();
 
     // ---- join the warps; write the result, or this share's part of it
-    const bool whole = use.lo == 0 && use.hi == use.tiles;
-    const uint32_t seg_lo = use.slot_at + use.seg * use.tiles, seg_hi = seg_lo + use.tiles;
-    const uint32_t c0 = seg_lo / quota, c1 = (seg_hi - 1) / quota;
+    const bool whole = use.lo == 0 && use.hi == use.size;
+    const uint32_t c0 = use.seg_at / quota, c1 = (use.seg_at + use.size - 1) / quota;
     constexpr size_t kPart = size_t(kRows) * (D + 2);
     float* mypart = P.partials + (size_t(blockIdx.x) * 2 + (use.lo == 0 ? 1 : 0)) * kPart;
     auto put = [&](int r, int d, float4 v, float top, float sum) {
