@@ -13,17 +13,24 @@
 // probabilities. Both products run transposed (codes are the 16-row operand,
 // 8 query rows the n side): a group of query heads of one key/value head fills
 // the instruction, and the scores' registers become the other operand of the
-// second product by an 8 x 8 transpose in the warp. p_t scale_v is rounded to
-// fp16 for that product; its exponent is taken out first (the running maximum is
-// that of score + exponent of scale_v), so that neither tiny nor huge values
-// lose bits, and the -8 is applied to the sum of the same rounded numbers, so
-// that the offset cancels exactly. Sums and statistics are fp32.
+// second product by an 8 x 8 transpose in the warp.
+//
+// Rounding. p_t scale_v is rounded to fp16, P_t, for the second product. Its
+// exponent is taken out first (the running maximum is that of score + exponent of
+// scale_v), so that neither tiny nor huge values lose bits. The result is
+//   (sum P (c - 8) + sum P base_v / scale_v) / sum P / scale_v,
+// the mean of the held values under the weights P / scale_v: rounded weights in
+// the numerator and the denominator, so that a row that one token rules has no
+// error from them. The log-sum-exp has its own sum of unrounded p. Sums and
+// statistics are fp32.
 //
 // The mma.sync form is used, not tcgen05: the product has 8 useful columns (one
 // group of heads), the codes reach the instruction from registers after one
 // logic operation per pair, and the kernel is bound by reading the cache and by
 // those logic operations, not by the matrix unit; tcgen05 would need the codes
 // expanded to fp16 in shared or tensor memory, four times the bytes of the cache.
+#include <algorithm>
+
 #include "felix_internal.h"
 #include "kv4_layout.cuh"
 #include "sm100_ptx.cuh"
@@ -33,8 +40,6 @@ namespace kv4 {
 
 using namespace felix_kv4;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 2;                     // blocks that a warp takes at once
 constexpr int kStepTokens = kStep * kBlock;  // 32: one per lane
 
@@ -49,7 +54,7 @@ struct AttnParams {
   uint32_t row_tiles;                // tiles of 8 * NT (row, head) pairs
   float scale_log2;                  // softmax scale * log2(e)
   uint32_t* counters;                // one per CTA, zero between launches
-  float* partials;                   // [CTA][2][8 NT][D + 2]
+  float* partials;                   // [CTA][2][8 NT][D + 3]
   unsigned* status;                  // watchdog word
   bool q_vec;                        // rows of q are 16-byte aligned
 };
@@ -142,18 +147,30 @@ struct alignas(16) Pair2 {
 struct alignas(16) TokenParams {
   Pair2 k[kStepTokens];  // scale_k; base_k - 8 scale_k
   Pair2 e[kStepTokens];  // exponent E of scale_v; 2^-E
-  Pair2 v[kStepTokens];  // scale_v 2^-E; base_v 2^-E
+  Pair2 v[kStepTokens];  // scale_v 2^-E; 1 / scale_v
+  F2 b[kStepTokens];     // base_v / scale_v
 };
 __device__ __forceinline__ float2 k_params(uint32_t p) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
   return make_float2(f.x, fmaf(-8.f, f.x, f.y));
 }
-// E is the exponent of the smallest normal where scale_v is subnormal or zero.
-__device__ __forceinline__ float4 v_params(uint32_t p) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-  const int e = max(int((p >> 10) & 31u), 1) - 15;
-  const float inv = __int_as_float((127 - e) << 23);
-  return make_float4(float(e), inv, f.x * inv, f.y * inv);
+struct VParams {
+  float e, inv, mant, rcp, base;
+};
+// A vector of equal values (scale 0) has all codes 8 and adds nothing beside its
+// base: any scale does, 1 is taken.
+__device__ __forceinline__ VParams v_params(uint32_t p) {
+  float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+  if (f.x == 0.f) f.x = 1.f;
+  // scales are not negative; a NaN counts as fp16's largest exponent
+  const int e = min(int(__float_as_uint(f.x) >> 23) - 127, 16);
+  VParams r;
+  r.e = float(e);
+  r.inv = __int_as_float((127 - e) << 23);
+  r.mant = f.x * r.inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.rcp) : "f"(f.x));
+  r.base = f.y * r.rcp;
+  return r;
 }
 
 template <typename T>
@@ -182,17 +199,19 @@ struct Attn {
   F2 f[NT], qs[NT];
   int lim[NT][2];                         // tokens that this thread's two rows see
   F2 o[NT][D / 16][2];                    // sums of p scale_v (c - 8); odd rows 16 times that
-  float m[NT][2];                         // running maximum
-  F2 l[NT], b_[NT];                       // sum of p, sum of p base_v
+  float m[NT][2];                         // what exponents are relative to
+  // sums of p, of P / scale_v and of P base_v / scale_v
+  F2 l[NT], w[NT], b[NT];
   int low;                                // the smallest of lim
 
+  // r0: the warp's first (row, head) pair of the segment's P.rows * P.group
   __device__ __forceinline__ void load_q(const AttnParams& P, uint32_t slot, uint32_t kvh,
-                                         uint32_t rt, int len, int count, int lane) {
+                                         uint32_t r0, int len, int count, int lane) {
     const int g = lane >> 2, t = lane & 3;
     low = len;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const uint32_t r = rt * kRows + 8 * n + g;
+      const uint32_t r = r0 + 8 * n + g;
       const uint32_t row = r / P.group, head = kvh * P.group + r % P.group;
       const bool live = row < P.rows && int(row) < count;
       float v[D / 4];
@@ -245,17 +264,17 @@ struct Attn {
         const float dn = __shfl_sync(~0u, down, from), sm = __shfl_sync(~0u, sum, from);
         fc[c] = P.scale_log2 * dn * 16777216.f;  // raw sums are of code * 2^-24
         qc[c] = sm * (1.f / 16777216.f);
-        const uint32_t rr = rt * kRows + 8 * n + 2 * t + c;
+        const uint32_t rr = r0 + 8 * n + 2 * t + c;
         const int rw = int(rr / P.group);
         lim[n][c] = (rw < int(P.rows) && rw < count) ? max(len - count + rw + 1, 0) : 0;
         m[n][c] = -INFINITY;
       }
       f[n] = f2(fc[0], fc[1]);
       qs[n] = f2(qc[0], qc[1]);
-      l[n] = b_[n] = f2(0.f, 0.f);
+      l[n] = w[n] = b[n] = f2(0.f, 0.f);
       // rows past the last do not narrow the unmasked range
-      const bool past = rt * kRows + 8 * n + 2 * t >= P.rows * P.group;
-      if (!past) low = min(low, min(lim[n][0], rt * kRows + 8 * n + 2 * t + 1 < P.rows * P.group
+      const bool past = r0 + 8 * n + 2 * t >= P.rows * P.group;
+      if (!past) low = min(low, min(lim[n][0], r0 + 8 * n + 2 * t + 1 < P.rows * P.group
                                                    ? lim[n][1] : lim[n][0]));
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
@@ -279,39 +298,42 @@ struct Attn {
       bool on[kStep][2][2];
       float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-      for (int b = 0; b < kStep; ++b)
+      for (int k = 0; k < kStep; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int i = b * 16 + h * 8 + g;
-          const Pair2 k = tp.k[i];
-          const F2 raw = f2(s[n][b][2 * h], s[n][b][2 * h + 1]);
-          x[b][h] = un(fma(fma(raw, k.a, mul(qs[n], k.b)), f[n], tp.e[i].a));
+          const int i = k * 16 + h * 8 + g;
+          const Pair2 kp = tp.k[i];
+          const F2 raw = f2(s[n][k][2 * h], s[n][k][2 * h + 1]);
+          x[k][h] = un(fma(fma(raw, kp.a, mul(qs[n], kp.b)), f[n], tp.e[i].a));
           if (kMask) {
-            const bool in = there >> b & 1;
-            on[b][h][0] = in && token0 + i < lim[n][0];
-            on[b][h][1] = in && token0 + i < lim[n][1];
-            if (!on[b][h][0]) x[b][h].x = -INFINITY;
-            if (!on[b][h][1]) x[b][h].y = -INFINITY;
+            const bool in = there >> k & 1;
+            on[k][h][0] = in && token0 + i < lim[n][0];
+            on[k][h][1] = in && token0 + i < lim[n][1];
+            if (!on[k][h][0]) x[k][h].x = -INFINITY;
+            if (!on[k][h][1]) x[k][h].y = -INFINITY;
           }
-          t0 = fmaxf(t0, x[b][h].x);
-          t1 = fmaxf(t1, x[b][h].y);
+          t0 = fmaxf(t0, x[k][h].x);
+          t1 = fmaxf(t1, x[k][h].y);
         }
-      // The sums are kept relative to a maximum that is only moved when a score
-      // passes it by 2^8: probabilities stay below 2^9 and fp16 holds them.
-      if (__any_sync(~0u, t0 > m[n][0] + 8.f || t1 > m[n][1] + 8.f)) {
+      // Exponents are relative to m, 2^6 below a maximum that is only moved when a
+      // score passes it by 2^8: P stays below 2^15, and fp16 holds what is 2^30
+      // smaller.
+      if (__any_sync(~0u, t0 > m[n][0] + 14.f || t1 > m[n][1] + 14.f)) {
         float keep[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float top = fmaxf(m[n][c], c ? t1 : t0);
+          float top = c ? t1 : t0;
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
           top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+          top = fmaxf(m[n][c], top - 6.f);
           keep[c] = top == -INFINITY ? 1.f : ex2(m[n][c] - top);
           m[n][c] = top;
         }
         const F2 kk = f2(keep[0], keep[1]);
         l[n] = mul(l[n], kk);
-        b_[n] = mul(b_[n], kk);
+        w[n] = mul(w[n], kk);
+        b[n] = mul(b[n], kk);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -319,27 +341,32 @@ struct Attn {
       }
       const F2 minus = f2(-m[n][0], -m[n][1]);
 #pragma unroll
-      for (int b = 0; b < kStep; ++b)
+      for (int k = 0; k < kStep; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int i = b * 16 + h * 8 + g;
-          const float2 d = un(add(f2(x[b][h].x, x[b][h].y), minus));
+          const int i = k * 16 + h * 8 + g;
+          const float2 d = un(add(f2(x[k][h].x, x[k][h].y), minus));
           float2 e = make_float2(ex2(d.x), ex2(d.y));
           Pair2 v = tp.v[i];
-          F2 inv = tp.e[i].b;
+          F2 inv = tp.e[i].b, base = tp.b[i];
           if (kMask) {  // a masked token's parameters may be anything
-            if (!on[b][h][0]) e.x = 0.f;
-            if (!on[b][h][1]) e.y = 0.f;
-            const float2 a = un(v.a), w = un(v.b), u = un(inv);
-            v.a = f2(on[b][h][0] ? a.x : 0.f, on[b][h][1] ? a.y : 0.f);
-            v.b = f2(on[b][h][0] ? w.x : 0.f, on[b][h][1] ? w.y : 0.f);
-            inv = f2(on[b][h][0] ? u.x : 0.f, on[b][h][1] ? u.y : 0.f);
+            auto seen = [&](F2 a) {
+              const float2 y = un(a);
+              return f2(on[k][h][0] ? y.x : 0.f, on[k][h][1] ? y.y : 0.f);
+            };
+            if (!on[k][h][0]) e.x = 0.f;
+            if (!on[k][h][1]) e.y = 0.f;
+            inv = seen(inv), base = seen(base), v.a = seen(v.a), v.b = seen(v.b);
           }
           const F2 ee = f2(e.x, e.y);
           l[n] = fma(ee, inv, l[n]);
-          b_[n] = fma(ee, v.b, b_[n]);
           const float2 p = un(mul(ee, v.a));
-          pt[n][b][h] = transpose8x8(felix_sm100::pack_half2(p.x, p.y));
+          const __half2 ph = __floats2half2_rn(p.x, p.y);
+          const float2 pr = __half22float2(ph);
+          const F2 P = f2(pr.x, pr.y);
+          w[n] = fma(P, v.b, w[n]);
+          b[n] = fma(P, base, b[n]);
+          pt[n][k][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ph));
         }
     }
   }
@@ -353,10 +380,11 @@ struct Attn {
     {
       const unsigned char* p = x + (lane / 16) * kB;
       const float2 k = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[lane & 15]);
-      const float4 v = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
+      const VParams v = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
       tp.k[lane] = {f2(k.x, k.x), f2(k.y, k.y)};
-      tp.e[lane] = {f2(v.x, v.x), f2(v.y, v.y)};
-      tp.v[lane] = {f2(v.z, v.z), f2(v.w, v.w)};
+      tp.e[lane] = {f2(v.e, v.e), f2(v.inv, v.inv)};
+      tp.v[lane] = {f2(v.mant, v.mant), f2(v.rcp, v.rcp)};
+      tp.b[lane] = f2(v.base, v.base);
     }
     __syncwarp();
     float s[NT][kStep][4];
@@ -442,22 +470,23 @@ struct Attn {
   }
 
   // Writes the warp's sums to shared memory: O [kRows][D] (base term included)
-  // and (m, l) of each row.
+  // and (m, l, w) of each row.
   __device__ __forceinline__ void park(float* so, float* sml, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float2 ls = un(l[n]), bs = un(b_[n]);
+      const float2 ls = un(l[n]), ws = un(w[n]), bs = un(b[n]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float lc = c ? ls.y : ls.x, off = c ? bs.y : bs.x;
+        float lc = c ? ls.y : ls.x, wc = c ? ws.y : ws.x, off = c ? bs.y : bs.x;
 #pragma unroll
         for (int x = 4; x < 32; x *= 2) {
           lc += __shfl_xor_sync(~0u, lc, x);
+          wc += __shfl_xor_sync(~0u, wc, x);
           off += __shfl_xor_sync(~0u, off, x);
         }
         const int r = 8 * n + 2 * t + c;
-        if (g == 0) sml[2 * r] = m[n][c], sml[2 * r + 1] = lc;
+        if (g == 0) sml[3 * r] = m[n][c], sml[3 * r + 1] = lc, sml[3 * r + 2] = wc;
         constexpr float u = 16777216.f;
         float4* dst = reinterpret_cast<float4*>(so + r * D + g * (D / 8));
         auto at = [&](int j, int h) {
@@ -465,27 +494,48 @@ struct Attn {
           return c ? v.y : v.x;
         };
 #pragma unroll
-        for (int w = 0; w < kW; ++w)
-          dst[w] = make_float4(fmaf(at(2 * w, 0), u, off), fmaf(at(2 * w, 1), u / 16, off),
-                               fmaf(at(2 * w + 1, 0), u, off), fmaf(at(2 * w + 1, 1), u / 16, off));
+        for (int j = 0; j < kW; ++j)
+          dst[j] = make_float4(fmaf(at(2 * j, 0), u, off), fmaf(at(2 * j, 1), u / 16, off),
+                               fmaf(at(2 * j + 1, 0), u, off), fmaf(at(2 * j + 1, 1), u / 16, off));
       }
     }
   }
 };
 
-template <int D, int NT>
+// A CTA: kCW consumer warps and one that fetches. The consumers are kRW groups
+// of rows times kTW = kCW / kRW that share a group's tokens; a stage of the ring
+// holds a step of each of the kTW.
+template <int D, int NT, int kRW, int kCW>
+struct Shape {
+  static constexpr int kTW = kCW / kRW;
+  static constexpr int kJoin = 32 * kCW;  // threads of the consumers
+  // Eight consumers are two warpgroups, the warp that fetches is in a third, which
+  // gives most of its registers to them.
+  static constexpr int kThreads = kCW == 8 ? 384 : 160;
+  static constexpr int kRows = 8 * NT;        // rows of a warp
+  static constexpr int kTileRows = kRW * kRows;
+  static constexpr int kBlocks = kTW * kStep;  // of a stage
+  static constexpr int kStageBytes = kBlocks * int(block_bytes(D));
+  // 50 KB of stages for a CTA of 4 consumers (three to an SM), 100 KB for one of 8
+  // (one to an SM)
+  static constexpr int kStages = (kCW == 4 ? 53000 : 100000) / kStageBytes;
+};
+// Registers of a CTA of 8 consumers: launched with 168 a thread (65536 / 384),
+// then 40 for the fetching warpgroup and 232 for the others: 40 * 128 + 232 * 256 =
+// 168 * 384. The host checks the launch count before the first launch.
+constexpr int kRegsLaunch = 168, kRegsFetch = 40, kRegsSums = 232;
+static_assert(kRegsFetch * 128 + kRegsSums * 256 <= kRegsLaunch * 384);
+
+template <int D, int NT, int kRW, int kCW>
 struct Smem {
-  // stages of kStep blocks per warp: 37 to 52 KB of cache are under way per CTA, about
-  // 150 KB per SM
-  static constexpr int kStages = D == 128 ? 3 : 4;
-  static constexpr int kRows = 8 * NT;
-  alignas(128) unsigned char ring[kWarps][kStages][kStep * block_bytes(D)];
-  alignas(16) float o[kWarps][kRows * D];
-  TokenParams tp[kWarps];
-  uint64_t full[kWarps][kStages];
-  uint32_t there[kWarps][kStages];
-  float ml[kWarps][2 * kRows];
-  uint32_t scan[kWarps], at[2], ticket;
+  using H = Shape<D, NT, kRW, kCW>;
+  alignas(128) unsigned char ring[H::kStages][H::kStageBytes];
+  alignas(16) float o[kCW][H::kRows * D];
+  TokenParams tp[kCW];
+  uint64_t full[H::kStages], empty[H::kStages];
+  uint32_t there[H::kStages];
+  float ml[kCW][3 * H::kRows];  // (m, l, w) of each row
+  uint32_t scan[H::kThreads / 32], at[2], ticket;
   int abort;
 };
 
@@ -527,16 +577,19 @@ struct Place {
 
 // Persistent grid. The work is a line of units (a segment's steps of 32 tokens and
 // kOpen for the segment itself, one after another), cut into equal shares, one
-// per CTA, whatever the slots' lengths; the warps of a CTA take its steps in turn.
-// Each warp has a ring of stages of its own in shared memory, filled by bulk
-// copies that it issues itself a few steps ahead, across segments: no barrier in
-// the loop, and the registers hold sums only. A segment that lies in several
-// shares is finished by the CTA that comes last to it, which joins the parts in a
-// fixed order: the result does not depend on who is last.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) {
-  constexpr int kRows = 8 * NT, kB = int(block_bytes(D)), kVec = kRows * D / 4;
-  using S = Smem<D, NT>;
+// per CTA, whatever the slots' lengths. The last warp looks pages up and fills the
+// ring of stages with bulk copies, across segments; the others take their steps
+// of each stage, and their registers hold sums only. A segment that lies in
+// several shares is finished by the CTA that comes last to it, which joins the
+// parts in a fixed order: the result does not depend on who is last.
+template <typename T, int D, int NT, int kRW, int kCW>
+__global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
+    kv4_attn_kernel(const AttnParams P) {
+  using H = Shape<D, NT, kRW, kCW>;
+  using S = Smem<D, NT, kRW, kCW>;
+  constexpr int kRows = H::kRows, kTW = H::kTW, kThreads = H::kThreads;
+  constexpr int kB = int(block_bytes(D));
+  constexpr int kVec = H::kTileRows * D / 4, kWarpVec = kRows * D / 4;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -558,20 +611,25 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
     if (lane >= x) upto += v;
   }
   if (lane == 31) sm.scan[warp] = upto;
-  if (tid == 0) sm.abort = 0;
-  if (lane < S::kStages) felix_sm100::mbar_init(&sm.full[warp][lane], 1);
-  felix_sm100::fence_mbar_init();
-  felix_sm100::fence_proxy_async_smem();
+  if (tid == 0) {
+    sm.abort = 0;
+    for (int s = 0; s < H::kStages; ++s) {
+      felix_sm100::mbar_init(&sm.full[s], 1);
+      felix_sm100::mbar_init(&sm.empty[s], kCW);
+    }
+    felix_sm100::fence_mbar_init();
+    felix_sm100::fence_proxy_async_smem();
+  }
   __syncthreads();
   uint32_t total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) upto += sm.scan[w];
     total += sm.scan[w];
   }
   // at least a segment's opening and one step for each warp: smaller parts cost
   // more to join than they save
-  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, kOpen + kWarps);
+  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, kOpen + kTW);
   const uint32_t first = min(blockIdx.x * quota, total), last = min(first + quota, total);
   if (first >= last) return;
   if (first >= upto - mine && first < upto) {
@@ -587,275 +645,286 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(const AttnParams P) 
   }
   __syncthreads();
 
-  Place use, get;  // the part being summed, and the one whose steps are being fetched
+  Place use;
   use.slot = sm.at[0], use.slot_at = sm.at[1];
   use.read(P);
   use.open(P, first, last);
-  get = use;
-  uint32_t get_t = get.first_step() + warp, get_end = get.end_step();
-  bool more = true;
-  const uint32_t blocks = 1u << (c.page_shift - 4);  // of a page and head
-  // the next step to fetch: lane b looks up the page of its block b
-  int page = -1;
-  uint32_t in_page = 0;
-  auto look = [&]() {
-    while (more && get_t >= get_end) {
-      const uint32_t u = get.end();
-      more = u < last;
-      if (more) {
-        get.open(P, u, last);
-        get_t = get.first_step() + warp;
-        get_end = get.end_step();
-      }
-    }
-    if (!more) return;
-    const uint32_t token = get_t * kStepTokens + lane * kBlock;
-    page = -1;
-    if (lane < kStep && int(token) < get.reach) {
-      page = c.table[size_t(get.slot) * c.width + (token >> c.page_shift)];
-      in_page = get.kvh * blocks + ((token >> 4) & (blocks - 1));
-    }
-    get_t += kWarps;
-  };
-  auto fetch = [&](int stage) {  // issues the step that look() found
-    if (!more) return;
-    const bool ok = page >= 0 && uint64_t(page) < c.num_pages;
-    const uint32_t there = __ballot_sync(~0u, ok);
-    if (lane == 0) {
-      sm.there[warp][stage] = there;
-      felix_sm100::mbar_arrive_expect_tx(&sm.full[warp][stage], __popc(there) * kB);
-    }
-    __syncwarp();
-    if (ok)
-      felix_sm100::bulk_load_1d(&sm.ring[warp][stage][lane * kB],
-                                c.pages + size_t(page) * c.page_bytes + size_t(in_page) * kB, kB,
-                                &sm.full[warp][stage]);
-  };
-  for (int s = 0; s < S::kStages; ++s) {
-    look();
-    fetch(s);
-  }
-  look();
-
   int stage = 0;
   uint32_t parity = 0;
-  for (;;) {
-    const uint32_t kvh = use.kvh, rt = use.rt;
-    const int count =
-        P.counts ? min(max(P.counts[use.slot], 0), int(P.rows)) : int(P.rows);
-    Attn<T, D, NT> A;
-    A.load_q(P, use.slot, kvh, rt, use.len, count, lane);
-    for (uint32_t t = use.first_step() + warp; t < use.end_step(); t += kWarps) {
-      if (felix_sm100::mbar_wait(&sm.full[warp][stage], parity, &sm.abort, P.status,
-                                 felix_sm100::kWdKv4Load)) {
-        const uint32_t there = sm.there[warp][stage];
-        if (there) A.step(sm.ring[warp][stage], sm.tp[warp], there, int(t) * kStepTokens, lane);
+  auto advance = [&]() {
+    if (++stage == H::kStages) stage = 0, parity ^= 1;
+  };
+
+  if (warp >= kCW) {  // ---- the warp that fetches: lane b has block b of a stage
+    if constexpr (kCW == 8) felix_sm100::setmaxnreg_dec<kRegsFetch>();
+    if (warp > kCW) return;
+    const uint32_t blocks = 1u << (c.page_shift - 4);  // of a page and head
+    uint32_t t = use.first_step(), end = use.end_step();
+    bool more = true;
+    int page = -1;
+    uint32_t in_page = 0;
+    auto look = [&]() {  // the next round's pages
+      while (more && t >= end) {
+        const uint32_t u = use.end();
+        more = u < last;
+        if (more) {
+          use.open(P, u, last);
+          t = use.first_step();
+          end = use.end_step();
+        }
+      }
+      if (!more) return;
+      const uint32_t token = t * kStepTokens + lane * kBlock;
+      page = -1;
+      if (lane < H::kBlocks && t + lane / kStep < end && int(token) < use.reach) {
+        page = c.table[size_t(use.slot) * c.width + (token >> c.page_shift)];
+        in_page = use.kvh * blocks + ((token >> 4) & (blocks - 1));
+      }
+      t += kTW;
+    };
+    look();
+    while (more) {
+      const bool ok = page >= 0 && uint64_t(page) < c.num_pages;
+      const unsigned char* src = c.pages + size_t(ok ? page : 0) * c.page_bytes + size_t(in_page) * kB;
+      const uint32_t there = __ballot_sync(~0u, ok);
+      look();  // the table is read while the stage is waited for
+      if (!felix_sm100::mbar_wait(&sm.empty[stage], parity ^ 1, &sm.abort, P.status,
+                                  felix_sm100::kWdKv4Load))
+        break;
+      if (lane == 0) {
+        sm.there[stage] = there;
+        felix_sm100::mbar_arrive_expect_tx(&sm.full[stage], __popc(there) * kB);
       }
       __syncwarp();
-      fetch(stage);
-      look();
-      if (++stage == S::kStages) stage = 0, parity ^= 1;
+      if (ok) felix_sm100::bulk_load_1d(&sm.ring[stage][lane * kB], src, kB, &sm.full[stage]);
+      advance();
+    }
+    // After a wait that gave up, copies may still be under way into this CTA's
+    // shared memory: they get time to land before it goes to another.
+    if (sm.abort) {
+      const uint64_t t0 = felix_sm100::globaltimer_ns();
+      while (felix_sm100::globaltimer_ns() - t0 < 1000000ull) {
+      }
+    }
+    return;
+  }
+  if constexpr (kCW == 8) felix_sm100::setmaxnreg_inc<kRegsSums>();
+
+  const int rw = warp / kTW, tw = warp - rw * kTW;  // group of rows, place among its tokens
+  for (;;) {
+    const uint32_t kvh = use.kvh, rt = use.rt;
+    const int count = P.counts ? min(max(P.counts[use.slot], 0), int(P.rows)) : int(P.rows);
+    Attn<T, D, NT> A;
+    A.load_q(P, use.slot, kvh, rt * H::kTileRows + rw * kRows, use.len, count, lane);
+    const uint32_t end = use.end_step();
+    for (uint32_t t = use.first_step(); t < end; t += kTW) {
+      if (felix_sm100::mbar_wait(&sm.full[stage], parity, &sm.abort, P.status,
+                                 felix_sm100::kWdKv4Load)) {
+        const uint32_t there = sm.there[stage] >> (tw * kStep) & ((1u << kStep) - 1);
+        if (there)
+          A.step(sm.ring[stage] + tw * kStep * kB, sm.tp[warp], there,
+                 int(t + tw) * kStepTokens, lane);
+      }
+      __syncwarp();
+      if (lane == 0) felix_sm100::mbar_arrive(&sm.empty[stage]);
+      advance();
     }
     A.park(sm.o[warp], sm.ml[warp], lane);
-    __syncthreads();
+    felix_sm100::named_barrier_sync(1, H::kJoin);
 
     // ---- join the warps; write the result, or this share's part of it
     const bool whole = use.lo == 0 && use.hi == use.size;
     const uint32_t c0 = use.seg_at / quota, c1 = (use.seg_at + use.size - 1) / quota;
-    constexpr size_t kPart = size_t(kRows) * (D + 2);
+    constexpr size_t kPart = size_t(H::kTileRows) * (D + 3);
     float* mypart = P.partials + (size_t(blockIdx.x) * 2 + (use.lo == 0 ? 1 : 0)) * kPart;
-    auto put = [&](int r, int d, float4 v, float top, float sum) {
-      const uint32_t rr = rt * kRows + r;
+    // Sums of a row: O is relative to `top`, as l and w are.
+    struct Row {
+      float top, l, w;
+    };
+    auto put = [&](int i, float4 v, Row s) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      const uint32_t rr = rt * H::kTileRows + r;
       const uint32_t row = rr / P.group, head = kvh * P.group + rr % P.group;
       if (row >= P.rows) return;
       const size_t at = (size_t(use.slot) * P.heads + head) * P.rows + row;
-      const float k = sum == 0.f ? 0.f : 1.f / sum;
-      T x[4] = {from_f<T>(sum == 0.f ? 0.f : v.x * k), from_f<T>(sum == 0.f ? 0.f : v.y * k),
-                from_f<T>(sum == 0.f ? 0.f : v.z * k), from_f<T>(sum == 0.f ? 0.f : v.w * k)};
+      const float k = s.l == 0.f ? 0.f : 1.f / s.w;  // l = 0: the row saw nothing, O is 0
+      const T x[4] = {from_f<T>(v.x * k), from_f<T>(v.y * k), from_f<T>(v.z * k),
+                      from_f<T>(v.w * k)};
       *reinterpret_cast<uint2*>(static_cast<T*>(P.out) + at * D + d) =
           *reinterpret_cast<const uint2*>(x);
       if (P.lse && d == 0)
-        P.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        P.lse[at] = s.l == 0.f ? -INFINITY : (s.top + log2f(s.l)) * 0.6931471805599453f;
     };
-    for (int i = tid; i < kVec; i += kThreads) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      float top = sm.ml[0][2 * r];
+    // O vector and statistics of a row from `n` sources as one: source(k, &m, &l, &w)
+    // gives its vector. A source that saw nothing of the row has l = 0 and O = 0;
+    // m = -inf with l not 0 is one that saw NaN only.
+    auto joined = [&](int n, auto&& stats, auto&& vec, Row* s) {
+      s->top = -INFINITY;
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][2 * r]);
+      for (int k = 0; k < n; ++k) s->top = fmaxf(s->top, stats(k)[0]);
+      s->l = s->w = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        // a warp that saw nothing of the row has l = 0 and O = 0; m = -inf with l
-        // not 0 is a warp that saw NaN only
-        const float wl = sm.ml[w][2 * r + 1], wm = sm.ml[w][2 * r];
-        if (wl == 0.f) continue;
-        const float k = wm == -INFINITY ? 1.f : ex2(wm - top);
-        const float4 x = reinterpret_cast<const float4*>(sm.o[w])[i];
-        v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y);
-        v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
-        sum = fmaf(wl, k, sum);
+      for (int k = 0; k < n; ++k) {
+        const float m = stats(k)[0], l = stats(k)[1];
+        if (l == 0.f) continue;
+        const float to = m == -INFINITY ? 1.f : ex2(m - s->top);
+        const float4 x = vec(k);
+        v.x = fmaf(x.x, to, v.x), v.y = fmaf(x.y, to, v.y);
+        v.z = fmaf(x.z, to, v.z), v.w = fmaf(x.w, to, v.w);
+        s->l = fmaf(l, to, s->l);
+        s->w = fmaf(stats(k)[2], to, s->w);
       }
+      return v;
+    };
+    for (int i = tid; i < kVec; i += H::kJoin) {
+      const int group = i / kWarpVec, j = i % kWarpVec;  // the rows' warps, place in them
+      Row s;
+      const float4 v = joined(
+          kTW, [&](int k) { return sm.ml[group * kTW + k] + 3 * (j / (D / 4)); },
+          [&](int k) { return reinterpret_cast<const float4*>(sm.o[group * kTW + k])[j]; }, &s);
       if (whole) {
-        put(r, d, v, top, sum);
+        put(i, v, s);
       } else {
         reinterpret_cast<float4*>(mypart)[i] = v;
-        if (d == 0) mypart[kRows * D + 2 * r] = top, mypart[kRows * D + 2 * r + 1] = sum;
+        if (i % (D / 4) == 0) {
+          float* x = mypart + H::kTileRows * D + 3 * (i / (D / 4));
+          x[0] = s.top, x[1] = s.l, x[2] = s.w;
+        }
       }
     }
     if (!whole) {
       __threadfence();
-      __syncthreads();
+      felix_sm100::named_barrier_sync(1, H::kJoin);
       if (tid == 0) sm.ticket = atomicAdd(P.counters + c0, 1u);
-      __syncthreads();
+      felix_sm100::named_barrier_sync(1, H::kJoin);
       if (sm.ticket == c1 - c0) {
         __threadfence();
-        // each warp joins every kWarps-th part, then the warps are joined: all
-        // loads of a warp are independent of one another
         auto part_at = [&](uint32_t k) {
           return P.partials + (size_t(k) * 2 + (k == c0 ? 1 : 0)) * kPart;
         };
-        for (int r = lane; r < kRows; r += 32) {
-          float top = -INFINITY, sum = 0.f;
-          for (uint32_t k = c0 + warp; k <= c1; k += kWarps)
-            top = fmaxf(top, __ldcg(part_at(k) + kRows * D + 2 * r));
-          for (uint32_t k = c0 + warp; k <= c1; k += kWarps) {
-            const float pm = __ldcg(part_at(k) + kRows * D + 2 * r);
-            const float pl = __ldcg(part_at(k) + kRows * D + 2 * r + 1);
-            if (pl != 0.f) sum = fmaf(pl, pm == -INFINITY ? 1.f : ex2(pm - top), sum);
-          }
-          sm.ml[warp][2 * r] = top;
-          sm.ml[warp][2 * r + 1] = sum;
-        }
-        __syncwarp();
-        constexpr int kPer = kVec / 32;  // vectors of a lane
-        for (int j0 = 0; j0 < kPer; j0 += 8) {
-          float4 v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-          for (uint32_t k = c0 + warp; k <= c1; k += kWarps) {
-            const float* pp = part_at(k);
+        // a thread joins its vectors over all parts, four parts' loads at a time
+        for (int i = tid; i < kVec; i += H::kJoin) {
+          const int r = i / (D / 4);
+          Row s = {-INFINITY, 0.f, 0.f};
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (uint32_t k0 = c0; k0 <= c1; k0 += 8) {
+            float m[8], l[8], w[8];
+            float4 x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              if (j0 + j >= kPer) break;
-              const int i = (j0 + j) * 32 + lane, r = i / (D / 4);
-              const float pm = __ldcg(pp + kRows * D + 2 * r), pl = __ldcg(pp + kRows * D + 2 * r + 1);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(pp) + i);
-              const float w = pl == 0.f ? 0.f : pm == -INFINITY ? 1.f : ex2(pm - sm.ml[warp][2 * r]);
-              v[j].x = fmaf(x.x, w, v[j].x), v[j].y = fmaf(x.y, w, v[j].y);
-              v[j].z = fmaf(x.z, w, v[j].z), v[j].w = fmaf(x.w, w, v[j].w);
+              const float* p = part_at(min(k0 + j, c1));
+              const float* q = p + H::kTileRows * D + 3 * r;
+              m[j] = __ldcg(q), l[j] = __ldcg(q + 1), w[j] = __ldcg(q + 2);
+              x[j] = __ldcg(reinterpret_cast<const float4*>(p) + i);
+              if (k0 + j > c1) l[j] = 0.f, m[j] = -INFINITY;
+            }
+            float top = s.top;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, m[j]);
+            const float keep = s.top == -INFINITY ? 1.f : ex2(s.top - top);
+            v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
+            s = {top, s.l * keep, s.w * keep};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (l[j] == 0.f) continue;
+              const float to = m[j] == -INFINITY ? 1.f : ex2(m[j] - top);
+              v.x = fmaf(x[j].x, to, v.x), v.y = fmaf(x[j].y, to, v.y);
+              v.z = fmaf(x[j].z, to, v.z), v.w = fmaf(x[j].w, to, v.w);
+              s.l = fmaf(l[j], to, s.l);
+              s.w = fmaf(w[j], to, s.w);
             }
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j0 + j < kPer)
-              reinterpret_cast<float4*>(sm.o[warp])[(j0 + j) * 32 + lane] = v[j];
-        }
-        __syncthreads();
-        for (int i = tid; i < kVec; i += kThreads) {
-          const int r = i / (D / 4), d = i % (D / 4) * 4;
-          float top = -INFINITY, sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.ml[w][2 * r]);
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float wl = sm.ml[w][2 * r + 1], wm = sm.ml[w][2 * r];
-            if (wl == 0.f) continue;
-            const float k = wm == -INFINITY ? 1.f : ex2(wm - top);
-            const float4 x = reinterpret_cast<const float4*>(sm.o[w])[i];
-            v.x = fmaf(x.x, k, v.x), v.y = fmaf(x.y, k, v.y);
-            v.z = fmaf(x.z, k, v.z), v.w = fmaf(x.w, k, v.w);
-            sum = fmaf(wl, k, sum);
-          }
-          put(r, d, v, top, sum);
+          put(i, v, s);
         }
         if (tid == 0) P.counters[c0] = 0;
       }
     }
-    __syncthreads();
+    felix_sm100::named_barrier_sync(1, H::kJoin);
     const uint32_t u = use.end();
     if (u >= last) break;
     use.open(P, u, last);
   }
-  // after a wait that gave up, copies may still be under way into this CTA's
-  // shared memory: give them time to land (with a limit) before it goes to another
-  if (sm.abort)
-    for (int s = 0; s < S::kStages; ++s) {
-      const uint64_t t0 = felix_sm100::globaltimer_ns();
-      while (!felix_sm100::mbar_try_wait(felix_sm100::smem_u32(&sm.full[warp][s]), parity) &&
-             felix_sm100::globaltimer_ns() - t0 < 1000000ull) {
-      }
-    }
 }
 
-// CTAs per SM that a caller's workspace has room for.
-constexpr int kMaxPerSm = 4;
-constexpr size_t ws_bytes_for(uint32_t grid, int rows, int D) {
-  return kWsCounterBytes + size_t(grid) * 2 * rows * (D + 2) * sizeof(float);
+// Scratch: counters, then two parts per CTA. A grid has at most three CTAs of 8
+// rows per SM, or one of up to kMaxRows(D).
+constexpr size_t part_bytes(uint32_t ctas, int rows, int D) {
+  return size_t(ctas) * 2 * rows * (D + 3) * sizeof(float);
 }
-// Tiles of 8 query rows that a warp keeps in registers: 5 of D = 64, 3 of D = 128.
-constexpr int max_nt(int D) { return D == 64 ? 5 : 3; }
+// Tiles of 8 query rows that a warp keeps in registers.
+constexpr int max_nt(int D) { return D == 64 ? 3 : 2; }
+constexpr int max_rows(int D) { return 4 * 8 * max_nt(D); }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int kRW, int kCW>
 FelixCode launch(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_bytes,
                  cudaStream_t stream) {
+  using H = Shape<D, NT, kRW, kCW>;
   static int per_sm[64];
   static PerDeviceOnce once;
-  constexpr int smem = int(sizeof(Smem<D, NT>));
+  constexpr int smem = int(sizeof(Smem<D, NT, kRW, kCW>));
+  auto* kernel = kv4_attn_kernel<T, D, NT, kRW, kCW>;
   const int rc = once.run(dev->ordinal, [&] {
-    if (cudaFuncSetAttribute(kv4_attn_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             smem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess)
       return -1;
+    cudaFuncAttributes attr;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) return -1;
+    if (kCW == 8 && attr.numRegs != kRegsLaunch) return -2;  // the split would wait for ever
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv4_attn_kernel<T, D, NT>, kThreads,
-                                                      smem) != cudaSuccess || n < 1)
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, H::kThreads, smem) !=
+            cudaSuccess || n < 1)
       return -1;
-    per_sm[dev->ordinal] = n < kMaxPerSm ? n : kMaxPerSm;
+    per_sm[dev->ordinal] = kCW == 4 ? (n < 3 ? n : 3) : 1;
     return 0;
   });
+  if (rc == -2) return api_error("kv4_attention: built with another register count than 168");
   if (rc != 0) return launch_error(cudaGetLastError(), "kv4_attention: occupancy");
   const uint32_t grid = uint32_t(dev->num_sms) * uint32_t(per_sm[dev->ordinal]);
-  const size_t need = ws_bytes_for(grid, 8 * NT, D);
+  const size_t need = kWsCounterBytes + part_bytes(grid, H::kTileRows, D);
   if (workspace && ws_bytes < need)
     return api_error("kv4_attention: workspace smaller than felix_kv4_attention_workspace_size");
   void* ws = workspace ? workspace : library_workspace(dev, stream, need);
   if (!ws) return launch_error(cudaErrorMemoryAllocation, "kv4_attention: workspace");
   P.counters = static_cast<uint32_t*>(ws);
   P.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + kWsCounterBytes);
-  P.row_tiles = (P.rows * P.group + 8 * NT - 1) / (8 * NT);
-  kv4_attn_kernel<T, D, NT><<<grid, kThreads, smem, stream>>>(P);
+  P.row_tiles = (P.rows * P.group + H::kTileRows - 1) / H::kTileRows;
+  kernel<<<grid, H::kThreads, smem, stream>>>(P);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return launch_error(e, "kv4_attention");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
-// The fewest row tiles that registers allow, then as even as possible: each tile
-// of rows reads the cache again.
+// Up to 8 rows: four consumers that share all tokens, three CTAs to an SM. More:
+// eight, in as many groups of rows as registers ask for, so that the cache is read
+// once for up to max_rows(D) rows; beyond that each further tile reads it again.
 template <typename T, int D>
-FelixCode launch_rows(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_bytes,
-                      cudaStream_t stream) {
-  const uint32_t eights = (P.rows * P.group + 7) / 8;
-  const uint32_t tiles = (eights + max_nt(D) - 1) / max_nt(D);
-  switch ((eights + tiles - 1) / tiles) {
-    case 1: return launch<T, D, 1>(P, dev, workspace, ws_bytes, stream);
-    case 2: return launch<T, D, 2>(P, dev, workspace, ws_bytes, stream);
-    case 3: return launch<T, D, 3>(P, dev, workspace, ws_bytes, stream);
-    default: break;
-  }
+FelixCode launch_rows(AttnParams& P, DeviceInfo* dev, void* ws, size_t n, cudaStream_t stream) {
+  const uint32_t eights = (P.rows * P.group + 7) / 8, most = max_nt(D);
+  if (eights == 1) return launch<T, D, 1, 1, 4>(P, dev, ws, n, stream);
+  const uint32_t tiles = (eights + 4 * most - 1) / (4 * most);
+  const uint32_t per_tile = (eights + tiles - 1) / tiles;
+  const uint32_t rw = per_tile <= most ? 1 : per_tile <= 2 * most ? 2 : 4;
+  const bool three = D == 64 && per_tile > 2 * rw;
   if constexpr (D == 64) {
-    if ((eights + tiles - 1) / tiles == 4) return launch<T, D, 4>(P, dev, workspace, ws_bytes, stream);
-    return launch<T, D, 5>(P, dev, workspace, ws_bytes, stream);
+    if (three) {
+      if (rw == 1) return launch<T, D, 3, 1, 8>(P, dev, ws, n, stream);
+      if (rw == 2) return launch<T, D, 3, 2, 8>(P, dev, ws, n, stream);
+      return launch<T, D, 3, 4, 8>(P, dev, ws, n, stream);
+    }
   }
-  return api_error("kv4_attention: rows");
+  if (rw == 1) return launch<T, D, 2, 1, 8>(P, dev, ws, n, stream);
+  if (rw == 2) return launch<T, D, 2, 2, 8>(P, dev, ws, n, stream);
+  return launch<T, D, 2, 4, 8>(P, dev, ws, n, stream);
 }
 
 }  // namespace kv4
 
 size_t kv4_attention_workspace_bytes(uint32_t head_dim, int num_sms) {
-  return kv4::ws_bytes_for(uint32_t(num_sms) * kv4::kMaxPerSm, 8 * kv4::max_nt(int(head_dim)),
-                           int(head_dim));
+  const uint32_t sms = uint32_t(num_sms);
+  const int D = int(head_dim);
+  return kWsCounterBytes + std::max(kv4::part_bytes(3 * sms, 8, D),
+                                    kv4::part_bytes(sms, kv4::max_rows(D), D));
 }
 
 FelixCode kv4_attention_launch(const felix_kv4::CacheView& c, uint32_t head_dim, const void* q,
