@@ -61,7 +61,7 @@ struct AttnParams {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -71,7 +71,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1,
                                          const float (&c)[4]) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -80,12 +80,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -315,6 +315,19 @@ struct Attn {
           t0 = fmaxf(t0, x[k][h].x);
           t1 = fmaxf(t1, x[k][h].y);
         }
+      // Probabilities with the m at hand; a vote says whether it holds.
+      float2 e[kStep][2];
+      auto exponents = [&]() {
+        const F2 minus = f2(-m[n][0], -m[n][1]);
+#pragma unroll
+        for (int k = 0; k < kStep; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 d = un(add(f2(x[k][h].x, x[k][h].y), minus));
+            e[k][h] = make_float2(ex2(d.x), ex2(d.y));
+          }
+      };
+      exponents();
       // Exponents are relative to m, 2^6 below a maximum that is only moved when a
       // score passes it by 2^8: P stays below 2^15, and fp16 holds what is 2^30
       // smaller.
@@ -338,15 +351,13 @@ struct Attn {
         for (int j = 0; j < D / 16; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) o[n][j][h] = mul(o[n][j][h], kk);
+        exponents();
       }
-      const F2 minus = f2(-m[n][0], -m[n][1]);
 #pragma unroll
       for (int k = 0; k < kStep; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = k * 16 + h * 8 + g;
-          const float2 d = un(add(f2(x[k][h].x, x[k][h].y), minus));
-          float2 e = make_float2(ex2(d.x), ex2(d.y));
           Pair2 v = tp.v[i];
           F2 inv = tp.e[i].b, base = tp.b[i];
           if (kMask) {  // a masked token's parameters may be anything
@@ -354,11 +365,11 @@ struct Attn {
               const float2 y = un(a);
               return f2(on[k][h][0] ? y.x : 0.f, on[k][h][1] ? y.y : 0.f);
             };
-            if (!on[k][h][0]) e.x = 0.f;
-            if (!on[k][h][1]) e.y = 0.f;
+            if (!on[k][h][0]) e[k][h].x = 0.f;
+            if (!on[k][h][1]) e[k][h].y = 0.f;
             inv = seen(inv), base = seen(base), v.a = seen(v.a), v.b = seen(v.b);
           }
-          const F2 ee = f2(e.x, e.y);
+          const F2 ee = f2(e[k][h].x, e[k][h].y);
           l[n] = fma(ee, inv, l[n]);
           const float2 p = un(mul(ee, v.a));
           const __half2 ph = __floats2half2_rn(p.x, p.y);
@@ -377,16 +388,16 @@ struct Attn {
     constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u;
     constexpr int kB = int(block_bytes(D));
     const int g = lane >> 2;
-    {
-      const unsigned char* p = x + (lane / 16) * kB;
-      const float2 k = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[lane & 15]);
-      const VParams v = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[lane & 15]);
-      tp.k[lane] = {f2(k.x, k.x), f2(k.y, k.y)};
-      tp.e[lane] = {f2(v.e, v.e), f2(v.inv, v.inv)};
-      tp.v[lane] = {f2(v.mant, v.mant), f2(v.rcp, v.rcp)};
-      tp.b[lane] = f2(v.base, v.base);
+#pragma unroll
+    for (int i = lane; i < kStepTokens; i += 32) {
+      const unsigned char* p = x + (i / 16) * kB;
+      const float2 k = k_params(reinterpret_cast<const uint32_t*>(p + k_params_at(D))[i & 15]);
+      const VParams v = v_params(reinterpret_cast<const uint32_t*>(p + v_params_at(D))[i & 15]);
+      tp.k[i] = {f2(k.x, k.x), f2(k.y, k.y)};
+      tp.e[i] = {f2(v.e, v.e), f2(v.inv, v.inv)};
+      tp.v[i] = {f2(v.mant, v.mant), f2(v.rcp, v.rcp)};
+      tp.b[i] = f2(v.base, v.base);
     }
-    __syncwarp();
     float s[NT][kStep][4];
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -418,6 +429,7 @@ struct Attn {
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[0][b][c] += s2[c];
     }
+    __syncwarp();  // tp is written
     uint32_t pt[NT][kStep][2];
     if (there == (1u << kStep) - 1 && token0 + kStepTokens <= low)
       softmax<false>(s, tp, there, token0, g, pt);
@@ -539,13 +551,16 @@ struct Smem {
   int abort;
 };
 
-// Units of a segment beyond its steps: what opening and closing it costs (q, the
-// join of the warps). Without them a share of many short segments takes longest.
-constexpr uint32_t kOpen = 12;
+// Units of a segment beyond its steps (`open` below): what opening and closing it
+// costs (q, the join of the warps), about 12 steps. Without them a share of many
+// short segments takes longest. Where there are few steps per CTA, the shares are
+// kept even in steps instead; at least 1, so that an empty slot is in a share too.
+constexpr uint32_t kMaxOpen = 12;
 
 // A place in a CTA's share of the work: the part [lo, hi) of a segment's units,
-// whose first kOpen units hold no steps.
+// whose first `open` units hold no steps.
 struct Place {
+  uint32_t open_units;
   uint32_t slot, slot_at;  // slot, and the units before it
   uint32_t size;           // units of each of the slot's segments
   int len, reach;
@@ -553,7 +568,7 @@ struct Place {
   __device__ __forceinline__ void read(const AttnParams& P) {
     len = slot_length(P.c, slot);
     reach = slot_reach(P.c, slot);
-    size = kOpen + (reach + kStepTokens - 1) / kStepTokens;
+    size = open_units + (reach + kStepTokens - 1) / kStepTokens;
   }
   // unit u, at or after the current slot's first
   __device__ __forceinline__ void open(const AttnParams& P, uint32_t u, uint32_t last) {
@@ -571,12 +586,12 @@ struct Place {
     hi = min(size, lo + (last - u));
   }
   __device__ __forceinline__ uint32_t end() const { return seg_at + hi; }
-  __device__ __forceinline__ uint32_t first_step() const { return lo > kOpen ? lo - kOpen : 0; }
-  __device__ __forceinline__ uint32_t end_step() const { return hi > kOpen ? hi - kOpen : 0; }
+  __device__ __forceinline__ uint32_t first_step() const { return lo > open_units ? lo - open_units : 0; }
+  __device__ __forceinline__ uint32_t end_step() const { return hi > open_units ? hi - open_units : 0; }
 };
 
 // Persistent grid. The work is a line of units (a segment's steps of 32 tokens and
-// kOpen for the segment itself, one after another), cut into equal shares, one
+// `open` for the segment itself, one after another), cut into equal shares, one
 // per CTA, whatever the slots' lengths. The last warp looks pages up and fills the
 // ring of stages with bulk copies, across segments; the others take their steps
 // of each stage, and their registers hold sums only. A segment that lies in
@@ -599,11 +614,11 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
   // ---- this CTA's share: units before each thread's run of slots, then the slot
   const uint32_t run = (c.slots + kThreads - 1) / kThreads;
   const uint32_t s0 = min(tid * run, c.slots), s1 = min(s0 + run, c.slots);
-  auto units = [&](uint32_t s) {
-    return (kOpen + uint32_t(slot_reach(c, s) + kStepTokens - 1) / kStepTokens) * per_seg;
+  auto steps = [&](uint32_t s) {
+    return uint32_t(slot_reach(c, s) + kStepTokens - 1) / kStepTokens * per_seg;
   };
   uint32_t mine = 0;
-  for (uint32_t s = s0; s < s1; ++s) mine += units(s);
+  for (uint32_t s = s0; s < s1; ++s) mine += steps(s);
   uint32_t upto = mine;
 #pragma unroll
   for (int x = 1; x < 32; x *= 2) {
@@ -627,15 +642,18 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
     if (w < warp) upto += sm.scan[w];
     total += sm.scan[w];
   }
-  // at least a segment's opening and one step for each warp: smaller parts cost
-  // more to join than they save
-  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, kOpen + kTW);
+  const uint32_t open = min(max(total / (4 * gridDim.x), 1u), kMaxOpen);
+  mine += open * (s1 - s0) * per_seg;
+  upto += open * s1 * per_seg;
+  total += open * c.slots * per_seg;
+  // at least a step for each warp: smaller parts cost more to join than they save
+  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, uint32_t(kTW));
   const uint32_t first = min(blockIdx.x * quota, total), last = min(first + quota, total);
   if (first >= last) return;
   if (first >= upto - mine && first < upto) {
     uint32_t at = upto - mine;
     for (uint32_t s = s0; s < s1; ++s) {
-      const uint32_t n = units(s);
+      const uint32_t n = steps(s) + open * per_seg;
       if (first < at + n) {
         sm.at[0] = s, sm.at[1] = at;
         break;
@@ -646,6 +664,7 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
   __syncthreads();
 
   Place use;
+  use.open_units = open;
   use.slot = sm.at[0], use.slot_at = sm.at[1];
   use.read(P);
   use.open(P, first, last);
@@ -794,48 +813,57 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
       }
     }
     if (!whole) {
-      __threadfence();
       felix_sm100::named_barrier_sync(1, H::kJoin);
-      if (tid == 0) sm.ticket = atomicAdd(P.counters + c0, 1u);
+      if (tid == 0) {
+        __threadfence();  // the barrier has ordered the CTA's stores before it
+        sm.ticket = atomicAdd(P.counters + c0, 1u);
+        __threadfence();
+      }
       felix_sm100::named_barrier_sync(1, H::kJoin);
       if (sm.ticket == c1 - c0) {
-        __threadfence();
         auto part_at = [&](uint32_t k) {
           return P.partials + (size_t(k) * 2 + (k == c0 ? 1 : 0)) * kPart;
         };
-        // a thread joins its vectors over all parts, four parts' loads at a time
-        for (int i = tid; i < kVec; i += H::kJoin) {
-          const int r = i / (D / 4);
-          Row s = {-INFINITY, 0.f, 0.f};
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (uint32_t k0 = c0; k0 <= c1; k0 += 8) {
-            float m[8], l[8], w[8];
-            float4 x[8];
+        // a thread joins two vectors of O over all parts, four parts' loads at a time
+        constexpr int kTwo = kVec / 2;
+        for (int i = tid; i < kTwo; i += H::kJoin) {
+          Row s[2] = {{-INFINITY, 0.f, 0.f}, {-INFINITY, 0.f, 0.f}};
+          float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+          for (uint32_t k0 = c0; k0 <= c1; k0 += 4) {
+            float m[2][4], l[2][4], w[2][4];
+            float4 x[2][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
               const float* p = part_at(min(k0 + j, c1));
-              const float* q = p + H::kTileRows * D + 3 * r;
-              m[j] = __ldcg(q), l[j] = __ldcg(q + 1), w[j] = __ldcg(q + 2);
-              x[j] = __ldcg(reinterpret_cast<const float4*>(p) + i);
-              if (k0 + j > c1) l[j] = 0.f, m[j] = -INFINITY;
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const float* q = p + H::kTileRows * D + 3 * ((i + y * kTwo) / (D / 4));
+                m[y][j] = __ldcg(q), l[y][j] = __ldcg(q + 1), w[y][j] = __ldcg(q + 2);
+                x[y][j] = __ldcg(reinterpret_cast<const float4*>(p) + i + y * kTwo);
+                if (k0 + j > c1) l[y][j] = 0.f, m[y][j] = -INFINITY;
+              }
             }
-            float top = s.top;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, m[j]);
-            const float keep = s.top == -INFINITY ? 1.f : ex2(s.top - top);
-            v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
-            s = {top, s.l * keep, s.w * keep};
+            for (int y = 0; y < 2; ++y) {
+              float top = s[y].top;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (l[j] == 0.f) continue;
-              const float to = m[j] == -INFINITY ? 1.f : ex2(m[j] - top);
-              v.x = fmaf(x[j].x, to, v.x), v.y = fmaf(x[j].y, to, v.y);
-              v.z = fmaf(x[j].z, to, v.z), v.w = fmaf(x[j].w, to, v.w);
-              s.l = fmaf(l[j], to, s.l);
-              s.w = fmaf(w[j], to, s.w);
+              for (int j = 0; j < 4; ++j) top = fmaxf(top, m[y][j]);
+              const float keep = s[y].top == -INFINITY ? 1.f : ex2(s[y].top - top);
+              v[y].x *= keep, v[y].y *= keep, v[y].z *= keep, v[y].w *= keep;
+              s[y] = {top, s[y].l * keep, s[y].w * keep};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (l[y][j] == 0.f) continue;
+                const float to = m[y][j] == -INFINITY ? 1.f : ex2(m[y][j] - top);
+                v[y].x = fmaf(x[y][j].x, to, v[y].x), v[y].y = fmaf(x[y][j].y, to, v[y].y);
+                v[y].z = fmaf(x[y][j].z, to, v[y].z), v[y].w = fmaf(x[y][j].w, to, v[y].w);
+                s[y].l = fmaf(l[y][j], to, s[y].l);
+                s[y].w = fmaf(w[y][j], to, s[y].w);
+              }
             }
           }
-          put(i, v, s);
+          put(i, v[0], s[0]);
+          put(i + kTwo, v[1], s[1]);
         }
         if (tid == 0) P.counters[c0] = 0;
       }
