@@ -318,7 +318,7 @@ int felix_kv4_copy_pages(const void* from, uint64_t from_pages, void* to, uint64
  * those with less than p of the kept mass before them, min-p those with
  * w >= min_p, and the first always stays; the token is the first by index at
  * which the running sum of kept mass exceeds floor(uniform * total). NaN counts
- * as -inf. logprobs: log of the probability with which the token was drawn (0
+ * as -inf. vocab is at most 524288. logprobs: log of the probability with which the token was drawn (0
  * where temperature <= 0). A row with nothing above -inf: -1 and -inf.
  */
 int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, int64_t stride,

@@ -616,7 +616,8 @@ int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, i
       return api_error("sample: logits must be fp16, bf16 or fp32");
     if (rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
     if (!logits || !uniform || !tokens || !logprobs) return api_error("sample: null pointer");
-    if (vocab == 0 || vocab > 0x7fffffffu) return api_error("sample: vocab must be 1..2^31-1");
+    if (vocab == 0 || vocab > 524288u) return api_error("sample: vocab must be 1..524288");
+    if (rows > (1u << 27)) return api_error("sample: at most 2^27 rows");
     if (stride < 0) return api_error("sample: stride must not be negative");
     return sample_launch({logits, dtype, rows, vocab, stride, uniform, temperature, top_k, top_p,
                           min_p, tokens, logprobs},

@@ -15,244 +15,551 @@
 // number give the same token in every batch. 2^-31 of the largest probability
 // is the resolution (a running sum in fp32 would have 2^-24 of the total).
 // All three filters keep a prefix of the order, so together they are a threshold
-// on the value and a number of ties to keep.
+// on (value, index), held as one 64-bit number that is larger for what comes first.
+//
+// A cluster of CTAs shares a row, and each keeps its part in shared memory: the
+// logits are read from HBM once. The threshold of top-k (by count) and that of
+// top-p (by mass) come from one histogram over the distance from the maximum
+// (2048 bins up to where masses round to 0; even in value, so that few tokens
+// share a bin), merged over the cluster by slices. The tokens of the bin in which
+// the threshold falls, a few dozen as a rule, are gathered by every CTA and ranked
+// by comparison with one another. Where a bin holds too many (equal values, a flat
+// row) it is split again into 2048 by (value, index) until it does not.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
 #include "felix_internal.h"
 #include "sm100_ptx.cuh"
-
-#include <cuda_bf16.h>
 
 namespace felix_impl {
 namespace smp {
 
-constexpr int kThreads = 1024;
+namespace cg = cooperative_groups;
+using u64 = unsigned long long;
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxCtas = 8;
+constexpr int kMost = 1024;  // tokens that are ranked by comparison
 
 template <typename T>
-__device__ __forceinline__ float value(const T* p, uint32_t i);
+__device__ __forceinline__ float to_f(T v);
 template <>
-__device__ __forceinline__ float value(const float* p, uint32_t i) { return p[i]; }
+__device__ __forceinline__ float to_f(float v) { return v; }
 template <>
-__device__ __forceinline__ float value(const __half* p, uint32_t i) { return __half2float(p[i]); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <>
-__device__ __forceinline__ float value(const __nv_bfloat16* p, uint32_t i) {
-  return __bfloat162float(p[i]);
-}
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Unsigned key in the order of the values; NaN as -inf, -0 as +0.
+// NaN as -inf, -0 as +0.
+__device__ __forceinline__ float plain(float x) { return x != x ? -INFINITY : x + 0.f; }
+// Unsigned key in the order of the values.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) x = -INFINITY;
-  x += 0.f;
   const uint32_t b = __float_as_uint(x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+__device__ __forceinline__ u64 place_of(float x, uint32_t i) { return u64(key_of(x)) << 32 | ~i; }
 __device__ __forceinline__ float scaled(float x, float top, float temp) {
   return x == top ? 0.f : __fdiv_rn(x - top, temp);
 }
-__device__ __forceinline__ uint32_t mass_of(float w) { return __float2uint_rn(w * 2147483648.f); }
+// expf, not an approximation: the masses are part of the definition.
+__device__ __forceinline__ uint32_t mass_of(float x, float top, float temp) {
+  return __float2uint_rn(expf(scaled(x, top, temp)) * 2147483648.f);
+}
 
-struct Shared {
-  unsigned long long sum[32];
-  uint32_t count[256];
-  unsigned long long mass[256];
-  unsigned long long before;  // mass or count above the digits chosen so far
-  uint32_t prefix, ties;
-  int found;
+struct Cut {  // a bin in which a threshold falls
+  int bin;    // kBins: what is past the bins
+  uint32_t count, before;  // tokens in it, and in the bins before it
+  u64 mass_before;
 };
 
-__device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
+struct Shared {
+  // Tokens of a bin, and their masses as sums of the low 16 and of the high bits: 32
+  // bits hold those of 65536 tokens, the most that a CTA has (vocab <= 8 * 65536).
+  uint32_t count[kBins], lo[kBins], hi[kBins];
+  u64 mine[kMost], all[kMost];
+  uint32_t mass[kMost];
+  u64 red[kWarps];
+  uint32_t red2[kWarps];
+  // for the other CTAs of the cluster
+  float top;
+  u64 slice_mass, kept, first, range[2];
+  uint32_t slice_count, gathered;
+  Cut cut;
+  u64 found;  // (threshold) of a ranking
+  u64 found_mass;
+};
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
   for (int d = 16; d; d /= 2) v += __shfl_xor_sync(~0u, v, d);
   return v;
 }
-// Exclusive prefix over the block; *total its sum.
-__device__ unsigned long long block_scan(unsigned long long v, Shared& sh, unsigned long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned long long x = v;
+__device__ __forceinline__ u64 warp_max(u64 v) {
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const unsigned long long y = __shfl_up_sync(~0u, x, d);
-    if (lane >= d) x += y;
+  for (int d = 16; d; d /= 2) {
+    const u64 o = __shfl_xor_sync(~0u, v, d);
+    v = o > v ? o : v;
   }
-  __syncthreads();
-  if (lane == 31) sh.sum[warp] = x;
-  __syncthreads();
-  unsigned long long w = sh.sum[lane];
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const unsigned long long y = __shfl_up_sync(~0u, w, d);
-    if (lane >= d) w += y;
-  }
-  const unsigned long long before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
-  *total = __shfl_sync(~0u, w, 31);
-  return x - v + (warp ? before : 0);
+  return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleArgs A) {
-  __shared__ Shared sh;
-  const uint32_t row = blockIdx.x, V = A.vocab, tid = threadIdx.x;
-  const T* x = static_cast<const T*>(A.logits) + int64_t(row) * A.stride;
-  const float temp = A.temperature ? A.temperature[row] : 1.f;
+// A row's part in one CTA: tokens lo .. lo + n - 1. Staged: in shared memory, else
+// read from global memory in each pass.
+template <typename T, bool kStaged>
+struct Row {
+  const T* g;     // the row
+  const T* s;     // token lo in shared memory
+  uint32_t lo, n;
+  __device__ __forceinline__ float at(uint32_t j) const {
+    return plain(to_f<T>(kStaged ? s[j] : g[lo + j]));
+  }
+};
 
-  // the largest value and its first index: (key, ~index) as one number
-  unsigned long long best = 0;
-  for (uint32_t i = tid; i < V; i += kThreads) {
-    const unsigned long long k = (unsigned long long)key_of(value<T>(x, i)) << 32 | ~i;
-    best = k > best ? k : best;
-  }
+template <typename T, bool kStaged>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t C = cluster.num_blocks(), rank = cluster.block_rank();
+  const uint32_t row = blockIdx.x / C, V = A.vocab;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float temp = A.temperature ? A.temperature[row] : 1.f;
+  const int k = A.top_k ? A.top_k[row] : 0;
+  const float p = A.top_p ? A.top_p[row] : 1.f, mp = A.min_p ? A.min_p[row] : 0.f;
+  auto of = [&](auto* x, uint32_t r) { return cluster.map_shared_rank(x, r); };
+
+  Row<T, kStaged> x;
+  x.g = static_cast<const T*>(A.logits) + int64_t(row) * A.stride;
+  const uint32_t run = ((V + C - 1) / C + 7) & ~7u;
+  x.lo = min(rank * run, V);
+  x.n = min(run, V - x.lo);
+
+  // ---- the maximum, and the part into shared memory: 16 bytes at a time, at the
+  // same offset from a 16-byte boundary in both memories
+  float top = -INFINITY;
+  if (kStaged) {
+    constexpr uint32_t kPer = 16 / sizeof(T);
+    const T* src = x.g + x.lo;
+    const uint32_t pad = uint32_t(reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T);
+    T* dst = reinterpret_cast<T*>(raw + ((sizeof(Shared) + 15) & ~size_t(15)));
+    x.s = dst + pad;
+    const uint32_t vecs = (pad + x.n + kPer - 1) / kPer;
+    const uint4* from = reinterpret_cast<const uint4*>(src - pad);
+#pragma unroll 4
+    for (uint32_t v = tid; v < vecs; v += kThreads) {
+      if (v * kPer >= pad && (v + 1) * kPer <= pad + x.n) {
+        const uint4 w = __ldg(from + v);
+        reinterpret_cast<uint4*>(dst)[v] = w;
+        const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-  for (int d = 16; d; d /= 2) {
-    const unsigned long long o = __shfl_xor_sync(~0u, best, d);
-    best = o > best ? o : best;
+        for (uint32_t i = 0; i < kPer; ++i) top = fmaxf(top, to_f<T>(e[i]));  // not NaN's
+      } else {
+        for (uint32_t i = v * kPer; i < (v + 1) * kPer; ++i)
+          if (i >= pad && i < pad + x.n) {
+            const T e = src[i - pad];
+            dst[i] = e;
+            top = fmaxf(top, to_f<T>(e));
+          }
+      }
+    }
+  } else {
+    for (uint32_t j = tid; j < x.n; j += kThreads) top = fmaxf(top, x.at(j));
   }
-  if ((tid & 31) == 0) sh.sum[tid >> 5] = best;
+  for (int b = tid; b < kBins; b += kThreads) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
+#pragma unroll
+  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  if (lane == 0) sh.red2[warp] = __float_as_uint(top);
   __syncthreads();
-  best = sh.sum[tid & 31];
+  top = __uint_as_float(sh.red2[lane % kWarps]);
 #pragma unroll
-  for (int d = 16; d; d /= 2) {
-    const unsigned long long o = __shfl_xor_sync(~0u, best, d);
-    best = o > best ? o : best;
-  }
-  const uint32_t top_key = uint32_t(best >> 32), first = ~uint32_t(best);
-  const float top = value_of(top_key);
-  if (top == -INFINITY || !(temp > 0.f)) {
-    if (tid == 0) {
-      A.tokens[row] = top == -INFINITY ? -1 : int32_t(first);
+  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  if (tid == 0) sh.top = top;
+  cluster.sync();
+  for (uint32_t r = 0; r < C; ++r) top = fmaxf(top, *of(&sh.top, r));
+  top += 0.f;
+
+  if (top == -INFINITY || !(temp > 0.f)) {  // the first of the largest, or none
+    u64 best = 0;
+    for (uint32_t j = tid; j < x.n; j += kThreads) {
+      const u64 c = place_of(x.at(j), x.lo + j);
+      best = c > best ? c : best;
+    }
+    best = warp_max(best);
+    if (lane == 0) sh.red[warp] = best;
+    __syncthreads();
+    best = warp_max(sh.red[lane % kWarps]);
+    if (tid == 0) sh.first = best;
+    cluster.sync();
+    for (uint32_t r = 0; r < C; ++r) best = max(best, *of(&sh.first, r));
+    if (rank == 0 && tid == 0) {
+      A.tokens[row] = top == -INFINITY ? -1 : int32_t(~uint32_t(best));
       A.logprobs[row] = top == -INFINITY ? -INFINITY : 0.f;
     }
+    cluster.sync();
     return;
   }
 
-  // threshold (key, ties): keys above it are kept, and `ties` of those equal to it
-  uint32_t key = 0, ties = 0xffffffffu;
-  const int k = A.top_k ? A.top_k[row] : 0;
-  const float p = A.top_p ? A.top_p[row] : 1.f, mp = A.min_p ? A.min_p[row] : 0.f;
-  const bool only_first = (A.top_p && !(p > 0.f)) || (A.min_p && !(mp <= 1.f));
-  for (int pass = 0; pass < 2 && !only_first; ++pass) {
-    const bool by_mass = pass == 1;
-    if (by_mass ? !(A.top_p && p < 1.f) : !(k > 0 && uint32_t(k) < V)) continue;
-    double want = double(k);
-    if (by_mass) {
-      unsigned long long mine = 0, total, tie_mass = 0;
-      uint32_t n_ties = 0;
-      for (uint32_t i = tid; i < V; i += kThreads) {
-        const uint32_t kk = key_of(value<T>(x, i));
-        if (kk > key) mine += mass_of(expf(scaled(value_of(kk), top, temp)));
-        n_ties += kk == key;
-      }
-      block_scan(mine, sh, &total);
-      if (ties == 0xffffffffu) {
-        block_scan(n_ties, sh, &tie_mass);
-      } else {
-        tie_mass = ties;
-      }
-      total += tie_mass * mass_of(expf(scaled(value_of(key), top, temp)));
-      want = double(p) * double(total);
-    }
-    if (tid == 0) sh.before = 0, sh.prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) sh.count[tid] = 0, sh.mass[tid] = 0;
-      __syncthreads();
-      const uint32_t prefix = sh.prefix;
-      for (uint32_t i = tid; i < V; i += kThreads) {
-        const uint32_t kk = key_of(value<T>(x, i));
-        if (kk < key || (shift < 24 && (kk ^ prefix) >> (shift + 8))) continue;
-        const uint32_t d = (kk >> shift) & 255u;
-        atomicAdd(&sh.count[d], 1u);
-        if (by_mass)
-          atomicAdd(&sh.mass[d], (unsigned long long)mass_of(expf(scaled(value_of(kk), top, temp))));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        // the last digit, from the top, that something before `want` falls in
-        unsigned long long acc = sh.before, at = acc;
-        int last = -1;
-        for (int d = 255; d >= 0; --d) {
-          if (!sh.count[d]) continue;
-          if (last >= 0 && !(double(acc) < want)) break;
-          last = d;
-          at = acc;
-          acc += by_mass ? sh.mass[d] : sh.count[d];
-        }
-        sh.before = at;
-        sh.prefix = prefix | uint32_t(last) << shift;
-        sh.ties = sh.count[last];
-      }
-      __syncthreads();
-    }
-    // of the equal ones, those with less than `want` before them
-    const uint32_t found = sh.prefix;
-    const unsigned long long each =
-        by_mass ? mass_of(expf(scaled(value_of(found), top, temp))) : 1ull;
-    uint32_t n = min(sh.ties, found == key ? ties : 0xffffffffu);
-    if (each) {
-      uint32_t lo = 1, hi = n;  // the largest n with before + (n - 1) each < want
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (double(sh.before + (unsigned long long)(mid - 1) * each) < want) lo = mid;
-        else hi = mid - 1;
-      }
-      n = lo;
-    }
-    key = found;
-    ties = n;
-    __syncthreads();
-  }
-  if (only_first) key = top_key, ties = 1;
-
-  // total of the kept masses, then the token
-  auto walk = [&](unsigned long long target, bool find) -> unsigned long long {
-    unsigned long long sum = 0;
-    uint32_t seen = 0;
-    for (uint32_t i0 = 0; i0 < V; i0 += kThreads) {
-      const uint32_t i = i0 + tid;
-      const uint32_t kk = i < V ? key_of(value<T>(x, i)) : 0;
-      unsigned long long tot;
-      const bool tie = i < V && kk == key;
-      uint32_t rank = 0;
-      if (ties != 0xffffffffu) {
-        rank = seen + uint32_t(block_scan(tie, sh, &tot));
-        seen += uint32_t(tot);
-      }
-      const float w = i < V ? expf(scaled(value_of(kk), top, temp)) : 0.f;
-      const bool keep = i < V && (kk > key || (tie && rank < ties)) && (kk == top_key || !(w < mp));
-      const unsigned long long mass = keep ? mass_of(w) : 0;
-      const unsigned long long at = sum + block_scan(mass, sh, &tot);
-      sum += tot;
-      if (find && at <= target && target < at + mass) sh.found = int(i);
-      if (find && sum > target) break;
-    }
-    return sum;
+  // ---- one histogram: the bins, then a slice of the merged ones in each CTA
+  const float to_bin = kBins / (22.5f * temp);  // exp(-22.5) 2^31 < 1/2: mass 0 from there
+  auto bin_of = [&](float v) {
+    if (v == top) return 0;
+    const float d = (top - v) * to_bin;
+    return d < float(kBins) ? int(d) : kBins;  // even where d is NaN
   };
-  const unsigned long long total = walk(0, false);
-  const double at = double(A.uniform[row]) * double(total);
-  unsigned long long target = at > 0. ? (unsigned long long)at : 0;
-  if (target >= total) target = total - 1;
-  walk(target, true);
-  __syncthreads();
-  if (tid == 0) {
-    const float z = scaled(value_of(key_of(value<T>(x, uint32_t(sh.found)))), top, temp);
-    A.tokens[row] = sh.found;
-    A.logprobs[row] = z - logf(__ull2float_rn(total) * 4.656612873077393e-10f);
+  // Adds a token to a bin; lanes that all name one bin add once.
+  auto tally = [&](int bin, uint32_t mass) {
+    const uint32_t on = __activemask();
+    int same;
+    __match_all_sync(on, bin, &same);
+    if (same) {
+      const uint32_t lo = __reduce_add_sync(on, mass & 0xffffu);
+      const uint32_t hi = __reduce_add_sync(on, mass >> 16);
+      if (lane == __ffs(on) - 1) {
+        atomicAdd(&sh.count[bin], __popc(on));
+        atomicAdd(&sh.lo[bin], lo);
+        atomicAdd(&sh.hi[bin], hi);
+      }
+    } else {
+      atomicAdd(&sh.count[bin], 1u);
+      if (mass) {
+        atomicAdd(&sh.lo[bin], mass & 0xffffu);
+        atomicAdd(&sh.hi[bin], mass >> 16);
+      }
+    }
+  };
+  // This CTA's slice of the merged histogram: kBins / C neighbouring bins, kEach in
+  // each of the first threads.
+  const uint32_t slice = kBins / C;
+  constexpr int kEach = kBins / kThreads;
+  uint32_t bc[kEach];
+  u64 bm[kEach];
+  auto merge = [&]() {  // call between cluster barriers
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) bc[e] = 0, bm[e] = 0;
+    if (uint32_t(tid) * kEach < slice) {
+      const uint32_t b = rank * slice + tid * kEach;
+      for (uint32_t r = 0; r < C; ++r) {
+        const uint32_t* c = of(sh.count, r) + b;
+        const uint32_t* l = of(sh.lo, r) + b;
+        const uint32_t* h = of(sh.hi, r) + b;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) bc[e] += c[e], bm[e] += u64(l[e]) + (u64(h[e]) << 16);
+      }
+    }
+  };
+  // Exclusive prefix of a thread's bins over the CTA, counts and masses; totals to
+  // slice_count / slice_mass.
+  uint32_t pc = 0;
+  u64 pm = 0;
+  auto prefix = [&]() {
+    uint32_t c = 0;
+    u64 m = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) c += bc[e], m += bm[e];
+    uint32_t ic = c;
+    u64 im = m;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const uint32_t yc = __shfl_up_sync(~0u, ic, d);
+      const u64 ym = __shfl_up_sync(~0u, im, d);
+      if (lane >= d) ic += yc, im += ym;
+    }
+    __syncthreads();
+    if (lane == 31) sh.red2[warp] = ic, sh.red[warp] = im;
+    __syncthreads();
+    pc = ic - c, pm = im - m;
+    for (int w = 0; w < warp; ++w) pc += sh.red2[w], pm += sh.red[w];
+    if (tid == kThreads - 1) sh.slice_count = pc + c, sh.slice_mass = pm + m;
+  };
+  // The last bin with tokens before which there is less than `want` (tokens or
+  // mass), told to every CTA. Bins are merged and slice totals are out; `base_*`
+  // are before the first bin, `members` are all tokens in question.
+  auto pick = [&](bool by_mass, double want, uint32_t base_count, u64 base_mass, uint32_t members,
+                  bool past) {
+    uint32_t c = base_count, inside = 0;
+    u64 m = base_mass, all_mass = 0;
+    for (uint32_t r = 0; r < C; ++r) {
+      const uint32_t sc = *of(&sh.slice_count, r);
+      const u64 sm = *of(&sh.slice_mass, r);
+      if (r < rank) c += sc, m += sm;
+      inside += sc, all_mass += sm;
+    }
+    c += pc, m += pm;
+    // this thread's last bin that qualifies, if the next qualifying one is not after
+    int hit = -1;
+    Cut cut{};
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      if (bc[e] && (by_mass ? double(m) : double(c)) < want) {
+        hit = e;
+        cut = {int(rank * slice) + tid * kEach + e, bc[e], c, m};
+      }
+      c += bc[e], m += bm[e];
+    }
+    // it is the last one if what comes after all of its bin does not qualify, or
+    // nothing comes after
+    const bool ends = hit >= 0 && [&] {
+      const uint32_t ac = cut.before + cut.count;
+      u64 am = cut.mass_before;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) am += e == hit ? bm[e] : 0;
+      const bool more = (by_mass ? double(am) : double(ac)) < want;
+      return !more || ac == base_count + inside;
+    }();
+    const bool beyond = past && base_count + inside < members &&
+                        (by_mass ? double(base_mass + all_mass) : double(base_count + inside)) < want;
+    if (ends && !beyond)
+      for (uint32_t r = 0; r < C; ++r) *of(&sh.cut, r) = cut;
+    if (beyond && tid == 0)
+      sh.cut = {kBins, members - base_count - inside, base_count + inside, base_mass + all_mass};
+    if (tid == 0) sh.gathered = 0;
+    cluster.sync();
+    return sh.cut;
+  };
+  // The threshold: the last token, in the order, before which there is less than
+  // `want`, among those of a cut, which `in(value, place)` tells. *mass: of all up
+  // to and with it.
+  auto resolve = [&](bool by_mass, double want, Cut cut, auto in0, u64* mass) -> u64 {
+    u64 low = 0, high = ~0ull;  // once the cut has been split: its range of places
+    bool split = false;
+    auto in = [&](float v, u64 c) { return split ? c >= low && c <= high : in0(v); };
+    while (cut.count > uint32_t(kMost)) {
+      if (!split) {  // the range of the cut
+        u64 least = 0, most = 0;  // as maxima of ~c and c
+        for (uint32_t j = tid; j < x.n; j += kThreads) {
+          const float v = x.at(j);
+          const u64 c = place_of(v, x.lo + j);
+          if (in(v, c)) least = max(least, ~c), most = max(most, c);
+        }
+        least = warp_max(least), most = warp_max(most);
+        __syncthreads();
+        if (lane == 0) sh.mine[warp] = least, sh.mine[kWarps + warp] = most;
+        __syncthreads();
+        least = warp_max(sh.mine[lane % kWarps]), most = warp_max(sh.mine[kWarps + lane % kWarps]);
+        if (tid == 0) sh.range[0] = least, sh.range[1] = most;
+        cluster.sync();
+        for (uint32_t r = 0; r < C; ++r)
+          least = max(least, of(sh.range, r)[0]), most = max(most, of(sh.range, r)[1]);
+        low = ~least, high = most;
+        split = true;
+      }
+      int shift = 0;
+      while ((high - low) >> shift >= u64(kBins)) ++shift;
+      cluster.sync();  // the histograms have been read
+      for (int b = tid; b < kBins; b += kThreads) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
+      __syncthreads();
+      for (uint32_t j = tid; j < x.n; j += kThreads) {
+        const float v = x.at(j);
+        const u64 c = place_of(v, x.lo + j);
+        if (c >= low && c <= high) tally(int((high - c) >> shift), mass_of(v, top, temp));
+      }
+      cluster.sync();
+      merge();
+      prefix();
+      cluster.sync();
+      cut = pick(by_mass, want, cut.before, cut.mass_before, 0, false);
+      const u64 up = high - (u64(cut.bin) << shift);
+      const u64 down = (u64(1) << shift) - 1;
+      low = up - low < down ? low : up - down;
+      high = up;
+    }
+    for (uint32_t j = tid; j < x.n; j += kThreads) {
+      const float v = x.at(j);
+      const u64 c = place_of(v, x.lo + j);
+      if (in(v, c)) sh.mine[atomicAdd(&sh.gathered, 1u)] = c;
+    }
+    cluster.sync();
+    uint32_t n = 0;
+    for (uint32_t r = 0; r < C; ++r) {
+      const uint32_t m = *of(&sh.gathered, r);
+      const u64* from = of(sh.mine, r);
+      for (uint32_t j = tid; j < m; j += kThreads) {
+        const u64 c = from[j];
+        sh.all[n + j] = c;
+        sh.mass[n + j] = mass_of(value_of(uint32_t(c >> 32)), top, temp);
+      }
+      n += m;
+    }
+    __syncthreads();
+    // the last one that stays is the one whose successor, in the order, does not
+    for (uint32_t j = tid; j < n; j += kThreads) {
+      const u64 c = sh.all[j];
+      uint32_t above = 0;
+      u64 mass_above = 0;
+      for (uint32_t i = 0; i < n; ++i)
+        if (sh.all[i] > c) ++above, mass_above += sh.mass[i];
+      const u64 m0 = cut.mass_before + mass_above, m1 = m0 + sh.mass[j];
+      const uint32_t c0 = cut.before + above;
+      const bool stays = (by_mass ? double(m0) : double(c0)) < want;
+      const bool next = above + 1 < n && (by_mass ? double(m1) : double(c0 + 1)) < want;
+      if (stays && !next) sh.found = c, sh.found_mass = m1;
+    }
+    __syncthreads();
+    *mass = sh.found_mass;
+    return sh.found;
+  };
+
+  u64 least = 0;  // what stays: places from here up
+  const bool only_first = (A.top_p && !(p > 0.f)) || (A.min_p && !(mp <= 1.f));
+  const bool by_count = k > 0 && uint32_t(k) < V, by_mass = A.top_p && p < 1.f;
+  if (only_first) {
+    least = ~0ull;
+  } else if (by_count || by_mass) {
+    for (uint32_t j = tid; j < x.n; j += kThreads) {
+      const float v = x.at(j);
+      const int b = bin_of(v);
+      if (b < kBins) tally(b, mass_of(v, top, temp));
+    }
+    cluster.sync();
+    merge();
+    prefix();
+    cluster.sync();
+    u64 total = 0;
+    for (uint32_t r = 0; r < C; ++r) total += *of(&sh.slice_mass, r);
+    if (by_count) {
+      // `resolve` may use the bins again
+      uint32_t oc[kEach], opc = pc;
+      u64 om[kEach], opm = pm;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) oc[e] = bc[e], om[e] = bm[e];
+      const uint32_t sc = sh.slice_count;
+      const u64 sm = sh.slice_mass;
+      const Cut cut = pick(false, double(k), 0, 0, V, true);
+      least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &total);
+      if (by_mass) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) bc[e] = oc[e], bm[e] = om[e];
+        pc = opc, pm = opm;
+        cluster.sync();  // lists and totals have been read
+        if (tid == 0) sh.slice_count = sc, sh.slice_mass = sm;
+        cluster.sync();
+      }
+    }
+    if (by_mass) {
+      const double want = double(p) * double(total);
+      const Cut cut = pick(true, want, 0, 0, V, false);
+      u64 m;
+      least = max(least, resolve(true, want, cut, [&](float v) { return bin_of(v) == cut.bin; }, &m));
+    }
   }
+
+  // ---- the kept mass: each warp a run of neighbouring tokens
+  const u64 top_place = key_of(top);
+  auto kept = [&](uint32_t j) -> uint32_t {
+    const float v = x.at(j);
+    const u64 c = place_of(v, x.lo + j);
+    if (only_first ? (c >> 32) != top_place : c < least) return 0u;
+    const float w = expf(scaled(v, top, temp));
+    if (v != top && w < mp) return 0u;
+    return __float2uint_rn(w * 2147483648.f);
+  };
+  const uint32_t part = ((x.n + kWarps - 1) / kWarps + 31) & ~31u;
+  const uint32_t j0 = min(warp * part, x.n), j1 = min(j0 + part, x.n);
+  u64 sum = 0;
+  for (uint32_t j = j0 + lane; j < j1; j += 32) sum += kept(j);
+  sum = warp_sum(sum);
+  if (lane == 0) sh.red[warp] = sum;
+  __syncthreads();
+  u64 here = 0, before_warp = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before_warp += sh.red[w];
+    here += sh.red[w];
+  }
+  if (tid == 0) sh.kept = here;
+  cluster.sync();
+  u64 total = 0, before = 0;
+  for (uint32_t r = 0; r < C; ++r) {
+    const u64 v = *of(&sh.kept, r);
+    if (r < rank) before += v;
+    total += v;
+  }
+  // only_first: of the largest ones the first, whatever u
+  const double u = only_first ? 0. : double(A.uniform[row]) * double(total);
+  u64 target = u > 0. ? u64(u) : 0;
+  if (target >= total) target = total - 1;
+  before += before_warp;
+  if (target >= before && target < before + sum) {  // in this warp's run
+    for (uint32_t b = j0; b < j1; b += 32) {
+      const uint32_t j = b + lane;
+      const uint32_t m = j < j1 ? kept(j) : 0u;
+      u64 upto = m;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const u64 y = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const uint32_t over = __ballot_sync(~0u, before + upto > target);
+      if (over) {
+        if (lane == __ffs(over) - 1) {
+          A.tokens[row] = int32_t(x.lo + j);
+          const u64 all = only_first ? u64(1) << 31 : total;
+          A.logprobs[row] = scaled(x.at(j), top, temp) -
+                            logf(__ull2float_rn(all) * 4.656612873077393e-10f);
+        }
+        break;
+      }
+      before += __shfl_sync(~0u, upto, 31);
+    }
+  }
+  cluster.sync();  // no CTA leaves while another reads from it
+}
+
+template <typename T>
+FelixCode launch(const SampleArgs& a, DeviceInfo* dev, cudaStream_t stream) {
+  const size_t fixed = (sizeof(Shared) + 15) & ~size_t(15);
+  // As many CTAs per row as fill the GPU, at least so many that the row fits their
+  // shared memory, and none with less than 2048 tokens.
+  uint32_t C = 1;
+  const uint32_t want = uint32_t(dev->num_sms) * 2;
+  auto bytes = [&](uint32_t c) {
+    return fixed + (size_t(((a.vocab + c - 1) / c + 7) & ~7u) + 16) * sizeof(T);
+  };
+  while (C < kMaxCtas && ((a.rows * uint64_t(C) < want && a.vocab / C > 4096) ||
+                          bytes(C) > 72 * 1024))
+    C *= 2;
+  const bool staged = bytes(C) <= size_t(dev->max_smem_optin);
+  static PerDeviceOnce once;
+  const int rc = once.run(dev->ordinal, [&] {
+    return cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                dev->max_smem_optin) == cudaSuccess &&
+                   cudaFuncSetAttribute(sample_kernel<T, false>,
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        int(fixed)) == cudaSuccess
+               ? 0 : -1;
+  });
+  if (rc != 0) return launch_error(cudaGetLastError(), "sample: attributes");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows * C);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = staged ? bytes(C) : fixed;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = C;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = staged ? cudaLaunchKernelEx(&cfg, sample_kernel<T, true>, a)
+                               : cudaLaunchKernelEx(&cfg, sample_kernel<T, false>, a);
+  if (e != cudaSuccess) return launch_error(e, "sample");
+  return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
 }  // namespace smp
 
 FelixCode sample_launch(const SampleArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+  DeviceInfo* dev = current_device_info();
+  if (!dev) return launch_error(cudaGetLastError(), "sample: no device");
   switch (a.dtype) {
-    case FELIX_F16: smp::sample_kernel<__half><<<a.rows, smp::kThreads, 0, stream>>>(a); break;
-    case FELIX_BF16:
-      smp::sample_kernel<__nv_bfloat16><<<a.rows, smp::kThreads, 0, stream>>>(a);
-      break;
-    default: smp::sample_kernel<float><<<a.rows, smp::kThreads, 0, stream>>>(a); break;
+    case FELIX_F16: return smp::launch<__half>(a, dev, stream);
+    case FELIX_BF16: return smp::launch<__nv_bfloat16>(a, dev, stream);
+    default: return smp::launch<float>(a, dev, stream);
   }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return launch_error(e, "sample");
-  return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
 }  // namespace felix_impl

@@ -172,6 +172,21 @@ def test_sample_frequencies():
     assert (np.abs(got - N * w / w.sum()) <= 2).all()
 
 
+def test_sample_largest_vocabularies():
+    # fp32 rows that do not fit a cluster's shared memory, up to the limit
+    rng = np.random.default_rng(5)
+    for V in (400000, 524288):
+        x = (rng.standard_normal((2, V)) * 3).astype(np.float32)
+        u = rng.random(2).astype(np.float32)
+        for temp, k, p, mp in ((1.0, 300000, 0.99, None), (0.5, 40, 0.9, 0.01), (1.0, None, None, None)):
+            tok, lp = sample(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(),
+                             temperature=temp, top_k=k, top_p=p, min_p=mp)
+            for i in range(2):
+                check_row(x[i], float(u[i]), int(tok[i]), float(lp[i]), temp, k,
+                          None if p is None else float(np.float32(p)),
+                          None if mp is None else float(np.float32(mp)))
+
+
 def test_sample_refusals(felix):
     x, u = torch.zeros(2, 5, device="cuda"), torch.zeros(2, device="cuda")
     for text, call in [
@@ -181,6 +196,7 @@ def test_sample_refusals(felix):
             ("one entry per row", lambda: sample(x, u[:1])),
             ("top_k must be", lambda: sample(x, u, top_k=torch.ones(2, device="cuda"))),
             ("vocab", lambda: sample(x[:, :0], u)),
+            ("vocab must be 1..524288", lambda: sample(torch.zeros(2, 524289, device="cuda"), u)),
             ("temperature must be on", lambda: sample(x, u, temperature=torch.ones(2)))]:
         with pytest.raises(RuntimeError, match=text):
             call()
