@@ -18,13 +18,17 @@
 // on (value, index), held as one 64-bit number that is larger for what comes first.
 //
 // A cluster of CTAs shares a row, and each keeps its part in shared memory: the
-// logits are read from HBM once. The threshold of top-k (by count) and that of
-// top-p (by mass) come from one histogram over the distance from the maximum
-// (2048 bins up to where masses round to 0; even in value, so that few tokens
-// share a bin), merged over the cluster by slices. The tokens of the bin in which
-// the threshold falls, a few dozen as a rule, are gathered by every CTA and ranked
-// by comparison with one another. Where a bin holds too many (equal values, a flat
-// row) it is split again into 2048 by (value, index) until it does not.
+// logits are read from HBM once. Thresholds come from a histogram over the distance
+// from the maximum (2048 bins up to where masses round to 0; even in value, so that
+// few tokens share a bin), which every CTA merges for itself. Where a bin holds too
+// many (equal values, a flat row) it is split again into 2048 by (value, index)
+// until it does not.
+//   top-k of up to 1024 (with or without the others): tokens are counted only, no
+//   exponentials; those down to the bin in which the k-th falls go to the first CTA
+//   of the cluster, which sorts them and finishes alone.
+//   else: the bins' masses are summed too; the tokens of the bin in which top-p (or a
+//   large top-k) cuts, a few dozen as a rule, are gathered by every CTA and ranked by
+//   comparison with one another, and a last pass sums what stays.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -62,12 +66,25 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 __device__ __forceinline__ u64 place_of(float x, uint32_t i) { return u64(key_of(x)) << 32 | ~i; }
-__device__ __forceinline__ float scaled(float x, float top, float temp) {
-  return x == top ? 0.f : __fdiv_rn(x - top, temp);
-}
+// (x - top) / T, correctly rounded. With r = RN(1 / T), q = RN(d r) is within a unit
+// in the last place, d - q T is exact in one fused operation and q + r (d - q T)
+// rounds to the quotient (Markstein, "Computation of elementary functions on the IBM
+// RISC System/6000 processor", 1990); quotients near the ends of the range, where
+// the remainder is not exact, are divided.
+struct Scale {
+  float top, temp, rcp;
+  bool quick;  // T where no quotient that matters leaves the range
+  __device__ __forceinline__ float operator()(float x) const {
+    if (x == top) return 0.f;
+    const float d = x - top;
+    const float q = d * rcp;
+    if (quick && q < -1e-20f && q > -1e20f) return fmaf(rcp, fmaf(-q, temp, d), q);
+    return __fdiv_rn(d, temp);
+  }
+};
 // expf, not an approximation: the masses are part of the definition.
-__device__ __forceinline__ uint32_t mass_of(float x, float top, float temp) {
-  return __float2uint_rn(expf(scaled(x, top, temp)) * 2147483648.f);
+__device__ __forceinline__ uint32_t mass_of(float x, const Scale& z) {
+  return __float2uint_rn(expf(z(x)) * 2147483648.f);
 }
 
 struct Cut {  // a bin in which a threshold falls
@@ -76,21 +93,29 @@ struct Cut {  // a bin in which a threshold falls
   u64 mass_before;
 };
 
+constexpr uint32_t kFew = 1024;  // the largest top-k that one CTA finishes
+constexpr int kList = 2048;      // tokens that it sorts
+
 struct Shared {
   // Tokens of a bin, and their masses as sums of the low 16 and of the high bits: 32
   // bits hold those of 65536 tokens, the most that a CTA has (vocab <= 8 * 65536).
-  uint32_t count[kBins], lo[kBins], hi[kBins];
+  alignas(16) uint32_t count[kBins];
+  union {
+    struct {
+      uint32_t lo[kBins], hi[kBins];
+    };
+    u64 list[kList];  // in the first CTA: tokens of a small top-k
+  };
   u64 mine[kMost], all[kMost];
   uint32_t mass[kMost];
   u64 red[kWarps];
   uint32_t red2[kWarps];
+  Cut cut;
+  u64 found, found_mass;  // of a ranking
   // for the other CTAs of the cluster
   float top;
-  u64 slice_mass, kept, first, range[2];
-  uint32_t slice_count, gathered;
-  Cut cut;
-  u64 found;  // (threshold) of a ranking
-  u64 found_mass;
+  u64 kept, first, range[2];
+  uint32_t gathered;
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -105,6 +130,24 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
     v = o > v ? o : v;
   }
   return v;
+}
+
+// Sorts a[0 .. n - 1] in shared memory (bitonic; a has room for the next power of two).
+__device__ __forceinline__ void sort(u64* a, uint32_t n, bool descending) {
+  uint32_t size = 2;
+  while (size < n) size *= 2;
+  const u64 pad = descending ? 0 : ~0ull;
+  for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) a[i] = pad;
+  __syncthreads();
+  for (uint32_t k = 2; k <= size; k *= 2)
+    for (uint32_t j = k / 2; j; j /= 2) {
+      for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
+        const uint32_t i = 2 * t - (t & (j - 1)), o = i + j;
+        const u64 x = a[i], y = a[o];
+        if ((x < y) == (((i & k) == 0) == descending) && x != y) a[i] = y, a[o] = x;
+      }
+      __syncthreads();
+    }
 }
 
 // A row's part in one CTA: tokens lo .. lo + n - 1. Staged: in shared memory, else
@@ -203,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     return;
   }
 
-  // ---- one histogram: the bins, then a slice of the merged ones in each CTA
+  // ---- the histogram
+  const Scale z = {top, temp, __frcp_rn(temp), temp > 1e-10f && temp < 1e10f};
   const float to_bin = kBins / (22.5f * temp);  // exp(-22.5) 2^31 < 1/2: mass 0 from there
   auto bin_of = [&](float v) {
     if (v == top) return 0;
@@ -231,33 +275,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       }
     }
   };
-  // This CTA's slice of the merged histogram: kBins / C neighbouring bins, kEach in
-  // each of the first threads.
-  const uint32_t slice = kBins / C;
+  // The merged histogram: each thread's kEach neighbouring bins, and what is before
+  // them. Call between cluster barriers. Masses are left out where none were summed.
   constexpr int kEach = kBins / kThreads;
-  uint32_t bc[kEach];
-  u64 bm[kEach];
-  auto merge = [&]() {  // call between cluster barriers
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) bc[e] = 0, bm[e] = 0;
-    if (uint32_t(tid) * kEach < slice) {
-      const uint32_t b = rank * slice + tid * kEach;
-      for (uint32_t r = 0; r < C; ++r) {
-        const uint32_t* c = of(sh.count, r) + b;
-        const uint32_t* l = of(sh.lo, r) + b;
-        const uint32_t* h = of(sh.hi, r) + b;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) bc[e] += c[e], bm[e] += u64(l[e]) + (u64(h[e]) << 16);
-      }
-    }
-  };
-  // Exclusive prefix of a thread's bins over the CTA, counts and masses; totals to
-  // slice_count / slice_mass.
-  uint32_t pc = 0;
-  u64 pm = 0;
-  auto prefix = [&]() {
+  static_assert(kEach == 4, "bins are read as vectors of four");
+  uint32_t bc[kEach], pc = 0, tokens = 0;
+  u64 bm[kEach], pm = 0, masses = 0;
+  auto merge = [&](bool with_mass) {
     uint32_t c = 0;
     u64 m = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) bc[e] = 0, bm[e] = 0;
+    for (uint32_t r = 0; r < C; ++r) {
+      const uint4 v = reinterpret_cast<const uint4*>(of(sh.count, r))[tid];
+      bc[0] += v.x, bc[1] += v.y, bc[2] += v.z, bc[3] += v.w;
+      if (!with_mass) continue;
+      const uint4 l = reinterpret_cast<const uint4*>(of(sh.lo, r))[tid];
+      const uint4 h = reinterpret_cast<const uint4*>(of(sh.hi, r))[tid];
+      bm[0] += l.x + (u64(h.x) << 16), bm[1] += l.y + (u64(h.y) << 16);
+      bm[2] += l.z + (u64(h.z) << 16), bm[3] += l.w + (u64(h.w) << 16);
+    }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) c += bc[e], m += bm[e];
     uint32_t ic = c;
@@ -271,53 +308,37 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     __syncthreads();
     if (lane == 31) sh.red2[warp] = ic, sh.red[warp] = im;
     __syncthreads();
-    pc = ic - c, pm = im - m;
-    for (int w = 0; w < warp; ++w) pc += sh.red2[w], pm += sh.red[w];
-    if (tid == kThreads - 1) sh.slice_count = pc + c, sh.slice_mass = pm + m;
+    pc = ic - c, pm = im - m, tokens = 0, masses = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) pc += sh.red2[w], pm += sh.red[w];
+      tokens += sh.red2[w], masses += sh.red[w];
+    }
   };
-  // The last bin with tokens before which there is less than `want` (tokens or
-  // mass), told to every CTA. Bins are merged and slice totals are out; `base_*`
-  // are before the first bin, `members` are all tokens in question.
-  auto pick = [&](bool by_mass, double want, uint32_t base_count, u64 base_mass, uint32_t members,
-                  bool past) {
-    uint32_t c = base_count, inside = 0;
-    u64 m = base_mass, all_mass = 0;
-    for (uint32_t r = 0; r < C; ++r) {
-      const uint32_t sc = *of(&sh.slice_count, r);
-      const u64 sm = *of(&sh.slice_mass, r);
-      if (r < rank) c += sc, m += sm;
-      inside += sc, all_mass += sm;
-    }
-    c += pc, m += pm;
-    // this thread's last bin that qualifies, if the next qualifying one is not after
-    int hit = -1;
-    Cut cut{};
+  // The last bin with tokens before which there is less than `want` (tokens or mass),
+  // of the merged ones, with base_* before the first; of `members` tokens those past
+  // the bins count as one more bin.
+  auto pick = [&](bool by_mass, double want, uint32_t base_count, u64 base_mass,
+                  uint32_t members) -> Cut {
+    uint32_t c = base_count + pc;
+    u64 m = base_mass + pm;
+    const uint32_t inside = base_count + tokens;
+    const bool beyond = inside < members &&
+                        (by_mass ? double(base_mass + masses) : double(inside)) < want;
+    if (tid == 0 && beyond) sh.cut = {kBins, members - inside, inside, base_mass + masses};
+    if (!beyond) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      if (bc[e] && (by_mass ? double(m) : double(c)) < want) {
-        hit = e;
-        cut = {int(rank * slice) + tid * kEach + e, bc[e], c, m};
+      for (int e = 0; e < kEach; ++e) {
+        const uint32_t ac = c + bc[e];
+        const u64 am = m + bm[e];
+        // it qualifies, and what comes after it does not or is nothing
+        if (bc[e] && (by_mass ? double(m) : double(c)) < want &&
+            (!((by_mass ? double(am) : double(ac)) < want) || ac == inside))
+          sh.cut = {tid * kEach + e, bc[e], c, m};
+        c = ac, m = am;
       }
-      c += bc[e], m += bm[e];
     }
-    // it is the last one if what comes after all of its bin does not qualify, or
-    // nothing comes after
-    const bool ends = hit >= 0 && [&] {
-      const uint32_t ac = cut.before + cut.count;
-      u64 am = cut.mass_before;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) am += e == hit ? bm[e] : 0;
-      const bool more = (by_mass ? double(am) : double(ac)) < want;
-      return !more || ac == base_count + inside;
-    }();
-    const bool beyond = past && base_count + inside < members &&
-                        (by_mass ? double(base_mass + all_mass) : double(base_count + inside)) < want;
-    if (ends && !beyond)
-      for (uint32_t r = 0; r < C; ++r) *of(&sh.cut, r) = cut;
-    if (beyond && tid == 0)
-      sh.cut = {kBins, members - base_count - inside, base_count + inside, base_mass + all_mass};
     if (tid == 0) sh.gathered = 0;
-    cluster.sync();
+    __syncthreads();
     return sh.cut;
   };
   // The threshold: the last token, in the order, before which there is less than
@@ -355,13 +376,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       for (uint32_t j = tid; j < x.n; j += kThreads) {
         const float v = x.at(j);
         const u64 c = place_of(v, x.lo + j);
-        if (c >= low && c <= high) tally(int((high - c) >> shift), mass_of(v, top, temp));
+        if (c >= low && c <= high) tally(int((high - c) >> shift), mass_of(v, z));
       }
       cluster.sync();
-      merge();
-      prefix();
-      cluster.sync();
-      cut = pick(by_mass, want, cut.before, cut.mass_before, 0, false);
+      merge(true);
+      cut = pick(by_mass, want, cut.before, cut.mass_before, 0);
       const u64 up = high - (u64(cut.bin) << shift);
       const u64 down = (u64(1) << shift) - 1;
       low = up - low < down ? low : up - down;
@@ -372,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       const u64 c = place_of(v, x.lo + j);
       if (in(v, c)) sh.mine[atomicAdd(&sh.gathered, 1u)] = c;
     }
-    cluster.sync();
+    cluster.sync();  // histograms have been read too
     uint32_t n = 0;
     for (uint32_t r = 0; r < C; ++r) {
       const uint32_t m = *of(&sh.gathered, r);
@@ -380,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       for (uint32_t j = tid; j < m; j += kThreads) {
         const u64 c = from[j];
         sh.all[n + j] = c;
-        sh.mass[n + j] = mass_of(value_of(uint32_t(c >> 32)), top, temp);
+        sh.mass[n + j] = mass_of(value_of(uint32_t(c >> 32)), z);
       }
       n += m;
     }
@@ -406,42 +425,131 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   u64 least = 0;  // what stays: places from here up
   const bool only_first = (A.top_p && !(p > 0.f)) || (A.min_p && !(mp <= 1.f));
   const bool by_count = k > 0 && uint32_t(k) < V, by_mass = A.top_p && p < 1.f;
+
+  if (by_count && uint32_t(k) <= kFew) {  // ---- a small top-k: the first CTA finishes
+    for (uint32_t j = tid; j < x.n; j += kThreads) {
+      const int b = bin_of(x.at(j));
+      if (b < kBins) atomicAdd(&sh.count[b], 1u);
+    }
+    cluster.sync();
+    merge(false);
+    const Cut cut = pick(false, double(k), 0, 0, V);
+    const bool fits = cut.before + cut.count <= uint32_t(kList);
+    if (!fits) {
+      u64 mass;
+      least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &mass);
+      cluster.sync();  // lists have been read
+      if (tid == 0) sh.gathered = 0;
+    }
+    cluster.sync();  // the counter and the list are free
+    uint32_t* counter = of(&sh.gathered, 0);
+    u64* list = of(sh.list, 0);
+    for (uint32_t j = tid; j < x.n; j += kThreads) {
+      const float v = x.at(j);
+      const u64 c = place_of(v, x.lo + j);
+      if (fits ? bin_of(v) <= cut.bin : c >= least) list[atomicAdd(counter, 1u)] = c;
+    }
+    cluster.sync();
+    if (rank != 0) return;
+    const uint32_t n = sh.gathered;
+    sort(sh.list, n, true);
+    // masses in the order, what stays of them, and those in the order of indexes
+    const uint32_t few = min(n, uint32_t(k));
+    u64 total = 0;
+    uint32_t m[2], stay = 0;
+    u64 upto[2];
+    auto scan2 = [&](const uint32_t (&m)[2]) {  // of the pairs 2 tid, 2 tid + 1
+      u64 v = u64(m[0]) + m[1];
+      const u64 own = v;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const u64 y = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh.red[warp] = v;
+      __syncthreads();
+      total = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) v += sh.red[w];
+        total += sh.red[w];
+      }
+      upto[0] = v - own;  // exclusive
+      upto[1] = upto[0] + m[0];
+    };
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = 2 * tid + e;
+      m[e] = i < few ? mass_of(value_of(uint32_t(sh.list[i] >> 32)), z) : 0u;
+    }
+    scan2(m);
+    const double want = double(p) * double(total);
+    u64 item[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = 2 * tid + e;
+      bool on = i < few && (!by_mass || double(upto[e]) < want);
+      if (on && A.min_p) on = !(expf(z(value_of(uint32_t(sh.list[i] >> 32)))) < mp);
+      if (only_first) on = false;
+      on |= i == 0;
+      item[e] = on ? u64(~uint32_t(sh.list[i])) << 32 | m[e] : ~0ull;
+      stay += on;
+    }
+    __syncthreads();
+    stay = uint32_t(__syncthreads_count(stay > 0)) + uint32_t(__syncthreads_count(stay > 1));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) sh.list[2 * tid + e] = item[e];
+    __syncthreads();
+    sort(sh.list, stay, false);  // what stays is a prefix: the first `stay`, by index
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      m[e] = 2 * tid + e < stay ? uint32_t(sh.list[2 * tid + e]) : 0u;
+    scan2(m);
+    const double u = double(A.uniform[row]) * double(total);
+    u64 target = u > 0. ? u64(u) : 0;
+    if (target >= total) target = total - 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (target >= upto[e] && target < upto[e] + m[e]) {
+        const uint32_t i = uint32_t(sh.list[2 * tid + e] >> 32);
+        const T* g = x.g;
+        A.tokens[row] = int32_t(i);
+        A.logprobs[row] =
+            z(plain(to_f<T>(g[i]))) - logf(__ull2float_rn(total) * 4.656612873077393e-10f);
+      }
+    return;
+  }
+
   if (only_first) {
     least = ~0ull;
   } else if (by_count || by_mass) {
     for (uint32_t j = tid; j < x.n; j += kThreads) {
       const float v = x.at(j);
       const int b = bin_of(v);
-      if (b < kBins) tally(b, mass_of(v, top, temp));
+      if (b < kBins) {
+        const uint32_t mass = mass_of(v, z);
+        atomicAdd(&sh.count[b], 1u);
+        atomicAdd(&sh.lo[b], mass & 0xffffu);
+        atomicAdd(&sh.hi[b], mass >> 16);
+      }
     }
     cluster.sync();
-    merge();
-    prefix();
-    cluster.sync();
-    u64 total = 0;
-    for (uint32_t r = 0; r < C; ++r) total += *of(&sh.slice_mass, r);
+    merge(true);
+    u64 total = masses;
     if (by_count) {
       // `resolve` may use the bins again
-      uint32_t oc[kEach], opc = pc;
-      u64 om[kEach], opm = pm;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) oc[e] = bc[e], om[e] = bm[e];
-      const uint32_t sc = sh.slice_count;
-      const u64 sm = sh.slice_mass;
-      const Cut cut = pick(false, double(k), 0, 0, V, true);
+      const uint32_t opc = pc, ot = tokens, oc[kEach] = {bc[0], bc[1], bc[2], bc[3]};
+      const u64 opm = pm, omass = masses, om[kEach] = {bm[0], bm[1], bm[2], bm[3]};
+      const Cut cut = pick(false, double(k), 0, 0, V);
       least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &total);
-      if (by_mass) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) bc[e] = oc[e], bm[e] = om[e];
-        pc = opc, pm = opm;
-        cluster.sync();  // lists and totals have been read
-        if (tid == 0) sh.slice_count = sc, sh.slice_mass = sm;
-        cluster.sync();
-      }
+      for (int e = 0; e < kEach; ++e) bc[e] = oc[e], bm[e] = om[e];
+      pc = opc, pm = opm, tokens = ot, masses = omass;
+      cluster.sync();  // lists have been read
     }
     if (by_mass) {
       const double want = double(p) * double(total);
-      const Cut cut = pick(true, want, 0, 0, V, false);
+      const Cut cut = pick(true, want, 0, 0, 0);
       u64 m;
       least = max(least, resolve(true, want, cut, [&](float v) { return bin_of(v) == cut.bin; }, &m));
     }
@@ -453,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     const float v = x.at(j);
     const u64 c = place_of(v, x.lo + j);
     if (only_first ? (c >> 32) != top_place : c < least) return 0u;
-    const float w = expf(scaled(v, top, temp));
+    const float w = expf(z(v));
     if (v != top && w < mp) return 0u;
     return __float2uint_rn(w * 2147483648.f);
   };
@@ -497,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
         if (lane == __ffs(over) - 1) {
           A.tokens[row] = int32_t(x.lo + j);
           const u64 all = only_first ? u64(1) << 31 : total;
-          A.logprobs[row] = scaled(x.at(j), top, temp) -
+          A.logprobs[row] = z(x.at(j)) -
                             logf(__ull2float_rn(all) * 4.656612873077393e-10f);
         }
         break;

@@ -187,6 +187,44 @@ def test_sample_largest_vocabularies():
                           None if mp is None else float(np.float32(mp)))
 
 
+def test_sample_quotients_are_correctly_rounded():
+    # two tokens, the second drawn (its mass is over 2^-24 of the total): its
+    # log-probability is q = (x1 - x0) / T less log(1 + exp(q)). q is in (8, 16),
+    # where a unit in the last place is 9.5e-7: with the last rounding of half of
+    # that, a quotient that is one unit off is seen
+    rng = np.random.default_rng(6)
+    n = 100000
+    t = np.exp(rng.uniform(-3, 3, n)).astype(np.float32)
+    z = rng.uniform(-15.9, -8.1, n)
+    x = np.stack([np.zeros(n), z * t], 1).astype(np.float32)
+    u = np.full(n, 1 - 2.0 ** -24, np.float32)
+    tok, lp = sample(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(),
+                     temperature=torch.from_numpy(t).cuda())
+    drawn = tok.cpu().numpy() == 1
+    q = x[:, 1] / t
+    assert drawn.all()
+    q = q.astype(np.float64)
+    np.testing.assert_allclose(lp.cpu().numpy(), q - np.log1p(np.exp(q)), rtol=0, atol=5.5e-7)
+
+
+@pytest.mark.parametrize("V", [1500, 30000, 131072])
+@pytest.mark.parametrize("k", [1, 2, 63, 64, 65, 1023, 1024, 1025, 5000])
+def test_sample_top_k_around_the_limits(V, k):
+    rng = np.random.default_rng(V + k)
+    for x in (rng.standard_normal((2, V)), np.round(rng.standard_normal((2, V)) * 2),
+              np.repeat([[0.0], [-np.inf]], V, 1) + (np.arange(V) == 7)):
+        x = x.astype(np.float32)
+        x[1, 7] = 1.0
+        u = rng.random(2).astype(np.float32)
+        for p, mp in ((None, None), (0.7, None), (0.9, 0.1)):
+            tok, lp = sample(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(),
+                             temperature=0.9, top_k=k, top_p=p, min_p=mp)
+            for i in range(2):
+                check_row(x[i], float(u[i]), int(tok[i]), float(lp[i]), float(np.float32(0.9)), k,
+                          None if p is None else float(np.float32(p)),
+                          None if mp is None else float(np.float32(mp)))
+
+
 def test_sample_refusals(felix):
     x, u = torch.zeros(2, 5, device="cuda"), torch.zeros(2, device="cuda")
     for text, call in [
