@@ -27,8 +27,8 @@
 //   exponentials; those down to the bin in which the k-th falls go to the first CTA
 //   of the cluster, which sorts them and finishes alone.
 //   else: the bins' masses are summed too; the tokens of the bin in which top-p (or a
-//   large top-k) cuts, a few dozen as a rule, are gathered by every CTA and ranked by
-//   comparison with one another, and a last pass sums what stays.
+//   large top-k) cuts, a few dozen as a rule, are gathered and sorted by every CTA, and a last
+//   pass sums what stays.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -44,7 +44,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCtas = 8;
-constexpr int kMost = 1024;  // tokens that are ranked by comparison
+constexpr int kMost = 1024;  // tokens of a bin that are sorted: two per thread
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -65,7 +65,9 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-__device__ __forceinline__ u64 place_of(float x, uint32_t i) { return u64(key_of(x)) << 32 | ~i; }
+__device__ __forceinline__ u64 place_of(float x, uint32_t i) {
+  return u64(key_of(plain(x))) << 32 | ~i;
+}
 // (x - top) / T, correctly rounded. With r = RN(1 / T), q = RN(d r) is within a unit
 // in the last place, d - q T is exact in one fused operation and q + r (d - q T)
 // rounds to the quotient (Markstein, "Computation of elementary functions on the IBM
@@ -94,7 +96,7 @@ struct Cut {  // a bin in which a threshold falls
 };
 
 constexpr uint32_t kFew = 1024;  // the largest top-k that one CTA finishes
-constexpr int kList = 2048;      // tokens that it sorts
+constexpr int kList = 1024;      // tokens that it sorts
 
 struct Shared {
   // Tokens of a bin, and their masses as sums of the low 16 and of the high bits: 32
@@ -107,15 +109,14 @@ struct Shared {
     u64 list[kList];  // in the first CTA: tokens of a small top-k
   };
   u64 mine[kMost], all[kMost];
-  uint32_t mass[kMost];
   u64 red[kWarps];
   uint32_t red2[kWarps];
   Cut cut;
   u64 found, found_mass;  // of a ranking
   // for the other CTAs of the cluster
   float top;
-  u64 kept, first, range[2];
-  uint32_t gathered;
+  u64 kept, first, range[2], slice_mass[2][kMaxCtas];
+  uint32_t gathered, slice_count[2][kMaxCtas];  // [0] of the bins, [1] of a bin split again
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -132,22 +133,70 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
   return v;
 }
 
-// Sorts a[0 .. n - 1] in shared memory (bitonic; a has room for the next power of two).
+// Sorts a[0 .. n - 1], n <= 2 * kThreads, in shared memory: bitonic, one or two items
+// a thread in registers (tid and tid + kThreads), exchanged by shuffles inside a warp
+// and through `a` between warps.
 __device__ __forceinline__ void sort(u64* a, uint32_t n, bool descending) {
-  uint32_t size = 2;
+  const uint32_t tid = threadIdx.x;
+  uint32_t size = 32;
   while (size < n) size *= 2;
-  const u64 pad = descending ? 0 : ~0ull;
-  for (uint32_t i = n + threadIdx.x; i < size; i += kThreads) a[i] = pad;
-  __syncthreads();
-  for (uint32_t k = 2; k <= size; k *= 2)
-    for (uint32_t j = k / 2; j; j /= 2) {
-      for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
-        const uint32_t i = 2 * t - (t & (j - 1)), o = i + j;
-        const u64 x = a[i], y = a[o];
-        if ((x < y) == (((i & k) == 0) == descending) && x != y) a[i] = y, a[o] = x;
-      }
-      __syncthreads();
+  const u64 flip = descending ? ~0ull : 0;  // sorts a ^ flip upwards
+  u64 x[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    x[e] = tid + e * kThreads < n ? a[tid + e * kThreads] ^ flip : ~0ull;
+  const bool two = size > kThreads;
+  if (tid < size || two) {  // whole warps
+    for (uint32_t k = 2; k <= 32; k *= 2)
+      for (uint32_t j = k / 2; j; j /= 2)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (e && !two) break;
+          const u64 y = __shfl_xor_sync(~0u, x[e], j);
+          const bool low = ((tid & j) == 0) == (((tid + e * kThreads) & k) == 0);
+          x[e] = (x[e] < y) == low ? x[e] : y;
+        }
+  }
+  for (uint32_t k = 64; k <= size; k *= 2) {
+    uint32_t j = k / 2;
+    if (j == kThreads) {
+      const u64 lo = min(x[0], x[1]);
+      x[1] = max(x[0], x[1]);
+      x[0] = lo;
+      j /= 2;
     }
+    for (; j >= 32; j /= 2) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (tid + e * kThreads < size) a[tid + e * kThreads] = x[e];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t i = tid + e * kThreads;
+        if (i < size) {
+          const u64 y = a[i ^ j];
+          const bool low = ((i & j) == 0) == ((i & k) == 0);
+          x[e] = (x[e] < y) == low ? x[e] : y;
+        }
+      }
+    }
+    if (tid < size || two) {
+      for (j = 16; j; j /= 2)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (e && !two) break;
+          const u64 y = __shfl_xor_sync(~0u, x[e], j);
+          const bool low = ((tid & j) == 0) == (((tid + e * kThreads) & k) == 0);
+          x[e] = (x[e] < y) == low ? x[e] : y;
+        }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (tid + e * kThreads < size) a[tid + e * kThreads] = x[e] ^ flip;
+  __syncthreads();
 }
 
 // A row's part in one CTA: tokens lo .. lo + n - 1. Staged: in shared memory, else
@@ -157,8 +206,33 @@ struct Row {
   const T* g;     // the row
   const T* s;     // token lo in shared memory
   uint32_t lo, n;
+  uint32_t pad;   // s is this many elements past a 16-byte boundary
   __device__ __forceinline__ float at(uint32_t j) const {
     return plain(to_f<T>(kStaged ? s[j] : g[lo + j]));
+  }
+  // f(value, j) for the CTA's tokens, spread over its threads, 16 bytes at a time.
+  // Values come as they are: NaN and -0 among them.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    if constexpr (kStaged) {
+      constexpr uint32_t kPer = 16 / sizeof(T);
+      const uint4* from = reinterpret_cast<const uint4*>(s - pad);
+      const uint32_t vecs = (pad + n + kPer - 1) / kPer;
+      for (uint32_t v = threadIdx.x; v < vecs; v += kThreads) {
+        const uint4 w = from[v];
+        const T* e = reinterpret_cast<const T*>(&w);
+        const uint32_t j = v * kPer - pad;
+        if (v * kPer >= pad && (v + 1) * kPer <= pad + n) {
+#pragma unroll
+          for (uint32_t i = 0; i < kPer; ++i) f(to_f<T>(e[i]), j + i);
+        } else {
+          for (uint32_t i = 0; i < kPer; ++i)
+            if (j + i < n) f(to_f<T>(s[j + i]), j + i);  // j wraps below 0
+        }
+      }
+    } else {
+      for (uint32_t j = threadIdx.x; j < n; j += kThreads) f(to_f<T>(g[lo + j]), j);
+    }
   }
 };
 
@@ -190,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     const uint32_t pad = uint32_t(reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T);
     T* dst = reinterpret_cast<T*>(raw + ((sizeof(Shared) + 15) & ~size_t(15)));
     x.s = dst + pad;
+    x.pad = pad;
     const uint32_t vecs = (pad + x.n + kPer - 1) / kPer;
     const uint4* from = reinterpret_cast<const uint4*>(src - pad);
 #pragma unroll 4
@@ -227,10 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 
   if (top == -INFINITY || !(temp > 0.f)) {  // the first of the largest, or none
     u64 best = 0;
-    for (uint32_t j = tid; j < x.n; j += kThreads) {
-      const u64 c = place_of(x.at(j), x.lo + j);
-      best = c > best ? c : best;
-    }
+    x.each([&](float v, uint32_t j) { best = max(best, place_of(v, x.lo + j)); });
     best = warp_max(best);
     if (lane == 0) sh.red[warp] = best;
     __syncthreads();
@@ -275,25 +347,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       }
     }
   };
-  // The merged histogram: each thread's kEach neighbouring bins, and what is before
-  // them. Call between cluster barriers. Masses are left out where none were summed.
+  // The merged histogram, a slice of kBins / C neighbouring bins in each CTA, kEach
+  // in each of its first threads, and what is before them in the slice. (Reading all
+  // bins of all CTAs in each took longer than the two barriers of the slices: 17
+  // against 6 us with masses.) Masses are left out where none were summed.
   constexpr int kEach = kBins / kThreads;
   static_assert(kEach == 4, "bins are read as vectors of four");
-  uint32_t bc[kEach], pc = 0, tokens = 0;
-  u64 bm[kEach], pm = 0, masses = 0;
-  auto merge = [&](bool with_mass) {
+  const uint32_t slice = kBins / C;
+  uint32_t bc[kEach], pc = 0;
+  u64 bm[kEach], pm = 0;
+  auto merge = [&](bool with_mass, int which) {
+    cluster.sync();
     uint32_t c = 0;
     u64 m = 0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) bc[e] = 0, bm[e] = 0;
-    for (uint32_t r = 0; r < C; ++r) {
-      const uint4 v = reinterpret_cast<const uint4*>(of(sh.count, r))[tid];
-      bc[0] += v.x, bc[1] += v.y, bc[2] += v.z, bc[3] += v.w;
-      if (!with_mass) continue;
-      const uint4 l = reinterpret_cast<const uint4*>(of(sh.lo, r))[tid];
-      const uint4 h = reinterpret_cast<const uint4*>(of(sh.hi, r))[tid];
-      bm[0] += l.x + (u64(h.x) << 16), bm[1] += l.y + (u64(h.y) << 16);
-      bm[2] += l.z + (u64(h.z) << 16), bm[3] += l.w + (u64(h.w) << 16);
+    if (uint32_t(tid) * kEach < slice) {
+      const uint32_t at = (rank * slice) / kEach + tid;
+#pragma unroll
+      for (uint32_t r0 = 0; r0 < uint32_t(kMaxCtas); r0 += 4) {
+        uint4 v[4], l[4], h[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t r = r0 + i;
+          v[i] = l[i] = h[i] = make_uint4(0, 0, 0, 0);
+          if (r < C) {
+            v[i] = reinterpret_cast<const uint4*>(of(sh.count, r))[at];
+            if (with_mass) {
+              l[i] = reinterpret_cast<const uint4*>(of(sh.lo, r))[at];
+              h[i] = reinterpret_cast<const uint4*>(of(sh.hi, r))[at];
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          bc[0] += v[i].x, bc[1] += v[i].y, bc[2] += v[i].z, bc[3] += v[i].w;
+          bm[0] += l[i].x + (u64(h[i].x) << 16), bm[1] += l[i].y + (u64(h[i].y) << 16);
+          bm[2] += l[i].z + (u64(h[i].z) << 16), bm[3] += l[i].w + (u64(h[i].w) << 16);
+        }
+        if (r0 + 4 >= C) break;
+      }
     }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) c += bc[e], m += bm[e];
@@ -308,23 +401,35 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     __syncthreads();
     if (lane == 31) sh.red2[warp] = ic, sh.red[warp] = im;
     __syncthreads();
-    pc = ic - c, pm = im - m, tokens = 0, masses = 0;
+    pc = ic - c, pm = im - m;
+    uint32_t tokens = 0;
+    u64 masses = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) pc += sh.red2[w], pm += sh.red[w];
       tokens += sh.red2[w], masses += sh.red[w];
     }
+    if (tid < int(C)) {
+      *of(&sh.slice_count[which][rank], tid) = tokens;
+      *of(&sh.slice_mass[which][rank], tid) = masses;
+    }
+    cluster.sync();
   };
   // The last bin with tokens before which there is less than `want` (tokens or mass),
   // of the merged ones, with base_* before the first; of `members` tokens those past
-  // the bins count as one more bin.
-  auto pick = [&](bool by_mass, double want, uint32_t base_count, u64 base_mass,
+  // the bins count as one more bin. One CTA finds it and tells the others.
+  auto pick = [&](int which, bool by_mass, double want, uint32_t base_count, u64 base_mass,
                   uint32_t members) -> Cut {
-    uint32_t c = base_count + pc;
-    u64 m = base_mass + pm;
-    const uint32_t inside = base_count + tokens;
-    const bool beyond = inside < members &&
-                        (by_mass ? double(base_mass + masses) : double(inside)) < want;
-    if (tid == 0 && beyond) sh.cut = {kBins, members - inside, inside, base_mass + masses};
+    uint32_t c = base_count + pc, inside = base_count;
+    u64 m = base_mass + pm, masses = base_mass;
+    for (uint32_t r = 0; r < C; ++r) {
+      const uint32_t tokens = sh.slice_count[which][r];
+      const u64 mass = sh.slice_mass[which][r];
+      if (r < rank) c += tokens, m += mass;
+      inside += tokens, masses += mass;
+    }
+    const bool beyond = inside < members && (by_mass ? double(masses) : double(inside)) < want;
+    if (tid == 0 && rank == 0 && beyond)
+      for (uint32_t r = 0; r < C; ++r) *of(&sh.cut, r) = {kBins, members - inside, inside, masses};
     if (!beyond) {
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
@@ -333,13 +438,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
         // it qualifies, and what comes after it does not or is nothing
         if (bc[e] && (by_mass ? double(m) : double(c)) < want &&
             (!((by_mass ? double(am) : double(ac)) < want) || ac == inside))
-          sh.cut = {tid * kEach + e, bc[e], c, m};
+          for (uint32_t r = 0; r < C; ++r)
+            *of(&sh.cut, r) = {int(rank * slice) + tid * kEach + e, bc[e], c, m};
         c = ac, m = am;
       }
     }
     if (tid == 0) sh.gathered = 0;
-    __syncthreads();
+    cluster.sync();
     return sh.cut;
+  };
+  // Exclusive prefix of the masses of items 2 tid and 2 tid + 1.
+  auto scan2 = [&](const uint32_t (&m)[2], u64 (&upto)[2], u64* total) {
+    u64 v = u64(m[0]) + m[1];
+    const u64 own = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const u64 y = __shfl_up_sync(~0u, v, d);
+      if (lane >= d) v += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh.red[warp] = v;
+    __syncthreads();
+    *total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) v += sh.red[w];
+      *total += sh.red[w];
+    }
+    upto[0] = v - own;
+    upto[1] = upto[0] + m[0];
   };
   // The threshold: the last token, in the order, before which there is less than
   // `want`, among those of a cut, which `in(value, place)` tells. *mass: of all up
@@ -351,11 +477,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     while (cut.count > uint32_t(kMost)) {
       if (!split) {  // the range of the cut
         u64 least = 0, most = 0;  // as maxima of ~c and c
-        for (uint32_t j = tid; j < x.n; j += kThreads) {
-          const float v = x.at(j);
+        x.each([&](float v, uint32_t j) {
           const u64 c = place_of(v, x.lo + j);
           if (in(v, c)) least = max(least, ~c), most = max(most, c);
-        }
+        });
         least = warp_max(least), most = warp_max(most);
         __syncthreads();
         if (lane == 0) sh.mine[warp] = least, sh.mine[kWarps + warp] = most;
@@ -373,24 +498,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       cluster.sync();  // the histograms have been read
       for (int b = tid; b < kBins; b += kThreads) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
       __syncthreads();
-      for (uint32_t j = tid; j < x.n; j += kThreads) {
-        const float v = x.at(j);
+      x.each([&](float v, uint32_t j) {
         const u64 c = place_of(v, x.lo + j);
         if (c >= low && c <= high) tally(int((high - c) >> shift), mass_of(v, z));
-      }
-      cluster.sync();
-      merge(true);
-      cut = pick(by_mass, want, cut.before, cut.mass_before, 0);
+      });
+      merge(true, 1);
+      cut = pick(1, by_mass, want, cut.before, cut.mass_before, 0);
       const u64 up = high - (u64(cut.bin) << shift);
       const u64 down = (u64(1) << shift) - 1;
       low = up - low < down ? low : up - down;
       high = up;
     }
-    for (uint32_t j = tid; j < x.n; j += kThreads) {
-      const float v = x.at(j);
+    x.each([&](float v, uint32_t j) {
       const u64 c = place_of(v, x.lo + j);
       if (in(v, c)) sh.mine[atomicAdd(&sh.gathered, 1u)] = c;
-    }
+    });
     cluster.sync();  // histograms have been read too
     uint32_t n = 0;
     for (uint32_t r = 0; r < C; ++r) {
@@ -399,23 +521,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       for (uint32_t j = tid; j < m; j += kThreads) {
         const u64 c = from[j];
         sh.all[n + j] = c;
-        sh.mass[n + j] = mass_of(value_of(uint32_t(c >> 32)), z);
       }
       n += m;
     }
     __syncthreads();
+    sort(sh.all, n, true);
+    uint32_t m[2];
+    u64 upto[2], sum;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      m[e] = 2 * tid + e < n ? mass_of(value_of(uint32_t(sh.all[2 * tid + e] >> 32)), z) : 0u;
+    scan2(m, upto, &sum);
     // the last one that stays is the one whose successor, in the order, does not
-    for (uint32_t j = tid; j < n; j += kThreads) {
-      const u64 c = sh.all[j];
-      uint32_t above = 0;
-      u64 mass_above = 0;
-      for (uint32_t i = 0; i < n; ++i)
-        if (sh.all[i] > c) ++above, mass_above += sh.mass[i];
-      const u64 m0 = cut.mass_before + mass_above, m1 = m0 + sh.mass[j];
-      const uint32_t c0 = cut.before + above;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t i = 2 * tid + e;
+      const u64 m0 = cut.mass_before + upto[e], m1 = m0 + m[e];
+      const uint32_t c0 = cut.before + i;
       const bool stays = (by_mass ? double(m0) : double(c0)) < want;
-      const bool next = above + 1 < n && (by_mass ? double(m1) : double(c0 + 1)) < want;
-      if (stays && !next) sh.found = c, sh.found_mass = m1;
+      const bool next = i + 1 < n && (by_mass ? double(m1) : double(c0 + 1)) < want;
+      if (i < n && stays && !next) sh.found = sh.all[i], sh.found_mass = m1;
     }
     __syncthreads();
     *mass = sh.found_mass;
@@ -427,13 +552,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   const bool by_count = k > 0 && uint32_t(k) < V, by_mass = A.top_p && p < 1.f;
 
   if (by_count && uint32_t(k) <= kFew) {  // ---- a small top-k: the first CTA finishes
-    for (uint32_t j = tid; j < x.n; j += kThreads) {
-      const int b = bin_of(x.at(j));
+    x.each([&](float v, uint32_t) {
+      const int b = bin_of(v);
       if (b < kBins) atomicAdd(&sh.count[b], 1u);
-    }
-    cluster.sync();
-    merge(false);
-    const Cut cut = pick(false, double(k), 0, 0, V);
+    });
+    merge(false, 0);
+    const Cut cut = pick(0, false, double(k), 0, 0, V);
     const bool fits = cut.before + cut.count <= uint32_t(kList);
     if (!fits) {
       u64 mass;
@@ -444,10 +568,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     cluster.sync();  // the counter and the list are free
     uint32_t* counter = of(&sh.gathered, 0);
     u64* list = of(sh.list, 0);
-    for (uint32_t j = tid; j < x.n; j += kThreads) {
-      const float v = x.at(j);
-      const u64 c = place_of(v, x.lo + j);
-      if (fits ? bin_of(v) <= cut.bin : c >= least) list[atomicAdd(counter, 1u)] = c;
+    if (fits && cut.bin < kBins) {
+      // the smallest value in the bin: bins go up as values go down
+      uint32_t low = key_of(-INFINITY), high = key_of(top);
+      while (low < high) {
+        const uint32_t mid = low + (high - low) / 2;
+        if (bin_of(value_of(mid)) <= cut.bin) high = mid;
+        else low = mid + 1;
+      }
+      const float from = value_of(high);
+      x.each([&](float v, uint32_t j) {
+        if (v >= from) list[atomicAdd(counter, 1u)] = place_of(v, x.lo + j);
+      });
+    } else {
+      x.each([&](float v, uint32_t j) {
+        const u64 c = place_of(v, x.lo + j);
+        if (c >= least) list[atomicAdd(counter, 1u)] = c;  // all of them where the bin is the rest
+      });
     }
     cluster.sync();
     if (rank != 0) return;
@@ -458,31 +595,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     u64 total = 0;
     uint32_t m[2], stay = 0;
     u64 upto[2];
-    auto scan2 = [&](const uint32_t (&m)[2]) {  // of the pairs 2 tid, 2 tid + 1
-      u64 v = u64(m[0]) + m[1];
-      const u64 own = v;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const u64 y = __shfl_up_sync(~0u, v, d);
-        if (lane >= d) v += y;
-      }
-      __syncthreads();
-      if (lane == 31) sh.red[warp] = v;
-      __syncthreads();
-      total = 0;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) v += sh.red[w];
-        total += sh.red[w];
-      }
-      upto[0] = v - own;  // exclusive
-      upto[1] = upto[0] + m[0];
-    };
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
       m[e] = i < few ? mass_of(value_of(uint32_t(sh.list[i] >> 32)), z) : 0u;
     }
-    scan2(m);
+    scan2(m, upto, &total);
     const double want = double(p) * double(total);
     u64 item[2];
 #pragma unroll
@@ -504,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       m[e] = 2 * tid + e < stay ? uint32_t(sh.list[2 * tid + e]) : 0u;
-    scan2(m);
+    scan2(m, upto, &total);
     const double u = double(A.uniform[row]) * double(total);
     u64 target = u > 0. ? u64(u) : 0;
     if (target >= total) target = total - 1;
@@ -523,8 +641,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   if (only_first) {
     least = ~0ull;
   } else if (by_count || by_mass) {
-    for (uint32_t j = tid; j < x.n; j += kThreads) {
-      const float v = x.at(j);
+    x.each([&](float v, uint32_t) {
       const int b = bin_of(v);
       if (b < kBins) {
         const uint32_t mass = mass_of(v, z);
@@ -532,24 +649,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
         atomicAdd(&sh.lo[b], mass & 0xffffu);
         atomicAdd(&sh.hi[b], mass >> 16);
       }
-    }
-    cluster.sync();
-    merge(true);
-    u64 total = masses;
+    });
+    merge(true, 0);
+    u64 total = 0;
+    for (uint32_t r = 0; r < C; ++r) total += sh.slice_mass[0][r];
     if (by_count) {
       // `resolve` may use the bins again
-      const uint32_t opc = pc, ot = tokens, oc[kEach] = {bc[0], bc[1], bc[2], bc[3]};
-      const u64 opm = pm, omass = masses, om[kEach] = {bm[0], bm[1], bm[2], bm[3]};
-      const Cut cut = pick(false, double(k), 0, 0, V);
+      const uint32_t opc = pc, oc[kEach] = {bc[0], bc[1], bc[2], bc[3]};
+      const u64 opm = pm, om[kEach] = {bm[0], bm[1], bm[2], bm[3]};
+      const Cut cut = pick(0, false, double(k), 0, 0, V);
       least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &total);
 #pragma unroll
       for (int e = 0; e < kEach; ++e) bc[e] = oc[e], bm[e] = om[e];
-      pc = opc, pm = opm, tokens = ot, masses = omass;
+      pc = opc, pm = opm;
       cluster.sync();  // lists have been read
     }
     if (by_mass) {
       const double want = double(p) * double(total);
-      const Cut cut = pick(true, want, 0, 0, 0);
+      const Cut cut = pick(0, true, want, 0, 0, 0);
       u64 m;
       least = max(least, resolve(true, want, cut, [&](float v) { return bin_of(v) == cut.bin; }, &m));
     }
