@@ -116,7 +116,7 @@ struct Shared {
   // for the other CTAs of the cluster
   float top;
   u64 kept, first, range[2], slice_mass[2][kMaxCtas];
-  uint32_t gathered, slice_count[2][kMaxCtas];  // [0] of the bins, [1] of a bin split again
+  uint32_t gathered, listed, slice_count[2][kMaxCtas];  // [0] of the bins, [1] of a bin split again
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   top = __uint_as_float(sh.red2[lane % kWarps]);
 #pragma unroll
   for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  if (tid == 0) sh.top = top;
+  if (tid == 0) sh.top = top, sh.listed = 0;
   cluster.sync();
   for (uint32_t r = 0; r < C; ++r) top = fmaxf(top, *of(&sh.top, r));
   top += 0.f;
@@ -326,26 +326,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     const float d = (top - v) * to_bin;
     return d < float(kBins) ? int(d) : kBins;  // even where d is NaN
   };
-  // Adds a token to a bin; lanes that all name one bin add once.
   auto tally = [&](int bin, uint32_t mass) {
-    const uint32_t on = __activemask();
-    int same;
-    __match_all_sync(on, bin, &same);
-    if (same) {
-      const uint32_t lo = __reduce_add_sync(on, mass & 0xffffu);
-      const uint32_t hi = __reduce_add_sync(on, mass >> 16);
-      if (lane == __ffs(on) - 1) {
-        atomicAdd(&sh.count[bin], __popc(on));
-        atomicAdd(&sh.lo[bin], lo);
-        atomicAdd(&sh.hi[bin], hi);
-      }
-    } else {
-      atomicAdd(&sh.count[bin], 1u);
-      if (mass) {
-        atomicAdd(&sh.lo[bin], mass & 0xffffu);
-        atomicAdd(&sh.hi[bin], mass >> 16);
-      }
-    }
+    atomicAdd(&sh.count[bin], 1u);
+    atomicAdd(&sh.lo[bin], mass & 0xffffu);
+    atomicAdd(&sh.hi[bin], mass >> 16);
   };
   // The merged histogram, a slice of kBins / C neighbouring bins in each CTA, kEach
   // in each of its first threads, and what is before them in the slice. (Reading all
@@ -468,12 +452,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     upto[1] = upto[0] + m[0];
   };
   // The threshold: the last token, in the order, before which there is less than
-  // `want`, among those of a cut, which `in(value, place)` tells. *mass: of all up
-  // to and with it.
-  auto resolve = [&](bool by_mass, double want, Cut cut, auto in0, u64* mass) -> u64 {
+  // `want`, among those of a cut of the bins. *mass: of all up to and with it.
+  auto resolve = [&](bool by_mass, double want, Cut cut, u64* mass) -> u64 {
     u64 low = 0, high = ~0ull;  // once the cut has been split: its range of places
     bool split = false;
-    auto in = [&](float v, u64 c) { return split ? c >= low && c <= high : in0(v); };
+    const int bin = cut.bin;
+    auto in = [&](float v, u64 c) { return split ? c >= low && c <= high : bin_of(v) == bin; };
     while (cut.count > uint32_t(kMost)) {
       if (!split) {  // the range of the cut
         u64 least = 0, most = 0;  // as maxima of ~c and c
@@ -551,54 +535,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   const bool only_first = (A.top_p && !(p > 0.f)) || (A.min_p && !(mp <= 1.f));
   const bool by_count = k > 0 && uint32_t(k) < V, by_mass = A.top_p && p < 1.f;
 
-  if (by_count && uint32_t(k) <= kFew) {  // ---- a small top-k: the first CTA finishes
+  // ---- a small top-k: the first CTA finishes
+  bool few = by_count && uint32_t(k) <= kFew;
+  if (few) {
     x.each([&](float v, uint32_t) {
       const int b = bin_of(v);
       if (b < kBins) atomicAdd(&sh.count[b], 1u);
     });
     merge(false, 0);
     const Cut cut = pick(0, false, double(k), 0, 0, V);
-    const bool fits = cut.before + cut.count <= uint32_t(kList);
-    if (!fits) {
-      u64 mass;
-      least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &mass);
-      cluster.sync();  // lists have been read
-      if (tid == 0) sh.gathered = 0;
-    }
-    cluster.sync();  // the counter and the list are free
-    uint32_t* counter = of(&sh.gathered, 0);
-    u64* list = of(sh.list, 0);
-    if (fits && cut.bin < kBins) {
+    few = cut.before + cut.count <= uint32_t(kList);
+    if (few) {
       // the smallest value in the bin: bins go up as values go down
       uint32_t low = key_of(-INFINITY), high = key_of(top);
-      while (low < high) {
+      while (cut.bin < kBins && low < high) {
         const uint32_t mid = low + (high - low) / 2;
         if (bin_of(value_of(mid)) <= cut.bin) high = mid;
         else low = mid + 1;
       }
-      const float from = value_of(high);
+      const float from = cut.bin < kBins ? value_of(high) : -INFINITY;
       x.each([&](float v, uint32_t j) {
-        if (v >= from) list[atomicAdd(counter, 1u)] = place_of(v, x.lo + j);
+        if (plain(v) >= from) sh.mine[atomicAdd(&sh.gathered, 1u)] = place_of(v, x.lo + j);
       });
-    } else {
-      x.each([&](float v, uint32_t j) {
-        const u64 c = place_of(v, x.lo + j);
-        if (c >= least) list[atomicAdd(counter, 1u)] = c;  // all of them where the bin is the rest
-      });
+      __syncthreads();
+      // its place in the first CTA's list, then the copy
+      const uint32_t n = sh.gathered;
+      if (tid == 0) sh.red2[0] = atomicAdd(of(&sh.listed, 0), n);
+      __syncthreads();
+      u64* list = of(sh.list, 0) + sh.red2[0];
+      for (uint32_t i = tid; i < n; i += kThreads) list[i] = sh.mine[i];
+    } else {  // many near the k-th: the other way, with the bins' masses
+      for (int b = tid; b < kBins; b += kThreads) sh.count[b] = 0;
     }
     cluster.sync();
+  }
+  if (few) {
     if (rank != 0) return;
-    const uint32_t n = sh.gathered;
+    const uint32_t n = sh.listed;
     sort(sh.list, n, true);
     // masses in the order, what stays of them, and those in the order of indexes
-    const uint32_t few = min(n, uint32_t(k));
+    const uint32_t first_k = min(n, uint32_t(k));
     u64 total = 0;
     uint32_t m[2], stay = 0;
     u64 upto[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
-      m[e] = i < few ? mass_of(value_of(uint32_t(sh.list[i] >> 32)), z) : 0u;
+      m[e] = i < first_k ? mass_of(value_of(uint32_t(sh.list[i] >> 32)), z) : 0u;
     }
     scan2(m, upto, &total);
     const double want = double(p) * double(total);
@@ -606,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
-      bool on = i < few && (!by_mass || double(upto[e]) < want);
+      bool on = i < first_k && (!by_mass || double(upto[e]) < want);
       if (on && A.min_p) on = !(expf(z(value_of(uint32_t(sh.list[i] >> 32)))) < mp);
       if (only_first) on = false;
       on |= i == 0;
@@ -643,32 +626,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   } else if (by_count || by_mass) {
     x.each([&](float v, uint32_t) {
       const int b = bin_of(v);
-      if (b < kBins) {
-        const uint32_t mass = mass_of(v, z);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd(&sh.lo[b], mass & 0xffffu);
-        atomicAdd(&sh.hi[b], mass >> 16);
-      }
+      if (b < kBins) tally(b, mass_of(v, z));
     });
     merge(true, 0);
     u64 total = 0;
     for (uint32_t r = 0; r < C; ++r) total += sh.slice_mass[0][r];
-    if (by_count) {
-      // `resolve` may use the bins again
-      const uint32_t opc = pc, oc[kEach] = {bc[0], bc[1], bc[2], bc[3]};
-      const u64 opm = pm, om[kEach] = {bm[0], bm[1], bm[2], bm[3]};
-      const Cut cut = pick(0, false, double(k), 0, 0, V);
-      least = resolve(false, double(k), cut, [&](float v) { return bin_of(v) == cut.bin; }, &total);
+    // top-k, then top-p of what it leaves; `resolve` may use the bins again
+    const uint32_t opc = pc, oc[kEach] = {bc[0], bc[1], bc[2], bc[3]};
+    const u64 opm = pm, om[kEach] = {bm[0], bm[1], bm[2], bm[3]};
+#pragma unroll 1
+    for (int pass = by_count ? 0 : 1; pass < (by_mass ? 2 : 1); ++pass) {
+      const double want = pass ? double(p) * double(total) : double(k);
+      const Cut cut = pick(0, pass, want, 0, 0, pass ? 0 : V);
+      least = max(least, resolve(pass, want, cut, &total));
+      if (pass || !by_mass) break;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) bc[e] = oc[e], bm[e] = om[e];
       pc = opc, pm = opm;
       cluster.sync();  // lists have been read
-    }
-    if (by_mass) {
-      const double want = double(p) * double(total);
-      const Cut cut = pick(0, true, want, 0, 0, 0);
-      u64 m;
-      least = max(least, resolve(true, want, cut, [&](float v) { return bin_of(v) == cut.bin; }, &m));
     }
   }
 
