@@ -135,8 +135,10 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
 
 // Sorts a[0 .. n - 1], n <= 2 * kThreads, in shared memory: bitonic, one or two items
 // a thread in registers (tid and tid + kThreads), exchanged by shuffles inside a warp
-// and through `a` between warps.
-__device__ __forceinline__ void sort(u64* a, uint32_t n, bool descending) {
+// and through `a` between warps. Not inlined, as other code that runs once: what a
+// row waits for here is, more than anything, instructions that are not yet in the
+// SM's cache.
+__device__ __noinline__ void sort(u64* a, uint32_t n, bool descending) {
   const uint32_t tid = threadIdx.x;
   uint32_t size = 32;
   while (size < n) size *= 2;
@@ -199,6 +201,32 @@ __device__ __forceinline__ void sort(u64* a, uint32_t n, bool descending) {
   __syncthreads();
 }
 
+// Exclusive prefix of the masses of items 2 tid and 2 tid + 1, and their sum.
+struct Prefix {
+  u64 upto[2], total;
+};
+__device__ __noinline__ Prefix scan2(uint32_t m0, uint32_t m1, u64* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 v = u64(m0) + m1;
+  const u64 own = v;
+  for (int d = 1; d < 32; d *= 2) {
+    const u64 y = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  Prefix r;
+  r.total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) v += red[w];
+    r.total += red[w];
+  }
+  r.upto[0] = v - own;
+  r.upto[1] = r.upto[0] + m0;
+  return r;
+}
+
 // A row's part in one CTA: tokens lo .. lo + n - 1. Staged: in shared memory, else
 // read from global memory in each pass.
 template <typename T, bool kStaged>
@@ -222,13 +250,9 @@ struct Row {
         const uint4 w = from[v];
         const T* e = reinterpret_cast<const T*>(&w);
         const uint32_t j = v * kPer - pad;
-        if (v * kPer >= pad && (v + 1) * kPer <= pad + n) {
 #pragma unroll
-          for (uint32_t i = 0; i < kPer; ++i) f(to_f<T>(e[i]), j + i);
-        } else {
-          for (uint32_t i = 0; i < kPer; ++i)
-            if (j + i < n) f(to_f<T>(s[j + i]), j + i);  // j wraps below 0
-        }
+        for (uint32_t i = 0; i < kPer; ++i)
+          if (j + i < n) f(to_f<T>(e[i]), j + i);  // j wraps below 0
       }
     } else {
       for (uint32_t j = threadIdx.x; j < n; j += kThreads) f(to_f<T>(g[lo + j]), j);
@@ -431,26 +455,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     cluster.sync();
     return sh.cut;
   };
-  // Exclusive prefix of the masses of items 2 tid and 2 tid + 1.
-  auto scan2 = [&](const uint32_t (&m)[2], u64 (&upto)[2], u64* total) {
-    u64 v = u64(m[0]) + m[1];
-    const u64 own = v;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const u64 y = __shfl_up_sync(~0u, v, d);
-      if (lane >= d) v += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh.red[warp] = v;
-    __syncthreads();
-    *total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) v += sh.red[w];
-      *total += sh.red[w];
-    }
-    upto[0] = v - own;
-    upto[1] = upto[0] + m[0];
-  };
   // The threshold: the last token, in the order, before which there is less than
   // `want`, among those of a cut of the bins. *mass: of all up to and with it.
   auto resolve = [&](bool by_mass, double want, Cut cut, u64* mass) -> u64 {
@@ -511,16 +515,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     __syncthreads();
     sort(sh.all, n, true);
     uint32_t m[2];
-    u64 upto[2], sum;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       m[e] = 2 * tid + e < n ? mass_of(value_of(uint32_t(sh.all[2 * tid + e] >> 32)), z) : 0u;
-    scan2(m, upto, &sum);
+    const Prefix at = scan2(m[0], m[1], sh.red);
     // the last one that stays is the one whose successor, in the order, does not
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
-      const u64 m0 = cut.mass_before + upto[e], m1 = m0 + m[e];
+      const u64 m0 = cut.mass_before + at.upto[e], m1 = m0 + m[e];
       const uint32_t c0 = cut.before + i;
       const bool stays = (by_mass ? double(m0) : double(c0)) < want;
       const bool next = i + 1 < n && (by_mass ? double(m1) : double(c0 + 1)) < want;
@@ -575,21 +578,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     sort(sh.list, n, true);
     // masses in the order, what stays of them, and those in the order of indexes
     const uint32_t first_k = min(n, uint32_t(k));
-    u64 total = 0;
     uint32_t m[2], stay = 0;
-    u64 upto[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
       m[e] = i < first_k ? mass_of(value_of(uint32_t(sh.list[i] >> 32)), z) : 0u;
     }
-    scan2(m, upto, &total);
-    const double want = double(p) * double(total);
+    Prefix at = scan2(m[0], m[1], sh.red);
+    const double want = double(p) * double(at.total);
     u64 item[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint32_t i = 2 * tid + e;
-      bool on = i < first_k && (!by_mass || double(upto[e]) < want);
+      bool on = i < first_k && (!by_mass || double(at.upto[e]) < want);
       if (on && A.min_p) on = !(expf(z(value_of(uint32_t(sh.list[i] >> 32)))) < mp);
       if (only_first) on = false;
       on |= i == 0;
@@ -605,13 +606,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       m[e] = 2 * tid + e < stay ? uint32_t(sh.list[2 * tid + e]) : 0u;
-    scan2(m, upto, &total);
+    at = scan2(m[0], m[1], sh.red);
+    const u64 total = at.total;
     const double u = double(A.uniform[row]) * double(total);
     u64 target = u > 0. ? u64(u) : 0;
     if (target >= total) target = total - 1;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if (target >= upto[e] && target < upto[e] + m[e]) {
+      if (target >= at.upto[e] && target < at.upto[e] + m[e]) {
         const uint32_t i = uint32_t(sh.list[2 * tid + e] >> 32);
         const T* g = x.g;
         A.tokens[row] = int32_t(i);
