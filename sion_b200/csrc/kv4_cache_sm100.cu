@@ -23,132 +23,195 @@ struct TokenParams {
   CacheView c;
   const int32_t* counts;  // new tokens of each slot, or nullptr: rows
   uint32_t rows;
+  uint32_t blocks;             // append: blocks that the rows of a slot can lie in
+  bool vec;                    // append: every row is 16-byte aligned
   const void *k, *v;           // append: sources
   int64_t ks[3], vs[3];        // element strides: slot, head, row
   __half *ko, *vo;             // read: [slots, kv_heads, rows, D]
 };
 
 template <typename T>
-__device__ __forceinline__ float load_f(const void* p, int64_t i);
+__device__ __forceinline__ float to_f(T v);
 template <>
-__device__ __forceinline__ float load_f<__half>(const void* p, int64_t i) {
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <>
-__device__ __forceinline__ float load_f<__nv_bfloat16>(const void* p, int64_t i) {
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// (scale, base) and codes of one head vector held by a warp, N values a lane:
+// A head vector is held by kLanes = 8 neighbouring lanes, D/8 dimensions each: that
+// is a V code's group g, so that a lane's codes of two tokens are one vector of the
+// layout, and a warp has four tokens under way with three shuffles to a minimum.
+constexpr int kLanes = 8;
+
+// (scale, base) and codes of a head vector, N values a lane:
 //   scale = fp16((max - min) / 15), base = fp16(min + 8 scale),
 //   code = clamp(rint((x - base) / scale) + 8, 0, 15).
 // Values past fp16's range count as its largest; a vector with an infinity or a
 // NaN has scale and base NaN. scale = 0 (all equal): the value is base alone.
 template <int N>
-__device__ __forceinline__ uint32_t quantise(float (&x)[N], uint32_t (&code)[N]) {
-  float lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
+__device__ __forceinline__ uint32_t quantise(float (&x)[N], uint32_t (&words)[N / 8]) {
+  float lo = INFINITY, hi = -INFINITY, worst = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    bad |= !(fabsf(x[i]) < INFINITY);
+    // infinity - infinity and NaN make the sum NaN, a finite x adds 0
+    worst += x[i] - x[i];
     x[i] = fminf(fmaxf(x[i], -65504.f), 65504.f);
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
 #pragma unroll
-  for (int d = 16; d; d /= 2) {
+  for (int d = kLanes / 2; d; d /= 2) {
     lo = fminf(lo, __shfl_xor_sync(~0u, lo, d));
     hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, d));
+    worst += __shfl_xor_sync(~0u, worst, d);
   }
-  bad = __any_sync(~0u, bad);
-  __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+  const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
   const float s = __half2float(sh);
-  __half bh = __float2half_rn(__fadd_rn(lo, 8.f * s));
+  const __half bh = __float2half_rn(__fadd_rn(lo, 8.f * s));
   const float b = __half2float(bh);
+  // The quotient correctly rounded (Markstein 1990): r = RN(1 / s), q = RN(d r) is
+  // within a unit in the last place, its remainder is exact in a fused operation.
+  const float r = __frcp_rn(s);
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    code[i] = s > 0.f ? uint32_t(fminf(fmaxf(rintf(__fdiv_rn(x[i] - b, s)) + 8.f, 0.f), 15.f)) : 8u;
-  if (bad) sh = bh = __ushort_as_half(0x7e00);
-  return uint32_t(__half_as_ushort(sh)) | (uint32_t(__half_as_ushort(bh)) << 16);
+  for (int w = 0; w < N / 8; ++w) words[w] = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = x[i] - b, q = d * r;
+    const float c = rintf(fmaf(fmaf(-q, s, d), r, q)) + 8.f;
+    const uint32_t code = s > 0.f ? uint32_t(fminf(fmaxf(c, 0.f), 15.f)) : 8u;
+    words[i / 8] |= code << (4 * (i % 8));
+  }
+  const uint32_t par = uint32_t(__half_as_ushort(sh)) | (uint32_t(__half_as_ushort(bh)) << 16);
+  return worst != worst ? 0x7e007e00u : par;
 }
 
-// One warp per (slot, row, head): a lane takes D/32 neighbouring dimensions.
+// One warp per (slot, head, block of the cache that has new tokens), four tokens at
+// a time. Bytes of other tokens are not touched.
 template <typename T, int D>
-__global__ void kv4_append_kernel(const TokenParams P) {
-  constexpr int N = D / 32;
-  const uint64_t item = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  const uint32_t heads = P.c.kv_heads;
-  if (item >= uint64_t(P.c.slots) * P.rows * heads) return;
-  const uint32_t head = uint32_t(item % heads), row = uint32_t(item / heads % P.rows),
-                 slot = uint32_t(item / heads / P.rows);
+__global__ void __launch_bounds__(256) kv4_append_kernel(const TokenParams P) {
+  constexpr int N = D / kLanes;
+  const int lane = threadIdx.x & 31, part = lane % kLanes;
+  const uint32_t head = blockIdx.y, nth = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  for (uint32_t slot = blockIdx.z; slot < P.c.slots; slot += gridDim.z) {
   const int len = slot_length(P.c, slot);
   const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
-  const int token = len - count + int(row);
-  if (int(row) >= count || token < 0) return;
-  unsigned char* blk = block_of(P.c, slot, token, head, D);
-  if (!blk) return;
-  const uint32_t r = uint32_t(token) % kBlock, d = lane * N;
+  const int start = len - count;  // token of row 0; tokens before 0 have no place
+  const int from = max(start, 0), t0 = (from / int(kBlock) + int(nth)) * int(kBlock);
+  if (t0 >= len || count <= 0) continue;
+  unsigned char* blk = block_of(P.c, slot, t0, head, D);
+  if (!blk) continue;
+  const int i1 = (min(len - t0, int(kBlock)) + 3) / 4;
+  for (int i = max(from - t0, 0) / 4; i < i1; ++i) {
+    const uint32_t r = 4 * i + lane / kLanes;
+    const int token = t0 + int(r), row = token - start;
+    const bool mine = token >= from && token < len;
+    float both_x[2][N];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const int64_t* st = which ? P.vs : P.ks;
-    const int64_t at = int64_t(slot) * st[0] + int64_t(head) * st[1] + int64_t(row) * st[2] + d;
-    float x[N];
-    uint32_t code[N];
+    for (int which = 0; which < 2; ++which) {
+      const int64_t* st = which ? P.vs : P.ks;
+      const T* src = static_cast<const T*>(which ? P.v : P.k) + int64_t(slot) * st[0] +
+                     int64_t(head) * st[1] + int64_t(row) * st[2] + part * N;
+      float (&x)[N] = both_x[which];
+      if (mine && P.vec) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = load_f<T>(which ? P.v : P.k, at + i);
-    const uint32_t par = quantise<N>(x, code);
-    unsigned char* dst =
-        which ? blk + v_codes_at(D) + v_code_byte(D, r, d) : blk + r * (D / 2) + d / 2;
-    if constexpr (N == 4) {
-      *reinterpret_cast<uint16_t*>(dst) =
-          uint16_t(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
-    } else {
-      *dst = (unsigned char)(code[0] | code[1] << 4);
+        for (int j = 0; j < N / 8; ++j) {
+          const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + j);
+          const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int y = 0; y < 8; ++y) x[8 * j + y] = to_f<T>(e[y]);
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < N; ++y) x[y] = mine ? to_f<T>(src[y]) : 0.f;
+      }
     }
-    if (lane == 0)
-      reinterpret_cast<uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D)))[r] = par;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float (&x)[N] = both_x[which];
+      uint32_t w[N / 8];
+      const uint32_t par = quantise<N>(x, w);
+      if (which == 0) {
+        if (mine) {
+          if constexpr (N == 16)
+            *reinterpret_cast<uint2*>(blk + r * (D / 2) + part * 8) = make_uint2(w[0], w[1]);
+          else
+            *reinterpret_cast<uint32_t*>(blk + r * (D / 2) + part * 4) = w[0];
+        }
+      } else {
+        // four codes of this token and of the pair's other one make a word
+        unsigned char* dst = blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) +
+                             (r % 8 / 2) * (D / 8);
+        const bool both = __shfl_xor_sync(~0u, int(mine), kLanes) && mine;
+        uint32_t o[N / 8], pair[N / 4];
+#pragma unroll
+        for (int j = 0; j < N / 8; ++j) {
+          o[j] = __shfl_xor_sync(~0u, w[j], kLanes);
+          pair[2 * j] = (w[j] & 0xffffu) | (o[j] << 16);
+          pair[2 * j + 1] = (w[j] >> 16) | (o[j] & 0xffff0000u);
+        }
+        if (both && !(r & 1)) {
+          if constexpr (N == 16)
+            *reinterpret_cast<uint4*>(dst) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+          else
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pair[0], pair[1]);
+        } else if (mine && !both) {
+#pragma unroll
+          for (int j = 0; j < N / 4; ++j)
+            *reinterpret_cast<uint16_t*>(dst + 4 * j + 2 * (r & 1)) =
+                uint16_t(w[j / 2] >> (16 * (j % 2)));
+        }
+      }
+      if (mine && part == 0)
+        reinterpret_cast<uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D)))[r] = par;
+    }
+  }
   }
 }
 
+// kLanes lanes per (slot, head, row).
 template <int D>
-__global__ void kv4_read_kernel(const TokenParams P) {
-  constexpr int N = D / 32;
-  const uint64_t item = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
-  const int lane = threadIdx.x & 31;
-  const uint32_t heads = P.c.kv_heads;
-  if (item >= uint64_t(P.c.slots) * P.rows * heads) return;
-  // rows innermost: neighbouring warps write neighbouring rows of the output
-  const uint32_t row = uint32_t(item % P.rows), head = uint32_t(item / P.rows % heads),
-                 slot = uint32_t(item / P.rows / heads);
+__global__ void __launch_bounds__(256) kv4_read_kernel(const TokenParams P) {
+  constexpr int N = D / kLanes;
+  const int part = threadIdx.x % kLanes;
+  const uint32_t head = blockIdx.y, row = (blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
+  if (row >= P.rows) return;
+  for (uint32_t slot = blockIdx.z; slot < P.c.slots; slot += gridDim.z) {
+  const uint64_t item = (uint64_t(slot) * P.c.kv_heads + head) * P.rows + row;
   const int len = slot_length(P.c, slot);
   const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
   const int token = len - count + int(row);
   const unsigned char* blk = (int(row) < count && token >= 0)
                                  ? block_of(P.c, slot, token, head, D) : nullptr;
-  const uint32_t r = uint32_t(token) % kBlock, d = lane * N;
+  const uint32_t r = uint32_t(token) % kBlock;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    __half out[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = __float2half_rn(0.f);
+    uint32_t w[N / 8] = {};
+    float2 sb = make_float2(0.f, 0.f);
     if (blk) {
-      const unsigned char* src =
-          which ? blk + v_codes_at(D) + v_code_byte(D, r, d) : blk + r * (D / 2) + d / 2;
-      const uint32_t w = N == 4 ? *reinterpret_cast<const uint16_t*>(src) : *src;
-      const uint32_t par =
-          reinterpret_cast<const uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D)))[r];
-      const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(&par));
+      if (which == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        out[i] = __float2half_rn(
-            __fadd_rn(sb.y, __fmul_rn(sb.x, float((w >> (4 * i)) & 15u) - 8.f)));
+        for (int j = 0; j < N / 8; ++j)
+          w[j] = __ldg(reinterpret_cast<const uint32_t*>(blk + r * (D / 2) + part * (N / 2)) + j);
+      } else {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(
+            blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) + (r % 8 / 2) * (D / 8) +
+            2 * (r & 1));
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) w[j / 2] |= uint32_t(__ldg(src + 2 * j)) << (16 * (j % 2));
+      }
+      const uint32_t par = __ldg(
+          reinterpret_cast<const uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D))) + r);
+      sb = __half22float2(*reinterpret_cast<const __half2*>(&par));
     }
-    __half* dst = (which ? P.vo : P.ko) + item * D + d;
-    if constexpr (N == 4)
-      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(out);
-    else
-      *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(out);
+    alignas(16) __half out[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float c = float((w[i / 8] >> (4 * (i % 8))) & 15u) - 8.f;
+      out[i] = __float2half_rn(blk ? __fadd_rn(sb.y, __fmul_rn(sb.x, c)) : 0.f);
+    }
+    uint4* dst = reinterpret_cast<uint4*>((which ? P.vo : P.ko) + item * D + part * N);
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) dst[j] = reinterpret_cast<const uint4*>(out)[j];
+  }
   }
 }
 
@@ -236,20 +299,42 @@ __device__ __forceinline__ uint32_t total_of(MetaShared& sh, int which, uint32_t
   return v;
 }
 
+// A CTA's pages are neighbouring, and so are the kRun of a thread in a pass: 65536
+// pages are one pass, one scan.
+constexpr uint32_t kRun = 8, kPass = kRun * kMeta;
 struct Range {
   uint32_t lo, hi;
 };
 __device__ __forceinline__ Range pages_of_cta(uint32_t pages, uint32_t rank) {
-  const uint32_t run = (pages + kCtas - 1) / kCtas;
+  const uint32_t run = ((pages + kCtas - 1) / kCtas + kRun - 1) & ~(kRun - 1);
   const uint32_t lo = min(rank * run, pages);
   return {lo, min(lo + run, pages)};
+}
+// refs of pages p0 .. p0 + kRun - 1, `none` past the range.
+__device__ __forceinline__ void load_run(const int32_t* refs, uint32_t p0, uint32_t hi, int none,
+                                         int (&v)[kRun]) {
+  if (p0 + kRun <= hi && (reinterpret_cast<uintptr_t>(refs) & 15) == 0) {
+    const int4 a = *reinterpret_cast<const int4*>(refs + p0);
+    const int4 b = *reinterpret_cast<const int4*>(refs + p0 + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e) v[e] = p0 + e < hi ? refs[p0 + e] : none;
+  }
 }
 
 // Counts the CTA's pages for which f holds, two predicates at once.
 template <class F, class G>
-__device__ __forceinline__ void count_pages(Range r, MetaShared& sh, F f, G g) {
+__device__ __forceinline__ void count_pages(const int32_t* refs, Range r, MetaShared& sh, F f, G g) {
   uint32_t nf = 0, ng = 0, sum;
-  for (uint32_t p = r.lo + threadIdx.x; p < r.hi; p += kMeta) nf += f(p), ng += g(p);
+  for (uint32_t p0 = r.lo + threadIdx.x * kRun; p0 < r.hi; p0 += kPass) {
+    int v[kRun];
+    load_run(refs, p0, r.hi, 0, v);
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e)
+      if (p0 + e < r.hi) nf += f(p0 + e, v[e]), ng += g(p0 + e, v[e]);
+  }
   scan(nf, sh, &sum);
   if (threadIdx.x == 0) sh.total[0] = sum;
   scan(ng, sh, &sum);
@@ -268,8 +353,8 @@ __device__ __forceinline__ int pages_for(int len, uint32_t shift) {
 // copied to refs_out with those pages at 1. Call with fits = want <= number.
 __device__ uint32_t count_free(const MetaParams& P, MetaShared& sh, Range r, uint32_t rank,
                                uint32_t* before) {
-  count_pages(r, sh, [&](uint32_t p) { return uint32_t(P.refs[p] <= 0); },
-              [](uint32_t) { return 0u; });
+  count_pages(P.refs, r, sh, [](uint32_t, int v) { return uint32_t(v <= 0); },
+              [](uint32_t, int) { return 0u; });
   csync();
   uint32_t all = 0;
   *before = 0;
@@ -282,14 +367,22 @@ __device__ uint32_t count_free(const MetaParams& P, MetaShared& sh, Range r, uin
 }
 __device__ void take_free(const MetaParams& P, MetaShared& sh, Range r, uint32_t before,
                           uint32_t want) {
-  for (uint32_t p0 = r.lo; p0 < r.hi; p0 += kMeta) {
-    const uint32_t p = p0 + threadIdx.x;
-    const int v = p < r.hi ? P.refs[p] : 1;
-    uint32_t sum;
-    const uint32_t at = before + scan(v <= 0, sh, &sum);
-    const bool take = v <= 0 && at < want;
-    if (take) P.fresh[at] = int32_t(p);
-    if (p < r.hi) P.refs_out[p] = take ? 1 : v;
+  for (uint32_t q = r.lo; q < r.hi; q += kPass) {
+    const uint32_t p0 = q + threadIdx.x * kRun;
+    int v[kRun];
+    load_run(P.refs, p0, r.hi, 1, v);
+    uint32_t mine = 0, sum;
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e) mine += v[e] <= 0;
+    uint32_t at = before + scan(mine, sh, &sum);
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e) {
+      if (p0 + e >= r.hi) break;
+      const bool is_free = v[e] <= 0, take = is_free && at < want;
+      if (take) P.fresh[at] = int32_t(p0 + e);
+      P.refs_out[p0 + e] = take ? 1 : v[e];
+      at += is_free;
+    }
     before += sum;
   }
 }
@@ -334,6 +427,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
     const int32_t* in = P.table + size_t(s) * P.width;
     int32_t* out = P.table_out + size_t(s) * P.width;
     const int lo = P.table == P.table_out ? now : 0, hi = P.table == P.table_out ? then : int(P.width);
+#pragma unroll 4
     for (int j = lo + int(threadIdx.x & 31); j < min(hi, int(P.width)); j += 32)
       out[j] = j >= now && j < then ? P.fresh[P.start[s] + j - now] : in[j];
     __syncwarp();
@@ -400,6 +494,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
     const int32_t* in = P.table + size_t(child ? uint32_t(P.a[i]) : s) * P.width;
     int32_t* out = P.table_out + size_t(s) * P.width;
     const int whole = child ? len >> P.page_shift : 0, at = child ? P.start[2 * i] : -1;
+#pragma unroll 4
     for (int j = lane; j < int(P.width); j += 32) {
       int v = in[j];
       if (child) {
@@ -439,6 +534,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
     if (gone || P.table != P.table_out) {
       const int32_t* in = P.table + size_t(s) * P.width;
       int32_t* out = P.table_out + size_t(s) * P.width;
+#pragma unroll 4
       for (int j = lane; j < int(P.width); j += 32) {
         const int v = in[j];
         if (gone && j < held && v >= 0 && uint32_t(v) < P.pages) atomicSub(&P.refs_out[v], 1);
@@ -460,8 +556,8 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
   const uint32_t live = P.pages - count_free(P, sh, r, rank, &before);
   csync();  // the totals have been read
   // live pages from `live` on move into the free ones below it, both in order
-  count_pages(r, sh, [&](uint32_t p) { return uint32_t(P.refs[p] > 0 && p >= live); },
-              [&](uint32_t p) { return uint32_t(P.refs[p] <= 0 && p < live); });
+  count_pages(P.refs, r, sh, [&](uint32_t p, int v) { return uint32_t(v > 0 && p >= live); },
+              [&](uint32_t p, int v) { return uint32_t(v <= 0 && p < live); });
   csync();
   uint32_t s_at = 0, d_at = 0, moves = 0;
   for (uint32_t k = 0; k < kCtas; ++k) {
@@ -469,16 +565,30 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
     if (k < rank) s_at += v, d_at += w;
     moves += v;
   }
-  for (uint32_t p0 = r.lo; p0 < r.hi; p0 += kMeta) {
-    const uint32_t p = p0 + threadIdx.x;
-    const int v = p < r.hi ? P.refs[p] : 0;
-    const bool from = p < r.hi && v > 0 && p >= live, into = p < r.hi && v <= 0 && p < live;
-    uint32_t sum, sum2;
-    const uint32_t a = s_at + scan(from, sh, &sum), b = d_at + scan(into, sh, &sum2);
-    if (from) P.src[a] = int32_t(p);
-    if (into) P.dst[b] = int32_t(p);
-    if (p < r.hi && !from) P.fresh[p] = int32_t(p);
-    if (p < r.hi && !from && !into) P.refs_out[p] = v > 0 ? v : 0;
+  for (uint32_t q = r.lo; q < r.hi; q += kPass) {
+    const uint32_t p0 = q + threadIdx.x * kRun;
+    int v[kRun];
+    load_run(P.refs, p0, r.hi, 0, v);
+    uint32_t nf = 0, ni = 0, sum, sum2;
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e) {
+      const uint32_t p = p0 + e;
+      nf += p < r.hi && v[e] > 0 && p >= live;
+      ni += p < r.hi && v[e] <= 0 && p < live;
+    }
+    uint32_t a = s_at + scan(nf, sh, &sum), b = d_at + scan(ni, sh, &sum2);
+#pragma unroll
+    for (uint32_t e = 0; e < kRun; ++e) {
+      const uint32_t p = p0 + e;
+      if (p >= r.hi) break;
+      if (v[e] > 0 && p >= live) {
+        P.src[a++] = int32_t(p);
+      } else {
+        P.fresh[p] = int32_t(p);
+        if (v[e] <= 0 && p < live) P.dst[b++] = int32_t(p);
+        else P.refs_out[p] = v[e] > 0 ? v[e] : 0;
+      }
+    }
     s_at += sum;
     d_at += sum2;
   }
@@ -492,6 +602,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
   }
   csync();
   const uint64_t entries = uint64_t(P.slots) * P.width;
+#pragma unroll 4
   for (uint64_t i = me; i < entries; i += all) {
     const int v = P.table[i];
     P.table_out[i] = v >= 0 && uint32_t(v) < P.pages ? P.fresh[v] : -1;
@@ -547,16 +658,20 @@ FelixCode kv4_append_launch(const felix_kv4::CacheView& c, uint32_t head_dim, co
   P.k = key;
   P.v = value;
   for (int i = 0; i < 3; ++i) P.ks[i] = ks[i], P.vs[i] = vs[i];
-  const uint64_t blocks = (uint64_t(c.slots) * rows * c.kv_heads + 7) / 8;
-  if (blocks == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
-  if (blocks > 0x7fffffffull) return api_error("kv4_append: too many tokens in one call");
-  const dim3 grid{uint32_t(blocks)};
+  uintptr_t bits = reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value);
+  for (int i = 0; i < 3; ++i) bits |= uintptr_t(ks[i] * 2) | uintptr_t(vs[i] * 2);
+  P.vec = (bits & 15) == 0;
+  // rows can start anywhere in a block
+  P.blocks = rows == 1 ? 1 : (rows + 14) / felix_kv4::kBlock + 1;
+  const dim3 grid((P.blocks + 7) / 8, c.kv_heads, c.slots < 65535u ? c.slots : 65535u);
+  if (grid.z == 0 || rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
+  const int threads = P.blocks < 8 ? int(P.blocks) * 32 : 256;
   if (bf16) {
-    if (head_dim == 128) kv4::kv4_append_kernel<__nv_bfloat16, 128><<<grid, 256, 0, stream>>>(P);
-    else kv4::kv4_append_kernel<__nv_bfloat16, 64><<<grid, 256, 0, stream>>>(P);
+    if (head_dim == 128) kv4::kv4_append_kernel<__nv_bfloat16, 128><<<grid, threads, 0, stream>>>(P);
+    else kv4::kv4_append_kernel<__nv_bfloat16, 64><<<grid, threads, 0, stream>>>(P);
   } else {
-    if (head_dim == 128) kv4::kv4_append_kernel<__half, 128><<<grid, 256, 0, stream>>>(P);
-    else kv4::kv4_append_kernel<__half, 64><<<grid, 256, 0, stream>>>(P);
+    if (head_dim == 128) kv4::kv4_append_kernel<__half, 128><<<grid, threads, 0, stream>>>(P);
+    else kv4::kv4_append_kernel<__half, 64><<<grid, threads, 0, stream>>>(P);
   }
   return kv4::done("kv4_append");
 }
@@ -569,10 +684,8 @@ FelixCode kv4_read_launch(const felix_kv4::CacheView& c, uint32_t head_dim, uint
   P.rows = rows;
   P.ko = key;
   P.vo = value;
-  const uint64_t blocks = (uint64_t(c.slots) * rows * c.kv_heads + 7) / 8;
-  if (blocks == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
-  if (blocks > 0x7fffffffull) return api_error("kv4_read: too many tokens in one call");
-  const dim3 grid{uint32_t(blocks)};
+  const dim3 grid((rows + 31) / 32, c.kv_heads, c.slots < 65535u ? c.slots : 65535u);
+  if (grid.z == 0 || rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
   if (head_dim == 128) kv4::kv4_read_kernel<128><<<grid, 256, 0, stream>>>(P);
   else kv4::kv4_read_kernel<64><<<grid, 256, 0, stream>>>(P);
   return kv4::done("kv4_read");

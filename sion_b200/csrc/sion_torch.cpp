@@ -14,9 +14,12 @@
 #include <sion/sion.hpp>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <felix/felix.hpp>
 #include <torch/extension.h>
+
+#include <array>
 
 namespace sion {
 
@@ -280,19 +283,27 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_attention_impl(
   return {O, L};
 }
 
+// Straight from the allocator: a page operation returns four small tensors, and the
+// dispatcher would take longer over them than the GPU over the operation.
+torch::Tensor empty_i32(at::IntArrayRef sizes, const torch::Device& dev) {
+  return at::Tensor(at::detail::empty_cuda(sizes, torch::kInt32, dev, std::nullopt));
+}
+
 // Outputs of a page operation: `out`, or new tensors of the inputs' shapes.
-std::vector<torch::Tensor> page_outputs(const std::vector<torch::Tensor>& in, const Kv4Out& out) {
-  std::vector<torch::Tensor> r;
-  if (!out) {
-    for (const auto& t : in) r.push_back(torch::empty_like(t));
-    return r;
-  }
-  TORCH_CHECK(out->size() == in.size(), "out must have ", in.size(), " tensors");
-  for (size_t i = 0; i < in.size(); ++i) {
+template <size_t N>
+std::array<torch::Tensor, N> page_outputs(const std::array<const torch::Tensor*, N>& in,
+                                          const Kv4Out& out) {
+  std::array<torch::Tensor, N> r;
+  if (out) TORCH_CHECK(out->size() == N, "out must have ", N, " tensors");
+  for (size_t i = 0; i < N; ++i) {
+    if (!out) {
+      r[i] = empty_i32(in[i]->sizes(), in[i]->device());
+      continue;
+    }
     const auto& t = (*out)[i];
-    check_i32(t, in[i].device(), in[i].dim(), "out");
-    TORCH_CHECK(t.sizes() == in[i].sizes(), "out must have the inputs' shapes");
-    r.push_back(t);
+    check_i32(t, in[i]->device(), in[i]->dim(), "out");
+    TORCH_CHECK(t.sizes() == in[i]->sizes(), "out must have the inputs' shapes");
+    r[i] = t;
   }
   return r;
 }
@@ -389,8 +400,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv4_reser
   const int32_t* n = counts_of(counts, lens);
   const uint32_t size = page_size_of(page_size);
   const c10::cuda::CUDAGuard guard(table.device());
-  const auto o = page_outputs({table, lens, refs}, out);
-  auto report = torch::empty({2}, lens.options());
+  const auto o = page_outputs<3>({&table, &lens, &refs}, out);
+  auto report = empty_i32({2}, lens.device());
   const auto status = felix::kv4_reserve_launch(
       pages_of(table, &lens, refs), n, uint32_t(table.size(0)), uint32_t(table.size(1)),
       uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]), report.data_ptr<int32_t>(),
@@ -410,8 +421,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv4_fork(
   TORCH_CHECK(parents.size(0) == children.size(0), "parents and children must have the same length");
   const uint32_t size = page_size_of(page_size);
   const c10::cuda::CUDAGuard guard(table.device());
-  const auto o = page_outputs({table, lens, refs}, out);
-  auto report = torch::empty({2}, lens.options());
+  const auto o = page_outputs<3>({&table, &lens, &refs}, out);
+  auto report = empty_i32({2}, lens.device());
   const auto status = felix::kv4_fork_launch(
       pages.data_ptr(), size_t(pages.size(1)), pages_of(table, &lens, refs), i32(parents),
       i32(children), uint32_t(parents.size(0)), uint32_t(table.size(0)), uint32_t(table.size(1)),
@@ -428,7 +439,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv4_free(
   check_i32(slots, table.device(), 1, "slots");
   const uint32_t size = page_size_of(page_size);
   const c10::cuda::CUDAGuard guard(table.device());
-  const auto o = page_outputs({table, lens, refs}, out);
+  const auto o = page_outputs<3>({&table, &lens, &refs}, out);
   const auto status = felix::kv4_free_launch(
       pages_of(table, &lens, refs), i32(slots), uint32_t(slots.size(0)), uint32_t(table.size(0)),
       uint32_t(table.size(1)), uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]),
@@ -444,7 +455,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_compact(const torch::Tensor& pages,
   check_state(table, nullptr, refs);
   check_pool(pages, refs);
   const c10::cuda::CUDAGuard guard(table.device());
-  const auto o = page_outputs({table, refs}, out);
+  const auto o = page_outputs<2>({&table, &refs}, out);
   const auto status = felix::kv4_compact_launch(
       pages.data_ptr(), size_t(pages.size(1)), pages_of(table, nullptr, refs),
       uint32_t(table.size(0)), uint32_t(table.size(1)), uint32_t(refs.size(0)),
@@ -500,8 +511,9 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits,
               *m = f32(min_p, "min_p");
   const c10::cuda::CUDAGuard guard(logits.device());
   const auto X = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
-  auto tokens = torch::empty({rows}, X.options().dtype(torch::kInt32));
-  auto logprobs = torch::empty({rows}, X.options().dtype(torch::kFloat32));
+  auto tokens = empty_i32({rows}, X.device());
+  auto logprobs =
+      at::Tensor(at::detail::empty_cuda({rows}, torch::kFloat32, X.device(), std::nullopt));
   const auto type = X.dtype() == torch::kFloat32 ? felix::ElementType::F32 : half_type(X, "logits");
   const auto status = felix::sample_launch(
       X.data_ptr(), type, uint32_t(rows), uint32_t(X.size(1)), X.stride(0),
