@@ -234,28 +234,37 @@ struct Row {
   const T* g;     // the row
   const T* s;     // token lo in shared memory
   uint32_t lo, n;
-  uint32_t pad;   // s is this many elements past a 16-byte boundary
+  uint32_t pad;   // the part starts this many elements past a 16-byte boundary
   __device__ __forceinline__ float at(uint32_t j) const {
     return plain(to_f<T>(kStaged ? s[j] : g[lo + j]));
   }
-  // f(value, j) for the CTA's tokens, spread over its threads, 16 bytes at a time.
-  // Values come as they are: NaN and -0 among them.
+  // f(value, j) for the CTA's tokens, spread over its threads: 16 bytes at a time,
+  // kBatch loads under way in a thread, the ends one by one. Values come as they are:
+  // NaN and -0 among them.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    if constexpr (kStaged) {
-      constexpr uint32_t kPer = 16 / sizeof(T);
-      const uint4* from = reinterpret_cast<const uint4*>(s - pad);
-      const uint32_t vecs = (pad + n + kPer - 1) / kPer;
-      for (uint32_t v = threadIdx.x; v < vecs; v += kThreads) {
-        const uint4 w = from[v];
-        const T* e = reinterpret_cast<const T*>(&w);
-        const uint32_t j = v * kPer - pad;
+    constexpr uint32_t kPer = 16 / sizeof(T), kBatch = kStaged ? 1 : 4;
+    const T* src = kStaged ? s : g + lo;
+    const uint32_t head = min((kPer - pad) % kPer, n), vecs = (n - head) / kPer;
+    const uint32_t ends = n - vecs * kPer;
+    const uint4* from = reinterpret_cast<const uint4*>(src + head);
+    for (uint32_t v0 = threadIdx.x; v0 < vecs; v0 += kBatch * kThreads) {
+      uint4 w[kBatch];
 #pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i)
-          if (j + i < n) f(to_f<T>(e[i]), j + i);  // j wraps below 0
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (v0 + k * kThreads < vecs) w[k] = from[v0 + k * kThreads];
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) {
+        const uint32_t v = v0 + k * kThreads;
+        if (v >= vecs) break;
+        const T* e = reinterpret_cast<const T*>(&w[k]);
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) f(to_f<T>(e[i]), head + v * kPer + i);
       }
-    } else {
-      for (uint32_t j = threadIdx.x; j < n; j += kThreads) f(to_f<T>(g[lo + j]), j);
+    }
+    for (uint32_t i = threadIdx.x; i < ends; i += kThreads) {
+      const uint32_t j = i < head ? i : n - ends + i;
+      f(to_f<T>(src[j]), j);
     }
   }
 };
@@ -282,13 +291,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
   // ---- the maximum, and the part into shared memory: 16 bytes at a time, at the
   // same offset from a 16-byte boundary in both memories
   float top = -INFINITY;
+  x.pad = uint32_t(reinterpret_cast<uintptr_t>(x.g + x.lo) & 15) / sizeof(T);
   if (kStaged) {
     constexpr uint32_t kPer = 16 / sizeof(T);
     const T* src = x.g + x.lo;
-    const uint32_t pad = uint32_t(reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T);
+    const uint32_t pad = x.pad;
     T* dst = reinterpret_cast<T*>(raw + ((sizeof(Shared) + 15) & ~size_t(15)));
     x.s = dst + pad;
-    x.pad = pad;
     const uint32_t vecs = (pad + x.n + kPer - 1) / kPer;
     const uint4* from = reinterpret_cast<const uint4*>(src - pad);
 #pragma unroll 4
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
       }
     }
   } else {
-    for (uint32_t j = tid; j < x.n; j += kThreads) top = fmaxf(top, x.at(j));
+    x.each([&](float v, uint32_t) { top = fmaxf(top, v); });
   }
   for (int b = tid; b < kBins; b += kThreads) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
 #pragma unroll
@@ -549,8 +558,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
     const Cut cut = pick(0, false, double(k), 0, 0, V);
     few = cut.before + cut.count <= uint32_t(kList);
     if (few) {
-      // the smallest value in the bin: bins go up as values go down
+      // The smallest value in the bin: bins go up as values go down. It is a few
+      // roundings from top - (bin + 1) / to_bin; where that does not bracket it, the
+      // whole range of values does.
       uint32_t low = key_of(-INFINITY), high = key_of(top);
+      const float guess = top - float(cut.bin + 1) / to_bin;
+      if (guess < top && guess > -INFINITY) {
+        const uint32_t l = max(key_of(guess - 1e-5f * (fabsf(top) + fabsf(guess))), low);
+        const uint32_t h = min(key_of(guess + 1e-5f * (fabsf(top) + fabsf(guess))), high);
+        if (bin_of(value_of(l)) > cut.bin) low = l;
+        if (bin_of(value_of(h)) <= cut.bin) high = h;
+      }
       while (cut.bin < kBins && low < high) {
         const uint32_t mid = low + (high - low) / 2;
         if (bin_of(value_of(mid)) <= cut.bin) high = mid;
@@ -713,17 +731,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 template <typename T>
 FelixCode launch(const SampleArgs& a, DeviceInfo* dev, cudaStream_t stream) {
   const size_t fixed = (sizeof(Shared) + 15) & ~size_t(15);
-  // As many CTAs per row as fill the GPU, at least so many that the row fits their
-  // shared memory, and none with less than 2048 tokens.
+  // Enough CTAs that every SM has one, as long as each has 4096 tokens or more; at most
+  // 65536 tokens in each (the histogram's sums) and 128 KB. Parts of which two fit
+  // an SM's shared memory are staged there; larger ones (many rows of a large
+  // vocabulary) are read again through the L2, which holds what 128 KB a CTA add up to:
+  // 256 rows of 131072 fp32 take 228 us in clusters of 8 that stage, waiting for one
+  // another, 160 us in clusters of 4 that do not, and 157 to 245 us in pairs, whose
+  // parts leave the L2 before they are read again.
   uint32_t C = 1;
-  const uint32_t want = uint32_t(dev->num_sms) * 2;
   auto bytes = [&](uint32_t c) {
     return fixed + (size_t(((a.vocab + c - 1) / c + 7) & ~7u) + 16) * sizeof(T);
   };
-  while (C < kMaxCtas && ((a.rows * uint64_t(C) < want && a.vocab / C > 4096) ||
-                          bytes(C) > 72 * 1024))
+  while (C < kMaxCtas && ((a.rows * uint64_t(C) < uint32_t(dev->num_sms) && a.vocab / C > 4096) ||
+                          a.vocab / C > 65536 || a.vocab / C * sizeof(T) > 128 * 1024))
     C *= 2;
-  const bool staged = bytes(C) <= size_t(dev->max_smem_optin);
+  const bool staged = bytes(C) <= 110 * 1024;
   static PerDeviceOnce once;
   const int rc = once.run(dev->ordinal, [&] {
     return cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
