@@ -142,78 +142,78 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const TokenParams P) {
   const int lane = threadIdx.x & 31, part = lane % kLanes;
   const uint32_t head = blockIdx.y, nth = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   for (uint32_t slot = blockIdx.z; slot < P.c.slots; slot += gridDim.z) {
-  const int len = slot_length(P.c, slot);
-  const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
-  const int start = len - count;  // token of row 0; tokens before 0 have no place
-  const int from = max(start, 0), t0 = (from / int(kBlock) + int(nth)) * int(kBlock);
-  if (t0 >= len || count <= 0) continue;
-  unsigned char* blk = block_of(P.c, slot, t0, head, D);
-  if (!blk) continue;
-  const int i1 = (min(len - t0, int(kBlock)) + 3) / 4;
-  for (int i = max(from - t0, 0) / 4; i < i1; ++i) {
-    const uint32_t r = 4 * i + lane / kLanes;
-    const int token = t0 + int(r), row = token - start;
-    const bool mine = token >= from && token < len;
-    float both_x[2][N];
+    const int len = slot_length(P.c, slot);
+    const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
+    const int start = len - count;  // token of row 0; tokens before 0 have no place
+    const int from = max(start, 0), t0 = (from / int(kBlock) + int(nth)) * int(kBlock);
+    if (t0 >= len || count <= 0) continue;
+    unsigned char* blk = block_of(P.c, slot, t0, head, D);
+    if (!blk) continue;
+    const int i1 = (min(len - t0, int(kBlock)) + 3) / 4;
+    for (int i = max(from - t0, 0) / 4; i < i1; ++i) {
+      const uint32_t r = 4 * i + lane / kLanes;
+      const int token = t0 + int(r), row = token - start;
+      const bool mine = token >= from && token < len;
+      float both_x[2][N];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int64_t* st = which ? P.vs : P.ks;
-      const T* src = static_cast<const T*>(which ? P.v : P.k) + int64_t(slot) * st[0] +
-                     int64_t(head) * st[1] + int64_t(row) * st[2] + part * N;
-      float (&x)[N] = both_x[which];
-      if (mine && P.vec) {
+      for (int which = 0; which < 2; ++which) {
+        const int64_t* st = which ? P.vs : P.ks;
+        const T* src = static_cast<const T*>(which ? P.v : P.k) + int64_t(slot) * st[0] +
+                       int64_t(head) * st[1] + int64_t(row) * st[2] + part * N;
+        float (&x)[N] = both_x[which];
+        if (mine && P.vec) {
 #pragma unroll
-        for (int j = 0; j < N / 8; ++j) {
-          const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + j);
-          const T* e = reinterpret_cast<const T*>(&w);
+          for (int j = 0; j < N / 8; ++j) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src) + j);
+            const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-          for (int y = 0; y < 8; ++y) x[8 * j + y] = to_f<T>(e[y]);
-        }
-      } else {
+            for (int y = 0; y < 8; ++y) x[8 * j + y] = to_f<T>(e[y]);
+          }
+        } else {
 #pragma unroll
-        for (int y = 0; y < N; ++y) x[y] = mine ? to_f<T>(src[y]) : 0.f;
-      }
-    }
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      float (&x)[N] = both_x[which];
-      uint32_t w[N / 8];
-      const uint32_t par = quantise<N>(x, w);
-      if (which == 0) {
-        if (mine) {
-          if constexpr (N == 16)
-            *reinterpret_cast<uint2*>(blk + r * (D / 2) + part * 8) = make_uint2(w[0], w[1]);
-          else
-            *reinterpret_cast<uint32_t*>(blk + r * (D / 2) + part * 4) = w[0];
-        }
-      } else {
-        // four codes of this token and of the pair's other one make a word
-        unsigned char* dst = blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) +
-                             (r % 8 / 2) * (D / 8);
-        const bool both = __shfl_xor_sync(~0u, int(mine), kLanes) && mine;
-        uint32_t o[N / 8], pair[N / 4];
-#pragma unroll
-        for (int j = 0; j < N / 8; ++j) {
-          o[j] = __shfl_xor_sync(~0u, w[j], kLanes);
-          pair[2 * j] = (w[j] & 0xffffu) | (o[j] << 16);
-          pair[2 * j + 1] = (w[j] >> 16) | (o[j] & 0xffff0000u);
-        }
-        if (both && !(r & 1)) {
-          if constexpr (N == 16)
-            *reinterpret_cast<uint4*>(dst) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
-          else
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pair[0], pair[1]);
-        } else if (mine && !both) {
-#pragma unroll
-          for (int j = 0; j < N / 4; ++j)
-            *reinterpret_cast<uint16_t*>(dst + 4 * j + 2 * (r & 1)) =
-                uint16_t(w[j / 2] >> (16 * (j % 2)));
+          for (int y = 0; y < N; ++y) x[y] = mine ? to_f<T>(src[y]) : 0.f;
         }
       }
-      if (mine && part == 0)
-        reinterpret_cast<uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D)))[r] = par;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        float (&x)[N] = both_x[which];
+        uint32_t w[N / 8];
+        const uint32_t par = quantise<N>(x, w);
+        if (which == 0) {
+          if (mine) {
+            if constexpr (N == 16)
+              *reinterpret_cast<uint2*>(blk + r * (D / 2) + part * 8) = make_uint2(w[0], w[1]);
+            else
+              *reinterpret_cast<uint32_t*>(blk + r * (D / 2) + part * 4) = w[0];
+          }
+        } else {
+          // four codes of this token and of the pair's other one make a word
+          unsigned char* dst = blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) +
+                               (r % 8 / 2) * (D / 8);
+          const bool both = __shfl_xor_sync(~0u, int(mine), kLanes) && mine;
+          uint32_t o[N / 8], pair[N / 4];
+#pragma unroll
+          for (int j = 0; j < N / 8; ++j) {
+            o[j] = __shfl_xor_sync(~0u, w[j], kLanes);
+            pair[2 * j] = (w[j] & 0xffffu) | (o[j] << 16);
+            pair[2 * j + 1] = (w[j] >> 16) | (o[j] & 0xffff0000u);
+          }
+          if (both && !(r & 1)) {
+            if constexpr (N == 16)
+              *reinterpret_cast<uint4*>(dst) = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+            else
+              *reinterpret_cast<uint2*>(dst) = make_uint2(pair[0], pair[1]);
+          } else if (mine && !both) {
+#pragma unroll
+            for (int j = 0; j < N / 4; ++j)
+              *reinterpret_cast<uint16_t*>(dst + 4 * j + 2 * (r & 1)) =
+                  uint16_t(w[j / 2] >> (16 * (j % 2)));
+          }
+        }
+        if (mine && part == 0)
+          reinterpret_cast<uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D)))[r] = par;
+      }
     }
-  }
   }
 }
 
@@ -225,54 +225,57 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const TokenParams P) {
   const uint32_t head = blockIdx.y, row = (blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
   if (row >= P.rows) return;
   for (uint32_t slot = blockIdx.z; slot < P.c.slots; slot += gridDim.z) {
-  const uint64_t item = (uint64_t(slot) * P.c.kv_heads + head) * P.rows + row;
-  const int len = slot_length(P.c, slot);
-  const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
-  const int token = len - count + int(row);
-  const unsigned char* blk = (int(row) < count && token >= 0)
-                                 ? block_of(P.c, slot, token, head, D) : nullptr;
-  const uint32_t r = uint32_t(token) % kBlock;
+    const uint64_t item = (uint64_t(slot) * P.c.kv_heads + head) * P.rows + row;
+    const int len = slot_length(P.c, slot);
+    const int count = P.counts ? min(P.counts[slot], int(P.rows)) : int(P.rows);
+    const int token = len - count + int(row);
+    const unsigned char* blk = (int(row) < count && token >= 0)
+                                   ? block_of(P.c, slot, token, head, D) : nullptr;
+    const uint32_t r = uint32_t(token) % kBlock;
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    uint32_t w[N / 8] = {};
-    float2 sb = make_float2(0.f, 0.f);
-    if (blk) {
-      if (which == 0) {
+    for (int which = 0; which < 2; ++which) {
+      uint32_t w[N / 8] = {};
+      float2 sb = make_float2(0.f, 0.f);
+      if (blk) {
+        if (which == 0) {
 #pragma unroll
-        for (int j = 0; j < N / 8; ++j)
-          w[j] = __ldg(reinterpret_cast<const uint32_t*>(blk + r * (D / 2) + part * (N / 2)) + j);
-      } else {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(
-            blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) + (r % 8 / 2) * (D / 8) +
-            2 * (r & 1));
+          for (int j = 0; j < N / 8; ++j)
+            w[j] = __ldg(reinterpret_cast<const uint32_t*>(blk + r * (D / 2) + part * (N / 2)) + j);
+        } else {
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(
+              blk + v_codes_at(D) + (r / 8) * 4 * D + part * (D / 2) + (r % 8 / 2) * (D / 8) +
+              2 * (r & 1));
 #pragma unroll
-        for (int j = 0; j < N / 4; ++j) w[j / 2] |= uint32_t(__ldg(src + 2 * j)) << (16 * (j % 2));
+          for (int j = 0; j < N / 4; ++j)
+            w[j / 2] |= uint32_t(__ldg(src + 2 * j)) << (16 * (j % 2));
+        }
+        const uint32_t par = __ldg(
+            reinterpret_cast<const uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D))) + r);
+        sb = __half22float2(*reinterpret_cast<const __half2*>(&par));
       }
-      const uint32_t par = __ldg(
-          reinterpret_cast<const uint32_t*>(blk + (which ? v_params_at(D) : k_params_at(D))) + r);
-      sb = __half22float2(*reinterpret_cast<const __half2*>(&par));
-    }
-    // 2^23 + code by its bits, less 2^23 + 8; scale times that is exact
-    alignas(16) __half2 out[N / 2];
-    const auto less = f2(-8388616.f, -8388616.f), scale = f2(sb.x, sb.x), base = f2(sb.y, sb.y);
+      // 2^23 + code by its bits, less 2^23 + 8; scale times that is exact
+      alignas(16) __half2 out[N / 2];
+      const auto less = f2(-8388616.f, -8388616.f), scale = f2(sb.x, sb.x), base = f2(sb.y, sb.y);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint32_t v = w[i / 8] >> (4 * (i % 8));
-      const auto c = add2(f2(__uint_as_float((v & 15u) | 0x4b000000u),
-                             __uint_as_float((v >> 4 & 15u) | 0x4b000000u)), less);
-      const float2 y = un2(fma2(scale, c, base));
-      out[i / 2] = __floats2half2_rn(y.x, y.y);
-    }
-    uint4* dst = reinterpret_cast<uint4*>((which ? P.vo : P.ko) + item * D + part * N);
+      for (int i = 0; i < N; i += 2) {
+        const uint32_t v = w[i / 8] >> (4 * (i % 8));
+        const auto c = add2(f2(__uint_as_float((v & 15u) | 0x4b000000u),
+                               __uint_as_float((v >> 4 & 15u) | 0x4b000000u)), less);
+        const float2 y = un2(fma2(scale, c, base));
+        out[i / 2] = __floats2half2_rn(y.x, y.y);
+      }
+      uint4* dst = reinterpret_cast<uint4*>((which ? P.vo : P.ko) + item * D + part * N);
 #pragma unroll
-    for (int j = 0; j < N / 8; ++j) dst[j] = reinterpret_cast<const uint4*>(out)[j];
-  }
+      for (int j = 0; j < N / 8; ++j) dst[j] = reinterpret_cast<const uint4*>(out)[j];
+    }
   }
 }
 
 // ---------------------------------------------------------------------- copies
 // Pages src[i] of one pool to dst[i] of another (or the same), `count` of them
-// (known on the device). Work is cut in chunks of 16 KB.
+// (known on the device). Work is cut in chunks of 16 KB. 515 pages of 35 KB take 5.4 us
+// in a graph (floor 5.5 at the card's copy rate; part of it stays in the L2), the 776
+// moved by a compaction of 6007 pages of 70 KB 19 us (16.5).
 constexpr uint32_t kChunk = 16384;
 
 __global__ void __launch_bounds__(256) kv4_copy_kernel(
@@ -295,7 +298,9 @@ __global__ void __launch_bounds__(256) kv4_copy_kernel(
 // ------------------------------------------------------------- page operations
 // One cluster of kCtas CTAs does each: scans over refs and slots run in the
 // CTAs, their totals are exchanged through distributed shared memory, and the
-// cluster barrier orders global reads and writes between the steps.
+// cluster barrier orders global reads and writes between the steps. Barriers and
+// dependent loads bound them: in a graph free, fork (with its copies) and reserve
+// take 20 us together for 16 slots and 1024 pages, 42 us for 512 slots and 65536.
 constexpr int kCtas = 8;
 constexpr int kMeta = 1024;
 
@@ -381,7 +386,8 @@ __device__ __forceinline__ void load_run(const int32_t* refs, uint32_t p0, uint3
 
 // Counts the CTA's pages for which f holds, two predicates at once.
 template <class F, class G>
-__device__ __forceinline__ void count_pages(const int32_t* refs, Range r, MetaShared& sh, F f, G g) {
+__device__ __forceinline__ void count_pages(const int32_t* refs, Range r, MetaShared& sh, F f,
+                                            G g) {
   uint32_t nf = 0, ng = 0, sum;
   for (uint32_t p0 = r.lo + threadIdx.x * kRun; p0 < r.hi; p0 += kPass) {
     int v[kRun];
@@ -481,7 +487,8 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
     const int then = fits ? pages_for(more, P.page_shift) : now;
     const int32_t* in = P.table + size_t(s) * P.width;
     int32_t* out = P.table_out + size_t(s) * P.width;
-    const int lo = P.table == P.table_out ? now : 0, hi = P.table == P.table_out ? then : int(P.width);
+    const bool inplace = P.table == P.table_out;
+    const int lo = inplace ? now : 0, hi = inplace ? then : int(P.width);
 #pragma unroll 4
     for (int j = lo + int(threadIdx.x & 31); j < min(hi, int(P.width)); j += 32)
       out[j] = j >= now && j < then ? P.fresh[P.start[s] + j - now] : in[j];
@@ -722,7 +729,8 @@ FelixCode kv4_append_launch(const felix_kv4::CacheView& c, uint32_t head_dim, co
   if (grid.z == 0 || rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
   const int threads = P.blocks < 8 ? int(P.blocks) * 32 : 256;
   if (bf16) {
-    if (head_dim == 128) kv4::kv4_append_kernel<__nv_bfloat16, 128><<<grid, threads, 0, stream>>>(P);
+    if (head_dim == 128)
+      kv4::kv4_append_kernel<__nv_bfloat16, 128><<<grid, threads, 0, stream>>>(P);
     else kv4::kv4_append_kernel<__nv_bfloat16, 64><<<grid, threads, 0, stream>>>(P);
   } else {
     if (head_dim == 128) kv4::kv4_append_kernel<__half, 128><<<grid, threads, 0, stream>>>(P);
@@ -763,7 +771,8 @@ FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {
   P.table_out = o.table_out, P.lens_out = o.lens_out, P.refs_out = o.refs_out;
   P.status = o.status;
   P.a = o.a, P.b = o.b;
-  P.slots = o.slots, P.width = o.width, P.pages = o.num_pages, P.page_shift = o.page_shift, P.n = o.n;
+  P.slots = o.slots, P.width = o.width, P.pages = o.num_pages;
+  P.page_shift = o.page_shift, P.n = o.n;
   FelixCode rc = kv4::scratch(dev, P, stream);
   if (rc.type != FELIX_SUCCESS) return rc;
   using namespace kv4;

@@ -17,18 +17,20 @@
 // All three filters keep a prefix of the order, so together they are a threshold
 // on (value, index), held as one 64-bit number that is larger for what comes first.
 //
-// A cluster of CTAs shares a row, and each keeps its part in shared memory: the
-// logits are read from HBM once. Thresholds come from a histogram over the distance
-// from the maximum (2048 bins up to where masses round to 0; even in value, so that
-// few tokens share a bin), which every CTA merges for itself. Where a bin holds too
-// many (equal values, a flat row) it is split again into 2048 by (value, index)
-// until it does not.
+// A cluster of CTAs shares a row, and each keeps its part in shared memory (or, where
+// that is too large, reads it again through the L2): the logits come from HBM once.
+// Thresholds come from a histogram over the distance from the maximum (2048 bins up to
+// where masses round to 0; even in value, so that few tokens share a bin), merged over
+// the cluster by slices. Where a bin holds too many (equal values, a flat row) it is
+// split again into 2048 by (value, index) until it does not.
 //   top-k of up to 1024 (with or without the others): tokens are counted only, no
 //   exponentials; those down to the bin in which the k-th falls go to the first CTA
-//   of the cluster, which sorts them and finishes alone.
+//   of the cluster, which sorts them and finishes alone. 1 x 32000 fp16: 16 us (21 by
+//   one CTA); 256 x 131072 fp32: 152 us for 134 MB, 13 % of the card's copy rate: three
+//   passes of 64 values a thread, barriers, and 15 us of the first CTA alone.
 //   else: the bins' masses are summed too; the tokens of the bin in which top-p (or a
-//   large top-k) cuts, a few dozen as a rule, are gathered and sorted by every CTA, and a last
-//   pass sums what stays.
+//   large top-k) cuts, a few dozen as a rule, are gathered and sorted by every CTA, and
+//   a last pass sums what stays. 33 x 50021 bf16: 41 us, whatever the cluster's size.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
