@@ -15,14 +15,19 @@
 // the instruction, and the scores' registers become the other operand of the
 // second product by an 8 x 8 transpose in the warp.
 //
-// Rounding. p_t scale_v is rounded to fp16, P_t, for the second product. Its
-// exponent is taken out first (the running maximum is that of score + exponent of
-// scale_v), so that neither tiny nor huge values lose bits. The result is
+// Rounding. p_t scale_v is rounded to fp16's 11 bits, P_t, for the second product.
+// Its exponent is taken out first (the running maximum is that of score + exponent
+// of scale_v). The result is
 //   (sum P (c - 8) + sum P base_v / scale_v) / sum P / scale_v,
 // the mean of the held values under the weights P / scale_v: rounded weights in
 // the numerator and the denominator, so that a row that one token rules has no
-// error from them. The log-sum-exp has its own sum of unrounded p. Sums and
-// statistics are fp32.
+// error from them. P is rounded with fp32's exponents, so that a weight keeps its 11
+// bits however far it is below the others. Only its copy for the product with (c - 8) goes
+// through fp16, where what is 2^-20 of the largest P (2^6 or more) is subnormal and
+// loses at most 2^-25: 2^-31 of the largest token's share, for each such token. (With
+// the weights taken from that copy too, a token whose scale is 2^-30 of another's
+// left the denominator, as if it were masked.) The log-sum-exp has its own sum of
+// unrounded p. Sums and statistics are fp32.
 //
 // Measured: 96 slots of up to 12288 tokens, 8 heads of 128: 129 to 137 us for 585 MB
 // (65 to 69 % of the card's copy rate; its loads alone take 100 us), 507 instructions a
@@ -124,6 +129,16 @@ __device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
   F2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
+}
+// Rounded to 11 bits, whatever the exponent: TF32 has fp16's significand and fp32's
+// exponents. (96 slots 137 us, 131071 x 40 rows 328; by Veltkamp's splitting 138 and
+// 332. Weights from the fp16 copy, wrong below 2^-14: 137 and 311.)
+__device__ __forceinline__ F2 round11(F2 a) {
+  const float2 x = un(a);
+  uint32_t r0, r1;
+  asm("cvt.rn.tf32.f32 %0, %1;" : "=r"(r0) : "f"(x.x));
+  asm("cvt.rn.tf32.f32 %0, %1;" : "=r"(r1) : "f"(x.y));
+  return f2(__uint_as_float(r0), __uint_as_float(r1));
 }
 
 template <int W>
@@ -337,8 +352,7 @@ struct Attn {
       };
       if (NT == 1) exponents();
       // Exponents are relative to m, 2^6 below a maximum that is only moved when a
-      // score passes it by 2^8: P stays below 2^15, and fp16 holds what is 2^30
-      // smaller.
+      // score passes it by 2^8: P stays below 2^15.
       if (__any_sync(~0u, t0 > m[n][0] + 14.f || t1 > m[n][1] + 14.f)) {
         float keep[2];
 #pragma unroll
@@ -380,10 +394,9 @@ struct Attn {
           }
           const F2 ee = f2(e[k][h].x, e[k][h].y);
           l[n] = fma(ee, inv, l[n]);
-          const float2 p = un(mul(ee, v.a));
-          const __half2 ph = __floats2half2_rn(p.x, p.y);
-          const float2 pr = __half22float2(ph);
-          const F2 P = f2(pr.x, pr.y);
+          const F2 P = round11(mul(ee, v.a));
+          const float2 pr = un(P);
+          const __half2 ph = __floats2half2_rn(pr.x, pr.y);  // exact but below 2^-14
           w[n] = fma(P, v.b, w[n]);
           b[n] = fma(P, base, b[n]);
           pt[n][k][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&ph));
