@@ -178,13 +178,15 @@ __device__ __forceinline__ float2 k_params(uint32_t p) {
 struct VParams {
   float e, inv, mant, rcp, base;
 };
-// A vector of equal values (scale 0) has all codes 8 and adds nothing beside its
-// base: any scale does, 1 is taken.
+// A vector of scale 0 is its base, whatever its codes (8 where it was appended, 0 in
+// a page that nobody has written). 2^-60 stands in for the scale: codes then add
+// nothing that shows, and the exponent leaves the maximum to the others, whose P a
+// likely token of zeros would otherwise push out of fp16's range.
 __device__ __forceinline__ VParams v_params(uint32_t p) {
   float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-  if (f.x == 0.f) f.x = 1.f;
-  // scales are not negative; a NaN counts as fp16's largest exponent
-  const int e = min(int(__float_as_uint(f.x) >> 23) - 127, 16);
+  if (f.x == 0.f) f.x = 0x1p-60f;
+  // a NaN counts as fp16's largest exponent
+  const int e = min(int(__float_as_uint(f.x) >> 23 & 255) - 127, 16);
   VParams r;
   r.e = float(e);
   r.inv = __int_as_float((127 - e) << 23);

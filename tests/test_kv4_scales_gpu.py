@@ -95,7 +95,7 @@ def test_equal_probabilities(dtype, D, rows, group, big, small):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("D,rows,group", [(128, 1, 4), (64, 5, 8)])
-@pytest.mark.parametrize("score", [8.0, 16.0])
+@pytest.mark.parametrize("score", [8.0, 16.0, 24.0])
 def test_unlikely_large_values_and_likely_small_ones(dtype, D, rows, group, score):
     # the small tokens are exp(score) times as likely as the large one, whose values
     # are about that much larger, so that both make the result; and the reverse
