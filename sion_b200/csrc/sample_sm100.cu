@@ -47,6 +47,15 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCtas = 8;
 constexpr int kMost = 1024;  // tokens of a bin that are sorted: two per thread
+// Tokens of a CTA at most: the low halves of as many masses fit 32 bits. A vocabulary
+// of kMaxCtas * kMaxPart, the largest that is taken, has parts of just that.
+constexpr uint32_t kMaxPart = 65536;
+static_assert(uint64_t(kMaxPart) * 0xffff <= 0xffffffffu);
+// Tokens of a CTA where C share a row of V; the last ones may have fewer.
+__host__ __device__ constexpr uint32_t part_of(uint32_t V, uint32_t C) {
+  return ((V + C - 1) / C + 7) & ~7u;
+}
+static_assert(part_of(524288, kMaxCtas) == kMaxPart);
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -102,7 +111,7 @@ constexpr int kList = 1024;      // tokens that it sorts
 
 struct Shared {
   // Tokens of a bin, and their masses as sums of the low 16 and of the high bits: 32
-  // bits hold those of 65536 tokens, the most that a CTA has (vocab <= 8 * 65536).
+  // bits hold those of kMaxPart tokens.
   alignas(16) uint32_t count[kBins];
   union {
     struct {
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 
   Row<T, kStaged> x;
   x.g = static_cast<const T*>(A.logits) + int64_t(row) * A.stride;
-  const uint32_t run = ((V + C - 1) / C + 7) & ~7u;
+  const uint32_t run = part_of(V, C);
   x.lo = min(rank * run, V);
   x.n = min(run, V - x.lo);
 
@@ -733,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs A)
 template <typename T>
 FelixCode launch(const SampleArgs& a, DeviceInfo* dev, cudaStream_t stream) {
   const size_t fixed = (sizeof(Shared) + 15) & ~size_t(15);
-  // Enough CTAs that every SM has one, as long as each has 4096 tokens or more; at most
-  // 65536 tokens in each (the histogram's sums) and 128 KB. Parts of which two fit
+  // Enough CTAs that every SM has one, as long as each has 2048 tokens or more; at most
+  // kMaxPart tokens in each (the histogram's sums) and about 128 KB. Parts of which two fit
   // an SM's shared memory are staged there; larger ones (many rows of a large
   // vocabulary) are read again through the L2, which holds what 128 KB a CTA add up to:
   // 256 rows of 131072 fp32 take 228 us in clusters of 8 that stage, waiting for one
@@ -742,10 +751,11 @@ FelixCode launch(const SampleArgs& a, DeviceInfo* dev, cudaStream_t stream) {
   // parts leave the L2 before they are read again.
   uint32_t C = 1;
   auto bytes = [&](uint32_t c) {
-    return fixed + (size_t(((a.vocab + c - 1) / c + 7) & ~7u) + 16) * sizeof(T);
+    return fixed + (size_t(part_of(a.vocab, c)) + 16) * sizeof(T);
   };
   while (C < kMaxCtas && ((a.rows * uint64_t(C) < uint32_t(dev->num_sms) && a.vocab / C > 4096) ||
-                          a.vocab / C > 65536 || a.vocab / C * sizeof(T) > 128 * 1024))
+                          part_of(a.vocab, C) > kMaxPart ||
+                          a.vocab / C * sizeof(T) > 128 * 1024))
     C *= 2;
   const bool staged = bytes(C) <= 110 * 1024;
   static PerDeviceOnce once;
