@@ -274,7 +274,8 @@ int felix_kv4_attention_workspace_size(uint32_t head_dim, size_t* bytes);
  *   reserve: lens grows by counts and each slot gets the pages for that (pages
  *            past a slot's width count as missing).
  *   fork:    slot children[i] becomes a copy of slot parents[i]: whole pages are
- *            shared, a last page that is not full is copied to a fresh one.
+ *            shared, a last page that is not full is copied to a fresh one (where
+ *            the table names no page for it, the child has none there either).
  *            Skipped: numbers out of range, a child that holds tokens, is its
  *            parent or was named before.
  *   free:    the listed slots become empty; pages that no slot holds any more

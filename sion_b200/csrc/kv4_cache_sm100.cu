@@ -525,6 +525,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kMeta, 1)
       if (valid) len = max(P.lens[p], 0);
       const uint32_t whole = uint32_t(len) >> P.page_shift;
       need = valid && (uint32_t(len) & ((1u << P.page_shift) - 1)) != 0 && whole < P.width;
+      // a last page that is not in the pool is missing in the copy too: a fresh one
+      // would show what its tokens held for an earlier slot
+      if (need) {
+        const int last = P.table[size_t(p) * P.width + whole];
+        need = last >= 0 && uint32_t(last) < P.pages;
+      }
     }
     uint32_t sum, sum2;
     const uint32_t at = want + scan(need, sh, &sum);
