@@ -11,6 +11,8 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <thread>
+#include <tuple>
 #include <utility>
 
 #include "felix_internal.h"
@@ -31,10 +33,14 @@ DeviceInfo g_dev[64];
 bool g_dev_ready[64] = {false};
 
 struct WsEntry {
+  std::mutex mu;  // held by a call from here to its last launch
   void* ptr = nullptr;
   size_t bytes = 0;
 };
-std::map<std::pair<int, cudaStream_t>, WsEntry> g_ws;
+// Device, stream, and the host thread where the handle stands for each thread's own
+// stream. Entries stay: a map's elements do not move.
+using WsKey = std::tuple<int, cudaStream_t, std::thread::id>;
+std::map<WsKey, WsEntry> g_ws;
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -83,10 +89,17 @@ DeviceInfo* current_device_info() {
   return &g_dev[d];
 }
 
-void* library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes) {
+static WsEntry& workspace_entry(int device, cudaStream_t stream) {
+  const auto thread =
+      stream == cudaStreamPerThread ? std::this_thread::get_id() : std::thread::id();
   std::lock_guard<std::mutex> lk(g_mu);
-  WsEntry& w = g_ws[{dev->ordinal, stream}];
-  if (w.bytes >= bytes) return w.ptr;
+  return g_ws[WsKey(device, stream, thread)];
+}
+
+Workspace library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes) {
+  WsEntry& w = workspace_entry(dev->ordinal, stream);
+  std::unique_lock<std::mutex> lk(w.mu);
+  if (w.bytes >= bytes) return {w.ptr, std::move(lk)};
   if (w.ptr) {
     // The old buffer may still be in use by work queued on this stream.
     cudaStreamSynchronize(stream);
@@ -97,11 +110,11 @@ void* library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes) {
   size_t sz = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
   if (cudaMalloc(&w.ptr, sz) != cudaSuccess) {
     w.ptr = nullptr;
-    return nullptr;
+    return {};
   }
-  if (cudaMemsetAsync(w.ptr, 0, sz, stream) != cudaSuccess) return nullptr;
+  if (cudaMemsetAsync(w.ptr, 0, sz, stream) != cudaSuccess) return {};
   w.bytes = sz;
-  return w.ptr;
+  return {w.ptr, std::move(lk)};
 }
 
 static int encode_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,

@@ -63,9 +63,18 @@ DeviceInfo* current_device_info();
 constexpr size_t kWsCounterBytes = 16384;
 constexpr uint32_t kWsMaxCounters = kWsCounterBytes / 4;
 
+// The library's scratch, held by one call: to be kept until the call's last launch.
+// Another host thread that uses the same stream waits for it, so that it neither
+// puts a launch of its own between two that hand data on through the scratch nor
+// replaces the buffer before a launch that was given it.
+struct Workspace {
+  void* ptr = nullptr;
+  std::unique_lock<std::mutex> held;
+};
 // Library-owned scratch for a (device, stream) pair, grown on demand and
-// zero-filled on (re)allocation. Kernels leave their counters at zero.
-void* library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes);
+// zero-filled on (re)allocation; ptr is null where there is no memory. Kernels
+// leave their counters at zero.
+Workspace library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes);
 
 // 2-D fp16 tensor map, 128-byte swizzle: inner extent `inner` elements,
 // `outer` rows, row pitch in bytes, box of box_inner x box_outer.

@@ -617,8 +617,10 @@ FelixCode flash_attn_bwd_launch(const __half* Q, const __half* K, const __half* 
 
   const size_t rows = size_t(bh) * seqlen;
   const size_t need = flash_attn_bwd_workspace_bytes(heads, batch, seqlen, head_dim);
+  Workspace scratch;  // until the last launch
   if (!workspace) {
-    workspace = library_workspace(dev, stream, need);
+    scratch = library_workspace(dev, stream, need);
+    workspace = scratch.ptr;
     if (!workspace) return launch_error(cudaErrorMemoryAllocation, "flash_attn_bwd: workspace");
   } else if (ws_bytes < need) {
     return api_error("flash_attn_bwd: workspace too small");

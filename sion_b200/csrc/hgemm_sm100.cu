@@ -1200,12 +1200,14 @@ FelixCode hgemm_launch(uint32_t M, uint32_t N, uint32_t K, float alpha, const __
   p.ksplit2 = pl.ksplit2 ? 1u : 0u;
   p.pair = pl.pair ? 1u : 0u;
   p.dyn = uses_dynamic_tiles(pl) ? 1u : 0u;
+  Workspace scratch;  // until the launch
   if (pl.sk_tiles || p.dyn) {
     if (uint64_t(pl.sk_tiles) * (pl.pair ? 2 : 1) > kWsMaxCounters - 2)
       return api_error("hgemm: too many stream-K tiles");
     const size_t need = workspace_need(pl);
     if (!workspace) {
-      workspace = library_workspace(dev, stream, need);
+      scratch = library_workspace(dev, stream, need);
+      workspace = scratch.ptr;
       if (!workspace) return launch_error(cudaErrorMemoryAllocation, "hgemm: workspace");
     } else if (ws_bytes < need) {
       return api_error("hgemm: workspace too small");

@@ -944,7 +944,9 @@ FelixCode launch(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_byte
   // the library's own is asked for at its largest, so that calls of other shapes do not
   // move it under a captured graph
   const size_t most = kv4_attention_workspace_bytes(128, dev->num_sms);
-  void* ws = workspace ? workspace : library_workspace(dev, stream, most);
+  Workspace scratch;  // until the launch
+  if (!workspace) scratch = library_workspace(dev, stream, most);
+  void* ws = workspace ? workspace : scratch.ptr;
   if (!ws) return launch_error(cudaErrorMemoryAllocation, "kv4_attention: workspace");
   P.counters = static_cast<uint32_t*>(ws);
   P.partials = reinterpret_cast<float*>(static_cast<char*>(ws) + kWsCounterBytes);

@@ -701,10 +701,10 @@ size_t scratch_bytes(uint32_t pages, uint32_t slots, uint32_t n) {
          sizeof(int32_t) * (size_t(pages) * 3 + size_t(slots) * 2 + size_t(n) * 4);
 }
 
-FelixCode scratch(DeviceInfo* dev, MetaParams& P, cudaStream_t stream) {
-  void* ws = library_workspace(dev, stream, scratch_bytes(P.pages, P.slots, P.n));
-  if (!ws) return launch_error(cudaErrorMemoryAllocation, "kv4: workspace");
-  char* p = static_cast<char*>(ws) + kWsCounterBytes;
+FelixCode scratch(DeviceInfo* dev, MetaParams& P, cudaStream_t stream, Workspace* ws) {
+  *ws = library_workspace(dev, stream, scratch_bytes(P.pages, P.slots, P.n));
+  if (!ws->ptr) return launch_error(cudaErrorMemoryAllocation, "kv4: workspace");
+  char* p = static_cast<char*>(ws->ptr) + kWsCounterBytes;
   P.moves = reinterpret_cast<uint32_t*>(p);
   P.fresh = reinterpret_cast<int32_t*>(p + 256);
   P.src = P.fresh + P.pages;
@@ -779,7 +779,8 @@ FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {
   P.a = o.a, P.b = o.b;
   P.slots = o.slots, P.width = o.width, P.pages = o.num_pages;
   P.page_shift = o.page_shift, P.n = o.n;
-  FelixCode rc = kv4::scratch(dev, P, stream);
+  Workspace ws;  // until the copies, which take their list from the plan, are launched
+  FelixCode rc = kv4::scratch(dev, P, stream, &ws);
   if (rc.type != FELIX_SUCCESS) return rc;
   using namespace kv4;
   switch (o.kind) {

@@ -804,10 +804,12 @@ FelixCode sgemm_launch(uint32_t M, uint32_t N, uint32_t K, float alpha, const fl
     if (e != cudaSuccess) return launch_error(e, "sgemm: launch failed");
     return FelixCode{FELIX_SUCCESS, cudaSuccess};
   };
+  Workspace scratch;  // until the launch
   auto attach = [&](size_t need) -> FelixCode {
     if (!workspace) {
       if (o.forbid_alloc) return api_error("sgemm: split-K scratch missing on an allocation-free call");
-      workspace = library_workspace(dev, stream, need);
+      scratch = library_workspace(dev, stream, need);
+      workspace = scratch.ptr;
       if (!workspace) return launch_error(cudaErrorMemoryAllocation, "sgemm: workspace");
     } else if (ws_bytes < need) {
       return api_error("sgemm: workspace too small");

@@ -746,7 +746,8 @@ FelixCode topk_select_launch(const float* data, float* out, uint32_t num_slices,
         data, out, slice_size, k, largest ? 1 : 0, staged, dev->status_word);
   } else {
     const size_t need = kWsCounterBytes + size_t(num_slices) * (256 * 4 + sizeof(SliceState));
-    uint8_t* ws = static_cast<uint8_t*>(library_workspace(dev, stream, need));
+    const Workspace scratch = library_workspace(dev, stream, need);  // until the last launch
+    uint8_t* ws = static_cast<uint8_t*>(scratch.ptr);
     if (!ws) return launch_error(cudaErrorMemoryAllocation, "topk: workspace");
     uint32_t* hist = reinterpret_cast<uint32_t*>(ws + kWsCounterBytes);
     SliceState* state = reinterpret_cast<SliceState*>(hist + size_t(num_slices) * 256);
