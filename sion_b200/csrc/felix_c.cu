@@ -74,6 +74,15 @@ FelixCode launch_error(cudaError_t e, const char* msg) {
 DeviceInfo* current_device_info() {
   int d = -1;
   if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) return nullptr;
+  // A host thread that has made no call of the runtime has no context yet, and
+  // encoding a tensor map, which is a call of the driver, would be refused there. The
+  // look-up gives it the device's (and leaves one that the caller has set as it is).
+  static thread_local int t_bound = -1;
+  if (t_bound != d) {
+    void* addr = nullptr;
+    if (cudaGetSymbolAddress(&addr, g_felix_watchdog_word) != cudaSuccess) return nullptr;
+    t_bound = d;
+  }
   std::lock_guard<std::mutex> lk(g_mu);
   if (!g_dev_ready[d]) {
     DeviceInfo& di = g_dev[d];

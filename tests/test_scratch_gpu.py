@@ -1,5 +1,5 @@
-"""The library's scratch: calls from several host threads, on one stream and on each
-thread's own."""
+"""Calls from several host threads, on one stream and on each thread's own: the
+library's scratch, and threads that have not used CUDA before."""
 import ctypes as C
 import threading
 
@@ -127,3 +127,50 @@ def test_attention_of_host_threads_on_their_own_streams(felix):
     for w, out in zip(want, outs):
         for o in out:
             assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("op", ["hgemm", "sgemm", "flash_attn_fwd"])
+def test_the_first_call_of_a_new_host_thread(felix, op):
+    # nothing has made the device's context current there
+    x = torch.randn(2, 2, 128, 128, device="cuda").to(torch.float32 if op == "sgemm" else torch.float16)
+    out = [torch.zeros_like(x) for _ in range(2)]
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(o):
+        if op == "flash_attn_fwd":
+            felix.flash_attn_fwd(x, x, x, o, stream=stream)
+        else:
+            getattr(felix, op)(x[0, 0], x[0, 1], o[0, 0], stream=stream)
+
+    call(out[0])
+    in_threads([lambda: call(out[1])])
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], out[1]) and out[0].abs().sum() > 0
+
+
+def test_hgemm_of_host_threads_while_the_scratch_grows(felix):
+    # each thread asks for more and more scratch on one stream
+    stream = torch.cuda.Stream().cuda_stream
+    sizes = [(256, 256, 4096), (512, 384, 4096), (1100, 1100, 4096), (2200, 2200, 2048)]
+    g = torch.Generator().manual_seed(1)
+    cases = []
+    for m, n, k in sizes:
+        a = torch.randn(m, k, generator=g).half().cuda()
+        b = torch.randn(n, k, generator=g).half().cuda()
+        cases.append((a, b, sion().hgemm_nt(a, b)))
+    outs = [[torch.zeros_like(c[2]) for c in cases] for _ in range(4)]
+    torch.cuda.synchronize()
+
+    def work(out):
+        def run():
+            for (a, b, _), o in zip(cases, out):
+                for _ in range(20):
+                    felix.hgemm(a, b, o, b_layout=felix.B_NK, stream=stream)
+        return run
+
+    in_threads([work(o) for o in outs])
+    torch.cuda.synchronize()
+    for out in outs:
+        for o, c in zip(out, cases):
+            # the order in which parts are added may differ: fp32 sums, fp16 results
+            assert (o.float() - c[2].float()).abs().max() <= 2.0 ** -10 * c[2].float().abs().max()
