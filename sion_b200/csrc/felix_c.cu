@@ -14,6 +14,7 @@
 #include <thread>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "felix_internal.h"
 #include "sm100_ptx.cuh"
@@ -32,10 +33,15 @@ std::mutex g_mu;
 DeviceInfo g_dev[64];
 bool g_dev_ready[64] = {false};
 
-struct WsEntry {
-  std::mutex mu;  // held by a call from here to its last launch
+struct Buffer {
   void* ptr = nullptr;
   size_t bytes = 0;
+};
+struct WsEntry {
+  std::mutex mu;  // held by a call from here to its last launch
+  Buffer own;
+  Buffer captured;                 // of the capture with this id, which owns it
+  unsigned long long capture = 0;
 };
 // Device, stream, and the host thread where the handle stands for each thread's own
 // stream. Entries stay: a map's elements do not move.
@@ -105,25 +111,116 @@ static WsEntry& workspace_entry(int device, cudaStream_t stream) {
   return g_ws[WsKey(device, stream, thread)];
 }
 
+// Allocations are no part of a capture, of this thread or another.
+struct NotCaptured {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  NotCaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~NotCaptured() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+constexpr size_t kWsLeast = size_t(1) << 20;
+
+// Buffers whose graphs are gone, for the next captures. They outlive the process's
+// static objects: graphs may be destroyed after those.
+struct Spare {
+  std::mutex mu;
+  std::vector<Buffer> free[64];
+};
+static Spare& spare() {
+  static Spare* s = new Spare;
+  return *s;
+}
+struct GraphBuffer {
+  int device;
+  Buffer b;
+};
+// Called when the last graph that holds the buffer is gone and has run to its end; may
+// not call CUDA.
+static void graph_gone(void* p) {
+  GraphBuffer* g = static_cast<GraphBuffer*>(p);
+  Spare& s = spare();
+  try {
+    std::lock_guard<std::mutex> lk(s.mu);
+    s.free[g->device].push_back(g->b);
+  } catch (...) {  // no memory for the list: the buffer is lost
+  }
+  delete g;
+}
+
+// A zeroed buffer that belongs to the graph. It cannot be zeroed on the stream, whose
+// work is being recorded.
+static Buffer graph_buffer(int device, cudaGraph_t graph, size_t bytes) {
+  NotCaptured outside;
+  Buffer b;
+  Spare& s = spare();
+  {
+    std::lock_guard<std::mutex> lk(s.mu);
+    auto& f = s.free[device];
+    auto best = f.end();
+    for (auto i = f.begin(); i != f.end(); ++i)
+      if (i->bytes >= bytes && (best == f.end() || i->bytes < best->bytes)) best = i;
+    if (best != f.end()) {
+      b = *best;
+      f.erase(best);
+    }
+  }
+  if (!b.ptr) {
+    b.bytes = bytes < kWsLeast ? kWsLeast : bytes;
+    if (cudaMalloc(&b.ptr, b.bytes) != cudaSuccess) return {};
+  }
+  auto* g = new GraphBuffer{device, b};
+  cudaStream_t side = nullptr;
+  cudaUserObject_t object = nullptr;
+  bool ok = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking) == cudaSuccess;
+  ok = ok && cudaMemsetAsync(b.ptr, 0, b.bytes, side) == cudaSuccess &&
+       cudaStreamSynchronize(side) == cudaSuccess;
+  if (side) cudaStreamDestroy(side);
+  ok = ok && cudaUserObjectCreate(&object, g, graph_gone, 1, cudaUserObjectNoDestructorSync) ==
+                 cudaSuccess;
+  if (!ok) {
+    graph_gone(g);
+    return {};
+  }
+  if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);  // back to the spare ones
+    return {};
+  }
+  return b;
+}
+
 Workspace library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes) {
   WsEntry& w = workspace_entry(dev->ordinal, stream);
   std::unique_lock<std::mutex> lk(w.mu);
-  if (w.bytes >= bytes) return {w.ptr, std::move(lk)};
-  if (w.ptr) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id, &graph) != cudaSuccess) {
+    cudaGetLastError();  // the launch will say so
+    status = cudaStreamCaptureStatusNone;
+  }
+  if (status == cudaStreamCaptureStatusActive) {
+    if (w.capture != id || w.captured.bytes < bytes) {
+      w.captured = graph_buffer(dev->ordinal, graph, bytes);  // a smaller one stays the graph's
+      w.capture = id;
+    }
+    return {w.captured.ptr, std::move(lk)};
+  }
+  if (w.own.bytes >= bytes) return {w.own.ptr, std::move(lk)};
+  NotCaptured outside;
+  if (w.own.ptr) {
     // The old buffer may still be in use by work queued on this stream.
     cudaStreamSynchronize(stream);
-    cudaFree(w.ptr);
-    w.ptr = nullptr;
-    w.bytes = 0;
+    cudaFree(w.own.ptr);
+    w.own = {};
   }
-  size_t sz = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
-  if (cudaMalloc(&w.ptr, sz) != cudaSuccess) {
-    w.ptr = nullptr;
+  const size_t sz = bytes < kWsLeast ? kWsLeast : bytes;
+  if (cudaMalloc(&w.own.ptr, sz) != cudaSuccess) {
+    w.own.ptr = nullptr;
     return {};
   }
-  if (cudaMemsetAsync(w.ptr, 0, sz, stream) != cudaSuccess) return {};
-  w.bytes = sz;
-  return {w.ptr, std::move(lk)};
+  if (cudaMemsetAsync(w.own.ptr, 0, sz, stream) != cudaSuccess) return {};
+  w.own.bytes = sz;
+  return {w.own.ptr, std::move(lk)};
 }
 
 static int encode_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,

@@ -73,7 +73,9 @@ struct Workspace {
 };
 // Library-owned scratch for a (device, stream) pair, grown on demand and
 // zero-filled on (re)allocation; ptr is null where there is no memory. Kernels
-// leave their counters at zero.
+// leave their counters at zero. A stream that is being captured gets a buffer of the
+// graph's own, which later calls neither free nor use, until the graph and what was
+// instantiated from it are destroyed; no call has to come before the capture.
 Workspace library_workspace(DeviceInfo* dev, cudaStream_t stream, size_t bytes);
 
 // 2-D fp16 tensor map, 128-byte swizzle: inner extent `inner` elements,

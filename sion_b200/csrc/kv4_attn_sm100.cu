@@ -941,8 +941,7 @@ FelixCode launch(AttnParams& P, DeviceInfo* dev, void* workspace, size_t ws_byte
   const size_t need = kWsCounterBytes + part_bytes(grid, H::kTileRows, D);
   if (workspace && ws_bytes < need)
     return api_error("kv4_attention: workspace smaller than felix_kv4_attention_workspace_size");
-  // the library's own is asked for at its largest, so that calls of other shapes do not
-  // move it under a captured graph
+  // the library's own is asked for at its largest: growing waits for the stream
   const size_t most = kv4_attention_workspace_bytes(128, dev->num_sms);
   Workspace scratch;  // until the launch
   if (!workspace) scratch = library_workspace(dev, stream, most);

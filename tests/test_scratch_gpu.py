@@ -174,3 +174,156 @@ def test_hgemm_of_host_threads_while_the_scratch_grows(felix):
         for o, c in zip(out, cases):
             # the order in which parts are added may differ: fp32 sums, fp16 results
             assert (o.float() - c[2].float()).abs().max() <= 2.0 ** -10 * c[2].float().abs().max()
+
+
+# ----------------------------------------------------------------------- graphs
+def capture(f, stream=None):
+    """f's work as a graph, with no call of it before."""
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        f()
+    return g
+
+
+def test_a_graph_keeps_its_scratch_while_the_stream_goes_on():
+    # a reserve alone is captured; then the same stream asks for far more scratch
+    rng = np.random.default_rng(5)
+    slots, width, pages, page = 50, 40, 1500, 16
+    lens0 = rng.integers(0, 100, slots).astype(np.int32)
+    empty = np.full((slots, width), -1, np.int32)
+    table0, _, refs0, status = R.reserve(empty, np.zeros(slots, np.int32), np.zeros(pages, np.int32),
+                                         lens0, page)
+    assert status == [0, 0]
+    counts = rng.integers(0, 60, slots).astype(np.int32)
+    want = R.reserve(table0, lens0, refs0, counts, page)
+    dev = [i32(x) for x in (table0, lens0, refs0, counts)]
+    side, got = torch.cuda.Stream(), []
+    g = capture(lambda: got.extend(sion().kv4_reserve(*dev, page)), side)
+    pool, table, lens, q = attend_case(4)
+    a = torch.randn(1100, 4096, device="cuda").half()
+    b = torch.randn(1100, 4096, device="cuda").half()
+    with torch.cuda.stream(side):
+        first = sion().kv4_attention(q, pool, table, lens, 2)
+        for _ in range(3):
+            sion().hgemm_nt(a, b)
+            g.replay()
+            o = sion().kv4_attention(q, pool, table, lens, 2)
+        junk = [torch.full((1 << 20,), -1, dtype=torch.int32, device="cuda") for _ in range(30)]
+        for x in got:
+            x.fill_(99)
+        g.replay()
+    torch.cuda.synchronize()
+    for x, w in zip(got, want):
+        np.testing.assert_array_equal(x.cpu().numpy(), np.asarray(w))
+    assert torch.equal(o, first) and all(int(j[0]) == -1 for j in junk[:2])
+
+
+def test_graphs_of_one_stream_run_at_once():
+    # two graphs captured one after the other, replayed on two streams, and eager calls
+    # on the stream of the captures beside them
+    cases = [attend_case(s) for s in (6, 7, 8)]
+    want = [sion().kv4_attention(q, pool, table, lens, 2) for pool, table, lens, q in cases]
+    side = torch.cuda.Stream()
+    outs, graphs = [], []
+    for pool, table, lens, q in cases[:2]:
+        o = []
+        graphs.append(capture(lambda: o.extend(sion().kv4_attention(q, pool, table, lens, 2)
+                                               for _ in range(20)), side))
+        outs.append(o)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    pool, table, lens, q = cases[2]
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(side):
+            eager = [sion().kv4_attention(q, pool, table, lens, 2) for _ in range(20)]
+        torch.cuda.synchronize()
+        for w, out in zip(want, [*outs, eager]):
+            assert all(torch.equal(o, w) for o in out)
+
+
+def test_branches_of_one_graph_have_their_own_scratch():
+    cases = [attend_case(s) for s in (9, 10)]
+    want = [sion().kv4_attention(q, pool, table, lens, 2) for pool, table, lens, q in cases]
+    main, other, outs = torch.cuda.Stream(), torch.cuda.Stream(), [[], []]
+
+    def run():
+        other.wait_stream(main)
+        for (pool, table, lens, q), out, s in zip(cases, outs, (main, other)):
+            with torch.cuda.stream(s):
+                out.extend(sion().kv4_attention(q, pool, table, lens, 2) for _ in range(20))
+        main.wait_stream(other)
+
+    g = capture(run, main)
+    for _ in range(10):
+        g.replay()
+        torch.cuda.synchronize()
+        for w, out in zip(want, outs):
+            assert all(torch.equal(o, w) for o in out)
+
+
+@pytest.mark.parametrize("op", ["hgemm", "sgemm", "topk", "fork", "backward"])
+def test_capture_without_a_call_before(felix, op):
+    gen = torch.Generator().manual_seed(3)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=gen).cuda()
+
+    if op in ("hgemm", "sgemm"):  # stream-K: parts and counters
+        a, b = rand(1100, 4096), rand(1100, 4096)
+        if op == "hgemm":
+            a, b = a.half(), b.half()
+            f = lambda o: o.append(sion().hgemm_nt(a, b))  # noqa: E731
+        else:
+            b = b.t().contiguous()
+            f = lambda o: o.append(sion().sgemm(a, b))  # noqa: E731
+    elif op == "topk":
+        x, out = rand(2, 3000001), torch.zeros(2, device="cuda")
+        f = lambda o: o.append(topk(felix, x, out).clone())  # noqa: E731
+    elif op == "fork":
+        s = Fork(11)
+        f = lambda o: o.extend(sion().kv4_fork(s.pool, *s.dev, s.page))  # noqa: E731
+    else:
+        q, k, v, do = (rand(1, 2, 300, 64).half() for _ in range(4))
+        out, lse = sion().flash_attention_lse(q, k, v)
+        f = lambda o: o.extend(sion().flash_attention_backward(q, k, v, out, lse, do))  # noqa: E731
+    got, want = [], []
+    g = capture(lambda: f(got), torch.cuda.Stream())
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    f(want)
+    torch.cuda.synchronize()
+    assert len(got) == len(want) > 0
+    for a, b in zip(got, want):
+        # sums of several CTAs may be added in another order
+        assert (a.double() - b.double()).abs().max() <= 2e-3 * max(b.double().abs().max(), 1e-30)
+
+
+def topk(felix, x, out):
+    felix.check(felix.lib().felix_topk_select(x.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], 5,
+                                              1, torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+def test_graphs_that_are_gone_give_their_scratch_back():
+    pool, table, lens, q = attend_case(12)
+    out = []
+
+    def once():
+        out.clear()
+        g = capture(lambda: out.append(sion().kv4_attention(q, pool, table, lens, 2)))
+        g.replay()
+        torch.cuda.synchronize()
+        del g
+
+    for _ in range(3):
+        once()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(30):  # 10 MB each
+        once()
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] < 100 << 20
