@@ -575,6 +575,22 @@ struct Smem {
   int abort;
 };
 
+// A bounded wait of a whole warp. Lanes may give up at different times; what follows
+// has warp-wide operations, so that all go on or none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* abort_flag,
+                                          unsigned* status) {
+  return __all_sync(~0u, felix_sm100::mbar_wait(bar, parity, abort_flag, status,
+                                                felix_sm100::kWdKv4Load));
+}
+// After a wait that gave up, copies may still be under way into this CTA's shared
+// memory: they get time to land before it goes to another. (Any warp may be the last to
+// leave: the one that fetches is mostly done by then.)
+__device__ __forceinline__ void let_copies_land() {
+  const uint64_t t0 = felix_sm100::globaltimer_ns();
+  while (felix_sm100::globaltimer_ns() - t0 < 1000000ull) {
+  }
+}
+
 // Units of a segment beyond its steps (`open` below): what opening and closing it
 // costs (q, the join of the warps), about 12 steps. Without them a share of many
 // short segments takes longest. Where there are few steps per CTA, the shares are
@@ -736,9 +752,7 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
           c.pages + size_t(ok ? page : 0) * c.page_bytes + size_t(in_page) * kB;
       const uint32_t there = __ballot_sync(~0u, ok);
       look();  // the table is read while the stage is waited for
-      if (!felix_sm100::mbar_wait(&sm.empty[stage], parity ^ 1, &sm.abort, P.status,
-                                  felix_sm100::kWdKv4Load))
-        break;
+      if (!warp_wait(&sm.empty[stage], parity ^ 1, &sm.abort, P.status)) break;
       if (lane == 0) {
         sm.there[stage] = there;
         felix_sm100::mbar_arrive_expect_tx(&sm.full[stage], __popc(there) * kB);
@@ -747,32 +761,28 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
       if (ok) felix_sm100::bulk_load_1d(&sm.ring[stage][lane * kB], src, kB, &sm.full[stage]);
       advance();
     }
-    // After a wait that gave up, copies may still be under way into this CTA's
-    // shared memory: they get time to land before it goes to another.
-    if (sm.abort) {
-      const uint64_t t0 = felix_sm100::globaltimer_ns();
-      while (felix_sm100::globaltimer_ns() - t0 < 1000000ull) {
-      }
-    }
+    if (sm.abort) let_copies_land();
     return;
   }
   if constexpr (kCW == 8) felix_sm100::setmaxnreg_inc<kRegsSums>();
 
   const int rw = warp / kTW, tw = warp - rw * kTW;  // group of rows, place among its tokens
+  bool gone = false;  // a wait gave up: the rest is passed over
   for (;;) {
     const uint32_t kvh = use.kvh, rt = use.rt;
     const int count = P.counts ? min(max(P.counts[use.slot], 0), int(P.rows)) : int(P.rows);
     Attn<T, D, NT> A;
     A.load_q(P, use.slot, kvh, rt * H::kTileRows + rw * kRows, use.len, count, lane);
     const uint32_t end = use.end_step();
-    for (uint32_t t = use.first_step(); t < end; t += kTW) {
-      if (felix_sm100::mbar_wait(&sm.full[stage], parity, &sm.abort, P.status,
-                                 felix_sm100::kWdKv4Load)) {
-        const uint32_t there = sm.there[stage] >> (tw * kStep) & ((1u << kStep) - 1);
-        if (there)
-          A.step(sm.ring[stage] + tw * kStep * kB, sm.tp[warp], there,
-                 int(t + tw) * kStepTokens, lane);
+    for (uint32_t t = use.first_step(); t < end && !gone; t += kTW) {
+      if (!warp_wait(&sm.full[stage], parity, &sm.abort, P.status)) {
+        gone = true;
+        break;
       }
+      const uint32_t there = sm.there[stage] >> (tw * kStep) & ((1u << kStep) - 1);
+      if (there)
+        A.step(sm.ring[stage] + tw * kStep * kB, sm.tp[warp], there, int(t + tw) * kStepTokens,
+               lane);
       __syncwarp();
       if (lane == 0) felix_sm100::mbar_arrive(&sm.empty[stage]);
       advance();
@@ -902,6 +912,7 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
     if (u >= last) break;
     use.open(P, u, last);
   }
+  if (gone) let_copies_land();
 }
 
 // Scratch: counters, then two parts per CTA. A grid has at most three CTAs of 8
