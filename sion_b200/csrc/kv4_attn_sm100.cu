@@ -455,7 +455,7 @@ struct Attn {
     }
     __syncwarp();  // tp is written
     uint32_t pt[NT][kStep][2];
-    if (there == (1u << kStep) - 1 && token0 + kStepTokens <= low)
+    if (there == (1u << kStep) - 1 && token0 <= low - kStepTokens)
       softmax<false>(s, tp, there, token0, g, pt);
     else
       softmax<true>(s, tp, there, token0, g, pt);
@@ -608,7 +608,7 @@ struct Place {
   __device__ __forceinline__ void read(const AttnParams& P) {
     len = slot_length(P.c, slot);
     reach = slot_reach(P.c, slot);
-    size = open_units + (reach + kStepTokens - 1) / kStepTokens;
+    size = open_units + (uint32_t(reach) + kStepTokens - 1) / kStepTokens;
   }
   // unit u, at or after the current slot's first
   __device__ __forceinline__ void open(const AttnParams& P, uint32_t u, uint32_t last) {
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
   const uint32_t run = (c.slots + kThreads - 1) / kThreads;
   const uint32_t s0 = min(tid * run, c.slots), s1 = min(s0 + run, c.slots);
   auto steps = [&](uint32_t s) {
-    return uint32_t(slot_reach(c, s) + kStepTokens - 1) / kStepTokens * per_seg;
+    return (uint32_t(slot_reach(c, s)) + kStepTokens - 1) / kStepTokens * per_seg;
   };
   uint32_t mine = 0;
   for (uint32_t s = s0; s < s1; ++s) mine += steps(s);
@@ -691,8 +691,10 @@ __global__ void __launch_bounds__(kCW == 8 ? 384 : 160, kCW == 8 ? 1 : 3)
   upto += open * s1 * per_seg;
   total += open * c.slots * per_seg;
   // at least a step for each warp: smaller parts cost more to join than they save
-  const uint32_t quota = max((total + gridDim.x - 1) / gridDim.x, uint32_t(kTW));
-  const uint32_t first = min(blockIdx.x * quota, total), last = min(first + quota, total);
+  // (the host keeps the total below 2^32; shares past it may lie beyond)
+  const uint32_t quota = max(total / gridDim.x + (total % gridDim.x != 0), uint32_t(kTW));
+  const uint32_t first = uint32_t(min(uint64_t(blockIdx.x) * quota, uint64_t(total)));
+  const uint32_t last = first + min(quota, total - first);
   if (first >= last) return;
   if (first >= upto - mine && first < upto) {
     uint32_t at = upto - mine;
