@@ -211,7 +211,8 @@ int felix_topk_select(const float* data, float* out, uint32_t num_slices, uint32
  * each slot in order, `lens` [slots] the tokens in it, new ones included.
  * Entries of `table` that name no page of the pool are not an error: tokens
  * there are not written, read as zero, and attention does not see them. All
- * arrays are on the device; pages is 16-byte aligned.
+ * arrays are on the device; pages is 16-byte aligned. Limits: 65535 heads, 2^24
+ * slots, width * page_size and rows below 2^31 (attention: 65535 rows).
  */
 typedef struct felix_kv4_cache {
   void* pages;

@@ -592,6 +592,8 @@ int felix_kv4_page_bytes(uint32_t kv_heads, uint32_t head_dim, uint32_t page_siz
   if (head_dim != 64 && head_dim != 128) return api_error("kv4: head_dim must be 64 or 128").type;
   if (page_shift_of(page_size) < 0)
     return api_error("kv4: page_size must be a power of two, 16..4096").type;
+  if (kv_heads == 0 || kv_heads > 65535)
+    return api_error("kv4: kv_heads must be 1..65535").type;
   if (bytes) *bytes = size_t(page_size) * kv_heads * (head_dim + 8);
   return FELIX_SUCCESS;
 }
@@ -605,6 +607,7 @@ int felix_kv4_append(const felix_kv4_cache* cache, const void* key, const void* 
     if (rc.type != FELIX_SUCCESS) return rc;
     if (dtype != FELIX_F16 && dtype != FELIX_BF16)
       return api_error("kv4_append: key and value must be fp16 or bf16");
+    if (rows > 0x7fffffffu) return api_error("kv4_append: at most 2^31-1 rows");
     if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
     if (!key || !value || !key_strides || !value_strides) return api_error("kv4_append: null pointer");
     return kv4_append_launch(v, cache->head_dim, key, value, dtype == FELIX_BF16, rows, key_strides,
@@ -618,6 +621,7 @@ int felix_kv4_read(const felix_kv4_cache* cache, uint32_t rows, const int32_t* c
     felix_kv4::CacheView v;
     const FelixCode rc = view_of(cache, &v);
     if (rc.type != FELIX_SUCCESS) return rc;
+    if (rows > 0x7fffffffu) return api_error("kv4_read: at most 2^31-1 rows");
     if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
     if (!key || !value) return api_error("kv4_read: null pointer");
     if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15)

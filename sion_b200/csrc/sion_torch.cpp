@@ -221,6 +221,12 @@ void check_i32(const torch::Tensor& t, const torch::Device& dev, int64_t dim, co
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 const int32_t* i32(const torch::Tensor& t) { return t.data_ptr<int32_t>(); }
+// A size as the C ABI takes it: what does not fit is refused, not cut off.
+constexpr int64_t kMostSlots = 1 << 24, kMostInt = 0x7fffffff, kMostHeads = 65535;
+uint32_t u32(int64_t n, int64_t most, const char* what) {
+  TORCH_CHECK(n <= most, what, " must be at most ", most);
+  return uint32_t(n);
+}
 const int32_t* counts_of(const OptTensor& counts, const torch::Tensor& lens) {
   if (!counts) return nullptr;
   check_i32(*counts, lens.device(), 1, "counts");
@@ -237,13 +243,20 @@ felix::Kv4Cache cache_of(const torch::Tensor& pages, const torch::Tensor& table,
   check_i32(lens, pages.device(), 1, "lens");
   TORCH_CHECK(table.size(0) == lens.size(0), "table and lens must have the same slots");
   TORCH_CHECK(kv_heads > 0, "kv_heads must be positive");
+  const uint32_t heads = u32(kv_heads, kMostHeads, "kv_heads");
   TORCH_CHECK(head_dim == 64 || head_dim == 128, "unsupported head dimension ", head_dim);
   const int64_t token = kv_heads * (head_dim + 8);
   TORCH_CHECK(pages.size(1) > 0 && pages.size(1) % token == 0,
               "a page's bytes must be page_size * kv_heads * (head_dim + 8)");
-  return {pages.data_ptr(), uint64_t(pages.size(0)), uint32_t(pages.size(1) / token),
-          uint32_t(kv_heads), uint32_t(head_dim), i32(table), i32(lens), uint32_t(table.size(0)),
-          uint32_t(table.size(1))};
+  return {pages.data_ptr(),
+          uint64_t(pages.size(0)),
+          u32(pages.size(1) / token, kMostInt, "page_size"),
+          heads,
+          uint32_t(head_dim),
+          i32(table),
+          i32(lens),
+          u32(table.size(0), kMostSlots, "slots"),
+          u32(table.size(1), kMostInt, "table's width")};
 }
 
 felix::ElementType half_type(const torch::Tensor& t, const char* name) {
@@ -269,6 +282,8 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_attention_impl(
   TORCH_CHECK(query.size(0) == table.size(0), "query must have one entry per slot");
   TORCH_CHECK(query.size(1) > 0 && query.size(1) % kv_heads == 0,
               "query's heads must be a multiple of kv_heads");
+  const uint32_t heads = u32(query.size(1), kMostHeads, "heads");
+  const uint32_t rows = u32(query.size(2), kMostHeads, "rows");
   const int32_t* n = counts_of(counts, lens);
   const c10::cuda::CUDAGuard guard(query.device());
   const auto Q = inner_contiguous(query);
@@ -276,7 +291,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv4_attention_impl(
   torch::Tensor L;
   if (want_lse) L = torch::empty(Q.sizes().slice(0, 3), Q.options().dtype(torch::kFloat32));
   const auto status = felix::kv4_attention_launch(
-      cache, Q.data_ptr(), type, uint32_t(Q.size(1)), uint32_t(Q.size(2)), Q.strides().data(), n,
+      cache, Q.data_ptr(), type, heads, rows, Q.strides().data(), n,
       float(scale), O.data_ptr(), want_lse ? L.data_ptr<float>() : nullptr,
       at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(status.ok(), "kv4_attention: kernel launch failed: ", status.str());
@@ -312,6 +327,9 @@ void check_state(const torch::Tensor& table, const torch::Tensor* lens, const to
   TORCH_CHECK(table.is_cuda(), "table must be CUDA tensor");
   check_i32(table, table.device(), 2, "table");
   check_i32(refs, table.device(), 1, "refs");
+  u32(table.size(0), kMostSlots, "slots");
+  u32(table.size(1), kMostInt, "table's width");
+  u32(refs.size(0), kMostInt, "pages");
   if (!lens) return;
   check_i32(*lens, table.device(), 1, "lens");
   TORCH_CHECK(table.size(0) == lens->size(0), "table and lens must have the same slots");
@@ -337,7 +355,7 @@ uint32_t page_size_of(int64_t page_size) {
 int64_t kv4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t page_size) {
   TORCH_CHECK(kv_heads > 0, "kv_heads must be positive");
   TORCH_CHECK(head_dim == 64 || head_dim == 128, "unsupported head dimension ", head_dim);
-  return int64_t(felix::kv4_page_bytes(uint32_t(kv_heads), uint32_t(head_dim),
+  return int64_t(felix::kv4_page_bytes(u32(kv_heads, kMostHeads, "kv_heads"), uint32_t(head_dim),
                                        page_size_of(page_size)));
 }
 
@@ -351,11 +369,12 @@ void kv4_append(const torch::Tensor& pages, const torch::Tensor& table, const to
   TORCH_CHECK(key.device() == pages.device() && value.device() == pages.device(),
               "key and value must be on ", pages.device());
   TORCH_CHECK(key.size(0) == table.size(0), "key must have one entry per slot");
+  const uint32_t rows = u32(key.size(2), kMostInt, "rows");
   const int32_t* n = counts_of(counts, lens);
   const c10::cuda::CUDAGuard guard(pages.device());
   const auto K = inner_contiguous(key), V = inner_contiguous(value);
   const auto status = felix::kv4_append_launch(
-      cache, K.data_ptr(), V.data_ptr(), type, uint32_t(K.size(2)), K.strides().data(),
+      cache, K.data_ptr(), V.data_ptr(), type, rows, K.strides().data(),
       V.strides().data(), n, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(status.ok(), "kv4_append: kernel launch failed: ", status.str());
 }
@@ -425,7 +444,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> kv4_fork(
   auto report = empty_i32({2}, lens.device());
   const auto status = felix::kv4_fork_launch(
       pages.data_ptr(), size_t(pages.size(1)), pages_of(table, &lens, refs), i32(parents),
-      i32(children), uint32_t(parents.size(0)), uint32_t(table.size(0)), uint32_t(table.size(1)),
+      i32(children), u32(parents.size(0), kMostSlots, "pairs"), uint32_t(table.size(0)),
+      uint32_t(table.size(1)),
       uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]), report.data_ptr<int32_t>(),
       at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(status.ok(), "kv4_fork: kernel launch failed: ", status.str());
@@ -441,8 +461,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> kv4_free(
   const c10::cuda::CUDAGuard guard(table.device());
   const auto o = page_outputs<3>({&table, &lens, &refs}, out);
   const auto status = felix::kv4_free_launch(
-      pages_of(table, &lens, refs), i32(slots), uint32_t(slots.size(0)), uint32_t(table.size(0)),
-      uint32_t(table.size(1)), uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]),
+      pages_of(table, &lens, refs), i32(slots), u32(slots.size(0), kMostSlots, "slots to free"),
+      uint32_t(table.size(0)), uint32_t(table.size(1)), uint32_t(refs.size(0)), size, pages_of(o[0], &o[1], o[2]),
       at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(status.ok(), "kv4_free: kernel launch failed: ", status.str());
   return {o[0], o[1], o[2]};
@@ -478,7 +498,7 @@ void kv4_copy_pages(const torch::Tensor& src_pages, const torch::Tensor& dst_pag
   const auto status = felix::kv4_copy_pages_launch(
       src_pages.data_ptr(), uint64_t(src_pages.size(0)), dst_pages.data_ptr(),
       uint64_t(dst_pages.size(0)), size_t(dst_pages.size(1)), i32(src), i32(dst),
-      uint32_t(src.size(0)), at::cuda::getCurrentCUDAStream());
+      u32(src.size(0), kMostInt, "pages to copy"), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(status.ok(), "kv4_copy_pages: kernel launch failed: ", status.str());
 }
 
@@ -493,7 +513,9 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits,
                   logits.dtype() == torch::kBFloat16,
               "logits must be float32, float16 or bfloat16");
   TORCH_CHECK(logits.size(1) > 0, "vocab must not be empty");
+  TORCH_CHECK(logits.size(1) <= 524288, "vocab must be 1..524288");
   const int64_t rows = logits.size(0);
+  u32(rows, 1 << 27, "rows");
   auto per_row = [&](const torch::Tensor& t, torch::ScalarType type, const char* name) {
     TORCH_CHECK(t.device() == logits.device(), name, " must be on ", logits.device());
     TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
