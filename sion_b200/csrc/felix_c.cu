@@ -421,7 +421,8 @@ static FelixCode pages_op(const Kv4PagesOp& o, uint32_t page_size, void* stream)
     return api_error("kv4: num_pages must be 1..2^31-1");
   if (o.slots > (1u << 24) || o.n > (1u << 24) || o.width > 0x7fffffffu / page_size)
     return api_error("kv4: too many slots, pages of a slot or list entries");
-  if (o.pages && ((reinterpret_cast<uintptr_t>(o.pages) & 15) || o.page_bytes % 16))
+  if (o.pages && ((reinterpret_cast<uintptr_t>(o.pages) & 15) || o.page_bytes == 0 ||
+                  o.page_bytes % 16))
     return api_error("kv4: pages must be 16-byte aligned and their size a multiple of 16");
   return kv4_pages_launch(o, static_cast<cudaStream_t>(stream));
 }

@@ -47,3 +47,12 @@ def test_torch_sizes_past_32_bits_are_refused():
         with pytest.raises(RuntimeError, match=text):
             call()
     assert torch.equal(pool, before)
+
+
+def test_pages_of_no_bytes_are_refused_before_any_change():
+    # (the plan would be made, and the copies then fail to launch)
+    L = abi.lib()
+    assert L.felix_kv4_compact(16, 0, 16, 16, 2, 2, 4, 16, 16, None) == abi.API_ERROR
+    assert "multiple of 16" in L.felix_last_error_message().decode()
+    rc = L.felix_kv4_fork(16, 0, 16, 16, 16, 16, 16, 1, 2, 2, 4, 16, 16, 16, 16, 16, None)
+    assert rc == abi.API_ERROR and "multiple of 16" in L.felix_last_error_message().decode()
