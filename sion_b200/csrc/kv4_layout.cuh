@@ -44,13 +44,6 @@ __host__ __device__ constexpr uint32_t v_codes_at(uint32_t D) { return kBlock * 
 __host__ __device__ constexpr uint32_t k_params_at(uint32_t D) { return kBlock * D; }
 __host__ __device__ constexpr uint32_t v_params_at(uint32_t D) { return kBlock * D + 4 * kBlock; }
 
-// Byte of the V code of token r (0..15), dimension d, in the V part.
-__host__ __device__ constexpr uint32_t v_code_byte(uint32_t D, uint32_t r, uint32_t d) {
-  const uint32_t e = d % (D / 8);
-  return (r / 8) * 4 * D + (d / (D / 8)) * (D / 2) + (r % 8 / 2) * (D / 8) + (e & ~3u) +
-         2 * (r & 1) + (e % 4) / 2;
-}
-
 // What the kernels need of a cache. `table` [slots, width] names the pages of
 // each slot, `lens` [slots] its tokens.
 struct CacheView {
