@@ -14,7 +14,7 @@
 #include "sm100_ptx.cuh"
 
 namespace felix_impl {
-namespace kv4 {
+namespace kv4_cache {
 
 using namespace felix_kv4;
 
@@ -714,12 +714,12 @@ FelixCode scratch(DeviceInfo* dev, MetaParams& P, cudaStream_t stream, Workspace
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
-}  // namespace kv4
+}  // namespace kv4_cache
 
 FelixCode kv4_append_launch(const felix_kv4::CacheView& c, uint32_t head_dim, const void* key,
                             const void* value, bool bf16, uint32_t rows, const int64_t* ks,
                             const int64_t* vs, const int32_t* counts, cudaStream_t stream) {
-  kv4::TokenParams P{};
+  kv4_cache::TokenParams P{};
   P.c = c;
   P.counts = counts;
   P.rows = rows;
@@ -736,18 +736,18 @@ FelixCode kv4_append_launch(const felix_kv4::CacheView& c, uint32_t head_dim, co
   const int threads = P.blocks < 8 ? int(P.blocks) * 32 : 256;
   if (bf16) {
     if (head_dim == 128)
-      kv4::kv4_append_kernel<__nv_bfloat16, 128><<<grid, threads, 0, stream>>>(P);
-    else kv4::kv4_append_kernel<__nv_bfloat16, 64><<<grid, threads, 0, stream>>>(P);
+      kv4_cache::kv4_append_kernel<__nv_bfloat16, 128><<<grid, threads, 0, stream>>>(P);
+    else kv4_cache::kv4_append_kernel<__nv_bfloat16, 64><<<grid, threads, 0, stream>>>(P);
   } else {
-    if (head_dim == 128) kv4::kv4_append_kernel<__half, 128><<<grid, threads, 0, stream>>>(P);
-    else kv4::kv4_append_kernel<__half, 64><<<grid, threads, 0, stream>>>(P);
+    if (head_dim == 128) kv4_cache::kv4_append_kernel<__half, 128><<<grid, threads, 0, stream>>>(P);
+    else kv4_cache::kv4_append_kernel<__half, 64><<<grid, threads, 0, stream>>>(P);
   }
-  return kv4::done("kv4_append");
+  return kv4_cache::done("kv4_append");
 }
 
 FelixCode kv4_read_launch(const felix_kv4::CacheView& c, uint32_t head_dim, uint32_t rows,
                           const int32_t* counts, __half* key, __half* value, cudaStream_t stream) {
-  kv4::TokenParams P{};
+  kv4_cache::TokenParams P{};
   P.c = c;
   P.counts = counts;
   P.rows = rows;
@@ -755,9 +755,9 @@ FelixCode kv4_read_launch(const felix_kv4::CacheView& c, uint32_t head_dim, uint
   P.vo = value;
   const dim3 grid((rows + 31) / 32, c.kv_heads, c.slots < 65535u ? c.slots : 65535u);
   if (grid.z == 0 || rows == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
-  if (head_dim == 128) kv4::kv4_read_kernel<128><<<grid, 256, 0, stream>>>(P);
-  else kv4::kv4_read_kernel<64><<<grid, 256, 0, stream>>>(P);
-  return kv4::done("kv4_read");
+  if (head_dim == 128) kv4_cache::kv4_read_kernel<128><<<grid, 256, 0, stream>>>(P);
+  else kv4_cache::kv4_read_kernel<64><<<grid, 256, 0, stream>>>(P);
+  return kv4_cache::done("kv4_read");
 }
 
 FelixCode kv4_copy_launch(const void* from, uint64_t from_pages, void* to, uint64_t to_pages,
@@ -765,14 +765,14 @@ FelixCode kv4_copy_launch(const void* from, uint64_t from_pages, void* to, uint6
                           cudaStream_t stream) {
   DeviceInfo* dev = current_device_info();
   if (!dev) return launch_error(cudaGetLastError(), "kv4_copy_pages: no device");
-  return kv4::copy(dev, from, from_pages, to, to_pages, page_bytes, src, dst, nullptr, count, count,
+  return kv4_cache::copy(dev, from, from_pages, to, to_pages, page_bytes, src, dst, nullptr, count, count,
                    stream);
 }
 
 FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {
   DeviceInfo* dev = current_device_info();
   if (!dev) return launch_error(cudaGetLastError(), "kv4: no device");
-  kv4::MetaParams P{};
+  kv4_cache::MetaParams P{};
   P.table = o.table, P.lens = o.lens, P.refs = o.refs;
   P.table_out = o.table_out, P.lens_out = o.lens_out, P.refs_out = o.refs_out;
   P.status = o.status;
@@ -780,9 +780,9 @@ FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {
   P.slots = o.slots, P.width = o.width, P.pages = o.num_pages;
   P.page_shift = o.page_shift, P.n = o.n;
   Workspace ws;  // until the copies, which take their list from the plan, are launched
-  FelixCode rc = kv4::scratch(dev, P, stream, &ws);
+  FelixCode rc = kv4_cache::scratch(dev, P, stream, &ws);
   if (rc.type != FELIX_SUCCESS) return rc;
-  using namespace kv4;
+  using namespace kv4_cache;
   switch (o.kind) {
     case Kv4PagesOp::kReserve: kv4_reserve_kernel<<<kCtas, kMeta, 0, stream>>>(P); break;
     case Kv4PagesOp::kFork: kv4_fork_kernel<<<kCtas, kMeta, 0, stream>>>(P); break;
@@ -793,7 +793,7 @@ FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {
   if (rc.type != FELIX_SUCCESS) return rc;
   const uint32_t most = o.kind == Kv4PagesOp::kFork ? o.n
                         : o.kind == Kv4PagesOp::kCompact ? o.num_pages / 2 + 1 : 0;
-  return kv4::copy(dev, o.pages, o.num_pages, o.pages, o.num_pages, o.page_bytes, P.src, P.dst,
+  return kv4_cache::copy(dev, o.pages, o.num_pages, o.pages, o.num_pages, o.page_bytes, P.src, P.dst,
                    P.moves, 0, most, stream);
 }
 

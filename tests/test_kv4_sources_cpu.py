@@ -19,3 +19,14 @@ def test_what_a_header_defines_is_used(header, names):
     assert names
     assert [n for n in names if not re.search(r"\b%s\b" % n, others) and
             len(re.findall(r"\b%s\b" % n, text)) == 1] == []
+
+
+def test_the_units_share_no_namespace_for_what_is_their_own():
+    # TokenParams and f2 mean different things in the cache's and in attention's file: in
+    # one namespace that would break the one-definition rule
+    inner = {}
+    for f in ("kv4_attn_sm100.cu", "kv4_cache_sm100.cu", "sample_sm100.cu"):
+        for name in re.findall(r"^namespace (\w+) \{", code(f), re.M):
+            if name != "felix_impl":
+                assert inner.setdefault(name, f) == f
+    assert len(inner) == 3
