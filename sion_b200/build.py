@@ -85,6 +85,36 @@ def check_attention_registers(ptxas_log: str) -> None:
                     f"-DFELIX_FA_REGSPLIT=0 or adjust kRegsLaunch)")
 
 
+# The same for the attention over the 4-bit cache with eight consumer warps
+# (kv4_attn_sm100.cu kRegsLaunch); its last template argument is their number.
+KV4_REGS_LAUNCH = 168
+
+
+def check_kv4_registers(ptxas_log: str) -> None:
+    """Raise if ptxas gave an eight-warp kv4_attn_kernel another count."""
+    cur, seen = None, 0
+    for line in ptxas_log.splitlines():
+        m = re.search(r"Compiling entry function '([^']+)'", line)
+        if m:
+            cur = m.group(1)
+            continue
+        m = re.search(r"Used (\d+) registers", line)
+        if m and cur and re.search(r"kv4_attn_kernelI.*Li8EEEv", cur):
+            seen += 1
+            if int(m.group(1)) != KV4_REGS_LAUNCH:
+                raise RuntimeError(
+                    f"{cur}: ptxas used {m.group(1)} registers per thread; the setmaxnreg split "
+                    f"of the attention over the 4-bit cache assumes {KV4_REGS_LAUNCH} "
+                    f"(kv4_attn_sm100.cu kRegsLaunch)")
+    if not seen:
+        raise RuntimeError("no eight-warp kv4_attn_kernel in ptxas's output")
+
+
+# Sources whose compiler output is checked.
+REGISTER_CHECKS = {"flash_attn_sm100.cu": check_attention_registers,
+                   "kv4_attn_sm100.cu": check_kv4_registers}
+
+
 def _headers() -> list[str]:
     hs = [os.path.join(CSRC, h) for h in HEADERS]
     for d, _, fs in os.walk(INC):
@@ -102,7 +132,7 @@ def build_felix(force: bool = False) -> str:
         obj = os.path.join(BUILD, s + ".o")
         objs.append(obj)
         if force or _newer(obj, [src] + hdrs):
-            extra = ["-Xptxas", "-v"] if s == "flash_attn_sm100.cu" else []
+            extra = ["-Xptxas", "-v"] if s in REGISTER_CHECKS else []
             jobs.append([NVCC, *NVCC_FLAGS, *extra, f"-I{INC}", "-c", src, "-o", obj])
     for s in CPP_SOURCES:
         src = os.path.join(CSRC, s)
@@ -115,8 +145,9 @@ def build_felix(force: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         logs = list(ex.map(_run, jobs))
     for job, log in zip(jobs, logs):
-        if "-Xptxas" in job:
-            check_attention_registers(log)
+        for s, check in REGISTER_CHECKS.items():
+            if os.path.join(CSRC, s) in job:
+                check(log)
     if force or jobs or _newer(LIB, objs):
         _run([NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a",
               "-cudart", "static", "-o", LIB, *objs, "-ldl"])
