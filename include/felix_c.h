@@ -258,7 +258,8 @@ int felix_kv4_read(const felix_kv4_cache* cache, uint32_t rows, const int32_t* c
  * type; lse (may be NULL) fp32 [slots][heads][rows], natural log. Rows that see
  * nothing (i >= n, an empty slot) give zeros and lse = -inf. scale <= 0 selects
  * 1/sqrt(head_dim). workspace: NULL = library-owned per (device, stream), else
- * felix_kv4_attention_workspace_size() bytes, zero-filled before its first use.
+ * felix_kv4_attention_workspace_size() bytes, 16-byte aligned and zero-filled before
+ * its first use. out is 8-byte aligned.
  */
 int felix_kv4_attention(const felix_kv4_cache* cache, const void* q, int dtype, uint32_t heads,
                         uint32_t rows, const int64_t* q_strides, const int32_t* counts,

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -381,6 +382,15 @@ static int guarded(F&& f) {
   }
 }
 
+// Whether a caller's pointers are multiples of n (a power of two). Kernels read and
+// write vectors there: what is not aligned is refused, it would fault the device.
+static bool aligned(size_t n, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) & (n - 1)) return false;
+  return true;
+}
+constexpr char kWorkspaceAlignment[] = "workspace must be 16-byte aligned";
+
 // log2 of a page size, or -1 where it is none.
 static int page_shift_of(uint32_t page_size) {
   if (page_size < felix_kv4::kBlock || page_size > felix_kv4::kMaxPageSize ||
@@ -451,6 +461,7 @@ int felix_sgemm_ex(uint32_t M, uint32_t N, uint32_t K, float alpha, const float*
                    const float* B, float beta, float* C, int split_k, void* workspace,
                    size_t workspace_bytes, void* stream) {
   if (split_k < 0) return api_error("sgemm: split_k must be >= 0").type;
+  if (!aligned(16, {workspace})) return api_error(kWorkspaceAlignment).type;
   SgemmOptions o;
   o.split_k = split_k;
   return finish(sgemm_launch(M, N, K, alpha, A, B, beta, C, o, workspace, workspace_bytes,
@@ -490,6 +501,7 @@ int felix_hgemm_ex(uint32_t M, uint32_t N, uint32_t K, float alpha, const void* 
     return api_error("hgemm: b_layout must be FELIX_B_KN or FELIX_B_NK").type;
   if (stream_k < 0 || stream_k > 2) return api_error("hgemm: stream_k must be 0, 1 or 2").type;
   if (max_ctas < 0) return api_error("hgemm: max_ctas must be >= 0").type;
+  if (!aligned(16, {workspace})) return api_error(kWorkspaceAlignment).type;
   HgemmOptions o;
   o.block_n = block_n;
   o.stream_k = stream_k;
@@ -507,6 +519,7 @@ int felix_hgemm_ex2(uint32_t M, uint32_t N, uint32_t K, float alpha, const void*
     return api_error("hgemm: b_layout must be FELIX_B_KN or FELIX_B_NK").type;
   if (stream_k < 0 || stream_k > 2) return api_error("hgemm: stream_k must be 0, 1 or 2").type;
   if (max_ctas < 0) return api_error("hgemm: max_ctas must be >= 0").type;
+  if (!aligned(16, {workspace})) return api_error(kWorkspaceAlignment).type;
   if (cta_pair < 0 || cta_pair > 2) return api_error("hgemm: cta_pair must be 0, 1 or 2").type;
   if (cta_pair == 2 && block_n != 0 && block_n != 256)
     return api_error("hgemm: CTA pairs use 256-wide tiles (block_n 0 or 256)").type;
@@ -611,6 +624,7 @@ int felix_kv4_append(const felix_kv4_cache* cache, const void* key, const void* 
     if (rows > 0x7fffffffu) return api_error("kv4_append: at most 2^31-1 rows");
     if (rows == 0 || v.slots == 0) return FelixCode{FELIX_SUCCESS, cudaSuccess};
     if (!key || !value || !key_strides || !value_strides) return api_error("kv4_append: null pointer");
+    if (!aligned(2, {key, value})) return api_error("kv4_append: key and value must be 2-byte aligned");
     return kv4_append_launch(v, cache->head_dim, key, value, dtype == FELIX_BF16, rows, key_strides,
                              value_strides, counts, static_cast<cudaStream_t>(stream));
   });
@@ -647,6 +661,9 @@ int felix_kv4_attention(const felix_kv4_cache* cache, const void* q, int dtype, 
     if (heads == 0 || heads > 65535 || heads % v.kv_heads)
       return api_error("kv4_attention: heads must be a multiple of kv_heads, at most 65535");
     if (rows > 65535) return api_error("kv4_attention: at most 65535 rows");
+    if (!aligned(2, {q}) || !aligned(8, {out}))
+      return api_error("kv4_attention: q must be 2-byte and out 8-byte aligned");
+    if (!aligned(16, {workspace})) return api_error(kWorkspaceAlignment);
     return kv4_attention_launch(v, cache->head_dim, q, dtype == FELIX_BF16, heads, rows, q_strides,
                                 counts, scale, out, lse, workspace, workspace_bytes,
                                 static_cast<cudaStream_t>(stream));
@@ -743,6 +760,8 @@ int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, i
     if (vocab == 0 || vocab > 524288u) return api_error("sample: vocab must be 1..524288");
     if (rows > (1u << 27)) return api_error("sample: at most 2^27 rows");
     if (stride < 0) return api_error("sample: stride must not be negative");
+    if (!aligned(dtype == FELIX_F32 ? 4 : 2, {logits}))
+      return api_error("sample: logits must be aligned to their type");
     return sample_launch({logits, dtype, rows, vocab, stride, uniform, temperature, top_k, top_p,
                           min_p, tokens, logprobs},
                          static_cast<cudaStream_t>(stream));

@@ -56,3 +56,32 @@ def test_pages_of_no_bytes_are_refused_before_any_change():
     assert "multiple of 16" in L.felix_last_error_message().decode()
     rc = L.felix_kv4_fork(16, 0, 16, 16, 16, 16, 16, 1, 2, 2, 4, 16, 16, 16, 16, 16, None)
     assert rc == abi.API_ERROR and "multiple of 16" in L.felix_last_error_message().decode()
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 8])
+def test_what_a_kernel_cannot_address_is_refused(off):
+    # each of these would be a misaligned access on the device
+    L, st = abi.lib(), (C.c_int64 * 3)(0, 0, 0)
+    c = abi.Kv4Cache(*[CACHE[f] for f, _ in abi.Kv4Cache._fields_])
+
+    def attend(q=64, out=64, ws=None):
+        return L.felix_kv4_attention(C.byref(c), q, abi.F16, 4, 1, st, None, 0.0, out, None, ws,
+                                     1 << 30, None)
+
+    bad = [attend(ws=64 + off),
+           L.felix_hgemm_ex(256, 256, 256, 1.0, 64, 64, 0.0, 64, 1, 0, 0, 0, 64 + off, 1 << 30, None),
+           L.felix_hgemm_ex2(256, 256, 256, 1.0, 64, 64, 0.0, 64, 1, 0, 0, 0, 0, 64 + off, 1 << 30,
+                             None),
+           L.felix_sgemm_ex(256, 256, 256, 1.0, 64, 64, 0.0, 64, 4, 64 + off, 1 << 30, None)]
+    if off < 2:
+        bad += [attend(q=64 + off),
+                L.felix_kv4_append(C.byref(c), 64 + off, 64, abi.F16, 1, st, st, None, None),
+                L.felix_kv4_append(C.byref(c), 64, 64 + off, abi.BF16, 1, st, st, None, None),
+                L.felix_sample(64 + off, abi.F16, 1, 5, 5, 64, None, None, None, None, 64, 64, None)]
+    if off < 8:
+        bad.append(attend(out=64 + off))
+    if off < 4:
+        bad.append(L.felix_sample(64 + off, abi.F32, 1, 5, 5, 64, None, None, None, None, 64, 64, None))
+    for rc in bad:
+        assert rc == abi.API_ERROR
+        assert "aligned" in L.felix_last_error_message().decode()
