@@ -132,7 +132,7 @@ __device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
 }
 // Rounded to 11 bits, whatever the exponent: TF32 has fp16's significand and fp32's
 // exponents. (96 slots 137 us, 131071 x 40 rows 328; by Veltkamp's splitting 138 and
-// 332. Weights from the fp16 copy, wrong below 2^-14: 137 and 311.)
+// 332. Weights from the fp16 copy, wrong below 2^-14, saved 5 % of the latter.)
 __device__ __forceinline__ F2 round11(F2 a) {
   const float2 x = un(a);
   uint32_t r0, r1;
@@ -338,9 +338,9 @@ struct Attn {
           t0 = fmaxf(t0, x[k][h].x);
           t1 = fmaxf(t1, x[k][h].y);
         }
-      // One tile of rows: probabilities with the m at hand, while a vote says whether it
-      // holds (it mostly does). With more tiles the others fill that wait, and the code
-      // of the loop has to stay short (313 against 311 us).
+      // Probabilities with the m at hand, while a vote says whether it holds (it mostly
+      // does). 131071 x 40 rows 317 us against 329 by voting first, 96 slots 138 against
+      // 139.
       float2 e[kStep][2];
       auto exponents = [&]() {
         const F2 minus = f2(-m[n][0], -m[n][1]);
@@ -352,7 +352,7 @@ struct Attn {
             e[k][h] = make_float2(ex2(d.x), ex2(d.y));
           }
       };
-      if (NT == 1) exponents();
+      exponents();
       // Exponents are relative to m, 2^6 below a maximum that is only moved when a
       // score passes it by 2^8: P stays below 2^15.
       if (__any_sync(~0u, t0 > m[n][0] + 14.f || t1 > m[n][1] + 14.f)) {
@@ -375,9 +375,8 @@ struct Attn {
         for (int j = 0; j < D / 16; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) o[n][j][h] = mul(o[n][j][h], kk);
-        if (NT == 1) exponents();
+        exponents();
       }
-      if (NT > 1) exponents();
 #pragma unroll
       for (int k = 0; k < kStep; ++k)
 #pragma unroll
