@@ -743,19 +743,20 @@ template <typename T>
 FelixCode launch(const SampleArgs& a, DeviceInfo* dev, cudaStream_t stream) {
   const size_t fixed = (sizeof(Shared) + 15) & ~size_t(15);
   // Enough CTAs that every SM has one, as long as each has 2048 tokens or more; at most
-  // kMaxPart tokens in each (the histogram's sums) and about 128 KB. Parts of which two fit
+  // kMaxPart tokens in each (the histogram's sums) and 208 KB. Parts of which two fit
   // an SM's shared memory are staged there; larger ones (many rows of a large
-  // vocabulary) are read again through the L2, which holds what 128 KB a CTA add up to:
-  // 256 rows of 131072 fp32 take 228 us in clusters of 8 that stage, waiting for one
-  // another, 160 us in clusters of 4 that do not, and 157 to 245 us in pairs, whose
-  // parts leave the L2 before they are read again.
+  // vocabulary) are read again through the L2: two CTAs an SM of 208 KB are half of it,
+  // what one die's half holds. With 256 rows of fp32, top-k 1000, in clusters of 2, 4
+  // and 8: 100000 tokens 128, 154 and 207 us; 131072 tokens 131 to 200, depending on
+  // where the rows lie, 155 and 220; 151936 tokens 176 and 229 by 4 and 8; 200003 tokens
+  // 205 and 256.
   uint32_t C = 1;
   auto bytes = [&](uint32_t c) {
     return fixed + (size_t(part_of(a.vocab, c)) + 16) * sizeof(T);
   };
   while (C < kMaxCtas && ((a.rows * uint64_t(C) < uint32_t(dev->num_sms) && a.vocab / C > 4096) ||
                           part_of(a.vocab, C) > kMaxPart ||
-                          a.vocab / C * sizeof(T) > 128 * 1024))
+                          a.vocab / C * sizeof(T) > 208 * 1024))
     C *= 2;
   const bool staged = bytes(C) <= 110 * 1024;
   static PerDeviceOnce once;
