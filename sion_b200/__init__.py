@@ -184,7 +184,8 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     """One token per row of logits [rows, vocab] from uniform [rows] in [0, 1):
     (tokens int32 [rows], log-probability of each under the kept tokens).
     temperature, top_p, min_p (fp32 [rows]) and top_k (int32 [rows]) may be
-    numbers, for all rows, or None."""
+    numbers, for all rows, or None. A number is written into a tensor by a small
+    kernel first (about 5 us each): a loop that keeps its tensors saves that."""
     import torch
 
     def rows(v, dtype):

@@ -29,16 +29,17 @@
 // left the denominator, as if it were masked.) The log-sum-exp has its own sum of
 // unrounded p. Sums and statistics are fp32.
 //
-// Measured: 96 slots of up to 12288 tokens, 8 heads of 128: 129 to 137 us for 585 MB
-// (65 to 69 % of the card's copy rate; its loads alone take 100 us), 507 instructions a
+// Measured: 96 slots of up to 12288 tokens, 8 heads of 128: 135 to 139 us for 585 MB
+// (64 to 66 % of the card's copy rate; its loads alone take 100 us), 517 instructions a
 // warp's step of 4352 bytes, 160 of them the masks and shifts of codes. Four slots of
-// 131071 tokens, 40 rows a group, heads of 64: 311 us, 578 instructions a step and 24
+// 131071 tokens, 40 rows a group, heads of 64: 317 us, 586 instructions a step and 24
 // rows. One slot of 1037 tokens: 8.8 us in the kernel, 14.4 us a call.
 //
 // The mma.sync form is used, not tcgen05: the product has 8 useful columns (one
 // group of heads), the codes reach the instruction from registers after one
-// logic operation per pair, and the kernel is bound by reading the cache and by
-// those logic operations, not by the matrix unit; tcgen05 would need the codes
+// logic operation per pair, and the kernel waits for its own latencies (half of the
+// issue slots, half of the ALU and a third of the matrix unit are used at three warps a
+// scheduler), not for the matrix unit; tcgen05 would need the codes
 // expanded to fp16 in shared or tensor memory, four times the bytes of the cache.
 #include <algorithm>
 

@@ -765,8 +765,8 @@ FelixCode kv4_copy_launch(const void* from, uint64_t from_pages, void* to, uint6
                           cudaStream_t stream) {
   DeviceInfo* dev = current_device_info();
   if (!dev) return launch_error(cudaGetLastError(), "kv4_copy_pages: no device");
-  return kv4_cache::copy(dev, from, from_pages, to, to_pages, page_bytes, src, dst, nullptr, count, count,
-                   stream);
+  return kv4_cache::copy(dev, from, from_pages, to, to_pages, page_bytes, src, dst, nullptr, count,
+                         count, stream);
 }
 
 FelixCode kv4_pages_launch(const Kv4PagesOp& o, cudaStream_t stream) {

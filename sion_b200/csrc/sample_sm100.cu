@@ -26,11 +26,11 @@
 //   top-k of up to 1024 (with or without the others): tokens are counted only, no
 //   exponentials; those down to the bin in which the k-th falls go to the first CTA
 //   of the cluster, which sorts them and finishes alone. 1 x 32000 fp16: 16 us (21 by
-//   one CTA); 256 x 131072 fp32: 152 us for 134 MB, 13 % of the card's copy rate: three
+//   one CTA); 256 x 131072 fp32: 152 to 165 us for 134 MB, 13 % of the card's copy rate: three
 //   passes of 64 values a thread, barriers, and 15 us of the first CTA alone.
 //   else: the bins' masses are summed too; the tokens of the bin in which top-p (or a
 //   large top-k) cuts, a few dozen as a rule, are gathered and sorted by every CTA, and
-//   a last pass sums what stays. 33 x 50021 bf16: 41 us, whatever the cluster's size.
+//   a last pass sums what stays. 33 x 50021 bf16: 41 to 42 us, whatever the cluster's size.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 

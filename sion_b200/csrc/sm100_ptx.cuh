@@ -31,10 +31,10 @@ enum WatchdogSite : unsigned {
   kWdAttnMma = 8,
   kWdAttnSoftmax = 9,
   kWdAttnCorrection = 10,
-  kWdSmemAlign = 11,
+  kWdSmemAlign = 11,  // dynamic shared memory not 1024-byte aligned: kernel did nothing
   kWdTileQueue = 12,  // HGEMM dynamic tile queue (producer push or consumer pop)
+  kWdTopkLoad = 13,   // top-k: bulk copy of a staged slice
   kWdKv4Load = 14,    // 4-bit cache attention: bulk copy of a step's blocks
-  kWdTopkLoad = 13,   // top-k: bulk copy of a staged slice  // dynamic shared memory not 1024-byte aligned: kernel did nothing
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
