@@ -106,6 +106,52 @@ FelixStatus sample_launch(const void* logits, ElementType type, uint32_t rows, u
                           const int32_t* top_k, const float* top_p, const float* min_p,
                           int32_t* tokens, float* logprobs, cudaStream_t stream);
 
+// new: feed-forward operators, fp16 or bf16 (felix_c.h describes the arguments and the
+// formulas): a linear layer with bias, activation and residual in the product's
+// epilogue, and a gated block, each with its backward pass. No reference counterpart.
+enum class Activation : int { None = 0, Relu = 1, Gelu = 2, GeluTanh = 3, Silu = 4, Sigmoid = 5 };
+
+struct Matrix {
+  void* data = nullptr;
+  int64_t stride = 0;  // elements from a row to the next
+};
+
+struct LinearArgs {
+  uint32_t tokens = 0, in_features = 0, out_features = 0;
+  ElementType type = ElementType::F16;
+  Activation activation = Activation::None;
+  Matrix x, weight, residual;
+  const void* bias = nullptr;
+  Matrix out, pre;
+  Matrix grad, dx, dweight;  // backward
+  void* dbias = nullptr;
+};
+
+struct GatedArgs {
+  uint32_t tokens = 0, features = 0, hidden = 0;
+  ElementType type = ElementType::F16;
+  Activation activation = Activation::Silu;
+  Matrix x, w_gate, w_up, w_down, residual;
+  Matrix out, gate, up;
+  Matrix grad, dx, dw_gate, dw_up, dw_down;  // backward
+};
+
+// workspace: nullptr = library-owned, else *_workspace_size bytes for these arguments.
+FelixStatus linear_launch(const LinearArgs& a, cudaStream_t stream, void* workspace = nullptr,
+                          size_t workspace_bytes = 0);
+FelixStatus linear_bwd_launch(const LinearArgs& a, cudaStream_t stream, void* workspace = nullptr,
+                              size_t workspace_bytes = 0);
+FelixStatus linear_workspace_size(const LinearArgs& a, bool backward, size_t* bytes);
+FelixStatus gated_linear_launch(const GatedArgs& a, cudaStream_t stream, void* workspace = nullptr,
+                                size_t workspace_bytes = 0);
+FelixStatus gated_linear_bwd_launch(const GatedArgs& a, cudaStream_t stream,
+                                    void* workspace = nullptr, size_t workspace_bytes = 0);
+FelixStatus gated_ffn_launch(const GatedArgs& a, cudaStream_t stream, void* workspace = nullptr,
+                             size_t workspace_bytes = 0);
+FelixStatus gated_ffn_bwd_launch(const GatedArgs& a, cudaStream_t stream, void* workspace = nullptr,
+                                 size_t workspace_bytes = 0);
+FelixStatus gated_workspace_size(const GatedArgs& a, bool ffn, bool backward, size_t* bytes);
+
 // new: reads (and clears) the device watchdog word; KERNEL_RUNTIME_ERROR when a
 // bounded wait inside a kernel gave up. Synchronises the device.
 FelixStatus check_watchdog();

@@ -330,6 +330,94 @@ int felix_sample(const void* logits, int dtype, uint32_t rows, uint32_t vocab, i
                  void* stream);
 
 /*
+ * Feed-forward operators (no reference counterpart: the reference has plain products
+ * only). fp16 or bf16 (`dtype`) in and out, sums in fp32, everything that follows a
+ * product done before its only rounding. Matrices are rows of contiguous elements,
+ * `stride` elements apart (rows of an input may repeat or overlap, stride 0 included).
+ * Any sizes from 1 up and any 2-byte alignment; rows that are no multiples of 16 bytes
+ * (or lie at other addresses) cost a copy of that input. Optional matrices have data
+ * NULL. Outputs may not overlap inputs or each other, but for `out`, which may be
+ * `residual` itself. tokens == 0 leaves outputs empty and sets the weights' gradients to zero.
+ *
+ * Activations: relu z < 0 ? 0 : z (derivative 0 at 0), gelu z Phi(z), gelu_tanh its
+ * form with tanh, silu z sigma(z), sigmoid sigma(z).
+ */
+#define FELIX_ACT_NONE 0
+#define FELIX_ACT_RELU 1
+#define FELIX_ACT_GELU 2
+#define FELIX_ACT_GELU_TANH 3
+#define FELIX_ACT_SILU 4
+#define FELIX_ACT_SIGMOID 5
+
+typedef struct felix_matrix {
+  void* data;
+  int64_t stride; /* elements from a row to the next; not used where there is one row */
+} felix_matrix;
+
+/*
+ * Linear layer. Forward, felix_linear: with z = x weight^T + bias,
+ *   out [tokens][out_features] = act(z) + residual, pre (optional) = z.
+ * x [tokens][in_features], weight [out_features][in_features], bias (optional)
+ * [out_features], residual (optional) as out.
+ * Backward, felix_linear_bwd: with dz = grad act'(pre) (pre is not read without an
+ * activation), each where wanted (not NULL): dx = dz weight, dweight = dz^T x, dbias =
+ * the sum of dz's rows. dz is rounded to 16 bits once, as the products read it; dbias
+ * sums it in fp32 before that. (The residual's gradient is grad itself.)
+ * Fields that a direction does not name are not read.
+ */
+typedef struct felix_linear_args {
+  uint32_t tokens, in_features, out_features;
+  int dtype, activation;
+  felix_matrix x, weight, residual;
+  const void* bias;
+  felix_matrix out, pre;
+  felix_matrix grad, dx, dweight;
+  void* dbias;
+} felix_linear_args;
+
+/*
+ * Gated feed-forward block. g = x w_gate^T, u = x w_up^T [tokens][hidden],
+ * h = act(g) u in one kernel; gate and up (optional) receive g and u.
+ *   felix_gated_linear: out [tokens][hidden] = h.
+ *   felix_gated_ffn:    out [tokens][features] = h w_down^T + residual (optional); h is
+ *                       rounded to 16 bits in between.
+ * w_gate, w_up [hidden][features], w_down [features][hidden].
+ * Backward from gate and up: dh = grad (felix_gated_linear_bwd, grad [tokens][hidden])
+ * or grad w_down (felix_gated_ffn_bwd, grad [tokens][features]; dh is never rounded),
+ *   dg = dh u act'(g), du = dh act(g), each rounded once;
+ * and where wanted dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x,
+ * dw_down = grad^T (act(g) u). (The residual's gradient is grad itself.)
+ */
+typedef struct felix_gated_args {
+  uint32_t tokens, features, hidden;
+  int dtype, activation;
+  felix_matrix x, w_gate, w_up, w_down, residual;
+  felix_matrix out, gate, up;
+  felix_matrix grad, dx, dw_gate, dw_up, dw_down;
+} felix_gated_args;
+
+/*
+ * workspace: NULL = library-owned per (device, stream), which stays as large as the
+ * largest call on the stream needed (the backward passes keep matrices of [tokens]
+ * [hidden] there); otherwise felix_*_workspace_size() bytes for these very arguments,
+ * 256-byte aligned, with any contents.
+ */
+int felix_linear(const felix_linear_args* args, void* workspace, size_t workspace_bytes,
+                 void* stream);
+int felix_linear_bwd(const felix_linear_args* args, void* workspace, size_t workspace_bytes,
+                     void* stream);
+int felix_linear_workspace_size(const felix_linear_args* args, int backward, size_t* bytes);
+int felix_gated_linear(const felix_gated_args* args, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int felix_gated_linear_bwd(const felix_gated_args* args, void* workspace, size_t workspace_bytes,
+                           void* stream);
+int felix_gated_ffn(const felix_gated_args* args, void* workspace, size_t workspace_bytes,
+                    void* stream);
+int felix_gated_ffn_bwd(const felix_gated_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream);
+int felix_gated_workspace_size(const felix_gated_args* args, int ffn, int backward, size_t* bytes);
+
+/*
  * Device watchdog. Every bounded wait inside the kernels records a nonzero
  * site code in a per-device status word when it gives up. Reads (and, when
  * clear != 0, resets) the word of the current device; synchronises the device.

@@ -2,6 +2,7 @@
 // reference (include/sion/sion.hpp:4-14); flash_attention_lse is new.
 #pragma once
 #include <optional>
+#include <string>
 #include <torch/torch.h>
 #include <tuple>
 #include <vector>
@@ -81,5 +82,51 @@ std::tuple<torch::Tensor, torch::Tensor> sample(
     const std::optional<torch::Tensor>& top_k = std::nullopt,
     const std::optional<torch::Tensor>& top_p = std::nullopt,
     const std::optional<torch::Tensor>& min_p = std::nullopt);
+
+// new: feed-forward operators in fp16 or bf16. x [..., in], weights as torch.nn.Linear
+// holds them ([out, in]), activation "none", "relu", "gelu", "gelu_tanh", "silu" or
+// "sigmoid". linear: act(x weight^T + bias) + residual; linear_save also returns what
+// stands in front of the activation, which linear_backward takes ((dx, dweight, dbias),
+// undefined where not wanted).
+torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight,
+                     const std::optional<torch::Tensor>& bias = std::nullopt,
+                     const std::optional<torch::Tensor>& residual = std::nullopt,
+                     const std::string& activation = "none");
+std::tuple<torch::Tensor, torch::Tensor> linear_save(
+    const torch::Tensor& x, const torch::Tensor& weight,
+    const std::optional<torch::Tensor>& bias = std::nullopt,
+    const std::optional<torch::Tensor>& residual = std::nullopt,
+    const std::string& activation = "none");
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& weight,
+    const std::optional<torch::Tensor>& pre, const std::string& activation = "none",
+    bool bias = false, bool need_x = true, bool need_weight = true);
+
+// new: act(x w_gate^T) * (x w_up^T); *_save also return both projections; gated_ffn
+// continues with w_down [in, hidden] and an optional residual.
+torch::Tensor gated_linear(const torch::Tensor& x, const torch::Tensor& w_gate,
+                           const torch::Tensor& w_up, const std::string& activation = "silu");
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_linear_save(
+    const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+    const std::string& activation = "silu");
+// (dx, dw_gate, dw_up)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_linear_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& w_gate,
+    const torch::Tensor& w_up, const torch::Tensor& gate, const torch::Tensor& up,
+    const std::string& activation = "silu", bool need_x = true, bool need_weights = true);
+torch::Tensor gated_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
+                        const torch::Tensor& w_up, const torch::Tensor& w_down,
+                        const std::optional<torch::Tensor>& residual = std::nullopt,
+                        const std::string& activation = "silu");
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn_save(
+    const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+    const torch::Tensor& w_down, const std::optional<torch::Tensor>& residual = std::nullopt,
+    const std::string& activation = "silu");
+// (dx, dw_gate, dw_up, dw_down)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& w_gate,
+    const torch::Tensor& w_up, const torch::Tensor& w_down, const torch::Tensor& gate,
+    const torch::Tensor& up, const std::string& activation = "silu", bool need_x = true,
+    bool need_weights = true);
 
 }  // namespace sion

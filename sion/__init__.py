@@ -13,6 +13,14 @@ from sion_b200 import (  # noqa: F401
     flash_attention_autograd,
     flash_attention_backward,
     flash_attention_lse,
+    gated_ffn,
+    gated_ffn_autograd,
+    gated_ffn_backward,
+    gated_ffn_save,
+    gated_linear,
+    gated_linear_autograd,
+    gated_linear_backward,
+    gated_linear_save,
     gemm,
     hgemm,
     hgemm_nt,
@@ -26,6 +34,10 @@ from sion_b200 import (  # noqa: F401
     kv4_page_bytes,
     kv4_read,
     kv4_reserve,
+    linear,
+    linear_autograd,
+    linear_backward,
+    linear_save,
     sample,
     sgemm,
 )
@@ -33,4 +45,7 @@ from sion_b200 import (  # noqa: F401
 __all__ = ["sgemm", "hgemm", "hgemm_nt", "gemm", "flash_attention", "flash_attention_lse",
            "flash_attention_backward", "flash_attention_autograd", "kv4_page_bytes", "kv4_append",
            "kv4_read", "kv4_attention", "kv4_attention_lse", "kv4_reserve", "kv4_fork", "kv4_free",
-           "kv4_compact", "kv4_copy_pages", "sample", "LIB_PATH"]
+           "kv4_compact", "kv4_copy_pages", "sample", "linear", "linear_save", "linear_backward",
+           "linear_autograd", "gated_linear", "gated_linear_save", "gated_linear_backward",
+           "gated_linear_autograd", "gated_ffn", "gated_ffn_save", "gated_ffn_backward",
+           "gated_ffn_autograd", "LIB_PATH"]

@@ -22,6 +22,14 @@ Decoding (no counterpart in the reference): a paged cache of keys and values in
     kv4_reserve / kv4_fork / kv4_free / kv4_compact / kv4_copy_pages
     sample(logits, uniform, temperature, top_k, top_p, min_p)
 
+Feed-forward (no counterpart in the reference), fp16 or bf16, weights [out, in]:
+
+    linear(x, W, bias, residual, activation)   act(x W^T + b) + r
+    gated_linear(x, Wg, Wu, activation)        act(x Wg^T) * (x Wu^T)
+    gated_ffn(x, Wg, Wu, Wd, residual, ...)    the whole block
+    *_save(...)                                also what the backward pass needs
+    *_backward(...), *_autograd(...)           gradients, torch.autograd
+
 These come from the native module ``_sion`` (LibTorch C++), which calls the
 felix:: C++ API in ``libfelix_b200.so``. The C ABI of that library
 (include/felix_c.h) is reachable through :mod:`sion_b200.abi`. There is no
@@ -198,7 +206,152 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
                               rows(min_p, torch.float32))
 
 
+def linear(x, weight, bias=None, residual=None, activation: str = "none"):
+    """act(x weight^T + bias) + residual in one kernel, rounded once. x [..., in] fp16 or
+    bf16, weight [out, in], bias [out], residual [..., out]. activation: "none", "relu",
+    "gelu", "gelu_tanh", "silu" or "sigmoid"."""
+    return _load_ext().linear(x, weight, bias, residual, activation)
+
+
+def linear_save(x, weight, bias=None, residual=None, activation: str = "none"):
+    """linear returning (y, pre), pre = x weight^T + bias for linear_backward."""
+    return _load_ext().linear_save(x, weight, bias, residual, activation)
+
+
+def linear_backward(grad, x, weight, pre=None, activation: str = "none", bias: bool = False,
+                    need_x: bool = True, need_weight: bool = True):
+    """(dx, dweight, dbias) of linear from grad [..., out] and, with an activation, pre;
+    None where not wanted. The residual's gradient is grad."""
+    return _load_ext().linear_backward(grad, x, weight, pre, activation, bias, need_x, need_weight)
+
+
+def gated_linear(x, w_gate, w_up, activation: str = "silu"):
+    """act(x w_gate^T) * (x w_up^T) in one kernel. x [..., in], both weights [hidden, in]."""
+    return _load_ext().gated_linear(x, w_gate, w_up, activation)
+
+
+def gated_linear_save(x, w_gate, w_up, activation: str = "silu"):
+    """gated_linear returning (h, gate, up), the projections for gated_linear_backward."""
+    return _load_ext().gated_linear_save(x, w_gate, w_up, activation)
+
+
+def gated_linear_backward(grad, x, w_gate, w_up, gate, up, activation: str = "silu",
+                          need_x: bool = True, need_weights: bool = True):
+    """(dx, dw_gate, dw_up) of gated_linear; None where not wanted."""
+    return _load_ext().gated_linear_backward(grad, x, w_gate, w_up, gate, up, activation, need_x,
+                                             need_weights)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, residual=None, activation: str = "silu"):
+    """gated_linear(x, w_gate, w_up) w_down^T + residual; w_down [in, hidden]."""
+    return _load_ext().gated_ffn(x, w_gate, w_up, w_down, residual, activation)
+
+
+def gated_ffn_save(x, w_gate, w_up, w_down, residual=None, activation: str = "silu"):
+    """gated_ffn returning (y, gate, up), the projections for gated_ffn_backward."""
+    return _load_ext().gated_ffn_save(x, w_gate, w_up, w_down, residual, activation)
+
+
+def gated_ffn_backward(grad, x, w_gate, w_up, w_down, gate, up, activation: str = "silu",
+                       need_x: bool = True, need_weights: bool = True):
+    """(dx, dw_gate, dw_up, dw_down) of gated_ffn; None where not wanted. The residual's
+    gradient is grad."""
+    return _load_ext().gated_ffn_backward(grad, x, w_gate, w_up, w_down, gate, up, activation,
+                                          need_x, need_weights)
+
+
+def _ffn_functions():
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class Linear(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, residual, activation):
+            pre = None
+            if activation == "none":
+                y = linear(x, weight, bias, residual, activation)
+            else:
+                y, pre = linear_save(x, weight, bias, residual, activation)
+            ctx.save_for_backward(x, weight, pre)
+            ctx.activation = activation
+            return y
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            x, weight, pre = ctx.saved_tensors
+            need = ctx.needs_input_grad
+            dx = dw = db = None
+            if need[0] or need[1] or need[2]:
+                dx, dw, db = linear_backward(grad, x, weight, pre, ctx.activation, need[2],
+                                             need[0], need[1])
+            return dx, dw, db, grad if need[3] else None, None
+
+    class GatedLinear(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w_gate, w_up, activation):
+            h, gate, up = gated_linear_save(x, w_gate, w_up, activation)
+            ctx.save_for_backward(x, w_gate, w_up, gate, up)
+            ctx.activation = activation
+            return h
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            need = ctx.needs_input_grad
+            return *gated_linear_backward(grad, *ctx.saved_tensors, ctx.activation, need[0],
+                                          need[1] or need[2]), None
+
+    class GatedFfn(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w_gate, w_up, w_down, residual, activation):
+            y, gate, up = gated_ffn_save(x, w_gate, w_up, w_down, residual, activation)
+            ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
+            ctx.activation = activation
+            return y
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            need = ctx.needs_input_grad
+            d = (None,) * 4
+            if any(need[:4]):
+                d = gated_ffn_backward(grad, *ctx.saved_tensors, ctx.activation, need[0],
+                                       any(need[1:4]))
+            return *d, grad if need[4] else None, None
+
+    return Linear, GatedLinear, GatedFfn
+
+
+_FFN_FNS = None
+
+
+def _ffn_function(i):
+    global _FFN_FNS
+    if _FFN_FNS is None:
+        _FFN_FNS = _ffn_functions()
+    return _FFN_FNS[i]
+
+
+def linear_autograd(x, weight, bias=None, residual=None, activation: str = "none"):
+    """linear that torch.autograd can differentiate (first derivatives)."""
+    return _ffn_function(0).apply(x, weight, bias, residual, activation)
+
+
+def gated_linear_autograd(x, w_gate, w_up, activation: str = "silu"):
+    """gated_linear that torch.autograd can differentiate (first derivatives)."""
+    return _ffn_function(1).apply(x, w_gate, w_up, activation)
+
+
+def gated_ffn_autograd(x, w_gate, w_up, w_down, residual=None, activation: str = "silu"):
+    """gated_ffn that torch.autograd can differentiate (first derivatives)."""
+    return _ffn_function(2).apply(x, w_gate, w_up, w_down, residual, activation)
+
+
 __all__ = ["sgemm", "hgemm", "hgemm_nt", "gemm", "flash_attention", "flash_attention_lse",
            "flash_attention_backward", "flash_attention_autograd", "kv4_page_bytes", "kv4_append",
            "kv4_read", "kv4_attention", "kv4_attention_lse", "kv4_reserve", "kv4_fork", "kv4_free",
-           "kv4_compact", "kv4_copy_pages", "sample", "LIB_PATH"]
+           "kv4_compact", "kv4_copy_pages", "sample", "linear", "linear_save", "linear_backward",
+           "linear_autograd", "gated_linear", "gated_linear_save", "gated_linear_backward",
+           "gated_linear_autograd", "gated_ffn", "gated_ffn_save", "gated_ffn_backward",
+           "gated_ffn_autograd", "LIB_PATH"]

@@ -56,6 +56,11 @@ _SIGS = {
                           [C.c_int, C.c_void_p]),
     "felix_flash_attn_fwd_ex": (C.c_int, [C.c_void_p] * 5 + [C.c_uint32] * 4 +
                                 [C.c_float, C.c_int, C.c_void_p]),
+    **{"felix_" + f: (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p])
+       for f in ("linear", "linear_bwd", "gated_linear", "gated_linear_bwd", "gated_ffn",
+                 "gated_ffn_bwd")},
+    "felix_linear_workspace_size": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_size_t)]),
+    "felix_gated_workspace_size": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
     "felix_kv4_page_bytes": (C.c_int, [C.c_uint32] * 3 + [C.POINTER(C.c_size_t)]),
     "felix_kv4_append": (C.c_int, [C.c_void_p] * 3 + [C.c_int, C.c_uint32] + [C.c_void_p] * 4),
     "felix_kv4_read": (C.c_int, [C.c_void_p, C.c_uint32] + [C.c_void_p] * 4),
@@ -79,6 +84,31 @@ _SIGS = {
 }
 
 F16, BF16, F32 = 0, 1, 2
+
+
+class Matrix(C.Structure):
+    """felix_matrix of the header: rows of contiguous elements, `stride` apart."""
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64)]
+
+
+class LinearArgs(C.Structure):
+    """felix_linear_args of the header."""
+    _fields_ = ([(f, C.c_uint32) for f in ("tokens", "in_features", "out_features")] +
+                [("dtype", C.c_int), ("activation", C.c_int)] +
+                [(f, Matrix) for f in ("x", "weight", "residual")] + [("bias", C.c_void_p)] +
+                [(f, Matrix) for f in ("out", "pre", "grad", "dx", "dweight")] +
+                [("dbias", C.c_void_p)])
+
+
+class GatedArgs(C.Structure):
+    """felix_gated_args of the header."""
+    _fields_ = ([(f, C.c_uint32) for f in ("tokens", "features", "hidden")] +
+                [("dtype", C.c_int), ("activation", C.c_int)] +
+                [(f, Matrix) for f in ("x", "w_gate", "w_up", "w_down", "residual", "out", "gate",
+                                       "up", "grad", "dx", "dw_gate", "dw_up", "dw_down")])
+
+
+ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid")
 
 
 class Kv4Cache(C.Structure):
@@ -293,6 +323,45 @@ def sample(logits, uniform, tokens, logprobs, temperature=None, top_k=None, top_
                              _ptr(uniform), _ptr(temperature), _ptr(top_k), _ptr(top_p),
                              _ptr(min_p), _ptr(tokens), _ptr(logprobs), _stream(stream)))
     return tokens, logprobs
+
+
+def matrix(t) -> Matrix:
+    """A 2-D tensor whose rows are contiguous (None: no matrix)."""
+    return Matrix(None, 0) if t is None else Matrix(t.data_ptr(), t.stride(0))
+
+
+def _ffn_args(cls, sizes, dtype, activation, fields):
+    a = cls(*sizes, dtype, ACTIVATIONS.index(activation))
+    for name, v in fields.items():
+        setattr(a, name, _ptr(v) if name in ("bias", "dbias") else matrix(v))
+    return a
+
+
+def linear_args(tokens, in_features, out_features, dtype, activation="none", **fields) -> LinearArgs:
+    """Arguments of felix_linear / felix_linear_bwd from 2-D tensors."""
+    return _ffn_args(LinearArgs, (tokens, in_features, out_features), dtype, activation, fields)
+
+
+def gated_args(tokens, features, hidden, dtype, activation="silu", **fields) -> GatedArgs:
+    """Arguments of felix_gated_linear / felix_gated_ffn and their backward passes."""
+    return _ffn_args(GatedArgs, (tokens, features, hidden), dtype, activation, fields)
+
+
+def ffn_call(name, args, workspace=None, stream=None):
+    """felix_<name>(args); name: linear, linear_bwd, gated_linear, gated_linear_bwd,
+    gated_ffn, gated_ffn_bwd."""
+    check(getattr(lib(), "felix_" + name)(C.byref(args), _ptr(workspace),
+                                          0 if workspace is None else workspace.nbytes,
+                                          _stream(stream)))
+
+
+def ffn_workspace_size(name, args) -> int:
+    n, back = C.c_size_t(), int(name.endswith("_bwd"))
+    if name.startswith("linear"):
+        check(lib().felix_linear_workspace_size(C.byref(args), back, C.byref(n)))
+    else:
+        check(lib().felix_gated_workspace_size(C.byref(args), int("ffn" in name), back, C.byref(n)))
+    return n.value
 
 
 def watchdog_status(clear=True) -> int:

@@ -311,6 +311,55 @@ FelixStatus sample_launch(const void* logits, ElementType type, uint32_t rows, u
                              temperature, top_k, top_p, min_p, tokens, logprobs, stream));
 }
 
+namespace {
+felix_matrix c_mat(const Matrix& m) { return {m.data, m.stride}; }
+felix_linear_args c_args(const LinearArgs& a) {
+  return {a.tokens, a.in_features, a.out_features, static_cast<int>(a.type),
+          static_cast<int>(a.activation), c_mat(a.x), c_mat(a.weight), c_mat(a.residual), a.bias,
+          c_mat(a.out), c_mat(a.pre), c_mat(a.grad), c_mat(a.dx), c_mat(a.dweight), a.dbias};
+}
+felix_gated_args c_args(const GatedArgs& a) {
+  return {a.tokens, a.features, a.hidden, static_cast<int>(a.type),
+          static_cast<int>(a.activation), c_mat(a.x), c_mat(a.w_gate), c_mat(a.w_up),
+          c_mat(a.w_down), c_mat(a.residual), c_mat(a.out), c_mat(a.gate), c_mat(a.up),
+          c_mat(a.grad), c_mat(a.dx), c_mat(a.dw_gate), c_mat(a.dw_up), c_mat(a.dw_down)};
+}
+}  // namespace
+
+FelixStatus linear_launch(const LinearArgs& a, cudaStream_t stream, void* ws, size_t bytes) {
+  const felix_linear_args c = c_args(a);
+  return from_c(felix_linear(&c, ws, bytes, stream));
+}
+FelixStatus linear_bwd_launch(const LinearArgs& a, cudaStream_t stream, void* ws, size_t bytes) {
+  const felix_linear_args c = c_args(a);
+  return from_c(felix_linear_bwd(&c, ws, bytes, stream));
+}
+FelixStatus linear_workspace_size(const LinearArgs& a, bool backward, size_t* bytes) {
+  const felix_linear_args c = c_args(a);
+  return from_c(felix_linear_workspace_size(&c, backward, bytes));
+}
+FelixStatus gated_linear_launch(const GatedArgs& a, cudaStream_t stream, void* ws, size_t bytes) {
+  const felix_gated_args c = c_args(a);
+  return from_c(felix_gated_linear(&c, ws, bytes, stream));
+}
+FelixStatus gated_linear_bwd_launch(const GatedArgs& a, cudaStream_t stream, void* ws,
+                                    size_t bytes) {
+  const felix_gated_args c = c_args(a);
+  return from_c(felix_gated_linear_bwd(&c, ws, bytes, stream));
+}
+FelixStatus gated_ffn_launch(const GatedArgs& a, cudaStream_t stream, void* ws, size_t bytes) {
+  const felix_gated_args c = c_args(a);
+  return from_c(felix_gated_ffn(&c, ws, bytes, stream));
+}
+FelixStatus gated_ffn_bwd_launch(const GatedArgs& a, cudaStream_t stream, void* ws, size_t bytes) {
+  const felix_gated_args c = c_args(a);
+  return from_c(felix_gated_ffn_bwd(&c, ws, bytes, stream));
+}
+FelixStatus gated_workspace_size(const GatedArgs& a, bool ffn, bool backward, size_t* bytes) {
+  const felix_gated_args c = c_args(a);
+  return from_c(felix_gated_workspace_size(&c, ffn, backward, bytes));
+}
+
 FelixStatus check_watchdog() {
   unsigned code = 0;
   return from_c(felix_watchdog_status(&code, 1));

@@ -358,7 +358,7 @@ FelixCode watchdog_probe_launch(uint32_t limit_us, cudaStream_t stream) {
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
-static int finish(FelixCode c) {
+int finish(FelixCode c) {
   if (c.type == FELIX_SUCCESS) {
     t_last_cuda = 0;
     t_last_msg.clear();

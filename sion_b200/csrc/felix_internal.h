@@ -22,6 +22,8 @@ struct FelixCode {
 // Record a message for felix_last_error_message() and return the code.
 FelixCode api_error(const char* msg, cudaError_t e = cudaErrorInvalidValue);
 FelixCode launch_error(cudaError_t e, const char* msg);
+// Ends an entry point: forgets the thread's last error after a success, returns the type.
+int finish(FelixCode c);
 
 struct DeviceInfo {
   int ordinal;

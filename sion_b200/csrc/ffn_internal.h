@@ -1,0 +1,56 @@
+// Host-side interfaces of the feed-forward operators' translation units.
+#pragma once
+#include "felix_internal.h"
+
+namespace felix_ffn {
+
+using felix_impl::DeviceInfo;
+using felix_impl::FelixCode;
+
+// A matrix of 16-bit elements whose rows are `ld` elements apart.
+struct Mat {
+  const void* p = nullptr;
+  int64_t ld = 0;
+};
+struct MutMat {
+  void* p = nullptr;
+  int64_t ld = 0;
+};
+
+// What a product's epilogue makes of the fp32 accumulators.
+enum Epilogue {
+  kLinear = 0,  // out0 = act(v + bias) + in0, out1 = v + bias
+  kGated = 1,   // v = g | u: out0 = act(g) u, out1 = g, out2 = u
+  kDGated = 2   // v = dh, in0 = g, in1 = u: out0 = dh u act'(g), out1 = dh act(g), out2 = act(g) u
+};
+
+// D[m][n] = sum over segments and k of A[m][k] B[n][k]. An operand is stored either
+// with k contiguous (A [m][k], B [n][k]) or, "mn", with m or n contiguous (A [k][m],
+// B [k][n]).
+struct Product {
+  Epilogue epilogue = kLinear;
+  bool bf16 = false;
+  bool a_mn = false, b_mn = false;
+  uint32_t k = 0;         // depth of one segment
+  uint32_t segments = 1;  // kLinear only: A and B of each segment in a[], b[]
+  uint32_t problems = 1;  // kLinear only: independent products of one depth, a[], b[], out[]
+  uint32_t m[3] = {}, n[3] = {};
+  Mat a[3], b[3];  // kGated: b[0] gate, b[1] up
+  MutMat out[3];   // null: not wanted (out1 of kLinear, out1 and out2 of kGated)
+  Mat in[2];
+  const void* bias = nullptr;
+  int act = FELIX_ACT_NONE;
+};
+
+// Whether TMA can address a matrix of these rows.
+inline bool tma_ok(const void* p, int64_t ld, uint32_t rows, uint64_t cols) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
+         (rows <= 1 || (ld % 8 == 0 && ld >= int64_t(cols) && ld < (int64_t(1) << 38)));
+}
+
+// Scratch of a product: kWsCounterBytes of counters that are zero before and after,
+// then fp32 partials. a and b must be addressable by TMA.
+size_t product_workspace_bytes(const Product& p, int num_sms);
+FelixCode product_launch(DeviceInfo* dev, const Product& p, void* workspace, cudaStream_t stream);
+
+}  // namespace felix_ffn

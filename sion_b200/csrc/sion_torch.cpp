@@ -545,6 +545,314 @@ std::tuple<torch::Tensor, torch::Tensor> sample(const torch::Tensor& logits,
   return {tokens, logprobs};
 }
 
+// ---------------------------------------------------------- feed-forward operators
+namespace {
+constexpr int64_t kMostFeatures = 1 << 30;
+
+felix::Activation activation_of(const std::string& name) {
+  constexpr const char* names[] = {"none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid"};
+  for (int i = 0; i < 6; ++i)
+    if (name == names[i]) return static_cast<felix::Activation>(i);
+  TORCH_CHECK(false, "unknown activation \"", name,
+              "\" (none, relu, gelu, gelu_tanh, silu, sigmoid)");
+}
+
+// A tensor as rows of contiguous elements; any leading dimensions, a copy only where the
+// last one is not contiguous or the rows are not evenly spaced.
+struct Rows {
+  torch::Tensor t;
+  int64_t rows = 0, cols = 0;
+  felix::Matrix m() const { return {t.data_ptr(), t.stride(0)}; }
+};
+Rows rows_of(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be CUDA tensor");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type());
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) > 0, name, " must have a last dimension that is not empty");
+  Rows r;
+  r.cols = t.size(-1);
+  r.rows = t.numel() / r.cols;
+  r.t = t.dim() == 2 ? t : t.reshape({r.rows, r.cols});
+  if (r.cols > 1 && r.t.stride(1) != 1) r.t = r.t.contiguous();
+  return r;
+}
+Rows weight_of(const torch::Tensor& w, const torch::Tensor& like, const char* name, int64_t rows,
+               int64_t cols) {
+  TORCH_CHECK(w.dim() == 2, name, " must be 2D");
+  TORCH_CHECK((rows < 0 || w.size(0) == rows) && w.size(1) == cols, name, " must be [",
+              rows < 0 ? std::string("out") : std::to_string(rows), ", ", cols, "]");
+  TORCH_CHECK(w.size(0) > 0, name, " must not be empty");
+  return rows_of(w, like, name);
+}
+std::vector<int64_t> with_last(const torch::Tensor& t, int64_t n) {
+  auto s = t.sizes().vec();
+  s.back() = n;
+  return s;
+}
+void check_sizes(const torch::Tensor& t, const std::vector<int64_t>& s, const char* name) {
+  TORCH_CHECK(t.sizes().vec() == s, name, " must have the shape ", at::IntArrayRef(s));
+}
+felix::Matrix out_of(const torch::Tensor& t) { return {t.data_ptr(), t.size(-1)}; }
+
+// Scratch past this size comes from torch's allocator and goes back to it; below it the
+// library keeps one per stream.
+constexpr size_t kOwnScratch = size_t(32) << 20;
+struct Scratch {
+  torch::Tensor t;
+  size_t bytes = 0;
+  void* ptr() const { return bytes ? t.data_ptr() : nullptr; }
+};
+Scratch scratch_of(size_t need, const torch::Tensor& like) {
+  if (need <= kOwnScratch) return {};
+  return {torch::empty({int64_t(need)}, like.options().dtype(torch::kUInt8)), need};
+}
+
+struct LinearCall {
+  felix::LinearArgs a;
+  std::vector<torch::Tensor> held;  // what the arguments point into
+  void hold(const Rows& r, felix::Matrix* to) {
+    held.push_back(r.t);
+    *to = r.m();
+  }
+};
+LinearCall linear_call(const torch::Tensor& x, const torch::Tensor& weight,
+                       const std::string& activation) {
+  LinearCall c;
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  c.a.type = half_type(x, "x");
+  c.a.activation = activation_of(activation);
+  const Rows X = rows_of(x, x, "x");
+  const Rows W = weight_of(weight, x, "weight", -1, X.cols);
+  c.a.tokens = u32(X.rows, kMostFeatures, "tokens");
+  c.a.in_features = u32(X.cols, kMostFeatures, "in_features");
+  c.a.out_features = u32(W.rows, kMostFeatures, "out_features");
+  c.hold(X, &c.a.x);
+  c.hold(W, &c.a.weight);
+  return c;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> linear_impl(const torch::Tensor& x,
+                                                     const torch::Tensor& weight,
+                                                     const OptTensor& bias,
+                                                     const OptTensor& residual,
+                                                     const std::string& activation, bool save) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  const c10::cuda::CUDAGuard guard(x.device());
+  LinearCall c = linear_call(x, weight, activation);
+  const auto shape = with_last(x, c.a.out_features);
+  if (bias) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0),
+                "bias must have one entry per output feature");
+    const Rows b = rows_of(*bias, x, "bias");
+    c.held.push_back(b.t);
+    c.a.bias = b.t.data_ptr();
+  }
+  if (residual) {
+    check_sizes(*residual, shape, "residual");
+    c.hold(rows_of(*residual, x, "residual"), &c.a.residual);
+  }
+  auto y = torch::empty(shape, x.options());
+  torch::Tensor pre;
+  c.a.out = out_of(y);
+  if (save) {
+    pre = torch::empty(shape, x.options());
+    c.a.pre = out_of(pre);
+  }
+  size_t need = 0;
+  auto status = felix::linear_workspace_size(c.a, false, &need);
+  TORCH_CHECK(status.ok(), "linear: ", status.str());
+  const Scratch s = scratch_of(need, x);
+  status = felix::linear_launch(c.a, at::cuda::getCurrentCUDAStream(), s.ptr(), s.bytes);
+  TORCH_CHECK(status.ok(), "linear: kernel launch failed: ", status.str());
+  return {y, pre};
+}
+
+struct GatedCall {
+  felix::GatedArgs a;
+  std::vector<torch::Tensor> held;
+  void hold(const Rows& r, felix::Matrix* to) {
+    held.push_back(r.t);
+    *to = r.m();
+  }
+};
+GatedCall gated_call(const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+                     const torch::Tensor* w_down, const std::string& activation) {
+  GatedCall c;
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  c.a.type = half_type(x, "x");
+  c.a.activation = activation_of(activation);
+  const Rows X = rows_of(x, x, "x");
+  const Rows G = weight_of(w_gate, x, "w_gate", -1, X.cols);
+  const Rows U = weight_of(w_up, x, "w_up", G.rows, X.cols);
+  c.a.tokens = u32(X.rows, kMostFeatures, "tokens");
+  c.a.features = u32(X.cols, kMostFeatures, "features");
+  c.a.hidden = u32(G.rows, kMostFeatures, "hidden");
+  c.hold(X, &c.a.x);
+  c.hold(G, &c.a.w_gate);
+  c.hold(U, &c.a.w_up);
+  if (w_down) c.hold(weight_of(*w_down, x, "w_down", X.cols, G.rows), &c.a.w_down);
+  return c;
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_impl(
+    const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+    const torch::Tensor* w_down, const OptTensor& residual, const std::string& activation,
+    bool save) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  const c10::cuda::CUDAGuard guard(x.device());
+  GatedCall c = gated_call(x, w_gate, w_up, w_down, activation);
+  const auto wide = with_last(x, c.a.hidden);
+  const auto shape = w_down ? x.sizes().vec() : wide;
+  if (residual) {
+    check_sizes(*residual, shape, "residual");
+    c.hold(rows_of(*residual, x, "residual"), &c.a.residual);
+  }
+  auto y = torch::empty(shape, x.options());
+  c.a.out = out_of(y);
+  torch::Tensor gate, up;
+  if (save) {
+    gate = torch::empty(wide, x.options());
+    up = torch::empty(wide, x.options());
+    c.a.gate = out_of(gate);
+    c.a.up = out_of(up);
+  }
+  size_t need = 0;
+  auto status = felix::gated_workspace_size(c.a, w_down != nullptr, false, &need);
+  TORCH_CHECK(status.ok(), "gated feed-forward: ", status.str());
+  const Scratch s = scratch_of(need, x);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  status = w_down ? felix::gated_ffn_launch(c.a, stream, s.ptr(), s.bytes)
+                  : felix::gated_linear_launch(c.a, stream, s.ptr(), s.bytes);
+  TORCH_CHECK(status.ok(), "gated feed-forward: kernel launch failed: ", status.str());
+  return {y, gate, up};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_backward_impl(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& w_gate,
+    const torch::Tensor& w_up, const torch::Tensor* w_down, const torch::Tensor& gate,
+    const torch::Tensor& up, const std::string& activation, bool need_x, bool need_weights) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  const c10::cuda::CUDAGuard guard(x.device());
+  GatedCall c = gated_call(x, w_gate, w_up, w_down, activation);
+  const auto wide = with_last(x, c.a.hidden);
+  check_sizes(grad, w_down ? x.sizes().vec() : wide, "grad");
+  check_sizes(gate, wide, "gate");
+  check_sizes(up, wide, "up");
+  c.hold(rows_of(grad, x, "grad"), &c.a.grad);
+  c.hold(rows_of(gate, x, "gate"), &c.a.gate);
+  c.hold(rows_of(up, x, "up"), &c.a.up);
+  torch::Tensor dx, dg, du, dd;
+  const auto opt = x.options();
+  if (need_x) {
+    dx = torch::empty(x.sizes(), opt);
+    c.a.dx = out_of(dx);
+  }
+  if (need_weights) {
+    dg = torch::empty(w_gate.sizes(), opt);
+    du = torch::empty(w_up.sizes(), opt);
+    c.a.dw_gate = out_of(dg);
+    c.a.dw_up = out_of(du);
+    if (w_down) {
+      dd = torch::empty(w_down->sizes(), opt);
+      c.a.dw_down = out_of(dd);
+    }
+  }
+  size_t need = 0;
+  auto status = felix::gated_workspace_size(c.a, w_down != nullptr, true, &need);
+  TORCH_CHECK(status.ok(), "gated feed-forward backward: ", status.str());
+  const Scratch s = scratch_of(need, x);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  status = w_down ? felix::gated_ffn_bwd_launch(c.a, stream, s.ptr(), s.bytes)
+                  : felix::gated_linear_bwd_launch(c.a, stream, s.ptr(), s.bytes);
+  TORCH_CHECK(status.ok(), "gated feed-forward backward: kernel launch failed: ", status.str());
+  return {dx, dg, du, dd};
+}
+}  // namespace
+
+torch::Tensor linear(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias,
+                     const OptTensor& residual, const std::string& activation) {
+  return std::get<0>(linear_impl(x, weight, bias, residual, activation, false));
+}
+std::tuple<torch::Tensor, torch::Tensor> linear_save(const torch::Tensor& x,
+                                                     const torch::Tensor& weight,
+                                                     const OptTensor& bias,
+                                                     const OptTensor& residual,
+                                                     const std::string& activation) {
+  return linear_impl(x, weight, bias, residual, activation, true);
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> linear_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& weight,
+    const OptTensor& pre, const std::string& activation, bool bias, bool need_x,
+    bool need_weight) {
+  TORCH_CHECK(x.is_cuda(), "x must be CUDA tensor");
+  const c10::cuda::CUDAGuard guard(x.device());
+  LinearCall c = linear_call(x, weight, activation);
+  const auto shape = with_last(x, c.a.out_features);
+  check_sizes(grad, shape, "grad");
+  c.hold(rows_of(grad, x, "grad"), &c.a.grad);
+  if (c.a.activation != felix::Activation::None) {
+    TORCH_CHECK(pre, "pre (from linear_save) is needed for the backward pass of ", activation);
+    check_sizes(*pre, shape, "pre");
+    c.hold(rows_of(*pre, x, "pre"), &c.a.pre);
+  }
+  torch::Tensor dx, dw, db;
+  const auto opt = x.options();
+  if (need_x) {
+    dx = torch::empty(x.sizes(), opt);
+    c.a.dx = out_of(dx);
+  }
+  if (need_weight) {
+    dw = torch::empty(weight.sizes(), opt);
+    c.a.dweight = out_of(dw);
+  }
+  if (bias) {
+    db = torch::empty({weight.size(0)}, opt);
+    c.a.dbias = db.data_ptr();
+  }
+  size_t need = 0;
+  auto status = felix::linear_workspace_size(c.a, true, &need);
+  TORCH_CHECK(status.ok(), "linear_backward: ", status.str());
+  const Scratch s = scratch_of(need, x);
+  status = felix::linear_bwd_launch(c.a, at::cuda::getCurrentCUDAStream(), s.ptr(), s.bytes);
+  TORCH_CHECK(status.ok(), "linear_backward: kernel launch failed: ", status.str());
+  return {dx, dw, db};
+}
+
+torch::Tensor gated_linear(const torch::Tensor& x, const torch::Tensor& w_gate,
+                           const torch::Tensor& w_up, const std::string& activation) {
+  return std::get<0>(gated_impl(x, w_gate, w_up, nullptr, std::nullopt, activation, false));
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_linear_save(
+    const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+    const std::string& activation) {
+  return gated_impl(x, w_gate, w_up, nullptr, std::nullopt, activation, true);
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_linear_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& w_gate,
+    const torch::Tensor& w_up, const torch::Tensor& gate, const torch::Tensor& up,
+    const std::string& activation, bool need_x, bool need_weights) {
+  auto r = gated_backward_impl(grad, x, w_gate, w_up, nullptr, gate, up, activation, need_x,
+                               need_weights);
+  return {std::get<0>(r), std::get<1>(r), std::get<2>(r)};
+}
+torch::Tensor gated_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
+                        const torch::Tensor& w_up, const torch::Tensor& w_down,
+                        const OptTensor& residual, const std::string& activation) {
+  return std::get<0>(gated_impl(x, w_gate, w_up, &w_down, residual, activation, false));
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn_save(
+    const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up,
+    const torch::Tensor& w_down, const OptTensor& residual, const std::string& activation) {
+  return gated_impl(x, w_gate, w_up, &w_down, residual, activation, true);
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn_backward(
+    const torch::Tensor& grad, const torch::Tensor& x, const torch::Tensor& w_gate,
+    const torch::Tensor& w_up, const torch::Tensor& w_down, const torch::Tensor& gate,
+    const torch::Tensor& up, const std::string& activation, bool need_x, bool need_weights) {
+  return gated_backward_impl(grad, x, w_gate, w_up, &w_down, gate, up, activation, need_x,
+                             need_weights);
+}
+
 }  // namespace sion
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -600,4 +908,32 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sample", &sion::sample, "one token per row of logits (tokens, log-probabilities)",
         py::arg("logits"), py::arg("uniform"), py::arg("temperature") = none,
         py::arg("top_k") = none, py::arg("top_p") = none, py::arg("min_p") = none);
+  m.def("linear", &sion::linear, "act(x weight^T + bias) + residual", py::arg("x"),
+        py::arg("weight"), py::arg("bias") = none, py::arg("residual") = none,
+        py::arg("activation") = "none");
+  m.def("linear_save", &sion::linear_save, "linear returning (y, what the activation was given)",
+        py::arg("x"), py::arg("weight"), py::arg("bias") = none, py::arg("residual") = none,
+        py::arg("activation") = "none");
+  m.def("linear_backward", &sion::linear_backward, "gradients of linear (dx, dweight, dbias)",
+        py::arg("grad"), py::arg("x"), py::arg("weight"), py::arg("pre") = none,
+        py::arg("activation") = "none", py::arg("bias") = false, py::arg("need_x") = true,
+        py::arg("need_weight") = true);
+  m.def("gated_linear", &sion::gated_linear, "act(x w_gate^T) * (x w_up^T)", py::arg("x"),
+        py::arg("w_gate"), py::arg("w_up"), py::arg("activation") = "silu");
+  m.def("gated_linear_save", &sion::gated_linear_save, "gated_linear returning (h, gate, up)",
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("activation") = "silu");
+  m.def("gated_linear_backward", &sion::gated_linear_backward,
+        "gradients of gated_linear (dx, dw_gate, dw_up)", py::arg("grad"), py::arg("x"),
+        py::arg("w_gate"), py::arg("w_up"), py::arg("gate"), py::arg("up"),
+        py::arg("activation") = "silu", py::arg("need_x") = true, py::arg("need_weights") = true);
+  m.def("gated_ffn", &sion::gated_ffn, "gated_linear, the down projection and a residual",
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"),
+        py::arg("residual") = none, py::arg("activation") = "silu");
+  m.def("gated_ffn_save", &sion::gated_ffn_save, "gated_ffn returning (y, gate, up)", py::arg("x"),
+        py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"), py::arg("residual") = none,
+        py::arg("activation") = "silu");
+  m.def("gated_ffn_backward", &sion::gated_ffn_backward,
+        "gradients of gated_ffn (dx, dw_gate, dw_up, dw_down)", py::arg("grad"), py::arg("x"),
+        py::arg("w_gate"), py::arg("w_up"), py::arg("w_down"), py::arg("gate"), py::arg("up"),
+        py::arg("activation") = "silu", py::arg("need_x") = true, py::arg("need_weights") = true);
 }
