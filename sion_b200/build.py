@@ -27,7 +27,8 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["felix_c.cu", "sgemm_sm100.cu", "hgemm_sm100.cu", "flash_attn_sm100.cu",
               "topk_sm100.cu", "flash_attn_bwd_sm100.cu", "kv4_attn_sm100.cu",
-              "kv4_cache_sm100.cu", "sample_sm100.cu", "ffn_sm100.cu", "ffn_product_sm100.cu"]
+              "kv4_cache_sm100.cu", "sample_sm100.cu", "ffn_sm100.cu", "ffn_product_sm100.cu",
+              "ffn_few_sm100.cu"]
 CPP_SOURCES = ["felix_api.cpp"]
 HEADERS = ["sm100_ptx.cuh", "felix_internal.h", "kv4_layout.cuh", "tile_queue.cuh",
            "activation.cuh", "ffn_internal.h"]

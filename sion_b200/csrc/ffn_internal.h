@@ -53,4 +53,9 @@ inline bool tma_ok(const void* p, int64_t ld, uint32_t rows, uint64_t cols) {
 size_t product_workspace_bytes(const Product& p, int num_sms);
 FelixCode product_launch(DeviceInfo* dev, const Product& p, void* workspace, cudaStream_t stream);
 
+// Whether a product (its fields but the pointers) is one of few tokens, and such a product:
+// operands of any address and stride, no scratch.
+bool few_tokens(const Product& p);
+FelixCode few_launch(const Product& p, cudaStream_t stream);
+
 }  // namespace felix_ffn

@@ -147,14 +147,18 @@ struct Call {
   DeviceInfo* dev;
   cudaStream_t stream;
   bool bf16;
-  uint8_t* base = nullptr;   // null: counting
-  size_t products = 0;       // bytes of the products' counters and partials, in front
+  enum { kCount, kLaunch } pass = kCount;
+  uint8_t* base = nullptr;
+  // bytes in front: the counters, which in the library's scratch other calls rely on
+  // even where this one has no product that uses them, and the products' partials
+  size_t products = felix_impl::kWsCounterBytes;
   size_t used = 0;           // bytes behind them
+  bool tiled = false;        // a product of more than a few tokens runs
   FelixCode code = kDone;
 
   bool ok() const { return code.type == FELIX_SUCCESS; }
-  bool counting() const { return base == nullptr; }
-  size_t total() const { return products + used; }
+  bool counting() const { return pass == kCount; }
+  size_t total() const { return tiled || used ? products + used : 0; }
 
   void* take(size_t bytes) {
     void* p = counting() ? nullptr : base + products + used;
@@ -182,11 +186,19 @@ struct Call {
     }
     return {c.p, c.ld};
   }
+  // An operand of a product: as it is for few tokens, else addressable by TMA.
+  Mat operand(const Product& p, const felix_matrix& m, uint32_t rows, uint32_t cols) {
+    return few_tokens(p) ? Mat{m.data, m.stride} : addressable(m, rows, cols);
+  }
   void run(const Product& p) {
-    if (counting())
+    if (few_tokens(p)) {
+      if (!counting() && ok()) code = few_launch(p, stream);
+    } else if (counting()) {
+      tiled = true;
       products = std::max(products, product_workspace_bytes(p, dev->num_sms));
-    else if (ok())
+    } else if (ok()) {
       code = product_launch(dev, p, base, stream);
+    }
   }
   void zero(const felix_matrix& m, uint32_t rows, uint32_t cols) {
     if (counting() || !ok() || !m.data) return;
@@ -266,8 +278,8 @@ void linear(Call& c, const felix_linear_args& a) {
   p.k = a.in_features;
   p.m[0] = a.tokens;
   p.n[0] = a.out_features;
-  p.a[0] = c.addressable(a.x, a.tokens, a.in_features);
-  p.b[0] = c.addressable(a.weight, a.out_features, a.in_features);
+  p.a[0] = c.operand(p, a.x, a.tokens, a.in_features);
+  p.b[0] = c.operand(p, a.weight, a.out_features, a.in_features);
   p.out[0] = as_mut(a.out);
   p.out[1] = as_mut(a.pre);
   p.in[0] = as_mat(a.residual);
@@ -318,9 +330,9 @@ void gated_product(Call& c, const felix_gated_args& a, const MutMat& h) {
   p.k = a.features;
   p.m[0] = a.tokens;
   p.n[0] = a.hidden;
-  p.a[0] = c.addressable(a.x, a.tokens, a.features);
-  p.b[0] = c.addressable(a.w_gate, a.hidden, a.features);
-  p.b[1] = c.addressable(a.w_up, a.hidden, a.features);
+  p.a[0] = c.operand(p, a.x, a.tokens, a.features);
+  p.b[0] = c.operand(p, a.w_gate, a.hidden, a.features);
+  p.b[1] = c.operand(p, a.w_up, a.hidden, a.features);
   p.out[0] = h;
   p.out[1] = as_mut(a.gate);
   p.out[2] = as_mut(a.up);
@@ -342,7 +354,7 @@ void gated_ffn(Call& c, const felix_gated_args& a) {
   p.m[0] = a.tokens;
   p.n[0] = a.features;
   p.a[0] = as_mat(h);
-  p.b[0] = c.addressable(a.w_down, a.features, a.hidden);
+  p.b[0] = c.operand(p, a.w_down, a.features, a.hidden);
   p.out[0] = as_mut(a.out);
   p.in[0] = as_mat(a.residual);
   c.run(p);
@@ -559,19 +571,20 @@ FelixCode perform(void (*op)(Call&, const Args&), const Args& a, void* workspace
   Call call = count;
   call.used = 0;
   felix_impl::Workspace scratch;  // until the last launch
-  if (!workspace) {
-    scratch = felix_impl::library_workspace(dev, stream, std::max<size_t>(count.total(), 16));
+  if (!workspace && count.total()) {
+    scratch = felix_impl::library_workspace(dev, stream, count.total());
     workspace = scratch.ptr;
     if (!workspace) return launch_error(cudaErrorMemoryAllocation, "feed-forward: workspace");
-  } else {
+  } else if (workspace) {
     if (bytes < count.total()) return api_error("feed-forward: workspace too small");
     // a caller's memory may hold anything: the products' counters start from zero
-    if (count.products) {
+    if (count.tiled) {
       const cudaError_t e =
           cudaMemsetAsync(workspace, 0, felix_impl::kWsCounterBytes, stream);
       if (e != cudaSuccess) return launch_error(e, "feed-forward: workspace");
     }
   }
+  call.pass = Call::kLaunch;
   call.base = static_cast<uint8_t*>(workspace);
   op(call, a);
   return call.code;
