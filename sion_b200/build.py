@@ -28,10 +28,10 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 CU_SOURCES = ["felix_c.cu", "sgemm_sm100.cu", "hgemm_sm100.cu", "flash_attn_sm100.cu",
               "topk_sm100.cu", "flash_attn_bwd_sm100.cu", "kv4_attn_sm100.cu",
               "kv4_cache_sm100.cu", "sample_sm100.cu", "ffn_sm100.cu", "ffn_product_sm100.cu",
-              "ffn_few_sm100.cu"]
+              "ffn_few_sm100.cu", "ffn_narrow_sm100.cu"]
 CPP_SOURCES = ["felix_api.cpp"]
 HEADERS = ["sm100_ptx.cuh", "felix_internal.h", "kv4_layout.cuh", "tile_queue.cuh",
-           "activation.cuh", "ffn_internal.h"]
+           "activation.cuh", "ffn_internal.h", "ffn_finish.cuh"]
 
 NVCC_FLAGS = [
     "-std=c++20", "-O3", "-lineinfo",
@@ -112,9 +112,35 @@ def check_kv4_registers(ptxas_log: str) -> None:
         raise RuntimeError("no eight-warp kv4_attn_kernel in ptxas's output")
 
 
+# The same for the wide tiles of the feed-forward products (ffn_product_sm100.cu
+# kRegsLaunch); the last template argument is the number of accumulators of a tile.
+FFN_REGS_LAUNCH = 168
+
+
+def check_ffn_registers(ptxas_log: str) -> None:
+    """Raise if ptxas gave a wide ffn_product_kernel another count."""
+    cur, seen = None, 0
+    for line in ptxas_log.splitlines():
+        m = re.search(r"Compiling entry function '([^']+)'", line)
+        if m:
+            cur = m.group(1)
+            continue
+        m = re.search(r"Used (\d+) registers", line)
+        if m and cur and re.search(r"ffn_product_kernelI.*Li2EEEv", cur):
+            seen += 1
+            if int(m.group(1)) != FFN_REGS_LAUNCH:
+                raise RuntimeError(
+                    f"{cur}: ptxas used {m.group(1)} registers per thread; the setmaxnreg split "
+                    f"of the feed-forward products' wide tiles assumes {FFN_REGS_LAUNCH} "
+                    f"(ffn_product_sm100.cu kRegsLaunch)")
+    if not seen:
+        raise RuntimeError("no wide ffn_product_kernel in ptxas's output")
+
+
 # Sources whose compiler output is checked.
 REGISTER_CHECKS = {"flash_attn_sm100.cu": check_attention_registers,
-                   "kv4_attn_sm100.cu": check_kv4_registers}
+                   "kv4_attn_sm100.cu": check_kv4_registers,
+                   "ffn_product_sm100.cu": check_ffn_registers}
 
 
 def _headers() -> list[str]:

@@ -18,16 +18,38 @@ __device__ __forceinline__ float reciprocal(float d) {
   return r;
 }
 
-// p = 1 / (1 + e^-z) and q = 1 - p without cancellation, from e^-|z| in (0, 1].
-__device__ __forceinline__ void logistic(float z, float& p, float& q) {
-  const float t = __expf(-fabsf(z)), r = reciprocal(1.f + t), tr = t * r;
-  p = z < 0.f ? tr : r;
-  q = z < 0.f ? r : tr;
+// 2^x, to 2 ulp.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// sqrt(8 / pi) (z + 0.044715 z^3): gelu_tanh is z p(that).
+// 1 / (1 + e^-z): to a few ulp everywhere (e^-z may be infinite, which gives 0).
+__device__ __forceinline__ float logistic(float z) {
+  return reciprocal(1.f + exp2_approx(-1.44269504f * z));
+}
+
+// sqrt(8 / pi) (z + 0.044715 z^3): gelu_tanh is z logistic(that).
 __device__ __forceinline__ float gelu_inner(float z) {
   return z * fmaf(0.0713548163f, z * z, 1.59576912f);
+}
+
+// The normal distribution function, and e^(-z^2 / 2). With s = |z| / sqrt 2 and
+// t = 1 / (1 + s / 2), erfc(s) e^(s^2) / (2 t) is smooth in t on (0, 1]; the polynomial is
+// its minimax fit of degree 6 for s up to 10 (where e^(-s^2) is 0), to 1.5e-6 relative in
+// fp32, so that small values for negative z keep their leading bits too.
+__device__ __forceinline__ float normal_area(float z, float& e) {
+  e = exp2_approx(-0.721347520f * z * z);
+  const float t = reciprocal(fmaf(0.353553391f, fabsf(z), 1.f));
+  float c = fmaf(0.04410203546f, t, -0.17836862803f);
+  c = fmaf(c, t, 0.19461159408f);
+  c = fmaf(c, t, 0.01894582063f);
+  c = fmaf(c, t, 0.14075168967f);
+  c = fmaf(c, t, 0.13879109917f);
+  c = fmaf(c, t, 0.14116570354f);
+  const float tail = c * t * e;
+  return z < 0.f ? tail : 1.f - tail;
 }
 
 // act(z). What is not a number stays one.
@@ -36,48 +58,45 @@ __device__ __forceinline__ float activate(float z) {
   if constexpr (ACT == FELIX_ACT_RELU) {
     return z < 0.f ? 0.f : z;
   } else if constexpr (ACT == FELIX_ACT_GELU) {
-    return 0.5f * z * erfcf(-0.707106781f * z);
+    float e;
+    return z * normal_area(z, e);
   } else if constexpr (ACT == FELIX_ACT_GELU_TANH) {
-    float p, q;
-    logistic(gelu_inner(z), p, q);
-    return z * p;
+    return z * logistic(gelu_inner(z));
   } else if constexpr (ACT == FELIX_ACT_SILU) {
-    float p, q;
-    logistic(z, p, q);
-    return z * p;
+    return z * logistic(z);
   } else if constexpr (ACT == FELIX_ACT_SIGMOID) {
-    float p, q;
-    logistic(z, p, q);
-    return p;
+    return logistic(z);
   } else {
     return z;
   }
 }
 
-// act(z) and act'(z). The derivative of relu is 0 at 0.
+// act(z) and act'(z). The derivative of relu is 0 at 0. 1 - p stands for the logistic of
+// -z where it is added to something that is larger; sigmoid's derivative is a product of
+// both and takes them without cancellation.
 template <int ACT>
 __device__ __forceinline__ void activate_both(float z, float& a, float& d) {
   if constexpr (ACT == FELIX_ACT_RELU) {
     a = z < 0.f ? 0.f : z;
     d = z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
   } else if constexpr (ACT == FELIX_ACT_GELU) {
-    const float area = 0.5f * erfcf(-0.707106781f * z);
+    float e;
+    const float area = normal_area(z, e);
     a = z * area;
-    d = fmaf(z * 0.398942280f, __expf(-0.5f * z * z), area);
+    d = fmaf(z * 0.398942280f, e, area);
   } else if constexpr (ACT == FELIX_ACT_GELU_TANH) {
-    float p, q;
-    logistic(gelu_inner(z), p, q);
+    const float p = logistic(gelu_inner(z));
     a = z * p;
-    d = fmaf(a * q, fmaf(0.214064449f, z * z, 1.59576912f), p);
+    // (z^2 bounded: where 1 - p is 0 the product is)
+    d = fmaf(a * (1.f - p), fmaf(0.214064449f, fminf(z * z, 1e6f), 1.59576912f), p);
   } else if constexpr (ACT == FELIX_ACT_SILU) {
-    float p, q;
-    logistic(z, p, q);
+    const float p = logistic(z);
     a = z * p;
-    d = fmaf(a, q, p);
+    d = fmaf(a, 1.f - p, p);
   } else if constexpr (ACT == FELIX_ACT_SIGMOID) {
-    float q;
-    logistic(z, a, q);
-    d = a * q;
+    const float t = exp2_approx(-1.44269504f * fabsf(z)), r = reciprocal(1.f + t);
+    a = z < 0.f ? t * r : r;
+    d = t * r * r;
   } else {
     a = z;
     d = 1.f;

@@ -1,8 +1,8 @@
-// Products of a few tokens (up to 32) with a layer's weights: y = x W^T with the same
+// Products of a few tokens (up to 8) with a layer's weights: y = x W^T with the same
 // epilogues as ffn_product_sm100.cu. Bound by reading W once.
 //
 // A CTA owns 16 rows of W (gated: 16 of the gate's and the same 16 of the up
-// projection's; more tokens: 32), its 8 warps take every 8th block of 64 k, so that a row
+// projection's), its 8 warps take every 8th block of 64 k, so that a row
 // is read 1 KB at a time, and their sums meet in shared memory: no second pass, no
 // atomics, and the result does not depend on the grid. W goes from memory straight into
 // the operands of m16n8k16 (rows of W x 8 tokens): a product does not care for the order of
@@ -68,11 +68,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// MT tiles of 16 rows of W, NT of 8 tokens, D steps under way.
-template <class T, int NT, int MT, int D, bool GATED, bool VEC>
-__global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(const Params p) {
-  constexpr uint32_t kRows = GATED ? MT * 8 : MT * 16;  // output features of a CTA
-  __shared__ float part[kWarps][MT * 16][NT * 8 + 1];
+// VEC: rows of whole 16-byte vectors.
+template <class T, bool GATED, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps, 2) few_kernel(const Params p) {
+  constexpr uint32_t kRows = 16;         // output features of a CTA
+  constexpr int MT = GATED ? 2 : 1;      // tiles of 16 rows of weights
+  constexpr int D = !VEC ? 1 : GATED ? 2 : 4;  // steps of a warp under way
+  __shared__ float part[kWarps][MT * 16][9];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const uint32_t n0 = blockIdx.x * kRows;
 
@@ -82,22 +84,15 @@ __global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(c
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int which = GATED ? m / (MT / 2) : 0;
-      const uint32_t row = n0 + (GATED ? m % (MT / 2) : m) * 16 + h * 8 + g;
+      const uint32_t row = n0 + h * 8 + g;
       wthere[m][h] = row < p.n;
-      wrow[m][h] = p.w[which] + int64_t(row) * p.w_ld[which];
+      wrow[m][h] = p.w[m] + int64_t(row) * p.w_ld[m];
     }
-  const uint16_t* xrow[NT];
-  bool xthere[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const uint32_t token = n * 8 + g;
-    xthere[n] = token < p.tokens;
-    xrow[n] = p.x + int64_t(token) * p.x_ld;
-  }
+  const bool xthere = g < p.tokens;
+  const uint16_t* xrow = p.x + int64_t(g) * p.x_ld;
 
-  float c[MT][NT][4] = {};
-  uint4 wv[D][MT][2][2], xv[D][NT][2];
+  float c[MT][4] = {};
+  uint4 wv[D][MT][2][2], xv[D][2];
   auto fetch = [&](int d, uint32_t step) {
     const uint32_t k = (step * kWarps + warp) * kBlock + t * 8;
 #pragma unroll
@@ -107,9 +102,7 @@ __global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(c
 #pragma unroll
         for (int r = 0; r < 2; ++r)
           wv[d][m][r][h] = load8<VEC, true>(wrow[m][r], k + 32 * h, p.k, wthere[m][r]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-        xv[d][n][h] = load8<VEC, false>(xrow[n], k + 32 * h, p.k, xthere[n]);
+      xv[d][h] = load8<VEC, false>(xrow, k + 32 * h, p.k, xthere);
     }
   };
   const uint32_t steps = (p.k + kBlock * kWarps - 1) / (kBlock * kWarps);
@@ -122,13 +115,9 @@ __global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(c
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const uint4 a = wv[d][m][0][h], b = wv[d][m][1][h];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 x = xv[d][n][h];
-            mma<T>(c[m][n], a.x, b.x, a.y, b.y, x.x, x.y);
-            mma<T>(c[m][n], a.z, b.z, a.w, b.w, x.z, x.w);
-          }
+          const uint4 a = wv[d][m][0][h], b = wv[d][m][1][h], x = xv[d][h];
+          mma<T>(c[m], a.x, b.x, a.y, b.y, x.x, x.y);
+          mma<T>(c[m], a.z, b.z, a.w, b.w, x.z, x.w);
         }
       fetch(d, s + D + d);
     }
@@ -137,10 +126,7 @@ __global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(c
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        part[warp][m * 16 + (i >> 1) * 8 + g][n * 8 + 2 * t + (i & 1)] = c[m][n][i];
+    for (int i = 0; i < 4; ++i) part[warp][m * 16 + (i >> 1) * 8 + g][2 * t + (i & 1)] = c[m][i];
   __syncthreads();
 
   // consecutive threads take consecutive features of a token
@@ -167,41 +153,17 @@ __global__ void __launch_bounds__(32 * kWarps, MT * NT > 4 ? 1 : 2) few_kernel(c
   }
 }
 
-template <class T, int NT, int MT, int D, bool GATED>
+template <class T, bool GATED>
 void launch(const Params& p, bool vec, cudaStream_t stream) {
-  constexpr uint32_t rows = GATED ? MT * 8 : MT * 16;
+  constexpr uint32_t rows = 16;
   const uint32_t grid = (p.n + rows - 1) / rows;
   if (vec)
-    few_kernel<T, NT, MT, D, GATED, true><<<grid, 32 * kWarps, 0, stream>>>(p);
+    few_kernel<T, GATED, true><<<grid, 32 * kWarps, 0, stream>>>(p);
   else
-    few_kernel<T, NT, MT, 1, GATED, false><<<grid, 32 * kWarps, 0, stream>>>(p);
-}
-
-template <class T>
-void launch(const Params& p, bool gated, bool vec, cudaStream_t stream) {
-  if (gated) {
-    if (p.tokens <= 8)
-      launch<T, 1, 2, 2, true>(p, vec, stream);
-    else if (p.tokens <= 16)
-      launch<T, 2, 2, 2, true>(p, vec, stream);
-    else
-      launch<T, 4, 2, 2, true>(p, vec, stream);
-  } else {
-    if (p.tokens <= 8)
-      launch<T, 1, 1, 4, false>(p, vec, stream);
-    else if (p.tokens <= 16)
-      launch<T, 2, 2, 2, false>(p, vec, stream);
-    else
-      launch<T, 4, 2, 2, false>(p, vec, stream);
-  }
+    few_kernel<T, GATED, false><<<grid, 32 * kWarps, 0, stream>>>(p);
 }
 
 }  // namespace few
-
-bool few_tokens(const Product& p) {
-  return p.m[0] <= 32 && p.epilogue != kDGated && p.segments == 1 && p.problems == 1 && !p.a_mn &&
-         !p.b_mn;
-}
 
 FelixCode few_launch(const Product& x, cudaStream_t stream) {
   few::Params p{};
@@ -228,8 +190,12 @@ FelixCode few_launch(const Product& x, cudaStream_t stream) {
   p.n = x.n[0];
   p.k = x.k;
   p.act = x.act;
-  x.bf16 ? few::launch<__nv_bfloat16>(p, gated, all, stream)
-         : few::launch<__half>(p, gated, all, stream);
+  if (gated)
+    x.bf16 ? few::launch<__nv_bfloat16, true>(p, all, stream)
+           : few::launch<__half, true>(p, all, stream);
+  else
+    x.bf16 ? few::launch<__nv_bfloat16, false>(p, all, stream)
+           : few::launch<__half, false>(p, all, stream);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return felix_impl::launch_error(e, "feed-forward: few tokens");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};

@@ -48,14 +48,18 @@ inline bool tma_ok(const void* p, int64_t ld, uint32_t rows, uint64_t cols) {
          (rows <= 1 || (ld % 8 == 0 && ld >= int64_t(cols) && ld < (int64_t(1) << 38)));
 }
 
-// Scratch of a product: kWsCounterBytes of counters that are zero before and after,
-// then fp32 partials. a and b must be addressable by TMA.
-size_t product_workspace_bytes(const Product& p, int num_sms);
+// A product of any size: a and b must be addressable by TMA; workspace: kWsCounterBytes of
+// counters that are zero before and after.
 FelixCode product_launch(DeviceInfo* dev, const Product& p, void* workspace, cudaStream_t stream);
 
-// Whether a product (its fields but the pointers) is one of few tokens, and such a product:
-// operands of any address and stride, no scratch.
-bool few_tokens(const Product& p);
+// Products of few tokens, for which reading the weights is all: up to 8 (operands of any
+// address and stride) and up to 64 (addressable by TMA). Neither needs scratch.
+inline bool forward_product(const Product& p) {
+  return p.epilogue != kDGated && p.segments == 1 && p.problems == 1 && !p.a_mn && !p.b_mn;
+}
+inline bool few_tokens(const Product& p) { return p.m[0] <= 8 && forward_product(p); }
 FelixCode few_launch(const Product& p, cudaStream_t stream);
+inline bool narrow_tokens(const Product& p) { return p.m[0] <= 64 && forward_product(p); }
+FelixCode narrow_launch(DeviceInfo* dev, const Product& p, cudaStream_t stream);
 
 }  // namespace felix_ffn

@@ -27,6 +27,7 @@
 #include <cstdint>
 
 #include "activation.cuh"
+#include "ffn_finish.cuh"
 #include "ffn_internal.h"
 #include "sm100_ptx.cuh"
 #include "tile_queue.cuh"
@@ -36,69 +37,75 @@ namespace product {
 
 using namespace felix_sm100;
 
-constexpr uint32_t kRows = 128;               // rows of A, and of B, of one CTA's stage
-constexpr uint32_t kDepth = 128;              // k of a stage
-constexpr uint32_t kOpBytes = kRows * kDepth * 2;
-constexpr uint32_t kStageBytes = 2 * kOpBytes;
-constexpr uint32_t kStages = 3;
+constexpr uint32_t kRows = 128;               // rows of an operand's tile in one CTA
 constexpr uint32_t kEpiWarps = 8;
-constexpr uint32_t kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kBoxBytes = 32 * 64;       // 32 rows x 32 columns
-constexpr uint32_t kStagingBytes = kEpiWarps * 2 * kBoxBytes;
+constexpr uint32_t kStagingBytes = kEpiWarps * kBoxBytes;
 constexpr uint32_t kBarBytes = 512;
-constexpr uint32_t kSmemBytes = kStages * kStageBytes + kStagingBytes + kBarBytes + 1024;
+constexpr uint32_t kRingBytes = 192 * 1024;
+constexpr uint32_t kSmemBytes = kRingBytes + kStagingBytes + kBarBytes + 1024;
+
+// CG CTAs per tile; HALVES accumulators of BN columns side by side in a tile.
+template <int CG, int BN_, int HALVES>
+struct Shape {
+  static constexpr uint32_t BN = BN_;
+  static constexpr uint32_t kDepth = HALVES == 2 ? 64 : 128;  // k of a stage
+  static constexpr uint32_t kBRows = BN / CG;                 // rows of B of one CTA, per half
+  static constexpr uint32_t kABytes = kRows * kDepth * 2, kBBytes = kBRows * kDepth * 2;
+  static constexpr uint32_t kStageBytes = kABytes + HALVES * kBBytes;
+  static constexpr uint32_t kStages = kRingBytes / kStageBytes;
+  static constexpr uint32_t kFirstEpi = HALVES == 2 ? 4 : 2;  // first epilogue warp
+  static constexpr uint32_t kThreads = 32 * (kFirstEpi + kEpiWarps);
+};
+// Wide tiles: the epilogue's two warpgroups hold 128 results a thread and take registers from
+// the first one (TMA, MMA and two idle warps): 128 x 80 + 256 x 208 <= 384 x 168, which the
+// host checks before the first launch.
+constexpr int kRegsLaunch = 168, kRegsFirst = 80, kRegsEpi = 208;
+static_assert(128 * kRegsFirst + 256 * kRegsEpi <= 384 * kRegsLaunch, "registers at launch");
+// Stages that a pair works through for one half of a wide tile before the other.
+constexpr uint32_t kSkew = 2;
 
 struct Problem {
   uint32_t m, n, tiles_m, tiles_n, tile0;
 };
 
 struct alignas(64) Params {
-  CUtensorMap a[3], b[3], out[3];
+  CUtensorMap a[3], b[3];
   Problem prob[3];
   uint32_t problems, tiles;
   uint32_t kb_seg, kb;         // 128-deep blocks of a segment, of a tile
   uint32_t a_mn, b_mn;         // operands stored with m / n contiguous
   uint32_t a_3d, b_3d;         // one request per operand and stage
   uint32_t group_m;
-  uint32_t split_tiles, parts; // the first tiles, cut into `parts` along k
-  uint32_t dyn;                // whole tiles come from the queue
-  void* out_ptr[3];
-  int64_t out_ld[3];
-  uint32_t out_tma, out_want;  // bit per output
-  const void* in_ptr[2];
-  int64_t in_ld[2];
-  uint32_t in_vec;             // bit per input: rows of whole 16-byte vectors
-  const void* bias;
-  int act;
-  unsigned* counters;          // [split tiles x CG], zero between launches
-  unsigned* dyn_counter;       // [0] next whole tile, [1] CTAs that are done
-  float* partials;             // [unit][CG][128 x 128 CG]
+  uint32_t parts;              // of each tile's depth, a cluster's CTAs or pairs
+  uint32_t dyn;                // tiles come from the queue
+  Finish fin;
+  // bit per output and input: rows of whole 16-byte vectors, of whole 32-byte sectors
+  uint32_t out_vec, out_sectors, in_vec, in_sectors;
+  unsigned* dyn_counter;       // [0] next tile, [1] CTAs that are done; zero between launches
   unsigned* status;
 };
 
 struct Unit {
   uint32_t tile, kb0, kb1;
-  bool split;
 };
 
-// The walk of every role of a CTA: its part of a split tile, then whole tiles.
+// The walk of every role of a CTA: a part of one tile, or whole tiles.
 struct Walk {
   uint32_t unit, units, next_tile;
-  bool first;
-  __device__ __forceinline__ void init(const Params& p, uint32_t cg) {
-    unit = blockIdx.x / cg;
+  __device__ __forceinline__ void init(uint32_t cg) {
+    unit = next_tile = blockIdx.x / cg;
     units = gridDim.x / cg;
-    first = unit < p.split_tiles * p.parts;
-    next_tile = p.split_tiles + unit;
   }
   __device__ __forceinline__ static void whole(const Params& p, Unit& u, uint32_t tile) {
-    u = {tile, 0, p.kb, false};
+    u = {tile, 0, p.kb};
   }
   __device__ __forceinline__ bool next(const Params& p, Unit& u) {
-    if (first) {
-      first = false;
+    if (p.parts > 1) {
+      if (next_tile != unit) return false;
       const uint32_t part = unit % p.parts;
-      u = {unit / p.parts, p.kb * part / p.parts, p.kb * (part + 1) / p.parts, true};
+      u = {unit / p.parts, p.kb * part / p.parts, p.kb * (part + 1) / p.parts};
+      next_tile = unit + 1;
       return true;
     }
     if (p.dyn || next_tile >= p.tiles) return false;
@@ -124,92 +131,120 @@ __device__ __forceinline__ Place place_of(const Params& p, uint32_t tile) {
   return r;
 }
 
-// float4 of (32-column chunk c, float4 j of it, row r) of a partial tile: a warp's rows
-// touch 512 contiguous bytes.
-__device__ __forceinline__ uint32_t partial_index(uint32_t c, uint32_t j, uint32_t r) {
-  return (c * 8 + j) * kRows + r;
+// A warp's box in shared memory: 32 rows of 64 bytes (32 columns), the 16-byte pieces of a
+// row swizzled so that neither 8 lanes of a row each nor 8 rows of 4 lanes conflict.
+__device__ __forceinline__ uint32_t box_offset(uint32_t row, uint32_t piece) {
+  return row * 64 + ((piece ^ ((row >> 1) & 3)) * 16);
 }
 
-// 32 columns of one row of an input, as 16 packed pairs; what lies outside reads as 0.
-// Rows that are no whole vectors go through the warp's staging, 64 bytes a row.
-template <class T>
+// 32 bytes of global memory at once (32-byte aligned), or as two vectors of 16.
+__device__ __forceinline__ void load32(const void* p, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                 "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 32 columns of this lane's row of an input, packed; what lies outside reads as 0. Rows
+// that are no whole vectors are read 64 bytes of a row at a time through the box.
 __device__ __forceinline__ void load_chunk(const Params& p, int which, uint32_t row0, uint32_t col,
-                                           uint32_t M, uint32_t N, uint8_t* stg, uint32_t lane,
+                                           uint32_t M, uint32_t N, uint8_t* box, uint32_t lane,
                                            uint32_t (&raw)[16]) {
-  const uint16_t* base = static_cast<const uint16_t*>(p.in_ptr[which]);
-  const int64_t ld = p.in_ld[which];
+  const uint16_t* base = static_cast<const uint16_t*>(p.fin.in[which]);
+  const int64_t ld = p.fin.in_ld[which];
   if (p.in_vec >> which & 1) {
     const uint32_t row = row0 + lane;
+    const bool sectors = p.in_sectors >> which & 1;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < M && col + 8 * j < N)
-        v = *reinterpret_cast<const uint4*>(base + int64_t(row) * ld + col + 8 * j);
-      raw[4 * j] = v.x, raw[4 * j + 1] = v.y, raw[4 * j + 2] = v.z, raw[4 * j + 3] = v.w;
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint16_t* at = base + int64_t(row) * ld + col + 16 * j;
+      if (sectors && row < M && col + 16 * j < N) {
+        load32(at, raw + 8 * j);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (row < M && col + 16 * j + 8 * i < N) v = *reinterpret_cast<const uint4*>(at + 8 * i);
+          raw[8 * j + 4 * i] = v.x, raw[8 * j + 4 * i + 1] = v.y;
+          raw[8 * j + 4 * i + 2] = v.z, raw[8 * j + 4 * i + 3] = v.w;
+        }
+      }
     }
     return;
   }
-  if (lane == 0) bulk_wait_group_read<0>();
   __syncwarp();
-  uint16_t* s = reinterpret_cast<uint16_t*>(stg);
   const uint32_t rows = min(32u, M - row0);
 #pragma unroll 8
   for (uint32_t r = 0; r < rows; ++r)
-    s[r * 32 + lane] = col + lane < N ? base[int64_t(row0 + r) * ld + col + lane] : uint16_t(0);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 v = reinterpret_cast<const uint4*>(stg + lane * 64)[j];
-    raw[4 * j] = v.x, raw[4 * j + 1] = v.y, raw[4 * j + 2] = v.z, raw[4 * j + 3] = v.w;
-  }
-  __syncwarp();
-}
-
-// Rounds 32 columns of each of the warp's rows and writes them: through a 64-byte
-// swizzled box and TMA, which clips the ragged edge, or, where rows are not 16-byte
-// multiples, row by row. `turn` alternates between the warp's two boxes.
-template <class T>
-__device__ __forceinline__ void store_chunk(const Params& p, int which, uint32_t row0, uint32_t col,
-                                            uint32_t M, uint32_t N, uint8_t* stg, uint32_t& turn,
-                                            uint32_t lane, const float (&v)[32]) {
-  uint8_t* box = stg + (turn++ & 1) * kBoxBytes;
-  if (lane == 0) bulk_wait_group_read<1>();
+    *reinterpret_cast<uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2) =
+        col + lane < N ? base[int64_t(row0 + r) * ld + col + lane] : uint16_t(0);
   __syncwarp();
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
-    uint4 w;
-    w.x = Pair<T>::pack(v[8 * j], v[8 * j + 1]);
-    w.y = Pair<T>::pack(v[8 * j + 2], v[8 * j + 3]);
-    w.z = Pair<T>::pack(v[8 * j + 4], v[8 * j + 5]);
-    w.w = Pair<T>::pack(v[8 * j + 6], v[8 * j + 7]);
-    *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = w;
+    const uint4 v = *reinterpret_cast<const uint4*>(box + box_offset(lane, j));
+    raw[4 * j] = v.x, raw[4 * j + 1] = v.y, raw[4 * j + 2] = v.z, raw[4 * j + 3] = v.w;
   }
-  if (p.out_tma >> which & 1) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(&p.out[which], box, int(col), int(row0));
-      bulk_commit_group();
+}
+
+// Writes 32 columns of each of the warp's rows: a lane its row, two sectors, straight from
+// registers (rows that are no whole vectors: through the box, 64 bytes of a row at a
+// time). Shared memory is busy with the operands.
+__device__ __forceinline__ void store_packed(const Params& p, int which, uint32_t row0,
+                                             uint32_t col, uint32_t M, uint32_t N, uint8_t* box,
+                                             uint32_t lane, const uint32_t (&w)[16]) {
+  uint16_t* base = static_cast<uint16_t*>(p.fin.out[which]);
+  const int64_t ld = p.fin.out_ld[which];
+  if (p.out_vec >> which & 1) {
+    const uint32_t row = row0 + lane;
+    if (row >= M) return;
+    uint16_t* at = base + int64_t(row) * ld + col;
+    if (p.out_sectors >> which & 1) {
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        if (col + 16 * j < N) store32(at + 16 * j, w + 8 * j);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        if (col + 8 * j < N)
+          *reinterpret_cast<uint4*>(at + 8 * j) =
+              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     }
-  } else {
-    __syncwarp();
-    uint16_t* base = static_cast<uint16_t*>(p.out_ptr[which]);
-    const int64_t ld = p.out_ld[which];
+    return;
+  }
+  __syncwarp();
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(box + box_offset(lane, j)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  __syncwarp();
+  if (col + lane < N) {
     const uint32_t rows = min(32u, M - row0);
-    if (col + lane < N) {
 #pragma unroll 8
-      for (uint32_t r = 0; r < rows; ++r)
-        base[int64_t(row0 + r) * ld + col + lane] = *reinterpret_cast<const uint16_t*>(
-            box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
-    }
-    if (lane == 0) bulk_commit_group();  // an empty one: the boxes' turns are counted in groups
+    for (uint32_t r = 0; r < rows; ++r)
+      base[int64_t(row0 + r) * ld + col + lane] =
+          *reinterpret_cast<const uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2);
   }
+}
+template <class T>
+__device__ __forceinline__ void store_chunk(const Params& p, int which, uint32_t row0, uint32_t col,
+                                            uint32_t M, uint32_t N, uint8_t* box, uint32_t lane,
+                                            const float (&v)[32]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = Pair<T>::pack(v[2 * j], v[2 * j + 1]);
+  store_packed(p, which, row0, col, M, N, box, lane, w);
 }
 
 // Bias of 32 columns (the same for every row: one broadcast load each).
 template <class T>
 __device__ __forceinline__ void add_bias(const Params& p, uint32_t col, uint32_t N, float (&v)[32]) {
-  const uint16_t* b = static_cast<const uint16_t*>(p.bias) + col;
+  const uint16_t* b = static_cast<const uint16_t*>(p.fin.bias) + col;
   if (col + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -229,12 +264,16 @@ __device__ __forceinline__ void add_bias(const Params& p, uint32_t col, uint32_t
   }
 }
 
-template <class T, int EPI, int CG>
-__global__ void __launch_bounds__(kThreads, 1)
+template <class T, int EPI, int CG, int BN_, int HALVES>
+__global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
     ffn_product_kernel(const __grid_constant__ Params p) {
-  constexpr uint32_t BN = kRows * CG;   // columns of a tile's accumulator
+  using S = Shape<CG, BN_, HALVES>;
+  constexpr uint32_t BN = BN_;  // columns of one accumulator
+  constexpr uint32_t kDepth = S::kDepth, kStageBytes = S::kStageBytes, kStages = S::kStages;
+  constexpr uint32_t kABytes = S::kABytes, kBBytes = S::kBBytes, kBRows = S::kBRows;
   constexpr uint32_t kTmemCols = 2 * BN;
-  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
+  const uint32_t cta = CG == 2 || p.parts > 1 ? cluster_ctarank() : 0u;  // in the cluster
+  const uint32_t rank = CG == 2 ? cta & 1u : 0u;                         // in the pair
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -245,14 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* tfull = empty + kStages;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
-  uint64_t* tq_full = drain + 1;
+  uint64_t* received = drain + 1;
+  uint64_t* tq_full = received + 1;
   uint64_t* tq_empty = tq_full + kTq;
   uint32_t* words = reinterpret_cast<uint32_t*>(tq_empty + kTq);
-  static_assert((2 * kStages + 5 + 2 * kTq) * 8 + (kTq + 3) * 4 <= kBarBytes, "barrier block");
+  static_assert((2 * kStages + 6 + 2 * kTq) * 8 + (kTq + 2) * 4 <= kBarBytes, "barrier block");
   TileQueue tq{words, tq_full, tq_empty, 0};
   uint32_t* tmem_slot = words + kTq;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(words + kTq + 1);
-  uint32_t* bcast = words + kTq + 2;
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -265,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&tempty[i], kEpiWarps * CG);  // a pair's leader counts both CTAs' warps
     }
     mbar_init(drain, 1);
+    mbar_init(received, 1);
     for (uint32_t i = 0; i < kTq; ++i) {
       mbar_init(&tq_full[i], 1);
       // the MMA warp and the epilogue warps; of the peer its producer and epilogue warps
@@ -292,42 +332,43 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    if constexpr (HALVES == 2) setmaxnreg_dec<kRegsFirst>();
     if (elect_one()) {
       Walk walk;
-      walk.init(p, CG);
+      walk.init(CG);
       Unit u;
       uint32_t stage = 0, phase = 0, filled = 0;
       bool ok = true;
       // loads of a pair's CTAs complete on the leader's barrier
       auto load2 = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, uint32_t x, uint32_t y) {
         if constexpr (CG == 2)
-          tma_load_2d_pair(dst, map, mapa_shared(smem_u32(bar), 0), int(x), int(y));
+          tma_load_2d_pair(dst, map, mapa_shared(smem_u32(bar), cta & ~1u), int(x), int(y));
         else
           tma_load_2d(dst, map, bar, int(x), int(y));
       };
       auto load3 = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, uint32_t y, uint32_t z) {
         if constexpr (CG == 2)
-          tma_load_3d_pair(dst, map, mapa_shared(smem_u32(bar), 0), 0, int(y), int(z));
+          tma_load_3d_pair(dst, map, mapa_shared(smem_u32(bar), cta & ~1u), 0, int(y), int(z));
         else
           tma_load_3d(dst, map, bar, 0, int(y), int(z));
       };
-      // 128 rows (of m or n, from mn0) of 128-deep block kb: two blocks of 64 k, or of 64
-      // m / n, 16 KB each
+      // `rows` (of m or n, from mn0) of k block kb: blocks of 64 k of all rows, or of 64
+      // m / n of all k
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, bool mn, bool whole,
-                      uint32_t mn0, uint32_t kb) {
-        if (whole) {
-          if (mn)
+                      uint32_t rows, uint32_t mn0, uint32_t kb) {
+        if (mn) {
+          if (whole) {
             load3(dst, map, bar, kb * kDepth, mn0 / 64);
-          else
-            load3(dst, map, bar, mn0, kb * 2);
+          } else {
+            for (uint32_t j = 0; j < rows / 64; ++j)
+              load2(dst + j * (kDepth * 128), map, bar, mn0 + 64 * j, kb * kDepth);
+          }
+        } else if (whole && kDepth == 128) {
+          load3(dst, map, bar, mn0, kb * 2);
         } else {
 #pragma unroll
-          for (uint32_t j = 0; j < 2; ++j) {
-            if (mn)
-              load2(dst + j * (kOpBytes / 2), map, bar, mn0 + 64 * j, kb * kDepth);
-            else
-              load2(dst + j * (kOpBytes / 2), map, bar, kb * kDepth + 64 * j, mn0);
-          }
+          for (uint32_t j = 0; j < kDepth / 64; ++j)
+            load2(dst + j * (rows * 128), map, bar, kb * kDepth + 64 * j, mn0);
         }
       };
       uint32_t ahead = 0;
@@ -337,11 +378,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!p.dyn) return false;
         uint32_t t;
         if (rank == 0) {
-          if (!have_ahead) ahead = p.split_tiles + atomicAdd(p.dyn_counter, 1u);
+          if (!have_ahead) ahead = atomicAdd(p.dyn_counter, 1u);
           t = ahead;
           if (!tq_push(tq, t, CG == 2, abort_flag, p.status)) return ok = false;
           have_ahead = t < p.tiles;
-          if (have_ahead) ahead = p.split_tiles + atomicAdd(p.dyn_counter, 1u);
+          if (have_ahead) ahead = atomicAdd(p.dyn_counter, 1u);
         } else {
           uint32_t slot;
           if (!tq_pop(tq, t, slot, abort_flag, p.status)) return ok = false;
@@ -354,27 +395,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && next_unit(u)) {
         const Place at = place_of(p, u.tile);
         const uint32_t m0 = (at.tm * CG + rank) * kRows;
-        const uint32_t n0 = EPI == kGated ? at.tn * (BN / 2) : (at.tn * CG + rank) * kRows;
+        const uint32_t n0 =
+            EPI == kGated ? at.tn * (BN / 2) : at.tn * (BN * HALVES) + rank * kBRows;
         for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kWdProducerEmpty)) {
+          if (!mbar_sleep_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
+                               kWdProducerEmpty)) {
             ok = false;
             break;
           }
           uint8_t* sa = ring + stage * kStageBytes;
-          uint8_t* sb = sa + kOpBytes;
+          uint8_t* sb = sa + kABytes;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * kStageBytes);
           const uint32_t seg = kb / p.kb_seg, k = kb - seg * p.kb_seg, op = at.prob + seg;
-          load(sa, &p.a[op], &full[stage], p.a_mn, p.a_3d, m0, k);
+          load(sa, &p.a[op], &full[stage], p.a_mn, p.a_3d, kRows, m0, k);
           if constexpr (EPI == kGated && CG == 1) {
             // 64 rows of the gate's weights, then 64 of the up projection's
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
               for (uint32_t j = 0; j < 2; ++j)
-                load2(sb + j * (kOpBytes / 2) + h * (kOpBytes / 4), &p.b[h], &full[stage],
+                load2(sb + j * (kBBytes / 2) + h * (kBBytes / 4), &p.b[h], &full[stage],
                       k * kDepth + 64 * j, n0);
           } else {
-            load(sb, &p.b[EPI == kGated ? rank : op], &full[stage], p.b_mn, p.b_3d, n0, k);
+#pragma unroll
+            for (uint32_t h = 0; h < HALVES; ++h)
+              load(sb + h * kBBytes, &p.b[EPI == kGated ? rank : op], &full[stage], p.b_mn, p.b_3d,
+                   kBRows, n0 + h * BN, k);
           }
           ++filled;
           if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -391,9 +437,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA
+    if constexpr (HALVES == 2) setmaxnreg_dec<kRegsFirst>();
     if (rank == 0) {
       auto wait_all = [&](uint64_t* bar, uint32_t parity, unsigned site) {
-        return __all_sync(~0u, mbar_wait(bar, parity, abort_flag, p.status, site)) != 0;
+        return __all_sync(~0u, mbar_sleep_wait(bar, parity, abort_flag, p.status, site)) != 0;
       };
       // bits 7 and 10: bf16 operands
       const uint32_t idesc = make_idesc_f16_f32(kRows * CG, BN, p.a_mn != 0, p.b_mn != 0) |
@@ -402,18 +449,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (CG == 2) {
           const uint32_t a = smem_u32(bar);
           umma_commit_pair(a);
-          umma_commit_pair(mapa_shared(a, 1));
+          umma_commit_pair(mapa_shared(a, cta | 1u));
         } else {
           umma_commit(bar);
         }
       };
       // per 16 k: K-major 32 bytes within the 128-byte rows of a 64-deep block, m / n
       // contiguous 16 rows of 128 bytes
-      const uint32_t lbo_a = p.a_mn ? kOpBytes / 2 : 16, lbo_b = p.b_mn ? kOpBytes / 2 : 16;
-      const uint32_t a_step = p.a_mn ? 2048 : 32, a_half = p.a_mn ? 4 * 2048 : kOpBytes / 2;
-      const uint32_t b_step = p.b_mn ? 2048 : 32, b_half = p.b_mn ? 4 * 2048 : kOpBytes / 2;
+      constexpr uint32_t kChunk = kDepth * 128;  // from 64 m or n to the next
+      const uint32_t lbo_a = p.a_mn ? kChunk : 16, lbo_b = p.b_mn ? kChunk : 16;
+      const uint32_t a_step = p.a_mn ? 2048 : 32, a_block = p.a_mn ? 4 * 2048 : kRows * 128;
+      const uint32_t b_step = p.b_mn ? 2048 : 32, b_block = p.b_mn ? 4 * 2048 : kBRows * 128;
+      // One stage's products into both halves' accumulators: rows of A that the first half's
+      // instruction has fetched stay for the second's.
+      auto issue_both = [&](uint32_t stage) {
+        const uint32_t a0 = smem_u32(ring + stage * kStageBytes);
+        const uint64_t ad0 = make_sdesc_sw128(a0, lbo_a, 1024);
+        const uint64_t bd0 = make_sdesc_sw128(a0 + kABytes, lbo_b, 1024);
+#pragma unroll
+        for (uint32_t k = 0; k < kDepth / 16; ++k) {
+          const uint64_t ad = ad0 + (((k >> 2) * a_block + (k & 3) * a_step) >> 4);
+          const uint64_t bd = bd0 + (((k >> 2) * b_block + (k & 3) * b_step) >> 4);
+          umma_f16_ss_pair_keep_a(tmem_base, ad, bd, idesc);
+          umma_f16_ss_pair_use_a(tmem_base + BN, ad, bd + (kBBytes >> 4), idesc);
+        }
+      };
+      // one stage's products into the accumulator of half h
+      auto issue = [&](uint32_t stage, uint32_t d, uint32_t h, bool add0) {
+        const uint32_t a0 = smem_u32(ring + stage * kStageBytes);
+        const uint64_t ad0 = make_sdesc_sw128(a0, lbo_a, 1024);
+        const uint64_t bd0 = make_sdesc_sw128(a0 + kABytes + h * kBBytes, lbo_b, 1024);
+#pragma unroll
+        for (uint32_t k = 0; k < kDepth / 16; ++k) {
+          const uint64_t ad = ad0 + (((k >> 2) * a_block + (k & 3) * a_step) >> 4);
+          const uint64_t bd = bd0 + (((k >> 2) * b_block + (k & 3) * b_step) >> 4);
+          const uint32_t add = add0 || k > 0;
+          if constexpr (CG == 2)
+            umma_f16_ss_pair(d, ad, bd, idesc, add);
+          else
+            umma_f16_ss(d, ad, bd, idesc, add);
+        }
+      };
       Walk walk;
-      walk.init(p, CG);
+      walk.init(CG);
       Unit u;
       uint32_t stage = 0, phase = 0, i = 0;
       bool ok = true;
@@ -428,39 +506,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         Walk::whole(p, uu, t);
         return true;
       };
+      auto advance = [&](uint32_t& st, uint32_t& ph) {
+        if (++st == kStages) st = 0, ph ^= 1u;
+      };
       while (ok && next_unit(u)) {
-        const uint32_t buf = i & 1u;
-        if (!wait_all(&tempty[buf], ((i >> 1) & 1u) ^ 1u, kWdMmaTmemEmpty)) break;
-        tc_fence_after();
-        const uint32_t d = tmem_base + buf * BN;
-        for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
-          if (!wait_all(&full[stage], phase, kWdMmaFull)) {
-            ok = false;
-            break;
-          }
+        if constexpr (HALVES == 1) {
+          const uint32_t buf = i & 1u;
+          if (!wait_all(&tempty[buf], ((i >> 1) & 1u) ^ 1u, kWdMmaTmemEmpty)) break;
           tc_fence_after();
-          if (elect_one()) {
-            const uint32_t a0 = smem_u32(ring + stage * kStageBytes);
-            const uint64_t ad0 = make_sdesc_sw128(a0, lbo_a, 1024);
-            const uint64_t bd0 = make_sdesc_sw128(a0 + kOpBytes, lbo_b, 1024);
-#pragma unroll
-            for (uint32_t k = 0; k < kDepth / 16; ++k) {
-              const uint64_t ad = ad0 + (((k >> 2) * a_half + (k & 3) * a_step) >> 4);
-              const uint64_t bd = bd0 + (((k >> 2) * b_half + (k & 3) * b_step) >> 4);
-              const uint32_t add = kb > u.kb0 || k > 0;
-              if constexpr (CG == 2)
-                umma_f16_ss_pair(d, ad, bd, idesc, add);
-              else
-                umma_f16_ss(d, ad, bd, idesc, add);
+          for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
+            if (!wait_all(&full[stage], phase, kWdMmaFull)) {
+              ok = false;
+              break;
             }
-            commit_all(&empty[stage]);
+            tc_fence_after();
+            if (elect_one()) {
+              issue(stage, tmem_base + buf * BN, 0, kb > u.kb0);
+              commit_all(&empty[stage]);
+            }
+            __syncwarp();
+            advance(stage, phase);
           }
+          if (!ok) break;
+          if (elect_one()) commit_all(&tfull[buf]);
           __syncwarp();
-          if (++stage == kStages) stage = 0, phase ^= 1u;
+        } else {
+          // The first and the last kSkew stages go through one half's accumulator, then
+          // through the other's: while the epilogue reads the first half, products of the
+          // second are still under way, and the next tile begins with the first.
+          for (uint32_t kb = u.kb0; ok && kb < u.kb1;) {
+            const bool first = kb == u.kb0;
+            const uint32_t left = u.kb1 - kb;
+            uint32_t n = 1;
+            if (first || left <= kSkew) n = min(kSkew, left);
+            const bool last = n == left;
+            if (!first && !last) {
+              if (!wait_all(&full[stage], phase, kWdMmaFull)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              if (elect_one()) {
+                issue_both(stage);
+                commit_all(&empty[stage]);
+              }
+              __syncwarp();
+              advance(stage, phase);
+              ++kb;
+              continue;
+            }
+#pragma unroll 1
+            for (uint32_t h = 0; ok && h < 2; ++h) {
+              if (first && !wait_all(&tempty[h], (i & 1u) ^ 1u, kWdMmaTmemEmpty)) {
+                ok = false;
+                break;
+              }
+              uint32_t st = stage, ph = phase;
+              for (uint32_t j = 0; j < n; ++j) {
+                if (h == 0 && !wait_all(&full[st], ph, kWdMmaFull)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+                if (elect_one()) {
+                  issue(st, tmem_base + h * BN, h, !first || j > 0);
+                  if (h == 1) commit_all(&empty[st]);
+                  if (last && j + 1 == n) commit_all(&tfull[h]);
+                }
+                __syncwarp();
+                advance(st, ph);
+              }
+              if (h == 1) stage = st, phase = ph;
+            }
+            kb += n;
+          }
+          if (!ok) break;
         }
-        if (!ok) break;
-        if (elect_one()) commit_all(&tfull[buf]);
-        __syncwarp();
         ++i;
       }
       // every product that was issued completes (bounded) before the memory goes away
@@ -474,18 +595,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       int none = 0;
       mbar_wait(drain, 0, &none, p.status, kWdDrain, 100000000ull);
     }
-  } else {
+  } else if (warp >= S::kFirstEpi) {
     // ------------------------------------------------------------ epilogue
-    const uint32_t e = warp - 2, q = warp & 3u, half = e >> 2;
+    if constexpr (HALVES == 2) setmaxnreg_inc<kRegsEpi>();
+    const uint32_t e = warp - S::kFirstEpi, q = warp & 3u, half = e >> 2;
     const uint32_t row_in_tile = q * 32 + lane;
-    uint8_t* stg = staging + e * 2 * kBoxBytes;
+    uint8_t* box = staging + e * kBoxBytes;
     auto wait_all = [&](uint64_t* bar, uint32_t parity, unsigned site) {
-      return __all_sync(~0u, mbar_wait(bar, parity, abort_flag, p.status, site)) != 0;
+      return __all_sync(~0u, mbar_sleep_wait(bar, parity, abort_flag, p.status, site)) != 0;
     };
     Walk walk;
-    walk.init(p, CG);
+    walk.init(CG);
     Unit u;
-    uint32_t i = 0, turn = 0;
+    uint32_t i = 0;
     auto next_unit = [&](Unit& uu) -> bool {
       if (walk.next(p, uu)) return true;
       if (!p.dyn) return false;
@@ -497,95 +619,149 @@ __global__ void __launch_bounds__(kThreads, 1)
       Walk::whole(p, uu, t);
       return true;
     };
-    while (next_unit(u)) {
-      const uint32_t buf = i & 1u;
-      if (!wait_all(&tfull[buf], (i >> 1) & 1u, kWdEpilogueTmemFull)) break;
-      tc_fence_after();
-      const uint32_t taddr = tmem_base + ((q * 32u) << 16) + buf * BN;
-      bool mine = true;  // whether this CTA finishes the tile
-      const float4* parts = nullptr;
-      if (u.split) {
-        // publish the fp32 part, take a ticket; the last one finishes the tile
-        float4* slot = reinterpret_cast<float4*>(p.partials) +
-                       (size_t(walk.unit) * CG + rank) * (kRows * BN / 4);
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      // Accumulator h of a tile: the tiles alternate between two, or each has both.
+      auto accumulator = [&](uint32_t h) { return HALVES == 2 ? h : i & 1u; };
+      auto wait_full = [&](uint32_t h) -> bool {
+        if (!wait_all(&tfull[accumulator(h)], (HALVES == 2 ? i : i >> 1) & 1u, kWdEpilogueTmemFull))
+          return ok = false;
+        tc_fence_after();
+        return true;
+      };
+      auto set_empty = [&](uint32_t h) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          uint64_t* bar = &tempty[accumulator(h)];
+          if (CG == 2 && rank == 1)
+            mbar_arrive_cluster(mapa_shared(smem_u32(bar), cta & ~1u));  // the leader's MMA warp waits
+          else
+            mbar_arrive(bar);
+        }
+      };
+      auto taddr = [&](uint32_t h) { return tmem_base + ((q * 32u) << 16) + accumulator(h) * BN; };
+      if constexpr (HALVES == 1) {
+        if (p.parts > 1) {
+          // a part: its sums to shared memory (the ring is idle once they are complete)
+          if (!wait_full(0)) break;
+          float4* part = reinterpret_cast<float4*>(ring);
 #pragma unroll 1
-        for (uint32_t c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c * 32, r);
-          tmem_ld_wait();
+          for (uint32_t c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(taddr(0) + c * 32, r);
+            tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            __stcg(slot + partial_index(c, j, row_in_tile),
-                   make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                               __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])));
+            for (uint32_t j = 0; j < 8; ++j)
+              part[part_index<BN>(row_in_tile, c * 8 + j)] =
+                  make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                              __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+          }
+          fence_proxy_async_smem();  // it will be sent from there
+          ++i;
+          continue;
         }
-        __threadfence();
-        named_barrier_sync(1, 32 * kEpiWarps);
-        if (e == 0 && lane == 0) {
-          unsigned* counter = &p.counters[u.tile * CG + rank];
-          const bool last = atomicAdd(counter, 1u) == p.parts - 1;
-          if (last) atomicExch(counter, 0u);
-          *bcast = last;
-        }
-        named_barrier_sync(1, 32 * kEpiWarps);
-        mine = *reinterpret_cast<volatile uint32_t*>(bcast) != 0;
-        if (mine) {
-          __threadfence();
-          parts = reinterpret_cast<const float4*>(p.partials) +
-                  (size_t(u.tile) * p.parts * CG + rank) * (kRows * BN / 4);
-        }
-        named_barrier_sync(1, 32 * kEpiWarps);  // the word is read before it is written again
       }
-      // columns 32 c .. of the tile's sums, from TMEM or from all parts in their order
-      auto sums = [&](uint32_t c, float (&v)[32]) {
-        if (!parts) {
+      const Place at = place_of(p, u.tile);
+      const uint32_t M = p.prob[at.prob].m, N = p.prob[at.prob].n;
+      const uint32_t row0 = (at.tm * CG + rank) * kRows + q * 32;
+      constexpr uint32_t kWide = EPI == kGated ? BN / 2 : BN;  // output columns of an accumulator
+      constexpr uint32_t kChunks = kWide / 64;                 // 32-column chunks of this warp
+      // The epilogue of wide tiles: bias, relu, residual.
+      auto light = [&](float (&v)[32], uint32_t col, const uint32_t (&res)[16],
+                       uint32_t (&out)[16]) {
+        if (p.fin.bias) add_bias<T>(p, col, N, v);
+        if (p.fin.act == FELIX_ACT_RELU) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = activate<FELIX_ACT_RELU>(v[j]);
+        }
+        if (p.fin.in[0]) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 f = Pair<T>::unpack(res[j]);
+            v[2 * j] += f.x;
+            v[2 * j + 1] += f.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[j] = Pair<T>::pack(v[2 * j], v[2 * j + 1]);
+      };
+      if constexpr (HALVES == 2) {
+        // Both halves are read, finished and rounded before anything is written: the next
+        // tile's products wait for the reads alone. (All CTAs write at about the same time,
+        // 64 KB each at 9 bytes a cycle; written in between, that took 7000 cycles a half.)
+        {
+          uint32_t hold[2][kChunks][16];  // the residual, then the results
+          const uint32_t col0 = at.tn * 2 * BN + half * kChunks * 32;
+          if (p.fin.in[0]) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+              for (uint32_t c = 0; c < kChunks; ++c)
+                if (row0 < M && col0 + h * BN + c * 32 < N)
+                  load_chunk(p, 0, row0, col0 + h * BN + c * 32, M, N, box, lane, hold[h][c]);
+          }
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) {
+            if (!wait_full(h)) break;
+#pragma unroll
+            for (uint32_t c = 0; c < kChunks; ++c) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(taddr(h) + (half * kChunks + c) * 32, r);
+              tmem_ld_wait();
+              float v[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+              light(v, col0 + h * BN + c * 32, hold[h][c], hold[h][c]);
+            }
+            set_empty(h);
+          }
+          if (ok) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+              for (uint32_t c = 0; c < kChunks; ++c)
+                if (row0 < M && col0 + h * BN + c * 32 < N)
+                  store_packed(p, int(at.prob), row0, col0 + h * BN + c * 32, M, N, box, lane,
+                               hold[h][c]);
+          }
+        }
+        ++i;
+        continue;
+      }
+      if constexpr (HALVES == 1) {
+        if (!wait_full(0)) break;
+        // columns 32 c .. of the accumulator's sums
+        auto sums = [&](uint32_t c, float (&v)[32]) {
           uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr + c * 32, r);
+          tmem_ld_32x32b_x32(taddr(0) + c * 32, r);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          return;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
-#pragma unroll 2
-        for (uint32_t s = 0; s < p.parts; ++s) {
-          const float4* src = parts + size_t(s) * CG * (kRows * BN / 4);
-          float4 x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __ldcg(src + partial_index(c, j, row_in_tile));
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[4 * j] += x[j].x;
-            v[4 * j + 1] += x[j].y;
-            v[4 * j + 2] += x[j].z;
-            v[4 * j + 3] += x[j].w;
-          }
-        }
-      };
-      if (mine) {
-        const Place at = place_of(p, u.tile);
-        const uint32_t M = p.prob[at.prob].m, N = p.prob[at.prob].n;
-        const uint32_t row0 = (at.tm * CG + rank) * kRows + q * 32;
-        constexpr uint32_t kWide = EPI == kGated ? BN / 2 : BN;  // output columns of a tile
-        constexpr uint32_t kChunks = kWide / 64;                 // 32-column chunks of this warp
+        };
+        const uint32_t col0 = at.tn * kWide + half * kChunks * 32;
+        // chunks that lie inside; the others hold zeros
+        const uint32_t chunks =
+            row0 < M && col0 < N ? min(kChunks, (N - col0 + 31) / 32) : 0u;
+        if (chunks == 0) set_empty(0);
 #pragma unroll 1
-        for (uint32_t cc = 0; cc < kChunks; ++cc) {
-          const uint32_t c = half * kChunks + cc, col = at.tn * kWide + c * 32;
-          if (row0 >= M || col >= N) break;  // this and the following chunks lie outside
+        for (uint32_t cc = 0; cc < chunks; ++cc) {
+          const uint32_t c = half * kChunks + cc, col = col0 + cc * 32;
+          // the accumulator is free for the next products once the last chunk is read
+          const bool done = cc + 1 == chunks;
           float v[32];
           if constexpr (EPI == kLinear) {
             uint32_t res[16];
-            if (p.in_ptr[0]) load_chunk<T>(p, 0, row0, col, M, N, stg, lane, res);
+            if (p.fin.in[0]) load_chunk(p, 0, row0, col, M, N, box, lane, res);
             sums(c, v);
-            if (p.bias) add_bias<T>(p, col, N, v);
-            if (p.out_want >> 1 & 1)
-              store_chunk<T>(p, 1, row0, col, M, N, stg, turn, lane, v);
-            with_activation(p.act, [&]<int ACT>() {
+            if (done) set_empty(0);
+            if (p.fin.bias) add_bias<T>(p, col, N, v);
+            if (p.fin.extra >> 1 & 1) store_chunk<T>(p, 1, row0, col, M, N, box, lane, v);
+            with_activation(p.fin.act, [&]<int ACT>() {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = activate<ACT>(v[j]);
             });
-            if (p.in_ptr[0]) {
+            if (p.fin.in[0]) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
                 const float2 f = Pair<T>::unpack(res[j]);
@@ -593,64 +769,70 @@ __global__ void __launch_bounds__(kThreads, 1)
                 v[2 * j + 1] += f.y;
               }
             }
-            store_chunk<T>(p, int(at.prob), row0, col, M, N, stg, turn, lane, v);
+            store_chunk<T>(p, int(at.prob), row0, col, M, N, box, lane, v);
           } else if constexpr (EPI == kGated) {
             float up[32];
             sums(c, v);
             sums(c + BN / 64, up);
-            if (p.out_want >> 1 & 1) store_chunk<T>(p, 1, row0, col, M, N, stg, turn, lane, v);
-            if (p.out_want >> 2 & 1) store_chunk<T>(p, 2, row0, col, M, N, stg, turn, lane, up);
-            with_activation(p.act, [&]<int ACT>() {
+            if (done) set_empty(0);
+            if (p.fin.extra >> 1 & 1) store_chunk<T>(p, 1, row0, col, M, N, box, lane, v);
+            if (p.fin.extra >> 2 & 1) store_chunk<T>(p, 2, row0, col, M, N, box, lane, up);
+            with_activation(p.fin.act, [&]<int ACT>() {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = activate<ACT>(v[j]) * up[j];
             });
-            store_chunk<T>(p, 0, row0, col, M, N, stg, turn, lane, v);
+            store_chunk<T>(p, 0, row0, col, M, N, box, lane, v);
           } else {
             uint32_t graw[16], uraw[16];
-            load_chunk<T>(p, 0, row0, col, M, N, stg, lane, graw);
-            load_chunk<T>(p, 1, row0, col, M, N, stg, lane, uraw);
+            load_chunk(p, 0, row0, col, M, N, box, lane, graw);
+            load_chunk(p, 1, row0, col, M, N, box, lane, uraw);
             sums(c, v);
-            float du[32], h[32];
-            with_activation(p.act, [&]<int ACT>() {
+            if (done) set_empty(0);
+            float du[32], hh[32];
+            with_activation(p.fin.act, [&]<int ACT>() {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
                 const float2 g = Pair<T>::unpack(graw[j]), up = Pair<T>::unpack(uraw[j]);
                 float a, d;
                 activate_both<ACT>(g.x, a, d);
                 du[2 * j] = v[2 * j] * a;
-                h[2 * j] = a * up.x;
+                hh[2 * j] = a * up.x;
                 v[2 * j] *= up.x * d;
                 activate_both<ACT>(g.y, a, d);
                 du[2 * j + 1] = v[2 * j + 1] * a;
-                h[2 * j + 1] = a * up.y;
+                hh[2 * j + 1] = a * up.y;
                 v[2 * j + 1] *= up.y * d;
               }
             });
-            store_chunk<T>(p, 0, row0, col, M, N, stg, turn, lane, v);
-            store_chunk<T>(p, 1, row0, col, M, N, stg, turn, lane, du);
-            store_chunk<T>(p, 2, row0, col, M, N, stg, turn, lane, h);
+            store_chunk<T>(p, 0, row0, col, M, N, box, lane, v);
+            store_chunk<T>(p, 1, row0, col, M, N, box, lane, du);
+            store_chunk<T>(p, 2, row0, col, M, N, box, lane, hh);
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 2 && rank == 1)
-          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[buf]), 0));  // the leader's MMA waits
-        else
-          mbar_arrive(&tempty[buf]);
-      }
       ++i;
     }
-    if (lane == 0) bulk_wait_group<0>();  // the boxes stay until they have been written out
-    __syncwarp();
+  } else {
+    if constexpr (HALVES == 2) setmaxnreg_dec<kRegsFirst>();
   }
 
   tc_fence_before();
-  if (CG == 2)
+  if (p.parts > 1) {
+    if constexpr (HALVES == 1) {
+      const Place at = place_of(p, blockIdx.x / (CG * p.parts));
+      const Problem& q = p.prob[at.prob];
+      constexpr uint32_t kWide = EPI == kGated ? BN / 2 : BN;
+      TilePlace place{at.prob, (at.tm * CG + rank) * kRows, at.tn * kWide, 0, 0};
+      place.tokens = place.t0 < q.m ? min(kRows, q.m - place.t0) : 0u;
+      place.features = min(kWide, q.n - place.f0);
+      finish_tile<T, EPI, BN, kRows>(p.fin, place, ring, p.parts, cta / CG, rank, CG, S::kThreads,
+                                     received, abort_flag, p.status);
+    }
+  } else if (CG == 2) {
     cluster_sync();  // no CTA exits while its peer may still use its memory
-  else
+  } else {
     __syncthreads();
+  }
   if (p.dyn && rank == 0 && threadIdx.x == 0) {
     // every leader has taken its final tile id: the last one puts the counter back
     __threadfence();
@@ -670,100 +852,158 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 struct Plan {
-  int cg;
-  uint32_t tiles, kb, units, split_tiles, parts;
+  int cg, bn_, halves;
+  uint32_t tiles, kb, depth, units, parts;
   bool dyn;
+  double cost;
+  uint32_t bm() const { return kRows * cg; }
+  uint32_t bn(const Product& p) const {
+    return bn_ * halves / (p.epilogue == kGated ? 2 : 1);
+  }
 };
 
-uint64_t count_tiles(const Product& p, int cg) {
-  const uint64_t bm = kRows * cg, bn = kRows * cg / (p.epilogue == kGated ? 2 : 1);
+uint64_t count_tiles(const Product& p, uint64_t bm, uint64_t bn) {
   uint64_t tiles = 0;
   for (uint32_t i = 0; i < p.problems; ++i)
     tiles += ((p.m[i] + bm - 1) / bm) * ((p.n[i] + bn - 1) / bn);
   return tiles;
 }
 
-Plan plan_for(const Product& p, int cg, int num_sms) {
+// Clusters of 1, 2, 4 and 8 CTAs that run at the same time, one CTA per SM.
+struct Clusters {
+  uint32_t n[4];
+};
+const Clusters* clusters_of(DeviceInfo* dev) {
+  static Clusters all[64];
+  static felix_impl::PerDeviceOnce once;
+  const int rc = once.run(dev->ordinal, [&] {
+    const auto kernel = ffn_product_kernel<__half, kLinear, 1, 128, 1>;
+    int rc = int(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kSmemBytes));
+    for (uint32_t i = 0; i < 4 && !rc; ++i) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(uint32_t(dev->num_sms) << i);
+      cfg.blockDim = dim3(Shape<1, 128, 1>::kThreads);
+      cfg.dynamicSmemBytes = kSmemBytes;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim = {1u << i, 1, 1};
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      rc = int(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+      all[dev->ordinal].n[i] = uint32_t(n);
+    }
+    return rc;
+  });
+  return rc ? nullptr : &all[dev->ordinal];
+}
+
+// Tiles of one shape, each in `parts` parts of its depth, with an estimate of the time in us:
+// waves of 128-deep blocks at the rate that the shape reaches with all SMs at work (one CTA's
+// and the narrow pair's tiles are bound by their operands from the L2, 120 GB/s an SM; 256
+// wide and more by the tensor cores), the start and the last epilogue, and for parts the
+// cluster's barrier, the exchange and the sums. Measured, tokens x depth x features, us, one
+// CTA | pair 128 | 256 | two halves wide: 500 x 4096 x 4096 23.2 | 20.8 | 29.0 | 47.8,
+// 500 x 11264 x 4096 54 | 45 | 66 | 111, 2000 x 4096 x 4096 75 | 59 | 51 | 51, 777 x 1024 x
+// 5008 13.7 | 16.9 | 17.6 | 19.7; one CTA's tiles of 128 x 4096 x 4096 in 1, 2, 4 parts 22.7,
+// 17.5, 14.5; pairs' of 500 x 11264 x 4096 in 2 42.
+Plan plan_for(const Product& p, int cg, int bn, int halves, uint32_t parts, uint32_t units) {
   Plan r{};
   r.cg = cg;
-  r.tiles = uint32_t(count_tiles(p, cg));
-  r.kb = (p.k + kDepth - 1) / kDepth * p.segments;
-  const uint32_t units = std::max(1u, uint32_t(num_sms) / cg);
-  const uint32_t rem = r.tiles % units, waves = (r.tiles + units - 1) / units;
-  // The last wave's tiles are cut along k where that fills at least twice as many units
-  // and whole waves would leave more than 5 % of them idle; a part is at least 2 blocks.
-  r.parts = 1;
-  if (rem && uint64_t(r.tiles) * 100 < uint64_t(waves) * units * 95)
-    r.parts = std::max(1u, std::min({units / rem, r.kb / 2, 8u}));
-  r.split_tiles = r.parts > 1 ? rem : 0;
-  r.units = std::min(units, r.tiles - r.split_tiles + r.split_tiles * r.parts);
-  r.dyn = r.tiles - r.split_tiles >= 4 * r.units;
+  r.bn_ = bn;
+  r.halves = halves;
+  r.depth = halves == 2 ? 64 : 128;
+  r.tiles = uint32_t(std::min<uint64_t>(count_tiles(p, r.bm(), r.bn(p)), 0x7fffffff));
+  r.kb = (p.k + r.depth - 1) / r.depth * p.segments;
+  r.parts = parts;
+  r.units = std::min(units, r.tiles);
+  r.dyn = parts == 1 && r.tiles >= 4 * r.units;
+  const bool one = cg == 1, pair = cg == 2 && bn == 128, wide = halves == 2;
+  double block = one ? 0.555 : pair ? 0.44 : wide ? 1.25 / 2 : 0.66;  // us a block of `depth`
+  if (p.epilogue != kLinear) block *= bn == 128 ? 1.15 : 1.06;  // two values a result
+  const double ends = one ? 5.4 : pair ? 6.7 : wide ? 10.5 : 7.9;
+  const double waves = double((r.tiles + units - 1) / units);
+  r.cost = ends + waves * block * ((r.kb + parts - 1) / parts);
+  if (parts > 1) r.cost += bn == 256 ? 4.5 : 2.5 + 0.3 * parts;
   return r;
 }
 
-// Time of a plan in units of one 128-deep block of a CTA pair's 256 x 256 tile. A single
-// CTA's 128 x 128 tile does half a CTA's share of that at about 0.7 of the rate (it reads
-// twice the bytes per product from the L2).
-double cost_of(const Plan& r, int num_sms) {
-  const double units = std::max(1, num_sms / r.cg);
-  const double block = r.cg == 2 ? 1.0 : 0.72;
-  const double whole = double((r.tiles - r.split_tiles + uint32_t(units) - 1) / uint32_t(units));
-  const double split = r.split_tiles ? 1.0 / r.parts : 0.0;
-  return block * (r.kb * (whole + split) + 6 * (whole + (r.split_tiles ? 2 : 0)));
-}
-
-Plan make_plan(const Product& p, int num_sms) {
-  const Plan one = plan_for(p, 1, num_sms), two = plan_for(p, 2, num_sms);
-  return cost_of(two, num_sms) <= cost_of(one, num_sms) ? two : one;
-}
-
-size_t workspace_need(const Plan& r) {
-  size_t n = felix_impl::kWsCounterBytes;
-  if (r.split_tiles)
-    n += size_t(r.split_tiles) * r.parts * r.cg * kRows * (kRows * r.cg) * sizeof(float);
-  return n;
+Plan make_plan(const Product& p, DeviceInfo* dev, const Clusters& clusters) {
+  Plan best = plan_for(p, 2, 256, 1, 1, clusters.n[1]);
+  auto consider = [&](const Plan& r) {
+    if (r.cost < best.cost) best = r;
+  };
+  consider(plan_for(p, 2, 128, 1, 1, clusters.n[1]));
+  consider(plan_for(p, 1, 128, 1, 1, clusters.n[0]));
+  if (p.epilogue == kLinear && p.act <= FELIX_ACT_RELU && !p.out[1].p)
+    consider(plan_for(p, 2, 256, 2, 1, clusters.n[1]));
+  // in parts: one wave of clusters of 2, 4 or 8 CTAs, parts of 256 at least
+  for (int i = 1; i < 4; ++i) {
+    auto split = [&](int cg, int bn) {
+      const Plan r = plan_for(p, cg, bn, 1, (1u << i) / cg, clusters.n[i]);
+      if (r.parts > 1 && r.tiles <= clusters.n[i] && r.kb >= 2 * r.parts) consider(r);
+    };
+    split(1, 128);
+    split(2, 128);
+    split(2, 256);
+  }
+  return best;
 }
 
 // Tensor map of an operand: whole 64-wide blocks as a third dimension where its
 // contiguous extent is a multiple of 64, two dimensions otherwise.
 int encode_operand(CUtensorMap* map, const Mat& x, bool mn, bool whole, uint32_t rows, uint32_t k,
-                   uint32_t box_rows) {
+                   uint32_t box_rows, uint32_t depth) {
   const uint64_t inner = mn ? rows : k, outer = mn ? k : rows;
   // a single row's distance to the next one is never used, but has to be encodable
   const uint64_t pitch = outer > 1 ? uint64_t(x.ld) * 2 : (inner * 2 + 15) / 16 * 16;
   if (whole)
     return felix_impl::encode_tmap_3d_f16(map, x.p, 64, outer, inner / 64, pitch, 128, 64,
-                                          mn ? kDepth : box_rows, 2);
-  return felix_impl::encode_tmap_2d_f16(map, x.p, inner, outer, pitch, 64, mn ? kDepth : box_rows);
+                                          mn ? depth : box_rows, mn ? box_rows / 64 : depth / 64);
+  return felix_impl::encode_tmap_2d_f16(map, x.p, inner, outer, pitch, 64, mn ? depth : box_rows);
 }
 
-template <class T, int EPI, int CG>
-FelixCode launch(DeviceInfo* dev, const Params& p, uint32_t units, cudaStream_t stream) {
+template <class T, int EPI, int CG, int BN, int HALVES>
+FelixCode launch_shape(DeviceInfo* dev, const Params& p, const Plan& r, cudaStream_t stream) {
+  const auto kernel = ffn_product_kernel<T, EPI, CG, BN, HALVES>;
   static felix_impl::PerDeviceOnce once;
-  const int rc = once.run(dev->ordinal, [] {
-    return int(cudaFuncSetAttribute(ffn_product_kernel<T, EPI, CG>,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  const int rc = once.run(dev->ordinal, [&] {
+    if (HALVES == 2) {
+      cudaFuncAttributes attr;
+      const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+      if (e != cudaSuccess) return int(e);
+      if (attr.numRegs != kRegsLaunch) return -1;
+    }
+    return int(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kSmemBytes));
   });
+  if (rc == -1)
+    return felix_impl::api_error("feed-forward product: built with another register count than "
+                                 "its register split assumes");
   if (rc) return felix_impl::launch_error(cudaError_t(rc), "feed-forward product: attributes");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(units * CG);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(r.units * r.parts * CG);
+  cfg.blockDim = dim3(Shape<CG, BN, HALVES>::kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {CG, 1, 1};
+  attr[0].val.clusterDim = {CG * r.parts, 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ffn_product_kernel<T, EPI, CG>, p);
+  cfg.numAttrs = CG * r.parts > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) return felix_impl::launch_error(e, "feed-forward product: launch failed");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }
 
 template <class T, int EPI>
 FelixCode launch(DeviceInfo* dev, const Params& p, const Plan& r, cudaStream_t stream) {
-  return r.cg == 2 ? launch<T, EPI, 2>(dev, p, r.units, stream)
-                   : launch<T, EPI, 1>(dev, p, r.units, stream);
+  if constexpr (EPI == kLinear)
+    if (r.halves == 2) return launch_shape<T, EPI, 2, 256, 2>(dev, p, r, stream);
+  return r.cg == 1      ? launch_shape<T, EPI, 1, 128, 1>(dev, p, r, stream)
+         : r.bn_ == 128 ? launch_shape<T, EPI, 2, 128, 1>(dev, p, r, stream)
+                        : launch_shape<T, EPI, 2, 256, 1>(dev, p, r, stream);
 }
 
 template <class T>
@@ -780,18 +1020,20 @@ FelixCode launch(DeviceInfo* dev, const Params& p, const Plan& r, int epilogue,
 
 using namespace product;
 
-size_t product_workspace_bytes(const Product& p, int num_sms) {
-  return workspace_need(make_plan(p, num_sms));
+// Whether rows consist of whole vectors of n elements.
+static bool whole(uint32_t n, const void* p, int64_t ld, uint32_t rows, uint32_t cols) {
+  return reinterpret_cast<uintptr_t>(p) % (2 * n) == 0 && cols % n == 0 && (rows <= 1 || ld % n == 0);
 }
 
 FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cudaStream_t stream) {
-  if (count_tiles(x, 1) > 0x3fffffffu)
+  if (count_tiles(x, kRows, kRows / 2) > 0x3fffffffu)
     return felix_impl::api_error("feed-forward product: too many tiles");
-  const Plan r = make_plan(x, dev->num_sms);
-  if (r.split_tiles * r.cg > felix_impl::kWsMaxCounters - 2)
-    return felix_impl::api_error("feed-forward product: too many split tiles");
+  const Clusters* clusters = clusters_of(dev);
+  if (!clusters) return felix_impl::launch_error(cudaGetLastError(), "feed-forward product: device");
+  const Plan r = make_plan(x, dev, *clusters);
   Params p{};
-  const uint32_t bm = kRows * r.cg, bn = kRows * r.cg / (x.epilogue == kGated ? 2 : 1);
+  p.fin = finish_of(x);
+  const uint32_t bm = r.bm(), bn = r.bn(x);
   const uint32_t operands = std::max(x.segments, x.problems);
   const bool gated = x.epilogue == kGated;
   uint32_t tile = 0;
@@ -803,35 +1045,28 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
     if ((x.b_mn ? x.n[i] : x.k) % 64) p.b_3d = 0;
   }
   if (gated && r.cg == 1) p.b_3d = 0;  // boxes of 64 rows, side by side in a stage
+  // a stage of 64 k is one block of K-major rows
+  if (r.depth == 64 && !x.a_mn) p.a_3d = 0;
+  if (r.depth == 64 && !x.b_mn) p.b_3d = 0;
   for (uint32_t i = 0; i < std::max(operands, gated ? 2u : 1u); ++i) {
     const uint32_t prob = std::min(i, x.problems - 1);
     if (i < operands &&
-        encode_operand(&p.a[i], x.a[i], x.a_mn, p.a_3d, x.m[prob], x.k, kRows))
+        encode_operand(&p.a[i], x.a[i], x.a_mn, p.a_3d, x.m[prob], x.k, kRows, r.depth))
       return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
     if (encode_operand(&p.b[i], x.b[i], x.b_mn, p.b_3d, x.n[prob], x.k,
-                       gated && r.cg == 1 ? 64 : kRows))
+                       gated && r.cg == 1 ? 64 : r.bn_ / r.cg, r.depth))
       return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
   }
   for (uint32_t i = 0; i < 3; ++i) {
     if (!x.out[i].p) continue;
     const uint32_t prob = std::min(i, x.problems - 1), m = x.m[prob], n = x.n[prob];
-    p.out_ptr[i] = x.out[i].p;
-    p.out_ld[i] = x.out[i].ld;
-    p.out_want |= 1u << i;
-    if (!tma_ok(x.out[i].p, x.out[i].ld, m, n)) continue;
-    const uint64_t pitch = m > 1 ? uint64_t(x.out[i].ld) * 2 : (uint64_t(n) * 2 + 15) / 16 * 16;
-    if (felix_impl::encode_tmap_2d_f16_swizzle(&p.out[i], x.out[i].p, n, m, pitch, 32, 32, 64))
-      return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
-    p.out_tma |= 1u << i;
+    p.out_vec |= uint32_t(whole(8, x.out[i].p, x.out[i].ld, m, n)) << i;
+    p.out_sectors |= uint32_t(whole(16, x.out[i].p, x.out[i].ld, m, n)) << i;
   }
-  if (x.problems > 1) p.out_want &= 1;  // there out[] are the problems' results
   for (uint32_t i = 0; i < 2; ++i) {
     if (!x.in[i].p) continue;
-    p.in_ptr[i] = x.in[i].p;
-    p.in_ld[i] = x.in[i].ld;
-    const bool vec = (reinterpret_cast<uintptr_t>(x.in[i].p) & 15) == 0 && x.n[0] % 8 == 0 &&
-                     (x.m[0] <= 1 || x.in[i].ld % 8 == 0);
-    p.in_vec |= uint32_t(vec) << i;
+    p.in_vec |= uint32_t(whole(8, x.in[i].p, x.in[i].ld, x.m[0], x.n[0])) << i;
+    p.in_sectors |= uint32_t(whole(16, x.in[i].p, x.in[i].ld, x.m[0], x.n[0])) << i;
   }
   p.problems = x.problems;
   p.tiles = r.tiles;
@@ -839,16 +1074,10 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
   p.kb_seg = r.kb / x.segments;
   p.a_mn = x.a_mn;
   p.b_mn = x.b_mn;
-  p.group_m = r.cg == 2 ? 8 : 16;
-  p.split_tiles = r.split_tiles;
+  p.group_m = r.halves == 2 ? 12 : r.cg == 2 ? 8 : 16;
   p.parts = r.parts;
   p.dyn = r.dyn;
-  p.bias = x.bias;
-  p.act = x.act;
-  p.counters = static_cast<unsigned*>(workspace);
-  p.dyn_counter = p.counters + (felix_impl::kWsMaxCounters - 2);
-  p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                        felix_impl::kWsCounterBytes);
+  p.dyn_counter = static_cast<unsigned*>(workspace) + (felix_impl::kWsMaxCounters - 2);
   p.status = dev->status_word;
   return x.bf16 ? launch<__nv_bfloat16>(dev, p, r, x.epilogue, stream)
                 : launch<__half>(dev, p, r, x.epilogue, stream);

@@ -8,6 +8,7 @@
 #include <initializer_list>
 
 #include "activation.cuh"
+#include "ffn_finish.cuh"
 #include "ffn_internal.h"
 
 namespace felix_ffn {
@@ -29,36 +30,6 @@ __global__ void __launch_bounds__(256)
     uint16_t* d = dst + int64_t(r) * dst_ld;
 #pragma unroll 4
     for (uint32_t c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) d[c] = s[c];
-  }
-}
-
-// V (1 or 8) elements as fp32.
-template <class T, int V>
-__device__ __forceinline__ void load_values(const uint16_t* p, float (&v)[V]) {
-  if constexpr (V == 8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pair<T>::unpack(x[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  } else {
-    v[0] = Pair<T>::to_float(*p);
-  }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_values(uint16_t* p, const float (&v)[V]) {
-  if constexpr (V == 8) {
-    uint4 w;
-    w.x = Pair<T>::pack(v[0], v[1]);
-    w.y = Pair<T>::pack(v[2], v[3]);
-    w.z = Pair<T>::pack(v[4], v[5]);
-    w.w = Pair<T>::pack(v[6], v[7]);
-    *reinterpret_cast<uint4*>(p) = w;
-  } else {
-    *p = Pair<T>::of_float(v[0]);
   }
 }
 
@@ -149,19 +120,19 @@ struct Call {
   bool bf16;
   enum { kCount, kLaunch } pass = kCount;
   uint8_t* base = nullptr;
-  // bytes in front: the counters, which in the library's scratch other calls rely on
-  // even where this one has no product that uses them, and the products' partials
-  size_t products = felix_impl::kWsCounterBytes;
-  size_t used = 0;           // bytes behind them
-  bool tiled = false;        // a product of more than a few tokens runs
+  // The products' counters come first. In the library's scratch other calls rely on them
+  // even where this one has no product that uses them.
+  static constexpr size_t kFront = felix_impl::kWsCounterBytes;
+  bool tiled = false;  // a product uses them
+  size_t used = 0;     // bytes behind them
   FelixCode code = kDone;
 
   bool ok() const { return code.type == FELIX_SUCCESS; }
   bool counting() const { return pass == kCount; }
-  size_t total() const { return tiled || used ? products + used : 0; }
+  size_t total() const { return tiled || used ? kFront + used : 0; }
 
   void* take(size_t bytes) {
-    void* p = counting() ? nullptr : base + products + used;
+    void* p = counting() ? nullptr : base + kFront + used;
     used += (bytes + 255) / 256 * 256;
     return p;
   }
@@ -193,9 +164,10 @@ struct Call {
   void run(const Product& p) {
     if (few_tokens(p)) {
       if (!counting() && ok()) code = few_launch(p, stream);
+    } else if (narrow_tokens(p)) {
+      if (!counting() && ok()) code = narrow_launch(dev, p, stream);
     } else if (counting()) {
       tiled = true;
-      products = std::max(products, product_workspace_bytes(p, dev->num_sms));
     } else if (ok()) {
       code = product_launch(dev, p, base, stream);
     }
