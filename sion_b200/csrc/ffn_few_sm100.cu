@@ -173,7 +173,7 @@ FelixCode few_launch(const Product& x, cudaStream_t stream) {
   };
   p.x = static_cast<const uint16_t*>(x.a[0].p);
   p.x_ld = x.a[0].ld;
-  bool all = x.k % 8 == 0 && vec(x.a[0], x.m[0]);
+  bool all = x.k[0] % 8 == 0 && vec(x.a[0], x.m[0]);
   for (int i = 0; i < (gated ? 2 : 1); ++i) {
     p.w[i] = static_cast<const uint16_t*>(x.b[i].p);
     p.w_ld[i] = x.b[i].ld;
@@ -188,7 +188,7 @@ FelixCode few_launch(const Product& x, cudaStream_t stream) {
   }
   p.tokens = x.m[0];
   p.n = x.n[0];
-  p.k = x.k;
+  p.k = x.k[0];
   p.act = x.act;
   if (gated)
     x.bf16 ? few::launch<__nv_bfloat16, true>(p, all, stream)

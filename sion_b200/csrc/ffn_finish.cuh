@@ -15,21 +15,14 @@ namespace felix_ffn {
 // Outputs and inputs of an epilogue (see Product). extra: bits 1 and 2 for outputs that are
 // wanted besides the first. vec: all rows are whole 16-byte vectors.
 struct Finish {
-  void* out[3];
-  int64_t out_ld[3];
+  void* out[kMaxProblems];
+  int64_t out_ld[kMaxProblems];
   const void* in[2];
   int64_t in_ld[2];
   const void* bias;
   int act;
   uint32_t extra, vec;
 };
-
-// float4 of 4 features of a token in a part of W features, swizzled: neither 8 tokens' same
-// features nor 32 features of a token conflict.
-template <uint32_t W>
-__device__ __forceinline__ uint32_t part_index(uint32_t token, uint32_t q) {
-  return token * (W / 4) + (q ^ (token & 7));
-}
 
 template <class T>
 __device__ __forceinline__ void unpack8(const uint4& w, float (&v)[8]) {
@@ -149,6 +142,9 @@ struct TilePlace {
   uint32_t prob, t0, f0, tokens, features;
 };
 
+// A part is [token][W features] in float4 of 4 features, the q-th of a token at q ^ (token & 7):
+// neither 8 tokens' same features nor 32 features of a token conflict.
+//
 // Rows [me, me + 1) R / P of a tile of R rows (tokens) of W features (kGated: the gate's, then
 // from W / 2 on the up projection's). own: this CTA's part, followed by what the others sent,
 // in their order.
@@ -228,7 +224,7 @@ inline Finish finish_of(const Product& x) {
   auto check = [&](const void* p, int64_t ld, uint32_t rows) {
     if (p && ((reinterpret_cast<uintptr_t>(p) & 15) || (rows > 1 && ld % 8))) vec = false;
   };
-  for (uint32_t i = 0; i < 3; ++i) {
+  for (uint32_t i = 0; i < kMaxProblems; ++i) {
     const uint32_t prob = i < x.problems ? i : x.problems - 1;
     f.out[i] = x.out[i].p;
     f.out_ld[i] = x.out[i].ld;

@@ -24,19 +24,22 @@ enum Epilogue {
   kDGated = 2   // v = dh, in0 = g, in1 = u: out0 = dh u act'(g), out1 = dh act(g), out2 = act(g) u
 };
 
-// D[m][n] = sum over segments and k of A[m][k] B[n][k]. An operand is stored either
-// with k contiguous (A [m][k], B [n][k]) or, "mn", with m or n contiguous (A [k][m],
+constexpr uint32_t kMaxProblems = 4, kMaxOperands = 5;
+
+// D[m][n] = sum over segments and k of A[m][k] B[n][k], for one or (kLinear without anything
+// behind the product) several independent problems, deepest first. An operand is stored
+// either with k contiguous (A [m][k], B [n][k]) or, "mn", with m or n contiguous (A [k][m],
 // B [k][n]).
 struct Product {
   Epilogue epilogue = kLinear;
   bool bf16 = false;
-  bool a_mn = false, b_mn = false;
-  uint32_t k = 0;         // depth of one segment
-  uint32_t segments = 1;  // kLinear only: A and B of each segment in a[], b[]
-  uint32_t problems = 1;  // kLinear only: independent products of one depth, a[], b[], out[]
-  uint32_t m[3] = {}, n[3] = {};
-  Mat a[3], b[3];  // kGated: b[0] gate, b[1] up
-  MutMat out[3];   // null: not wanted (out1 of kLinear, out1 and out2 of kGated)
+  uint32_t problems = 1;
+  uint32_t m[kMaxProblems] = {}, n[kMaxProblems] = {};
+  uint32_t k[kMaxProblems] = {};                    // depth of one segment
+  uint32_t segments[kMaxProblems] = {1, 1, 1, 1};   // kLinear only
+  bool a_mn[kMaxProblems] = {}, b_mn[kMaxProblems] = {};
+  Mat a[kMaxOperands], b[kMaxOperands];  // problem after problem; kGated: b[0] gate, b[1] up
+  MutMat out[kMaxProblems];  // of the problems, or one problem's (null: not wanted)
   Mat in[2];
   const void* bias = nullptr;
   int act = FELIX_ACT_NONE;
@@ -55,7 +58,7 @@ FelixCode product_launch(DeviceInfo* dev, const Product& p, void* workspace, cud
 // Products of few tokens, for which reading the weights is all: up to 8 (operands of any
 // address and stride) and up to 64 (addressable by TMA). Neither needs scratch.
 inline bool forward_product(const Product& p) {
-  return p.epilogue != kDGated && p.segments == 1 && p.problems == 1 && !p.a_mn && !p.b_mn;
+  return p.epilogue != kDGated && p.problems == 1 && p.segments[0] == 1 && !p.a_mn[0] && !p.b_mn[0];
 }
 inline bool few_tokens(const Product& p) { return p.m[0] <= 8 && forward_product(p); }
 FelixCode few_launch(const Product& p, cudaStream_t stream);

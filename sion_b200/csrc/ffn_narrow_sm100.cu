@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
         tmem_ld_wait();
 #pragma unroll
         for (uint32_t j = 0; j < 32; ++j)
-          part[part_index<128>(c + j, row / 4) * 4 + row % 4] = __uint_as_float(r[j]);
+          part[((c + j) * 32 + ((row / 4) ^ ((c + j) & 7))) * 4 + row % 4] = __uint_as_float(r[j]);
       }
       fence_proxy_async_smem();  // it will be sent from there
     } else {
@@ -238,18 +238,18 @@ FelixCode narrow_launch(DeviceInfo* dev, const Product& x, cudaStream_t stream) 
   p.features = x.n[0];
   p.tiles_t = (p.tokens + bn - 1) / bn;
   const uint32_t tiles = (p.features + wide - 1) / wide * p.tiles_t;
-  p.kb = (x.k + kDepth - 1) / kDepth;
+  p.kb = (x.k[0] + kDepth - 1) / kDepth;
   // Parts of 256 k at least. Measured with 24 tokens, 4096 deep, us: 32 tiles in 2, 4, 8 parts
   // 15.5, 11.6, 13.2; 128 tiles in 1, 2, 4 28.5, 26.2, 31.6; 176 (gated) in 1, 2 36.9, 41.3.
   p.parts = 1;
   while (p.parts < 8 && tiles * p.parts * 2 <= 2 * uint32_t(dev->num_sms) &&
          p.kb >= 4 * p.parts && (p.parts < 4 || tiles * p.parts * 2 <= uint32_t(dev->num_sms)))
     p.parts *= 2;
-  p.whole = x.k % 64 == 0;
+  p.whole = x.k[0] % 64 == 0;
   int rc = 0;
   for (int i = 0; i < (gated ? 2 : 1); ++i)
-    rc |= encode(&p.w[i], x.b[i], p.whole && !gated, p.features, x.k, wide);
-  rc |= encode(&p.x, x.a[0], p.whole, p.tokens, x.k, bn);
+    rc |= encode(&p.w[i], x.b[i], p.whole && !gated, p.features, x.k[0], wide);
+  rc |= encode(&p.x, x.a[0], p.whole, p.tokens, x.k[0], bn);
   if (rc) return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
   p.fin = finish_of(x);
   p.status = dev->status_word;

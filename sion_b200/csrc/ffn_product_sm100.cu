@@ -5,21 +5,23 @@
 //            TMEM, so that one thread holds both of an element: act(g) u
 //   kDGated  dh = dy Wd never leaves the SM: dg, du and h are written from it
 //
-// Tiles. CG = 2: a CTA pair (cta_group::2) computes 256 x 256, each CTA loading 128
-// rows of A and 128 of B per stage and holding 128 rows of the tile in its TMEM; for
-// kGated one CTA's 128 rows of B are the gate's and the other's the up projection's.
-// CG = 1: 128 x 128, for products of few tiles. A stage is 128 deep: 32 KB per operand
-// (one request where the tensor map can say it, two of 16 KB where a size is no multiple
-// of 64), three stages. Two accumulators, so that the epilogue of a tile overlaps the
-// next tile's products. An operand may be stored with k or with m / n contiguous: the
-// three products of a training step need x W^T, dz W and dz^T x, without a transpose.
+// Tiles. CG = 2: a CTA pair (cta_group::2) computes 256 rows x BN columns, each CTA loading
+// its 128 rows of A and BN / 2 of B per stage and holding its rows of the tile in its TMEM;
+// for kGated one CTA's rows of B are the gate's and the other's the up projection's. CG = 1:
+// 128 x 128. Two accumulators, so that the epilogue of a tile overlaps the next tile's
+// products. HALVES = 2: two accumulators of one tile of 256 x 512; its epilogue has to be short.
+// What bounds a tile is the L2's 64 bytes a cycle and SM: per 128 k a pair's CTA needs 1024
+// cycles for 64 KB at BN = 256, as long as its products take, 768 for 48 KB at BN = 128
+// (products 512), 768 a half at 512 columns; so few tiles are cut along k rather than made
+// small. An operand may be stored with k or with m / n contiguous: a training step's x W^T,
+// dz W and dz^T x need no transpose. One launch may do several products (a backward pass does
+// all of its own), deepest tiles first.
 //
-// Warps: 0 TMA, 1 MMA, 2-9 epilogue (two per quarter of the TMEM lanes, each with half
-// the columns: activations cost 10 to 50 instructions a value).
+// Warps: 0 TMA, 1 MMA, 8 of the epilogue (two per quarter of the TMEM lanes, which take every
+// other 32 columns: activations cost 10 to 50 instructions a value).
 //
-// Schedule: persistent; the tiles of an incomplete last wave are cut along k in equal
-// parts, first of all, and finished by the last contributor in the order of the parts
-// (repeatable); from four waves on whole tiles are handed out at run time (tile_queue.cuh).
+// Schedule: persistent, tiles from a queue (tile_queue.cuh) where there are several per CTA;
+// or, where tiles are few, each tile in parts of its depth over a cluster (ffn_finish.cuh).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -37,7 +39,7 @@ namespace product {
 
 using namespace felix_sm100;
 
-constexpr uint32_t kRows = 128;               // rows of an operand's tile in one CTA
+constexpr uint32_t kRows = 128;               // rows of A, and of a tile, in one CTA
 constexpr uint32_t kEpiWarps = 8;
 constexpr uint32_t kBoxBytes = 32 * 64;       // 32 rows x 32 columns
 constexpr uint32_t kStagingBytes = kEpiWarps * kBoxBytes;
@@ -45,12 +47,13 @@ constexpr uint32_t kBarBytes = 512;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr uint32_t kSmemBytes = kRingBytes + kStagingBytes + kBarBytes + 1024;
 
-// CG CTAs per tile; HALVES accumulators of BN columns side by side in a tile.
-template <int CG, int BN_, int HALVES>
+// CG CTAs per tile, HALVES accumulators of BN columns side by side in a tile. Stages of 64 k
+// where operands are wide (16 KB requests, 6 of them under way: 730 -> 711 us for 8192 x 4096
+// x 16384), of 128 k (32 KB) where smaller requests would cost more than their bytes.
+template <int CG, int BN, int HALVES>
 struct Shape {
-  static constexpr uint32_t BN = BN_;
-  static constexpr uint32_t kDepth = HALVES == 2 ? 64 : 128;  // k of a stage
-  static constexpr uint32_t kBRows = BN / CG;                 // rows of B of one CTA, per half
+  static constexpr uint32_t kDepth = BN == 256 ? 64 : 128;
+  static constexpr uint32_t kBRows = BN / CG;
   static constexpr uint32_t kABytes = kRows * kDepth * 2, kBBytes = kBRows * kDepth * 2;
   static constexpr uint32_t kStageBytes = kABytes + HALVES * kBBytes;
   static constexpr uint32_t kStages = kRingBytes / kStageBytes;
@@ -67,16 +70,16 @@ constexpr uint32_t kSkew = 2;
 
 struct Problem {
   uint32_t m, n, tiles_m, tiles_n, tile0;
+  uint32_t kb, kb_seg;      // blocks of kDepth of a tile, of a segment
+  uint32_t map;             // its first operands in a[], b[]
+  uint32_t a_mn, b_mn;      // operands stored with m / n contiguous
+  uint32_t a_3d, b_3d;      // one request per operand and stage
 };
 
 struct alignas(64) Params {
-  CUtensorMap a[3], b[3];
-  Problem prob[3];
-  uint32_t problems, tiles;
-  uint32_t kb_seg, kb;         // 128-deep blocks of a segment, of a tile
-  uint32_t a_mn, b_mn;         // operands stored with m / n contiguous
-  uint32_t a_3d, b_3d;         // one request per operand and stage
-  uint32_t group_m;
+  CUtensorMap a[kMaxOperands], b[kMaxOperands];
+  Problem prob[kMaxProblems];
+  uint32_t problems, tiles, group_m;
   uint32_t parts;              // of each tile's depth, a cluster's CTAs or pairs
   uint32_t dyn;                // tiles come from the queue
   Finish fin;
@@ -87,8 +90,22 @@ struct alignas(64) Params {
 };
 
 struct Unit {
-  uint32_t tile, kb0, kb1;
+  uint32_t prob, tm, tn, kb0, kb1;
 };
+
+// Where a tile stands. Grouped raster: runs of group_m tiles along m sweep across n, so that
+// CTAs that run together share panels of A and B in the L2.
+__device__ __forceinline__ Unit unit_of(const Params& p, uint32_t tile) {
+  Unit u{};
+  while (u.prob + 1 < p.problems && tile >= p.prob[u.prob + 1].tile0) ++u.prob;
+  const Problem& q = p.prob[u.prob];
+  const uint32_t t = tile - q.tile0, per_group = p.group_m * q.tiles_n, g = t / per_group;
+  const uint32_t m0 = g * p.group_m, gm = min(p.group_m, q.tiles_m - m0), i = t - g * per_group;
+  u.tm = m0 + i % gm;
+  u.tn = i / gm;
+  u.kb1 = q.kb;
+  return u;
+}
 
 // The walk of every role of a CTA: a part of one tile, or whole tiles.
 struct Walk {
@@ -97,39 +114,22 @@ struct Walk {
     unit = next_tile = blockIdx.x / cg;
     units = gridDim.x / cg;
   }
-  __device__ __forceinline__ static void whole(const Params& p, Unit& u, uint32_t tile) {
-    u = {tile, 0, p.kb};
-  }
   __device__ __forceinline__ bool next(const Params& p, Unit& u) {
     if (p.parts > 1) {
       if (next_tile != unit) return false;
-      const uint32_t part = unit % p.parts;
-      u = {unit / p.parts, p.kb * part / p.parts, p.kb * (part + 1) / p.parts};
       next_tile = unit + 1;
+      const uint32_t part = unit % p.parts;
+      u = unit_of(p, unit / p.parts);
+      u.kb0 = u.kb1 * part / p.parts;
+      u.kb1 = u.kb1 * (part + 1) / p.parts;
       return true;
     }
     if (p.dyn || next_tile >= p.tiles) return false;
-    whole(p, u, next_tile);
+    u = unit_of(p, next_tile);
     next_tile += units;
     return true;
   }
 };
-
-struct Place {
-  uint32_t prob, tm, tn;
-};
-// Grouped raster: runs of group_m tiles along m sweep across n, so that CTAs that run
-// together share panels of A and B in the L2.
-__device__ __forceinline__ Place place_of(const Params& p, uint32_t tile) {
-  Place r{0, 0, 0};
-  while (r.prob + 1 < p.problems && tile >= p.prob[r.prob + 1].tile0) ++r.prob;
-  const Problem& q = p.prob[r.prob];
-  const uint32_t t = tile - q.tile0, per_group = p.group_m * q.tiles_n, g = t / per_group;
-  const uint32_t m0 = g * p.group_m, gm = min(p.group_m, q.tiles_m - m0), i = t - g * per_group;
-  r.tm = m0 + i % gm;
-  r.tn = i / gm;
-  return r;
-}
 
 // A warp's box in shared memory: 32 rows of 64 bytes (32 columns), the 16-byte pieces of a
 // row swizzled so that neither 8 lanes of a row each nor 8 rows of 4 lanes conflict.
@@ -178,12 +178,16 @@ __device__ __forceinline__ void load_chunk(const Params& p, int which, uint32_t 
     }
     return;
   }
+  const uint32_t rows = M - row0;
+  const uint16_t* at = base + int64_t(row0) * ld + col + lane;
+  uint16_t v[32];  // all 32 rows under way together
+#pragma unroll
+  for (uint32_t r = 0; r < 32; ++r)
+    v[r] = r < rows && col + lane < N ? at[int64_t(r) * ld] : uint16_t(0);
   __syncwarp();
-  const uint32_t rows = min(32u, M - row0);
-#pragma unroll 8
-  for (uint32_t r = 0; r < rows; ++r)
-    *reinterpret_cast<uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2) =
-        col + lane < N ? base[int64_t(row0 + r) * ld + col + lane] : uint16_t(0);
+#pragma unroll
+  for (uint32_t r = 0; r < 32; ++r)
+    *reinterpret_cast<uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2) = v[r];
   __syncwarp();
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
@@ -224,11 +228,13 @@ __device__ __forceinline__ void store_packed(const Params& p, int which, uint32_
         make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
   __syncwarp();
   if (col + lane < N) {
-    const uint32_t rows = min(32u, M - row0);
-#pragma unroll 8
-    for (uint32_t r = 0; r < rows; ++r)
-      base[int64_t(row0 + r) * ld + col + lane] =
-          *reinterpret_cast<const uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2);
+    const uint32_t rows = M - row0;
+    uint16_t* at = base + int64_t(row0) * ld + col + lane;
+#pragma unroll
+    for (uint32_t r = 0; r < 32; ++r)
+      if (r < rows)
+        at[int64_t(r) * ld] =
+            *reinterpret_cast<const uint16_t*>(box + box_offset(r, lane / 8) + lane % 8 * 2);
   }
 }
 template <class T>
@@ -264,20 +270,18 @@ __device__ __forceinline__ void add_bias(const Params& p, uint32_t col, uint32_t
   }
 }
 
-template <class T, int EPI, int CG, int BN_, int HALVES>
-__global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
+template <class T, int EPI, int CG, int BN, int HALVES>
+__global__ void __launch_bounds__((Shape<CG, BN, HALVES>::kThreads), 1)
     ffn_product_kernel(const __grid_constant__ Params p) {
-  using S = Shape<CG, BN_, HALVES>;
-  constexpr uint32_t BN = BN_;  // columns of one accumulator
-  constexpr uint32_t kDepth = S::kDepth, kStageBytes = S::kStageBytes, kStages = S::kStages;
-  constexpr uint32_t kABytes = S::kABytes, kBBytes = S::kBBytes, kBRows = S::kBRows;
-  constexpr uint32_t kTmemCols = 2 * BN;
+  using S = Shape<CG, BN, HALVES>;
+  constexpr uint32_t kDepth = S::kDepth, kABytes = S::kABytes, kBBytes = S::kBBytes;
+  constexpr uint32_t kBRows = S::kBRows, kStages = S::kStages, kStageBytes = S::kStageBytes;
   const uint32_t cta = CG == 2 || p.parts > 1 ? cluster_ctarank() : 0u;  // in the cluster
   const uint32_t rank = CG == 2 ? cta & 1u : 0u;                         // in the pair
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* staging = ring + kStages * kStageBytes;
+  uint8_t* staging = ring + kRingBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(staging + kStagingBytes);
   uint64_t* full = bars;
   uint64_t* empty = full + kStages;
@@ -295,6 +299,8 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.a[0]);
+    tma_prefetch_desc(&p.b[0]);
     for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -312,16 +318,14 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
     }
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&p.a[0]);
-    tma_prefetch_desc(&p.b[0]);
   }
   if (CG == 2) cluster_sync();  // the peer uses this CTA's barriers
   if (warp == 1) {
     if constexpr (CG == 2) {
-      tmem_alloc_pair(tmem_slot, kTmemCols);
+      tmem_alloc_pair(tmem_slot, 2 * BN);
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(tmem_slot, kTmemCols);
+      tmem_alloc(tmem_slot, 2 * BN);
       tmem_relinquish();
     }
   }
@@ -329,6 +333,19 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+
+  // A warp's next unit from the queue (MMA and epilogue warps); false at the end, or where a
+  // wait gave up.
+  auto pop_unit = [&](Unit& u, uint32_t who) -> bool {
+    if (!p.dyn) return false;
+    uint32_t t, slot;
+    const bool got = tq_pop(tq, t, slot, abort_flag, p.status);
+    if (__all_sync(~0u, got) == 0) return false;
+    if (lane == 0) tq_release(tq, slot, who);
+    if (t >= p.tiles) return false;
+    u = unit_of(p, t);
+    return true;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -389,14 +406,14 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
           tq_release(tq, slot, rank);
         }
         if (t >= p.tiles) return false;
-        Walk::whole(p, uu, t);
+        uu = unit_of(p, t);
         return true;
       };
       while (ok && next_unit(u)) {
-        const Place at = place_of(p, u.tile);
-        const uint32_t m0 = (at.tm * CG + rank) * kRows;
+        const Problem& q = p.prob[u.prob];
+        const uint32_t m0 = (u.tm * CG + rank) * kRows;
         const uint32_t n0 =
-            EPI == kGated ? at.tn * (BN / 2) : at.tn * (BN * HALVES) + rank * kBRows;
+            EPI == kGated ? u.tn * (BN / 2) : u.tn * (BN * HALVES) + rank * kBRows;
         for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_sleep_wait(&empty[stage], phase ^ 1u, abort_flag, p.status,
                                kWdProducerEmpty)) {
@@ -406,20 +423,20 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
           uint8_t* sa = ring + stage * kStageBytes;
           uint8_t* sb = sa + kABytes;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * kStageBytes);
-          const uint32_t seg = kb / p.kb_seg, k = kb - seg * p.kb_seg, op = at.prob + seg;
-          load(sa, &p.a[op], &full[stage], p.a_mn, p.a_3d, kRows, m0, k);
+          const uint32_t seg = kb / q.kb_seg, k = kb - seg * q.kb_seg, op = q.map + seg;
+          load(sa, &p.a[op], &full[stage], q.a_mn, q.a_3d, kRows, m0, k);
           if constexpr (EPI == kGated && CG == 1) {
-            // 64 rows of the gate's weights, then 64 of the up projection's
+            // half the rows of B are the gate's, then the up projection's
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-              for (uint32_t j = 0; j < 2; ++j)
-                load2(sb + j * (kBBytes / 2) + h * (kBBytes / 4), &p.b[h], &full[stage],
+              for (uint32_t j = 0; j < kDepth / 64; ++j)
+                load2(sb + (j * 2 + h) * (kBRows / 2 * 128), &p.b[h], &full[stage],
                       k * kDepth + 64 * j, n0);
           } else {
 #pragma unroll
             for (uint32_t h = 0; h < HALVES; ++h)
-              load(sb + h * kBBytes, &p.b[EPI == kGated ? rank : op], &full[stage], p.b_mn, p.b_3d,
+              load(sb + h * kBBytes, &p.b[EPI == kGated ? rank : op], &full[stage], q.b_mn, q.b_3d,
                    kBRows, n0 + h * BN, k);
           }
           ++filled;
@@ -442,9 +459,6 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
       auto wait_all = [&](uint64_t* bar, uint32_t parity, unsigned site) {
         return __all_sync(~0u, mbar_sleep_wait(bar, parity, abort_flag, p.status, site)) != 0;
       };
-      // bits 7 and 10: bf16 operands
-      const uint32_t idesc = make_idesc_f16_f32(kRows * CG, BN, p.a_mn != 0, p.b_mn != 0) |
-                             (Pair<T>::kBf16 ? (1u << 7 | 1u << 10) : 0u);
       auto commit_all = [&](uint64_t* bar) {
         if constexpr (CG == 2) {
           const uint32_t a = smem_u32(bar);
@@ -454,12 +468,21 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
           umma_commit(bar);
         }
       };
-      // per 16 k: K-major 32 bytes within the 128-byte rows of a 64-deep block, m / n
-      // contiguous 16 rows of 128 bytes
-      constexpr uint32_t kChunk = kDepth * 128;  // from 64 m or n to the next
-      const uint32_t lbo_a = p.a_mn ? kChunk : 16, lbo_b = p.b_mn ? kChunk : 16;
-      const uint32_t a_step = p.a_mn ? 2048 : 32, a_block = p.a_mn ? 4 * 2048 : kRows * 128;
-      const uint32_t b_step = p.b_mn ? 2048 : 32, b_block = p.b_mn ? 4 * 2048 : kBRows * 128;
+      // Operands of a unit's problem. Per 16 k: K-major 32 bytes within the 128-byte rows of
+      // a 64-deep block, m / n contiguous 16 rows of 128 bytes.
+      uint32_t idesc = 0, lbo_a = 0, lbo_b = 0, a_step = 0, b_step = 0, a_block = 0, b_block = 0;
+      auto use_problem = [&](const Problem& q) {
+        constexpr uint32_t kChunk = kDepth * 128;  // from 64 m or n to the next
+        // bits 7 and 10: bf16 operands
+        idesc = make_idesc_f16_f32(kRows * CG, BN, q.a_mn != 0, q.b_mn != 0) |
+                (Pair<T>::kBf16 ? (1u << 7 | 1u << 10) : 0u);
+        lbo_a = q.a_mn ? kChunk : 16;
+        lbo_b = q.b_mn ? kChunk : 16;
+        a_step = q.a_mn ? 2048 : 32;
+        b_step = q.b_mn ? 2048 : 32;
+        a_block = q.a_mn ? 4 * 2048 : kRows * 128;
+        b_block = q.b_mn ? 4 * 2048 : kBRows * 128;
+      };
       // One stage's products into both halves' accumulators: rows of A that the first half's
       // instruction has fetched stay for the second's.
       auto issue_both = [&](uint32_t stage) {
@@ -495,21 +518,11 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
       Unit u;
       uint32_t stage = 0, phase = 0, i = 0;
       bool ok = true;
-      auto next_unit = [&](Unit& uu) -> bool {
-        if (walk.next(p, uu)) return true;
-        if (!p.dyn) return false;
-        uint32_t t, slot;
-        const bool got = tq_pop(tq, t, slot, abort_flag, p.status);
-        if (__all_sync(~0u, got) == 0) return ok = false;
-        if (lane == 0) tq_release(tq, slot, 0);
-        if (t >= p.tiles) return false;
-        Walk::whole(p, uu, t);
-        return true;
-      };
       auto advance = [&](uint32_t& st, uint32_t& ph) {
         if (++st == kStages) st = 0, ph ^= 1u;
       };
-      while (ok && next_unit(u)) {
+      while (ok && (walk.next(p, u) || pop_unit(u, 0))) {
+        use_problem(p.prob[u.prob]);
         if constexpr (HALVES == 1) {
           const uint32_t buf = i & 1u;
           if (!wait_all(&tempty[buf], ((i >> 1) & 1u) ^ 1u, kWdMmaTmemEmpty)) break;
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
           if (elect_one()) commit_all(&tfull[buf]);
           __syncwarp();
         } else {
-          // The first and the last kSkew stages go through one half's accumulator, then
+          // The first and the last kSkew kStages go through one half's accumulator, then
           // through the other's: while the epilogue reads the first half, products of the
           // second are still under way, and the next tile begins with the first.
           for (uint32_t kb = u.kb0; ok && kb < u.kb1;) {
@@ -608,19 +621,8 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
     walk.init(CG);
     Unit u;
     uint32_t i = 0;
-    auto next_unit = [&](Unit& uu) -> bool {
-      if (walk.next(p, uu)) return true;
-      if (!p.dyn) return false;
-      uint32_t t, slot;
-      const bool got = tq_pop(tq, t, slot, abort_flag, p.status);
-      if (__all_sync(~0u, got) == 0) return false;
-      if (lane == 0) tq_release(tq, slot, rank);
-      if (t >= p.tiles) return false;
-      Walk::whole(p, uu, t);
-      return true;
-    };
     bool ok = true;
-    while (ok && next_unit(u)) {
+    while (ok && (walk.next(p, u) || pop_unit(u, rank))) {
       // Accumulator h of a tile: the tiles alternate between two, or each has both.
       auto accumulator = [&](uint32_t h) { return HALVES == 2 ? h : i & 1u; };
       auto wait_full = [&](uint32_t h) -> bool {
@@ -640,20 +642,22 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
             mbar_arrive(bar);
         }
       };
-      auto taddr = [&](uint32_t h) { return tmem_base + ((q * 32u) << 16) + accumulator(h) * BN; };
+      auto taddr = [&](uint32_t h) {
+        return tmem_base + ((q * 32u) << 16) + accumulator(h) * BN;
+      };
       if constexpr (HALVES == 1) {
         if (p.parts > 1) {
           // a part: its sums to shared memory (the ring is idle once they are complete)
           if (!wait_full(0)) break;
           float4* part = reinterpret_cast<float4*>(ring);
 #pragma unroll 1
-          for (uint32_t c = half * (BN / 64); c < (half + 1) * (BN / 64); ++c) {
+          for (uint32_t c = half; c < BN / 32; c += 2) {
             uint32_t r[32];
             tmem_ld_32x32b_x32(taddr(0) + c * 32, r);
             tmem_ld_wait();
 #pragma unroll
             for (uint32_t j = 0; j < 8; ++j)
-              part[part_index<BN>(row_in_tile, c * 8 + j)] =
+              part[row_in_tile * (BN / 4) + ((c * 8 + j) ^ (row_in_tile & 7))] =
                   make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
                               __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
           }
@@ -662,98 +666,89 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
           continue;
         }
       }
-      const Place at = place_of(p, u.tile);
-      const uint32_t M = p.prob[at.prob].m, N = p.prob[at.prob].n;
-      const uint32_t row0 = (at.tm * CG + rank) * kRows + q * 32;
-      constexpr uint32_t kWide = EPI == kGated ? BN / 2 : BN;  // output columns of an accumulator
-      constexpr uint32_t kChunks = kWide / 64;                 // 32-column chunks of this warp
-      // The epilogue of wide tiles: bias, relu, residual.
-      auto light = [&](float (&v)[32], uint32_t col, const uint32_t (&res)[16],
-                       uint32_t (&out)[16]) {
-        if (p.fin.bias) add_bias<T>(p, col, N, v);
-        if (p.fin.act == FELIX_ACT_RELU) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = activate<FELIX_ACT_RELU>(v[j]);
-        }
+      const uint32_t M = p.prob[u.prob].m;
+      const uint32_t row0 = (u.tm * CG + rank) * kRows + q * 32;
+      if constexpr (HALVES == 2) {
+        // Wide tiles: bias, relu, residual. Both halves are read, finished and rounded before
+        // anything is written: the next tile's products wait for the reads alone. (All CTAs
+        // write at about the same time, 64 KB each at 9 bytes a cycle; written in between,
+        // that took 7000 cycles a half.)
+        constexpr uint32_t kChunks = BN / 64;  // 32-column chunks of this warp in a half
+        const uint32_t N = p.prob[u.prob].n;
+        const uint32_t col0 = u.tn * 2 * BN + half * 32;
+        uint32_t hold[2][kChunks][16];  // the residual, then the results
         if (p.fin.in[0]) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 f = Pair<T>::unpack(res[j]);
-            v[2 * j] += f.x;
-            v[2 * j + 1] += f.y;
-          }
+          for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+            for (uint32_t c = 0; c < kChunks; ++c)
+              if (row0 < M && col0 + h * BN + c * 64 < N)
+                load_chunk(p, 0, row0, col0 + h * BN + c * 64, M, N, box, lane, hold[h][c]);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) out[j] = Pair<T>::pack(v[2 * j], v[2 * j + 1]);
-      };
-      if constexpr (HALVES == 2) {
-        // Both halves are read, finished and rounded before anything is written: the next
-        // tile's products wait for the reads alone. (All CTAs write at about the same time,
-        // 64 KB each at 9 bytes a cycle; written in between, that took 7000 cycles a half.)
-        {
-          uint32_t hold[2][kChunks][16];  // the residual, then the results
-          const uint32_t col0 = at.tn * 2 * BN + half * kChunks * 32;
-          if (p.fin.in[0]) {
+        for (uint32_t h = 0; h < 2; ++h) {
+          if (!wait_full(h)) break;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
+          for (uint32_t c = 0; c < kChunks; ++c) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(taddr(h) + (half + 2 * c) * 32, r);
+            tmem_ld_wait();
+            float v[32];
 #pragma unroll
-              for (uint32_t c = 0; c < kChunks; ++c)
-                if (row0 < M && col0 + h * BN + c * 32 < N)
-                  load_chunk(p, 0, row0, col0 + h * BN + c * 32, M, N, box, lane, hold[h][c]);
-          }
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            if (p.fin.bias) add_bias<T>(p, col0 + h * BN + c * 64, N, v);
+            if (p.fin.act == FELIX_ACT_RELU) {
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            if (!wait_full(h)) break;
-#pragma unroll
-            for (uint32_t c = 0; c < kChunks; ++c) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(taddr(h) + (half * kChunks + c) * 32, r);
-              tmem_ld_wait();
-              float v[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-              light(v, col0 + h * BN + c * 32, hold[h][c], hold[h][c]);
+              for (int j = 0; j < 32; ++j) v[j] = activate<FELIX_ACT_RELU>(v[j]);
             }
-            set_empty(h);
-          }
-          if (ok) {
+            if (p.fin.in[0]) {
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
+              for (int j = 0; j < 16; ++j) {
+                const float2 f = Pair<T>::unpack(hold[h][c][j]);
+                v[2 * j] += f.x;
+                v[2 * j + 1] += f.y;
+              }
+            }
 #pragma unroll
-              for (uint32_t c = 0; c < kChunks; ++c)
-                if (row0 < M && col0 + h * BN + c * 32 < N)
-                  store_packed(p, int(at.prob), row0, col0 + h * BN + c * 32, M, N, box, lane,
-                               hold[h][c]);
+            for (int j = 0; j < 16; ++j) hold[h][c][j] = Pair<T>::pack(v[2 * j], v[2 * j + 1]);
           }
+          set_empty(h);
         }
-        ++i;
-        continue;
-      }
-      if constexpr (HALVES == 1) {
+        if (ok) {
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+            for (uint32_t c = 0; c < kChunks; ++c)
+              if (row0 < M && col0 + h * BN + c * 64 < N)
+                store_packed(p, int(u.prob), row0, col0 + h * BN + c * 64, M, N, box, lane,
+                             hold[h][c]);
+        }
+      } else {
         if (!wait_full(0)) break;
         // columns 32 c .. of the accumulator's sums
-        auto sums = [&](uint32_t c, float (&v)[32]) {
+        auto sums = [&](uint32_t column, float (&v)[32]) {
           uint32_t r[32];
-          tmem_ld_32x32b_x32(taddr(0) + c * 32, r);
+          tmem_ld_32x32b_x32(taddr(0) + column, r);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         };
-        const uint32_t col0 = at.tn * kWide + half * kChunks * 32;
-        // chunks that lie inside; the others hold zeros
-        const uint32_t chunks =
-            row0 < M && col0 < N ? min(kChunks, (N - col0 + 31) / 32) : 0u;
-        if (chunks == 0) set_empty(0);
+        constexpr uint32_t wide = EPI == kGated ? BN / 2 : BN;  // output columns of the tile
+        const uint32_t first = u.tn * wide;
+        const uint32_t N = min(p.prob[u.prob].n, first + wide);
+        // chunks of 32 columns that lie inside, every other one this warp's
+        const uint32_t chunks = row0 < M ? (N - first + 31) / 32 : 0u;
+        if (chunks <= half) set_empty(0);
 #pragma unroll 1
-        for (uint32_t cc = 0; cc < chunks; ++cc) {
-          const uint32_t c = half * kChunks + cc, col = col0 + cc * 32;
+        for (uint32_t c = half; c < chunks; c += 2) {
+          const uint32_t col = first + c * 32;
           // the accumulator is free for the next products once the last chunk is read
-          const bool done = cc + 1 == chunks;
+          const bool done = c + 2 >= chunks;
           float v[32];
           if constexpr (EPI == kLinear) {
             uint32_t res[16];
             if (p.fin.in[0]) load_chunk(p, 0, row0, col, M, N, box, lane, res);
-            sums(c, v);
+            sums(c * 32, v);
             if (done) set_empty(0);
             if (p.fin.bias) add_bias<T>(p, col, N, v);
             if (p.fin.extra >> 1 & 1) store_chunk<T>(p, 1, row0, col, M, N, box, lane, v);
@@ -769,11 +764,11 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
                 v[2 * j + 1] += f.y;
               }
             }
-            store_chunk<T>(p, int(at.prob), row0, col, M, N, box, lane, v);
+            store_chunk<T>(p, int(u.prob), row0, col, M, N, box, lane, v);
           } else if constexpr (EPI == kGated) {
             float up[32];
-            sums(c, v);
-            sums(c + BN / 64, up);
+            sums(c * 32, v);
+            sums(wide + c * 32, up);
             if (done) set_empty(0);
             if (p.fin.extra >> 1 & 1) store_chunk<T>(p, 1, row0, col, M, N, box, lane, v);
             if (p.fin.extra >> 2 & 1) store_chunk<T>(p, 2, row0, col, M, N, box, lane, up);
@@ -786,9 +781,9 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
             uint32_t graw[16], uraw[16];
             load_chunk(p, 0, row0, col, M, N, box, lane, graw);
             load_chunk(p, 1, row0, col, M, N, box, lane, uraw);
-            sums(c, v);
+            sums(c * 32, v);
             if (done) set_empty(0);
-            float du[32], hh[32];
+            float du[32], h[32];
             with_activation(p.fin.act, [&]<int ACT>() {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
@@ -796,17 +791,17 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
                 float a, d;
                 activate_both<ACT>(g.x, a, d);
                 du[2 * j] = v[2 * j] * a;
-                hh[2 * j] = a * up.x;
+                h[2 * j] = a * up.x;
                 v[2 * j] *= up.x * d;
                 activate_both<ACT>(g.y, a, d);
                 du[2 * j + 1] = v[2 * j + 1] * a;
-                hh[2 * j + 1] = a * up.y;
+                h[2 * j + 1] = a * up.y;
                 v[2 * j + 1] *= up.y * d;
               }
             });
             store_chunk<T>(p, 0, row0, col, M, N, box, lane, v);
             store_chunk<T>(p, 1, row0, col, M, N, box, lane, du);
-            store_chunk<T>(p, 2, row0, col, M, N, box, lane, hh);
+            store_chunk<T>(p, 2, row0, col, M, N, box, lane, h);
           }
         }
       }
@@ -819,13 +814,13 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
   tc_fence_before();
   if (p.parts > 1) {
     if constexpr (HALVES == 1) {
-      const Place at = place_of(p, blockIdx.x / (CG * p.parts));
-      const Problem& q = p.prob[at.prob];
-      constexpr uint32_t kWide = EPI == kGated ? BN / 2 : BN;
-      TilePlace place{at.prob, (at.tm * CG + rank) * kRows, at.tn * kWide, 0, 0};
-      place.tokens = place.t0 < q.m ? min(kRows, q.m - place.t0) : 0u;
-      place.features = min(kWide, q.n - place.f0);
-      finish_tile<T, EPI, BN, kRows>(p.fin, place, ring, p.parts, cta / CG, rank, CG, S::kThreads,
+      const Unit u = unit_of(p, blockIdx.x / (CG * p.parts));
+      const Problem& q = p.prob[u.prob];
+      constexpr uint32_t wide = EPI == kGated ? BN / 2 : BN;
+      TilePlace at{u.prob, (u.tm * CG + rank) * kRows, u.tn * wide, 0, 0};
+      at.tokens = at.t0 < q.m ? min(kRows, q.m - at.t0) : 0u;
+      at.features = min(wide, q.n - at.f0);
+      finish_tile<T, EPI, BN, kRows>(p.fin, at, ring, p.parts, cta / CG, rank, CG, S::kThreads,
                                      received, abort_flag, p.status);
     }
   } else if (CG == 2) {
@@ -845,29 +840,25 @@ __global__ void __launch_bounds__((Shape<CG, BN_, HALVES>::kThreads), 1)
     __syncwarp();
     tc_fence_after();
     if constexpr (CG == 2)
-      tmem_dealloc_pair(tmem_base, kTmemCols);
+      tmem_dealloc_pair(tmem_base, 2 * BN);
     else
-      tmem_dealloc(tmem_base, kTmemCols);
+      tmem_dealloc(tmem_base, 2 * BN);
   }
 }
+
+// ------------------------------------------------------------------------------ host
+uint64_t over(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
-  int cg, bn_, halves;
-  uint32_t tiles, kb, depth, units, parts;
-  bool dyn;
+  int cg, halves;
+  uint32_t bn, parts, units, tiles;
   double cost;
   uint32_t bm() const { return kRows * cg; }
-  uint32_t bn(const Product& p) const {
-    return bn_ * halves / (p.epilogue == kGated ? 2 : 1);
+  uint32_t wide(const Product& p) const {
+    return bn * halves / (p.epilogue == kGated ? 2 : 1);
   }
+  uint32_t depth() const { return bn == 256 ? 64 : 128; }
 };
-
-uint64_t count_tiles(const Product& p, uint64_t bm, uint64_t bn) {
-  uint64_t tiles = 0;
-  for (uint32_t i = 0; i < p.problems; ++i)
-    tiles += ((p.m[i] + bm - 1) / bm) * ((p.n[i] + bn - 1) / bn);
-  return tiles;
-}
 
 // Clusters of 1, 2, 4 and 8 CTAs that run at the same time, one CTA per SM.
 struct Clusters {
@@ -893,56 +884,85 @@ const Clusters* clusters_of(DeviceInfo* dev) {
       int n = 0;
       rc = int(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
       all[dev->ordinal].n[i] = uint32_t(n);
+      if (!rc && n == 0) rc = int(cudaErrorInvalidConfiguration);
     }
     return rc;
   });
   return rc ? nullptr : &all[dev->ordinal];
 }
 
+// When the last of `units` is done that take tiles off one queue, problem after problem, in
+// units of blocks of a tile's depth.
+double makespan(const Product& p, const Plan& r, uint32_t units) {
+  // units by the time at which they are free, in whole waves: at most two times differ
+  double early = 0, late = 0;  // `ahead` units are free at `late`, the others at `early`
+  uint32_t ahead = 0;
+  for (uint32_t i = 0; i < p.problems; ++i) {
+    const uint64_t tiles = over(p.m[i], r.bm()) * over(p.n[i], r.wide(p));
+    const double length = double(over(over(p.k[i], r.depth()) * p.segments[i], r.parts));
+    // (those that are late finish as if they had started when the others are done)
+    const uint64_t open = units - ahead;
+    if (ahead && tiles <= open) {
+      late = std::max(late, early + length);
+      ahead = tiles == open ? 0 : ahead + uint32_t(tiles);
+      if (!ahead) early = late;
+      continue;
+    }
+    const uint64_t rest = ahead ? tiles - open : tiles;
+    const double start = ahead ? std::max(late, early + length) : early;
+    const uint64_t waves = rest / units;
+    early = start + waves * length;
+    ahead = uint32_t(rest % units);
+    late = early + length;
+  }
+  return ahead ? late : early;
+}
+
 // Tiles of one shape, each in `parts` parts of its depth, with an estimate of the time in us:
 // waves of 128-deep blocks at the rate that the shape reaches with all SMs at work (one CTA's
-// and the narrow pair's tiles are bound by their operands from the L2, 120 GB/s an SM; 256
-// wide and more by the tensor cores), the start and the last epilogue, and for parts the
-// cluster's barrier, the exchange and the sums. Measured, tokens x depth x features, us, one
-// CTA | pair 128 | 256 | two halves wide: 500 x 4096 x 4096 23.2 | 20.8 | 29.0 | 47.8,
+// and narrow pairs' tiles are bound by their operands from the L2, 120 GB/s an SM; 256 wide
+// and more by the tensor cores), the start and the last epilogue, and for parts the cluster's
+// barrier, the exchange and the sums. Measured, tokens x depth x features, us, one CTA |
+// pair 128 | 256 | two halves wide: 500 x 4096 x 4096 23.2 | 20.8 | 29.0 | 47.8,
 // 500 x 11264 x 4096 54 | 45 | 66 | 111, 2000 x 4096 x 4096 75 | 59 | 51 | 51, 777 x 1024 x
 // 5008 13.7 | 16.9 | 17.6 | 19.7; one CTA's tiles of 128 x 4096 x 4096 in 1, 2, 4 parts 22.7,
 // 17.5, 14.5; pairs' of 500 x 11264 x 4096 in 2 42.
-Plan plan_for(const Product& p, int cg, int bn, int halves, uint32_t parts, uint32_t units) {
+Plan plan_for(const Product& p, int cg, uint32_t bn, int halves, uint32_t parts, uint32_t units) {
   Plan r{};
   r.cg = cg;
-  r.bn_ = bn;
+  r.bn = bn;
   r.halves = halves;
-  r.depth = halves == 2 ? 64 : 128;
-  r.tiles = uint32_t(std::min<uint64_t>(count_tiles(p, r.bm(), r.bn(p)), 0x7fffffff));
-  r.kb = (p.k + r.depth - 1) / r.depth * p.segments;
   r.parts = parts;
+  uint64_t tiles = 0;
+  for (uint32_t i = 0; i < p.problems; ++i) tiles += over(p.m[i], r.bm()) * over(p.n[i], r.wide(p));
+  r.tiles = uint32_t(std::min<uint64_t>(tiles, 0x7fffffff));
   r.units = std::min(units, r.tiles);
-  r.dyn = parts == 1 && r.tiles >= 4 * r.units;
-  const bool one = cg == 1, pair = cg == 2 && bn == 128, wide = halves == 2;
-  double block = one ? 0.555 : pair ? 0.44 : wide ? 1.25 / 2 : 0.66;  // us a block of `depth`
-  if (p.epilogue != kLinear) block *= bn == 128 ? 1.15 : 1.06;  // two values a result
-  const double ends = one ? 5.4 : pair ? 6.7 : wide ? 10.5 : 7.9;
-  const double waves = double((r.tiles + units - 1) / units);
-  r.cost = ends + waves * block * ((r.kb + parts - 1) / parts);
+  double block = cg == 1 ? 0.555 : halves == 2 ? 1.16 : bn == 256 ? 0.63 : 0.44;
+  if (p.epilogue != kLinear) block *= bn == 256 ? 1.06 : 1.15;  // two values a result
+  block *= r.depth() / 128.0;
+  const double ends = cg == 1 ? 5.4 : halves == 2 ? 10.5 : bn == 256 ? 7.9 : 6.7;
+  r.cost = ends + block * makespan(p, r, units);
   if (parts > 1) r.cost += bn == 256 ? 4.5 : 2.5 + 0.3 * parts;
   return r;
 }
 
-Plan make_plan(const Product& p, DeviceInfo* dev, const Clusters& clusters) {
+Plan make_plan(const Product& p, const Clusters& clusters) {
   Plan best = plan_for(p, 2, 256, 1, 1, clusters.n[1]);
   auto consider = [&](const Plan& r) {
     if (r.cost < best.cost) best = r;
   };
   consider(plan_for(p, 2, 128, 1, 1, clusters.n[1]));
   consider(plan_for(p, 1, 128, 1, 1, clusters.n[0]));
-  if (p.epilogue == kLinear && p.act <= FELIX_ACT_RELU && !p.out[1].p)
+  if (p.epilogue == kLinear && p.act <= FELIX_ACT_RELU && (p.problems > 1 || !p.out[1].p))
     consider(plan_for(p, 2, 256, 2, 1, clusters.n[1]));
   // in parts: one wave of clusters of 2, 4 or 8 CTAs, parts of 256 at least
+  uint32_t least = ~0u;
+  for (uint32_t i = 0; i < p.problems; ++i)
+    least = std::min<uint32_t>(least, uint32_t(over(p.k[i], 128)) * p.segments[i]);
   for (int i = 1; i < 4; ++i) {
-    auto split = [&](int cg, int bn) {
+    auto split = [&](int cg, uint32_t bn) {
       const Plan r = plan_for(p, cg, bn, 1, (1u << i) / cg, clusters.n[i]);
-      if (r.parts > 1 && r.tiles <= clusters.n[i] && r.kb >= 2 * r.parts) consider(r);
+      if (r.parts > 1 && r.tiles <= clusters.n[i] && least >= 2 * r.parts) consider(r);
     };
     split(1, 128);
     split(2, 128);
@@ -1001,9 +1021,9 @@ template <class T, int EPI>
 FelixCode launch(DeviceInfo* dev, const Params& p, const Plan& r, cudaStream_t stream) {
   if constexpr (EPI == kLinear)
     if (r.halves == 2) return launch_shape<T, EPI, 2, 256, 2>(dev, p, r, stream);
-  return r.cg == 1      ? launch_shape<T, EPI, 1, 128, 1>(dev, p, r, stream)
-         : r.bn_ == 128 ? launch_shape<T, EPI, 2, 128, 1>(dev, p, r, stream)
-                        : launch_shape<T, EPI, 2, 256, 1>(dev, p, r, stream);
+  return r.cg == 1     ? launch_shape<T, EPI, 1, 128, 1>(dev, p, r, stream)
+         : r.bn == 256 ? launch_shape<T, EPI, 2, 256, 1>(dev, p, r, stream)
+                       : launch_shape<T, EPI, 2, 128, 1>(dev, p, r, stream);
 }
 
 template <class T>
@@ -1016,48 +1036,60 @@ FelixCode launch(DeviceInfo* dev, const Params& p, const Plan& r, int epilogue,
   }
 }
 
+// Whether rows consist of whole vectors of n elements.
+bool whole(uint32_t n, const void* p, int64_t ld, uint32_t rows, uint32_t cols) {
+  return reinterpret_cast<uintptr_t>(p) % (2 * n) == 0 && cols % n == 0 && (rows <= 1 || ld % n == 0);
+}
+
 }  // namespace product
 
 using namespace product;
 
-// Whether rows consist of whole vectors of n elements.
-static bool whole(uint32_t n, const void* p, int64_t ld, uint32_t rows, uint32_t cols) {
-  return reinterpret_cast<uintptr_t>(p) % (2 * n) == 0 && cols % n == 0 && (rows <= 1 || ld % n == 0);
-}
-
 FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cudaStream_t stream) {
-  if (count_tiles(x, kRows, kRows / 2) > 0x3fffffffu)
-    return felix_impl::api_error("feed-forward product: too many tiles");
   const Clusters* clusters = clusters_of(dev);
   if (!clusters) return felix_impl::launch_error(cudaGetLastError(), "feed-forward product: device");
-  const Plan r = make_plan(x, dev, *clusters);
+  const Plan r = make_plan(x, *clusters);
+  if (r.tiles > 0x3fffffffu)
+    return felix_impl::api_error("feed-forward product: too many tiles");
+  const bool gated = x.epilogue == kGated;
   Params p{};
   p.fin = finish_of(x);
-  const uint32_t bm = r.bm(), bn = r.bn(x);
-  const uint32_t operands = std::max(x.segments, x.problems);
-  const bool gated = x.epilogue == kGated;
-  uint32_t tile = 0;
-  p.a_3d = p.b_3d = 1;
+  p.problems = x.problems;
+  p.tiles = r.tiles;
+  p.parts = r.parts;
+  p.group_m = r.halves == 2 ? 12 : r.cg == 2 ? 8 : 16;
+  p.dyn = r.parts == 1 && (x.problems > 1 ? r.tiles > r.units : r.tiles >= 4 * r.units);
+  const uint32_t depth = r.depth(), wide = r.wide(x), b_rows = r.bn / r.cg;
+  uint32_t tile = 0, map = 0;
   for (uint32_t i = 0; i < x.problems; ++i) {
-    p.prob[i] = {x.m[i], x.n[i], (x.m[i] + bm - 1) / bm, (x.n[i] + bn - 1) / bn, tile};
-    tile += p.prob[i].tiles_m * p.prob[i].tiles_n;
-    if ((x.a_mn ? x.m[i] : x.k) % 64) p.a_3d = 0;
-    if ((x.b_mn ? x.n[i] : x.k) % 64) p.b_3d = 0;
+    Problem& q = p.prob[i];
+    q.m = x.m[i];
+    q.n = x.n[i];
+    q.tiles_m = uint32_t(over(q.m, r.bm()));
+    q.tiles_n = uint32_t(over(q.n, wide));
+    q.tile0 = tile;
+    tile += q.tiles_m * q.tiles_n;
+    q.kb_seg = uint32_t(over(x.k[i], depth));
+    q.kb = q.kb_seg * x.segments[i];
+    q.map = map;
+    q.a_mn = x.a_mn[i];
+    q.b_mn = x.b_mn[i];
+    // whole 64-wide blocks (a stage of 64 k is one block of K-major rows; a gated CTA's two
+    // boxes lie side by side)
+    q.a_3d = q.a_mn ? q.m % 64 == 0 : x.k[i] % 64 == 0 && depth == 128;
+    q.b_3d = q.b_mn ? q.n % 64 == 0
+                    : x.k[i] % 64 == 0 && depth == 128 && !(gated && r.cg == 1);
+    const uint32_t operands = gated ? 2 : x.segments[i];
+    for (uint32_t s = 0; s < operands; ++s, ++map) {
+      if (s < x.segments[i] &&
+          encode_operand(&p.a[map], x.a[map], q.a_mn, q.a_3d, q.m, x.k[i], kRows, depth))
+        return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
+      if (encode_operand(&p.b[map], x.b[map], q.b_mn, q.b_3d, q.n, x.k[i],
+                         gated && r.cg == 1 ? b_rows / 2 : b_rows, depth))
+        return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
+    }
   }
-  if (gated && r.cg == 1) p.b_3d = 0;  // boxes of 64 rows, side by side in a stage
-  // a stage of 64 k is one block of K-major rows
-  if (r.depth == 64 && !x.a_mn) p.a_3d = 0;
-  if (r.depth == 64 && !x.b_mn) p.b_3d = 0;
-  for (uint32_t i = 0; i < std::max(operands, gated ? 2u : 1u); ++i) {
-    const uint32_t prob = std::min(i, x.problems - 1);
-    if (i < operands &&
-        encode_operand(&p.a[i], x.a[i], x.a_mn, p.a_3d, x.m[prob], x.k, kRows, r.depth))
-      return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
-    if (encode_operand(&p.b[i], x.b[i], x.b_mn, p.b_3d, x.n[prob], x.k,
-                       gated && r.cg == 1 ? 64 : r.bn_ / r.cg, r.depth))
-      return felix_impl::api_error("feed-forward product: cuTensorMapEncodeTiled failed");
-  }
-  for (uint32_t i = 0; i < 3; ++i) {
+  for (uint32_t i = 0; i < kMaxProblems; ++i) {
     if (!x.out[i].p) continue;
     const uint32_t prob = std::min(i, x.problems - 1), m = x.m[prob], n = x.n[prob];
     p.out_vec |= uint32_t(whole(8, x.out[i].p, x.out[i].ld, m, n)) << i;
@@ -1068,15 +1100,6 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
     p.in_vec |= uint32_t(whole(8, x.in[i].p, x.in[i].ld, x.m[0], x.n[0])) << i;
     p.in_sectors |= uint32_t(whole(16, x.in[i].p, x.in[i].ld, x.m[0], x.n[0])) << i;
   }
-  p.problems = x.problems;
-  p.tiles = r.tiles;
-  p.kb = r.kb;
-  p.kb_seg = r.kb / x.segments;
-  p.a_mn = x.a_mn;
-  p.b_mn = x.b_mn;
-  p.group_m = r.halves == 2 ? 12 : r.cg == 2 ? 8 : 16;
-  p.parts = r.parts;
-  p.dyn = r.dyn;
   p.dyn_counter = static_cast<unsigned*>(workspace) + (felix_impl::kWsMaxCounters - 2);
   p.status = dev->status_word;
   return x.bf16 ? launch<__nv_bfloat16>(dev, p, r, x.epilogue, stream)

@@ -21,15 +21,36 @@ constexpr FelixCode kDone{FELIX_SUCCESS, cudaSuccess};
 
 // ------------------------------------------------------------ element-wise passes
 // Rows that TMA cannot address (odd sizes, addresses or strides, repeated rows) are
-// copied to rows of a multiple of 16 bytes; what lies behind a row is never read.
+// copied to rows of a multiple of 16 bytes; what lies behind a row is never read. A thread
+// writes one vector from the 4 or 5 aligned words that hold it (10 MB: 13 -> 6 us against one
+// element at a time).
 __global__ void __launch_bounds__(256)
     pack_kernel(const uint16_t* src, int64_t src_ld, uint16_t* dst, int64_t dst_ld, uint32_t rows,
                 uint32_t cols) {
-  for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    const uint16_t* s = src + int64_t(r) * src_ld;
-    uint16_t* d = dst + int64_t(r) * dst_ld;
-#pragma unroll 4
-    for (uint32_t c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) d[c] = s[c];
+  const uint32_t vectors = (cols + 7) / 8;
+  const uint64_t all = uint64_t(rows) * vectors, stride = uint64_t(gridDim.x) * 256;
+#pragma unroll 2
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += stride) {
+    const uint32_t r = uint32_t(i / vectors), c = uint32_t(i - uint64_t(r) * vectors) * 8;
+    const uint16_t* s = src + int64_t(r) * src_ld + c;
+    uint32_t v[4];
+    if (c + 8 <= cols) {
+      const uint32_t odd = uint32_t(reinterpret_cast<uintptr_t>(s) >> 1) & 1;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(s - odd);
+      uint32_t x[5];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = w[j];
+      x[4] = odd ? w[4] : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __funnelshift_r(x[j], x[j + 1], 16 * odd);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < cols ? s[2 * j] : 0u, hi = c + 2 * j + 1 < cols ? s[2 * j + 1] : 0u;
+        v[j] = lo | hi << 16;
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + int64_t(r) * dst_ld + c) = make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -39,13 +60,16 @@ struct Elementwise {
   uint16_t *out, *out_up;  // dz, or dg and du
   int64_t out_ld;
   float* sums;  // [row blocks][cols], may be null
+  uint16_t* bias;      // the bias' gradient
+  unsigned* counters;  // one per block of columns, zero before and after
   uint32_t rows, cols, rows_per_block;
   int act;
 };
 
-// dz = grad act'(z) (z null: grad), or gated dg = grad up act'(z), du = grad act(z), and
-// per block of rows the columns' sums of dz for the bias' gradient. One pass: a warp
-// reads 32 V columns of a row, the block's 8 warps take every 8th row.
+// dz = grad act'(z) (z null: grad), or gated dg = grad up act'(z), du = grad act(z), and the
+// columns' sums of dz for the bias' gradient. One pass: a warp reads 32 V columns of a row,
+// the block's 8 warps take every 8th row; the last block of a range of columns adds up all
+// blocks' sums in their order. Bound by memory: 8192 x 16384 with sums 147 us (5.5 TB/s).
 template <class T, int V, bool GATED>
 __global__ void __launch_bounds__(256) elementwise_kernel(const Elementwise p) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -70,7 +94,7 @@ __global__ void __launch_bounds__(256) elementwise_kernel(const Elementwise p) {
             g[i] *= up[i] * d;
           }
           store_values<T, V>(p.out_up + int64_t(r) * p.out_ld + col, du);
-        } else if (ACT != FELIX_ACT_NONE) {
+        } else if constexpr (ACT != FELIX_ACT_NONE) {
           load_values<T, V>(p.z + int64_t(r) * p.z_ld + col, z);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
@@ -87,29 +111,32 @@ __global__ void __launch_bounds__(256) elementwise_kernel(const Elementwise p) {
   if constexpr (!GATED) {
     if (!p.sums) return;
     __shared__ float part[8][32 * V];
+    __shared__ bool last;
 #pragma unroll
     for (int i = 0; i < V; ++i) part[warp][i * 32 + lane] = sum[i];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 32 * V; i += 256) {
+    const uint32_t i = threadIdx.x, c = (blockIdx.x * 32 + i % 32) * V + i / 32;
+    const bool mine = i < 32 * V && c < p.cols;
+    if (mine) {
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) s += part[w][i];
-      const uint32_t c = (blockIdx.x * 32 + i % 32) * V + i / 32;
-      if (c < p.cols) p.sums[size_t(blockIdx.y) * p.cols + c] = s;
+      __stcg(p.sums + size_t(blockIdx.y) * p.cols + c, s);
     }
-  }
-}
-
-// The bias' gradient: the row blocks' sums in their order.
-template <class T>
-__global__ void __launch_bounds__(128)
-    bias_kernel(const float* sums, uint16_t* out, uint32_t blocks, uint32_t cols) {
-  const uint32_t c = blockIdx.x * 128 + threadIdx.x;
-  if (c >= cols) return;
-  float s = 0.f;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last = atomicAdd(&p.counters[blockIdx.x], 1u) == gridDim.y - 1;
+      if (last) p.counters[blockIdx.x] = 0;
+    }
+    __syncthreads();
+    if (!last || !mine) return;
+    __threadfence();
+    float s = 0.f;
 #pragma unroll 8
-  for (uint32_t b = 0; b < blocks; ++b) s += sums[size_t(b) * cols + c];
-  out[c] = Pair<T>::of_float(s);
+    for (uint32_t b = 0; b < gridDim.y; ++b) s += __ldcg(p.sums + size_t(b) * p.cols + c);
+    p.bias[c] = Pair<T>::of_float(s);
+  }
 }
 
 // ------------------------------------------------------------------------ a call
@@ -150,7 +177,8 @@ struct Call {
     if (tma_ok(m.data, m.stride, rows, cols)) return {m.data, m.stride};
     const MutMat c = matrix(rows, cols);
     if (!counting() && ok()) {
-      const dim3 grid(std::min(8u, (cols + 1023) / 1024), std::min(rows, 16384u));
+      const uint64_t vectors = uint64_t(rows) * ((cols + 7) / 8);
+      const uint32_t grid = uint32_t(std::min<uint64_t>((vectors + 255) / 256, 16u * dev->num_sms));
       pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(m.data), m.stride,
                                             static_cast<uint16_t*>(c.p), c.ld, rows, cols);
       check_launch("feed-forward: copy");
@@ -171,6 +199,11 @@ struct Call {
     } else if (ok()) {
       code = product_launch(dev, p, base, stream);
     }
+  }
+  void zero_bytes(void* p, size_t bytes) {
+    if (counting() || !ok()) return;
+    const cudaError_t e = cudaMemsetAsync(p, 0, bytes, stream);
+    if (e != cudaSuccess) code = launch_error(e, "feed-forward: zero");
   }
   void zero(const felix_matrix& m, uint32_t rows, uint32_t cols) {
     if (counting() || !ok() || !m.data) return;
@@ -197,6 +230,49 @@ void elementwise(Call& c, Elementwise& e, uint32_t blocks, bool vec) {
   c.check_launch("feed-forward: element-wise pass");
 }
 
+Mat as_mat(const felix_matrix& m) { return {m.data, m.stride}; }
+MutMat as_mut(const felix_matrix& m) { return {m.data, m.stride}; }
+Mat as_mat(const MutMat& m) { return {m.p, m.ld}; }
+
+// The products of a backward pass, in one launch, deepest first: B always lies with n
+// contiguous, A with k (dx) or m (the weights' gradients).
+struct Backward {
+  struct One {
+    uint32_t m, n, k, segments;
+    bool a_mn;
+    Mat a[2], b[2];
+    MutMat out;
+  };
+  One list[kMaxProblems];
+  uint32_t count = 0;
+  void add(const One& one) { list[count++] = one; }
+  void run(Call& c) {
+    if (!count) return;
+    std::stable_sort(list, list + count, [](const One& x, const One& y) {
+      return uint64_t(x.k) * x.segments > uint64_t(y.k) * y.segments;
+    });
+    Product p;
+    p.bf16 = c.bf16;
+    p.problems = count;
+    uint32_t operand = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+      const One& one = list[i];
+      p.m[i] = one.m;
+      p.n[i] = one.n;
+      p.k[i] = one.k;
+      p.segments[i] = one.segments;
+      p.a_mn[i] = one.a_mn;
+      p.b_mn[i] = true;
+      p.out[i] = one.out;
+      for (uint32_t s = 0; s < one.segments; ++s, ++operand) {
+        p.a[operand] = one.a[s];
+        p.b[operand] = one.b[s];
+      }
+    }
+    c.run(p);
+  }
+};
+
 // dz and the bias' gradient; returns dz as the products read it.
 Mat linear_gradient(Call& c, const felix_linear_args& a) {
   const uint32_t T = a.tokens, N = a.out_features;
@@ -205,12 +281,23 @@ Mat linear_gradient(Call& c, const felix_linear_args& a) {
                     (acts || !tma_ok(a.grad.data, a.grad.stride, T, N));
   MutMat dz;
   if (copy) dz = c.matrix(T, N);
-  // as many blocks of rows as fill the device twice, of 64 rows at least
-  const uint32_t columns = (N + 255) / 256, sms = uint32_t(c.dev->num_sms);
+  const bool vec = vectors({as_mat(a.grad), {acts ? a.pre.data : nullptr, a.pre.stride}}, T, N);
+  // blocks of rows for some 8 CTAs per SM, of 16 rows at least (two a warp)
+  const uint32_t columns = (N + (vec ? 255 : 31)) / (vec ? 256 : 32), sms = uint32_t(c.dev->num_sms);
   const uint32_t want = std::max(1u, 16 * sms / columns);
-  const uint32_t per = std::max(64u, ((T + want - 1) / want + 7) / 8 * 8);
+  const uint32_t per = std::max(16u, ((T + want - 1) / want + 7) / 8 * 8);
   const uint32_t blocks = (T + per - 1) / per;
-  float* sums = a.dbias ? static_cast<float*>(c.take(size_t(blocks) * N * 4)) : nullptr;
+  float* sums = nullptr;
+  unsigned* counters = nullptr;
+  if (a.dbias) {
+    sums = static_cast<float*>(c.take(size_t(blocks) * N * 4));
+    // in front of the scratch, or of their own where there are very many columns
+    c.tiled = true;
+    counters = static_cast<unsigned*>(columns <= felix_impl::kWsMaxCounters - 2
+                                          ? c.base
+                                          : c.take(size_t(columns) * 4));
+    if (columns > felix_impl::kWsMaxCounters - 2) c.zero_bytes(counters, size_t(columns) * 4);
+  }
   if (!c.counting() && c.ok() && (copy || a.dbias)) {
     Elementwise e{};
     e.grad = static_cast<const uint16_t*>(a.grad.data);
@@ -220,34 +307,23 @@ Mat linear_gradient(Call& c, const felix_linear_args& a) {
     e.out = static_cast<uint16_t*>(dz.p);
     e.out_ld = dz.ld;
     e.sums = sums;
+    e.bias = static_cast<uint16_t*>(a.dbias);
+    e.counters = counters;
     e.rows = T;
     e.cols = N;
     e.rows_per_block = per;
     e.act = a.activation;
-    const bool vec = vectors({{e.grad, e.grad_ld}, {acts ? e.z : nullptr, e.z_ld}}, T, N);
     c.bf16 ? elementwise<__nv_bfloat16, false>(c, e, blocks, vec)
            : elementwise<__half, false>(c, e, blocks, vec);
-    if (a.dbias && c.ok()) {
-      uint16_t* out = static_cast<uint16_t*>(a.dbias);
-      if (c.bf16)
-        bias_kernel<__nv_bfloat16><<<(N + 127) / 128, 128, 0, c.stream>>>(sums, out, blocks, N);
-      else
-        bias_kernel<__half><<<(N + 127) / 128, 128, 0, c.stream>>>(sums, out, blocks, N);
-      c.check_launch("feed-forward: bias");
-    }
   }
   return copy ? Mat{dz.p, dz.ld} : Mat{a.grad.data, a.grad.stride};
 }
-
-Mat as_mat(const felix_matrix& m) { return {m.data, m.stride}; }
-MutMat as_mut(const felix_matrix& m) { return {m.data, m.stride}; }
-Mat as_mat(const MutMat& m) { return {m.p, m.ld}; }
 
 void linear(Call& c, const felix_linear_args& a) {
   if (!a.tokens) return;
   Product p;
   p.bf16 = c.bf16;
-  p.k = a.in_features;
+  p.k[0] = a.in_features;
   p.m[0] = a.tokens;
   p.n[0] = a.out_features;
   p.a[0] = c.operand(p, a.x, a.tokens, a.in_features);
@@ -268,30 +344,12 @@ void linear_bwd(Call& c, const felix_linear_args& a) {
     return;
   }
   const Mat dz = linear_gradient(c, a);
-  if (a.dx.data) {
-    Product p;
-    p.bf16 = c.bf16;
-    p.k = N;
-    p.m[0] = T;
-    p.n[0] = K;
-    p.a[0] = dz;
-    p.b[0] = c.addressable(a.weight, N, K);
-    p.b_mn = true;
-    p.out[0] = as_mut(a.dx);
-    c.run(p);
-  }
-  if (a.dweight.data) {
-    Product p;
-    p.bf16 = c.bf16;
-    p.k = T;
-    p.m[0] = N;
-    p.n[0] = K;
-    p.a[0] = dz;
-    p.b[0] = c.addressable(a.x, T, K);
-    p.a_mn = p.b_mn = true;
-    p.out[0] = as_mut(a.dweight);
-    c.run(p);
-  }
+  Backward all;
+  if (a.dx.data)
+    all.add({T, K, N, 1, false, {dz}, {c.addressable(a.weight, N, K)}, as_mut(a.dx)});
+  if (a.dweight.data)
+    all.add({N, K, T, 1, true, {dz}, {c.addressable(a.x, T, K)}, as_mut(a.dweight)});
+  all.run(c);
 }
 
 // h = act(x Wg^T) (x Wu^T), and g, u where they are wanted.
@@ -299,7 +357,7 @@ void gated_product(Call& c, const felix_gated_args& a, const MutMat& h) {
   Product p;
   p.epilogue = kGated;
   p.bf16 = c.bf16;
-  p.k = a.features;
+  p.k[0] = a.features;
   p.m[0] = a.tokens;
   p.n[0] = a.hidden;
   p.a[0] = c.operand(p, a.x, a.tokens, a.features);
@@ -322,7 +380,7 @@ void gated_ffn(Call& c, const felix_gated_args& a) {
   gated_product(c, a, h);
   Product p;
   p.bf16 = c.bf16;
-  p.k = a.hidden;
+  p.k[0] = a.hidden;
   p.m[0] = a.tokens;
   p.n[0] = a.features;
   p.a[0] = as_mat(h);
@@ -336,41 +394,17 @@ void gated_ffn(Call& c, const felix_gated_args& a) {
 void gated_products(Call& c, const felix_gated_args& a, const MutMat& dg, const MutMat& du,
                     const Mat& grad, const MutMat& h) {
   const uint32_t T = a.tokens, K = a.features, F = a.hidden;
-  if (a.dx.data) {
-    Product p;
-    p.bf16 = c.bf16;
-    p.k = F;
-    p.segments = 2;
-    p.m[0] = T;
-    p.n[0] = K;
-    p.a[0] = as_mat(dg);
-    p.a[1] = as_mat(du);
-    p.b[0] = c.addressable(a.w_gate, F, K);
-    p.b[1] = c.addressable(a.w_up, F, K);
-    p.b_mn = true;
-    p.out[0] = as_mut(a.dx);
-    c.run(p);
-  }
-  // three products of one depth, in one launch
-  Product p;
-  p.bf16 = c.bf16;
-  p.k = T;
-  p.a_mn = p.b_mn = true;
-  p.problems = 0;
-  auto add = [&](const Mat& x, const Mat& y, uint32_t m, uint32_t n, const felix_matrix& out) {
-    p.a[p.problems] = x;
-    p.b[p.problems] = y;
-    p.m[p.problems] = m;
-    p.n[p.problems] = n;
-    p.out[p.problems++] = as_mut(out);
-  };
+  Backward all;
+  if (a.dx.data)
+    all.add({T, K, F, 2, false, {as_mat(dg), as_mat(du)},
+             {c.addressable(a.w_gate, F, K), c.addressable(a.w_up, F, K)}, as_mut(a.dx)});
   if (a.dw_gate.data || a.dw_up.data) {
     const Mat x = c.addressable(a.x, T, K);
-    if (a.dw_gate.data) add(as_mat(dg), x, F, K, a.dw_gate);
-    if (a.dw_up.data) add(as_mat(du), x, F, K, a.dw_up);
+    if (a.dw_gate.data) all.add({F, K, T, 1, true, {as_mat(dg)}, {x}, as_mut(a.dw_gate)});
+    if (a.dw_up.data) all.add({F, K, T, 1, true, {as_mat(du)}, {x}, as_mut(a.dw_up)});
   }
-  if (a.dw_down.data) add(grad, as_mat(h), K, F, a.dw_down);
-  if (p.problems) c.run(p);
+  if (a.dw_down.data) all.add({K, F, T, 1, true, {grad}, {as_mat(h)}, as_mut(a.dw_down)});
+  all.run(c);
 }
 
 void no_tokens(Call& c, const felix_gated_args& a) {
@@ -414,12 +448,12 @@ void gated_ffn_bwd(Call& c, const felix_gated_args& a) {
   Product p;
   p.epilogue = kDGated;
   p.bf16 = c.bf16;
-  p.k = K;
+  p.k[0] = K;
   p.m[0] = T;
   p.n[0] = F;
   p.a[0] = grad;
   p.b[0] = c.addressable(a.w_down, K, F);
-  p.b_mn = true;
+  p.b_mn[0] = true;
   p.in[0] = as_mat(a.gate);
   p.in[1] = as_mat(a.up);
   p.out[0] = dg;
