@@ -3,9 +3,9 @@
 //
 // Roles are swapped: the tensor core's 128 rows are 128 rows of W (gated: 64 of the gate's and
 // the same 64 of the up projection's), its columns 32 or 64 tokens, so that nearly all of a
-// stage is what has to be read. A tile's depth is cut into parts over a cluster until there
-// are about two CTAs per SM (two small rings hide each other's ends; one CTA with a deeper
-// ring where there are fewer). Each CTA leaves its fp32 part in its own shared memory as
+// stage is what has to be read. Where there are fewer tiles than SMs, their depth is cut into
+// parts over clusters; where there are more, two CTAs with smaller rings share an SM and hide
+// each other's ends. Each CTA leaves its fp32 part in its own shared memory as
 // [token][feature]; after a cluster barrier each takes a share of the tile, adds the parts
 // in their order and finishes it (ffn_finish.cuh).
 #include <cuda.h>
@@ -239,11 +239,12 @@ FelixCode narrow_launch(DeviceInfo* dev, const Product& x, cudaStream_t stream) 
   p.tiles_t = (p.tokens + bn - 1) / bn;
   const uint32_t tiles = (p.features + wide - 1) / wide * p.tiles_t;
   p.kb = (x.k[0] + kDepth - 1) / kDepth;
-  // Parts of 256 k at least. Measured with 24 tokens, 4096 deep, us: 32 tiles in 2, 4, 8 parts
-  // 15.5, 11.6, 13.2; 128 tiles in 1, 2, 4 28.5, 26.2, 31.6; 176 (gated) in 1, 2 36.9, 41.3.
+  // Parts of 256 k at least, one CTA per SM at most. Measured, tokens x depth x features in 1,
+  // 2, 4, 8 parts, us: 24 x 4096 x 4096 17.0, 12.2, 10.6, 11.1; 40 x 8192 x 1024 31.4, 19.2,
+  // 12.8, 9.8; 64 x 8192 x 8192 33.6, 28.1, 27.3, 33.6; 24 x 4096 x 16384 26.2, 26.2, 29.9, 35.4;
+  // gated 40 x 2048 x 5632 12.9, 14.8, 17.7, 22.9.
   p.parts = 1;
-  while (p.parts < 8 && tiles * p.parts * 2 <= 2 * uint32_t(dev->num_sms) &&
-         p.kb >= 4 * p.parts && (p.parts < 4 || tiles * p.parts * 2 <= uint32_t(dev->num_sms)))
+  while (p.parts < 8 && tiles * p.parts * 2 <= uint32_t(dev->num_sms) && p.kb >= 4 * p.parts)
     p.parts *= 2;
   p.whole = x.k[0] % 64 == 0;
   int rc = 0;

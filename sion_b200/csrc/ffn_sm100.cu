@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) elementwise_kernel(const Elementwise p) {
     if (!last || !mine) return;
     __threadfence();
     float s = 0.f;
-#pragma unroll 8
+#pragma unroll 16
     for (uint32_t b = 0; b < gridDim.y; ++b) s += __ldcg(p.sums + size_t(b) * p.cols + c);
     p.bias[c] = Pair<T>::of_float(s);
   }
@@ -282,10 +282,11 @@ Mat linear_gradient(Call& c, const felix_linear_args& a) {
   MutMat dz;
   if (copy) dz = c.matrix(T, N);
   const bool vec = vectors({as_mat(a.grad), {acts ? a.pre.data : nullptr, a.pre.stride}}, T, N);
-  // blocks of rows for some 8 CTAs per SM, of 16 rows at least (two a warp)
+  // blocks of rows for some 16 CTAs per SM, of 32 rows at least: the last one adds up all
+  // blocks' sums, 16 at a time
   const uint32_t columns = (N + (vec ? 255 : 31)) / (vec ? 256 : 32), sms = uint32_t(c.dev->num_sms);
   const uint32_t want = std::max(1u, 16 * sms / columns);
-  const uint32_t per = std::max(16u, ((T + want - 1) / want + 7) / 8 * 8);
+  const uint32_t per = std::max(32u, ((T + want - 1) / want + 7) / 8 * 8);
   const uint32_t blocks = (T + per - 1) / per;
   float* sums = nullptr;
   unsigned* counters = nullptr;
