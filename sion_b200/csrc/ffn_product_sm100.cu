@@ -107,26 +107,28 @@ __device__ __forceinline__ Unit unit_of(const Params& p, uint32_t tile) {
   return u;
 }
 
-// The walk of every role of a CTA: a part of one tile, or whole tiles.
+// The walk of every role of a CTA: a part of one tile, or whole tiles. Every other wave runs
+// backwards: who had one of the first, deepest tiles comes last.
 struct Walk {
-  uint32_t unit, units, next_tile;
+  uint32_t unit, units, wave;
   __device__ __forceinline__ void init(uint32_t cg) {
-    unit = next_tile = blockIdx.x / cg;
+    unit = blockIdx.x / cg;
     units = gridDim.x / cg;
+    wave = 0;
   }
   __device__ __forceinline__ bool next(const Params& p, Unit& u) {
     if (p.parts > 1) {
-      if (next_tile != unit) return false;
-      next_tile = unit + 1;
+      if (wave++) return false;
       const uint32_t part = unit % p.parts;
       u = unit_of(p, unit / p.parts);
       u.kb0 = u.kb1 * part / p.parts;
       u.kb1 = u.kb1 * (part + 1) / p.parts;
       return true;
     }
-    if (p.dyn || next_tile >= p.tiles) return false;
-    u = unit_of(p, next_tile);
-    next_tile += units;
+    const uint32_t tile = wave * units + (wave & 1 ? units - 1 - unit : unit);
+    ++wave;
+    if (p.dyn || tile >= p.tiles) return false;
+    u = unit_of(p, tile);
     return true;
   }
 };
@@ -891,31 +893,51 @@ const Clusters* clusters_of(DeviceInfo* dev) {
   return rc ? nullptr : &all[dev->ordinal];
 }
 
-// When the last of `units` is done that take tiles off one queue, problem after problem, in
-// units of blocks of a tile's depth.
-double makespan(const Product& p, const Plan& r, uint32_t units) {
-  // units by the time at which they are free, in whole waves: at most two times differ
-  double early = 0, late = 0;  // `ahead` units are free at `late`, the others at `early`
-  uint32_t ahead = 0;
+// When the last of `units` is done that take tiles off one queue, problem after problem, each
+// for `block` us per block of its depth (more by `ragged` where operands' rows are) and some
+// more, `least` us at any rate.
+double makespan(const Product& p, const Plan& r, uint32_t units, double block, double least,
+                double ragged) {
+  struct Group {
+    double free;     // when these units are
+    uint64_t units;
+  };
+  Group groups[16] = {{0.0, units}};  // by time; at most two more per problem are open at once
+  uint32_t n = 1;
   for (uint32_t i = 0; i < p.problems; ++i) {
-    const uint64_t tiles = over(p.m[i], r.bm()) * over(p.n[i], r.wide(p));
-    const double length = double(over(over(p.k[i], r.depth()) * p.segments[i], r.parts));
-    // (those that are late finish as if they had started when the others are done)
-    const uint64_t open = units - ahead;
-    if (ahead && tiles <= open) {
-      late = std::max(late, early + length);
-      ahead = tiles == open ? 0 : ahead + uint32_t(tiles);
-      if (!ahead) early = late;
-      continue;
+    uint64_t tiles = over(p.m[i], r.bm()) * over(p.n[i], r.wide(p));
+    // rows of no whole 128-byte lines: two requests for one, each row in two lines
+    const bool ragged_a = (p.a_mn[i] ? p.m[i] : p.k[i]) % 64, ragged_b = (p.b_mn[i] ? p.n[i] : p.k[i]) % 64;
+    const double rows = 1 + ragged / 2 * (int(ragged_a) + int(ragged_b));
+    const double length = std::max(
+        rows * block * double(over(over(p.k[i], r.depth()) * p.segments[i], r.parts)) + 0.3 * least,
+        least);
+    // many waves keep the units' distances: all but the first few and the last go at once
+    if (tiles > 8 * uint64_t(units)) {
+      const uint64_t waves = tiles / units - 4;
+      for (uint32_t j = 0; j < n; ++j) groups[j].free += double(waves) * length;
+      tiles -= waves * units;
     }
-    const uint64_t rest = ahead ? tiles - open : tiles;
-    const double start = ahead ? std::max(late, early + length) : early;
-    const uint64_t waves = rest / units;
-    early = start + waves * length;
-    ahead = uint32_t(rest % units);
-    late = early + length;
+    while (tiles) {
+      const uint64_t take = std::min(tiles, groups[0].units);
+      const double until = groups[0].free + length;
+      tiles -= take;
+      groups[0].units -= take;
+      if (!groups[0].units) std::copy(groups + 1, groups + n--, groups);
+      uint32_t at = n;
+      while (at && groups[at - 1].free > until) --at;
+      if (at && groups[at - 1].free == until) {
+        groups[at - 1].units += take;
+      } else if (n < 16) {
+        std::copy_backward(groups + at, groups + n, groups + n + 1);
+        groups[at] = {until, take};
+        ++n;
+      } else {
+        groups[at ? at - 1 : 0].units += take;
+      }
+    }
   }
-  return ahead ? late : early;
+  return groups[n - 1].free;
 }
 
 // Tiles of one shape, each in `parts` parts of its depth, with an estimate of the time in us:
@@ -940,8 +962,12 @@ Plan plan_for(const Product& p, int cg, uint32_t bn, int halves, uint32_t parts,
   double block = cg == 1 ? 0.555 : halves == 2 ? 1.16 : bn == 256 ? 0.63 : 0.44;
   if (p.epilogue != kLinear) block *= bn == 256 ? 1.06 : 1.15;  // two values a result
   block *= r.depth() / 128.0;
-  const double ends = cg == 1 ? 5.4 : halves == 2 ? 10.5 : bn == 256 ? 7.9 : 6.7;
-  r.cost = ends + block * makespan(p, r, units);
+  // a tile's own: its turn in the queue, its epilogue where that is longer than its products
+  const double least = cg == 1 ? 1.9 : halves == 2 ? 9.0 : bn == 256 ? 5.8 : 3.9;
+  const double ends = cg == 1 ? 4.8 : halves == 2 ? 7.8 : bn == 256 ? 6.2 : 5.5;
+  // 2000 x 4104 x 4096 against 4096 deep: 106, 85, 61, 53 us for 74, 59, 50, 51
+  const double ragged = bn == 128 ? 0.42 : halves == 2 ? 0.05 : 0.2;
+  r.cost = ends + makespan(p, r, units, block, least, ragged);
   if (parts > 1) r.cost += bn == 256 ? 4.5 : 2.5 + 0.3 * parts;
   return r;
 }
@@ -1058,7 +1084,7 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
   p.tiles = r.tiles;
   p.parts = r.parts;
   p.group_m = r.halves == 2 ? 12 : r.cg == 2 ? 8 : 16;
-  p.dyn = r.parts == 1 && (x.problems > 1 ? r.tiles > r.units : r.tiles >= 4 * r.units);
+  p.dyn = r.parts == 1 && r.tiles >= 4 * r.units;
   const uint32_t depth = r.depth(), wide = r.wide(x), b_rows = r.bn / r.cg;
   uint32_t tile = 0, map = 0;
   for (uint32_t i = 0; i < x.problems; ++i) {
