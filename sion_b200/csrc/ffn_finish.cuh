@@ -175,8 +175,8 @@ __device__ __forceinline__ void finish_share(const Finish& p, const TilePlace& a
 // cluster (this one: j = me), and finishes this one's. Every thread of the cluster comes here,
 // after the parts have been written and fence_proxy_async_smem() by whoever wrote. received:
 // a barrier with count 1, in its first phase. Behind `own`, R * W * 4 bytes, there is room for
-// as much again.
-template <class T, int EPI, uint32_t W, uint32_t R>
+// (MAXP - 1) / MAXP as much; parts: 1, 2, 4 or 8, MAXP at most.
+template <class T, int EPI, uint32_t W, uint32_t R, uint32_t MAXP>
 __device__ __forceinline__ void finish_tile(const Finish& p, const TilePlace& at, uint8_t* own,
                                             uint32_t parts, uint32_t me, uint32_t first,
                                             uint32_t step, uint32_t threads, uint64_t* received,
@@ -208,11 +208,15 @@ __device__ __forceinline__ void finish_tile(const Finish& p, const TilePlace& at
     else
       finish_share<T, EPI, W, R, P, 1>(p, at, own, me, threads);
   };
-  switch (parts) {
-    case 1: go.template operator()<1>(); break;
-    case 2: go.template operator()<2>(); break;
-    case 4: go.template operator()<4>(); break;
-    default: go.template operator()<8>(); break;
+  if (parts == 1)
+    go.template operator()<1>();
+  else if (parts == 2)
+    go.template operator()<2>();
+  else if constexpr (MAXP >= 4) {
+    if (parts == 4)
+      go.template operator()<4>();
+    else
+      go.template operator()<8>();
   }
   if (parts > 1) cluster_wait();  // what this CTA sent has arrived
 }

@@ -47,16 +47,19 @@ constexpr uint32_t kBarBytes = 512;
 constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr uint32_t kSmemBytes = kRingBytes + kStagingBytes + kBarBytes + 1024;
 
-// CG CTAs per tile, HALVES accumulators of BN columns side by side in a tile. Stages of 64 k
-// where operands are wide (16 KB requests, 6 of them under way: 730 -> 711 us for 8192 x 4096
-// x 16384), of 128 k (32 KB) where smaller requests would cost more than their bytes.
+// CG CTAs per tile, HALVES accumulators of BN columns side by side in a tile. Stages of 128 k:
+// with stages of 64 k and requests of 16 KB a pair's 256 x 256 tiles ran 2 % faster alone
+// (8192 x 4096 x 16384: 730 -> 711 us), but 3 % slower under the power cap (843 -> 871).
 template <int CG, int BN, int HALVES>
 struct Shape {
-  static constexpr uint32_t kDepth = BN == 256 ? 64 : 128;
+  static constexpr uint32_t kDepth = HALVES == 2 ? 64 : 128;
   static constexpr uint32_t kBRows = BN / CG;
   static constexpr uint32_t kABytes = kRows * kDepth * 2, kBBytes = kBRows * kDepth * 2;
   static constexpr uint32_t kStageBytes = kABytes + HALVES * kBBytes;
   static constexpr uint32_t kStages = kRingBytes / kStageBytes;
+  // a tile's parts: a CTA's own and what it receives of the others' lie in the ring
+  static constexpr uint32_t kMaxParts = BN == 256 ? 2 : 8;
+  static_assert(kRows * BN * 4 + (kMaxParts - 1) * (kRows / kMaxParts) * BN * 4 <= kRingBytes);
   static constexpr uint32_t kFirstEpi = HALVES == 2 ? 4 : 2;  // first epilogue warp
   static constexpr uint32_t kThreads = 32 * (kFirstEpi + kEpiWarps);
 };
@@ -822,7 +825,7 @@ __global__ void __launch_bounds__((Shape<CG, BN, HALVES>::kThreads), 1)
       TilePlace at{u.prob, (u.tm * CG + rank) * kRows, u.tn * wide, 0, 0};
       at.tokens = at.t0 < q.m ? min(kRows, q.m - at.t0) : 0u;
       at.features = min(wide, q.n - at.f0);
-      finish_tile<T, EPI, BN, kRows>(p.fin, at, ring, p.parts, cta / CG, rank, CG, S::kThreads,
+      finish_tile<T, EPI, BN, kRows, S::kMaxParts>(p.fin, at, ring, p.parts, cta / CG, rank, CG, S::kThreads,
                                      received, abort_flag, p.status);
     }
   } else if (CG == 2) {
@@ -859,7 +862,10 @@ struct Plan {
   uint32_t wide(const Product& p) const {
     return bn * halves / (p.epilogue == kGated ? 2 : 1);
   }
-  uint32_t depth() const { return bn == 256 ? 64 : 128; }
+  uint32_t max_parts() const {
+    return bn == 256 ? Shape<2, 256, 1>::kMaxParts : Shape<1, 128, 1>::kMaxParts;
+  }
+  uint32_t depth() const { return halves == 2 ? 64 : 128; }
 };
 
 // Clusters of 1, 2, 4 and 8 CTAs that run at the same time, one CTA per SM.
@@ -988,7 +994,9 @@ Plan make_plan(const Product& p, const Clusters& clusters) {
   for (int i = 1; i < 4; ++i) {
     auto split = [&](int cg, uint32_t bn) {
       const Plan r = plan_for(p, cg, bn, 1, (1u << i) / cg, clusters.n[i]);
-      if (r.parts > 1 && r.tiles <= clusters.n[i] && least >= 2 * r.parts) consider(r);
+      if (r.parts > 1 && r.parts <= r.max_parts() && r.tiles <= clusters.n[i] &&
+          least >= 2 * r.parts)
+        consider(r);
     };
     split(1, 128);
     split(2, 128);

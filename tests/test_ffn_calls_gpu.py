@@ -29,7 +29,9 @@ def watchdog():
 # tiles, pairs in parts, wide tiles, several waves from the queue, columns past the last tile
 SHAPES = [(128, 2048, 4096), (128, 4096, 4096), (100, 8192, 1024), (256, 4096, 4096),
           (500, 8192, 4096), (4096, 512, 8200), (8192, 512, 5120), (9000, 264, 2056),
-          (700, 4096, 130)]
+          (700, 4096, 130),
+          # few tiles and great depth: as many parts as a tile may have
+          (256, 16384, 2048), (250, 16000, 1024), (512, 16384, 512), (130, 20000, 256)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
