@@ -15,6 +15,7 @@
 
 #include "activation.cuh"
 #include "ffn_internal.h"
+#include "sm100_ptx.cuh"
 
 namespace felix_ffn {
 namespace few {
@@ -107,6 +108,8 @@ __global__ void __launch_bounds__(32 * kWarps, GATED ? 3 : 2) few_kernel(const P
       xv[d][h] = load8<VEC, false>(xrow, k + 32 * h, p.k, xthere);
     }
   };
+  felix_sm100::launch_dependents();
+  felix_sm100::wait_for_earlier_launches();
   const uint32_t steps = (p.k + kBlock * kWarps - 1) / (kBlock * kWarps);
 #pragma unroll
   for (int d = 0; d < D; ++d) fetch(d, d);
@@ -156,13 +159,10 @@ __global__ void __launch_bounds__(32 * kWarps, GATED ? 3 : 2) few_kernel(const P
 }
 
 template <class T, bool GATED>
-void launch(const Params& p, bool vec, cudaStream_t stream) {
-  constexpr uint32_t rows = 16;
-  const uint32_t grid = (p.n + rows - 1) / rows;
-  if (vec)
-    few_kernel<T, GATED, true><<<grid, 32 * kWarps, 0, stream>>>(p);
-  else
-    few_kernel<T, GATED, false><<<grid, 32 * kWarps, 0, stream>>>(p);
+cudaError_t launch(const Params& p, bool vec, cudaStream_t stream) {
+  const uint32_t grid = (p.n + 15) / 16;
+  return vec ? launch_behind(few_kernel<T, GATED, true>, grid, 1, 32 * kWarps, 0, 1, stream, p)
+             : launch_behind(few_kernel<T, GATED, false>, grid, 1, 32 * kWarps, 0, 1, stream, p);
 }
 
 }  // namespace few
@@ -192,13 +192,11 @@ FelixCode few_launch(const Product& x, cudaStream_t stream) {
   p.n = x.n[0];
   p.k = x.k[0];
   p.act = x.act;
-  if (gated)
-    x.bf16 ? few::launch<__nv_bfloat16, true>(p, all, stream)
-           : few::launch<__half, true>(p, all, stream);
-  else
-    x.bf16 ? few::launch<__nv_bfloat16, false>(p, all, stream)
-           : few::launch<__half, false>(p, all, stream);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      gated ? x.bf16 ? few::launch<__nv_bfloat16, true>(p, all, stream)
+                     : few::launch<__half, true>(p, all, stream)
+            : x.bf16 ? few::launch<__nv_bfloat16, false>(p, all, stream)
+                     : few::launch<__half, false>(p, all, stream);
   if (e != cudaSuccess) return felix_impl::launch_error(e, "feed-forward: few tokens");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }

@@ -1,5 +1,7 @@
 // Host-side interfaces of the feed-forward operators' translation units.
 #pragma once
+#include <utility>
+
 #include "felix_internal.h"
 
 namespace felix_ffn {
@@ -44,6 +46,31 @@ struct Product {
   const void* bias = nullptr;
   int act = FELIX_ACT_NONE;
 };
+
+// A launch that may be set up while the one before it runs or drains (the kernel waits for
+// that one itself, wait_for_earlier_launches): 2.3 us less for one token x 4096 x 4096, 3.5
+// us for a gated block. The kernels of a few tokens and the element-wise ones let the next
+// launch in from their start; those that fill an SM's shared memory do not (the next
+// launch's CTAs would scatter their clusters: 1031 x 768 x 2312 backward 31 instead of 25 us).
+template <class... K, class... A>
+cudaError_t launch_behind(void (*kernel)(K...), uint32_t grid_x, uint32_t grid_y, uint32_t threads,
+                          uint32_t smem, uint32_t cluster, cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid_x, grid_y);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
 
 // Whether TMA can address a matrix of these rows.
 inline bool tma_ok(const void* p, int64_t ld, uint32_t rows, uint64_t cols) {

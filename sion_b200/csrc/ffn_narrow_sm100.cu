@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_for_earlier_launches();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -193,17 +194,8 @@ FelixCode launch(DeviceInfo* dev, Params& p, uint32_t tiles, cudaStream_t stream
                                     Shape<BN>::bytes(Shape<BN>::kAlone)));
   });
   if (rc) return felix_impl::launch_error(cudaError_t(rc), "feed-forward product: attributes");
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles * p.parts);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<BN>::bytes(p.stages);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {p.parts, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = p.parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  const cudaError_t e = launch_behind(kernel, tiles * p.parts, 1, kThreads,
+                                      Shape<BN>::bytes(p.stages), p.parts, stream, p);
   if (e != cudaSuccess) return felix_impl::launch_error(e, "feed-forward product: launch failed");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }

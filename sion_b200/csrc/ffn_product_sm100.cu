@@ -338,6 +338,7 @@ __global__ void __launch_bounds__((Shape<CG, BN, HALVES>::kThreads), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  wait_for_earlier_launches();
 
   // A warp's next unit from the queue (MMA and epilogue warps); false at the end, or where a
   // wait gave up.
@@ -1036,17 +1037,9 @@ FelixCode launch_shape(DeviceInfo* dev, const Params& p, const Plan& r, cudaStre
     return felix_impl::api_error("feed-forward product: built with another register count than "
                                  "its register split assumes");
   if (rc) return felix_impl::launch_error(cudaError_t(rc), "feed-forward product: attributes");
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(r.units * r.parts * CG);
-  cfg.blockDim = dim3(Shape<CG, BN, HALVES>::kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {CG * r.parts, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = CG * r.parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  const cudaError_t e =
+      launch_behind(kernel, r.units * r.parts * CG, 1, Shape<CG, BN, HALVES>::kThreads, kSmemBytes,
+                    CG * r.parts, stream, p);
   if (e != cudaSuccess) return felix_impl::launch_error(e, "feed-forward product: launch failed");
   return FelixCode{FELIX_SUCCESS, cudaSuccess};
 }

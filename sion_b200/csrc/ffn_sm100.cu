@@ -10,6 +10,7 @@
 #include "activation.cuh"
 #include "ffn_finish.cuh"
 #include "ffn_internal.h"
+#include "sm100_ptx.cuh"
 
 namespace felix_ffn {
 namespace {
@@ -27,6 +28,8 @@ constexpr FelixCode kDone{FELIX_SUCCESS, cudaSuccess};
 __global__ void __launch_bounds__(256)
     pack_kernel(const uint16_t* src, int64_t src_ld, uint16_t* dst, int64_t dst_ld, uint32_t rows,
                 uint32_t cols) {
+  felix_sm100::launch_dependents();
+  felix_sm100::wait_for_earlier_launches();
   const uint32_t vectors = (cols + 7) / 8;
   const uint64_t all = uint64_t(rows) * vectors, stride = uint64_t(gridDim.x) * 256;
 #pragma unroll 2
@@ -72,6 +75,8 @@ struct Elementwise {
 // blocks' sums in their order. Bound by memory: 8192 x 16384 with sums 147 us (5.5 TB/s).
 template <class T, int V, bool GATED>
 __global__ void __launch_bounds__(256) elementwise_kernel(const Elementwise p) {
+  felix_sm100::launch_dependents();
+  felix_sm100::wait_for_earlier_launches();
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t col = (blockIdx.x * 32 + lane) * V;
   const uint32_t r0 = blockIdx.y * p.rows_per_block;
@@ -168,8 +173,7 @@ struct Call {
     const int64_t ld = (int64_t(cols) + 7) / 8 * 8;
     return {take(size_t(rows) * ld * 2), ld};
   }
-  void check_launch(const char* what) {
-    const cudaError_t e = cudaGetLastError();
+  void check(cudaError_t e, const char* what) {
     if (ok() && e != cudaSuccess) code = launch_error(e, what);
   }
   // m itself, or a copy where TMA cannot address it.
@@ -179,9 +183,10 @@ struct Call {
     if (!counting() && ok()) {
       const uint64_t vectors = uint64_t(rows) * ((cols + 7) / 8);
       const uint32_t grid = uint32_t(std::min<uint64_t>((vectors + 255) / 256, 16u * dev->num_sms));
-      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(m.data), m.stride,
-                                            static_cast<uint16_t*>(c.p), c.ld, rows, cols);
-      check_launch("feed-forward: copy");
+      check(launch_behind(pack_kernel, grid, 1, 256, 0, 1, stream,
+                          static_cast<const uint16_t*>(m.data), m.stride,
+                          static_cast<uint16_t*>(c.p), c.ld, rows, cols),
+            "feed-forward: copy");
     }
     return {c.p, c.ld};
   }
@@ -222,12 +227,10 @@ bool vectors(std::initializer_list<Mat> list, uint32_t rows, uint32_t cols) {
 
 template <class T, bool GATED>
 void elementwise(Call& c, Elementwise& e, uint32_t blocks, bool vec) {
-  const dim3 grid((e.cols + (vec ? 255 : 31)) / (vec ? 256 : 32), blocks);
-  if (vec)
-    elementwise_kernel<T, 8, GATED><<<grid, 256, 0, c.stream>>>(e);
-  else
-    elementwise_kernel<T, 1, GATED><<<grid, 256, 0, c.stream>>>(e);
-  c.check_launch("feed-forward: element-wise pass");
+  const auto kernel = vec ? elementwise_kernel<T, 8, GATED> : elementwise_kernel<T, 1, GATED>;
+  c.check(launch_behind(kernel, (e.cols + (vec ? 255 : 31)) / (vec ? 256 : 32), blocks, 256, 0, 1,
+                        c.stream, e),
+          "feed-forward: element-wise pass");
 }
 
 Mat as_mat(const felix_matrix& m) { return {m.data, m.stride}; }

@@ -145,6 +145,19 @@ __device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity,
   }
 }
 
+// ------------------------------------------------- launches that follow one another
+// In a kernel launched with programmatic stream serialization: the next such launch may be
+// set up from here on (once all CTAs have come here), and everything that was launched
+// before is complete and visible after the wait. No memory that another launch writes or
+// reads is touched before it. Not for a kernel that allocates tensor memory: a CTA of the
+// next launch on the same SM could take the columns first and hold them while it waits.
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_earlier_launches() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- cluster
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

@@ -384,3 +384,53 @@ def test_arguments_of_the_binding_stay_as_they_are(S):
     abi.ffn_call("linear", a)
     C.memset(C.byref(a), 255, C.sizeof(a))
     assert torch.equal(y, S.linear(x, w))
+
+
+def test_calls_that_follow_one_another(S):
+    """Each call reads what the one before wrote, into memory that earlier ones read: the same
+    bits whether the calls are apart, follow at once, change streams or are replayed."""
+    dtype = torch.bfloat16
+    K, F = 512, 2304
+    w = [rand(K, K, dtype=dtype, seed=i, scale=K ** -0.5) for i in range(4)]
+    up = [rand(F, K, dtype=dtype, seed=i, scale=K ** -0.5) for i in range(2)]
+    down = rand(K, F, dtype=dtype, seed=5, scale=F ** -0.5)
+    odd = rand(K, K + 1, dtype=dtype, seed=6, scale=K ** -0.5)[:, 1:]  # copied for TMA
+    start = rand(700, K, dtype=dtype, seed=7)
+    other = torch.cuda.Stream()
+
+    def chain(between):
+        kept, a = [], start.clone()
+        for i, n in enumerate([1, 7, 33, 64, 200, 700, 40, 3]):
+            b = S.linear(a[:n], w[i % 4])
+            between()
+            b = S.linear(b, odd, residual=a[:n], activation="gelu")
+            between()
+            b = S.gated_ffn(b, *up, down, residual=b)
+            between()
+            if i % 2:
+                b.mul_(0.5)
+            y, pre = S.linear_save(b, w[1], activation="silu")
+            between()
+            grads = S.linear_backward(y, b, w[1], pre, "silu", bias=True)
+            between()
+            a[:n].copy_(S.linear(grads[0], w[2]))
+            kept += [y, *grads]
+        return [*kept, a]
+
+    def move():
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            start.add_(0)
+        here.wait_stream(other)
+
+    want = chain(torch.cuda.synchronize)
+    assert all(torch.isfinite(t).all() and t.abs().max() > 0 for t in want)
+    for between in (lambda: None, move):
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(want, chain(between)))
+    graph, out = capture(lambda: chain(lambda: None))
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out))
