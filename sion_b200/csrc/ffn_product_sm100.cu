@@ -919,13 +919,13 @@ double makespan(const Product& p, const Plan& r, uint32_t units, double block, d
     const double length = std::max(
         rows * block * double(over(over(p.k[i], r.depth()) * p.segments[i], r.parts)) + 0.3 * least,
         least);
-    // many waves keep the units' distances: all but the first few and the last go at once
-    if (tiles > 8 * uint64_t(units)) {
-      const uint64_t waves = tiles / units - 4;
-      for (uint32_t j = 0; j < n; ++j) groups[j].free += double(waves) * length;
-      tiles -= waves * units;
-    }
     while (tiles) {
+      // many waves of units that are level keep their distances: all but the last few at once
+      if (tiles > 8 * uint64_t(units) && groups[n - 1].free - groups[0].free <= 2 * length) {
+        const uint64_t waves = tiles / units - 4;
+        for (uint32_t j = 0; j < n; ++j) groups[j].free += double(waves) * length;
+        tiles -= waves * units;
+      }
       const uint64_t take = std::min(tiles, groups[0].units);
       const double until = groups[0].free + length;
       tiles -= take;
@@ -1006,6 +1006,51 @@ Plan make_plan(const Product& p, const Clusters& clusters) {
   return best;
 }
 
+// Problems [from, to) of a product of several.
+Product some_of(const Product& x, uint32_t from, uint32_t to) {
+  Product y;
+  y.bf16 = x.bf16;
+  y.problems = to - from;
+  uint32_t first = 0, operand = 0;
+  for (uint32_t i = 0; i < from; ++i) first += x.segments[i];
+  for (uint32_t i = from; i < to; ++i) {
+    const uint32_t j = i - from;
+    y.m[j] = x.m[i];
+    y.n[j] = x.n[i];
+    y.k[j] = x.k[i];
+    y.segments[j] = x.segments[i];
+    y.a_mn[j] = x.a_mn[i];
+    y.b_mn[j] = x.b_mn[i];
+    y.out[j] = x.out[i];
+    for (uint32_t s = 0; s < x.segments[i]; ++s, ++operand) {
+      y.a[operand] = x.a[first + operand];
+      y.b[operand] = x.b[first + operand];
+    }
+  }
+  return y;
+}
+
+// How many of a product's problems, which come deepest first, make the first of two launches;
+// 0: one launch is best. Problems of very different depth have no parts in common: 479 x 128
+// x 10880 backward, dx 21760 deep and the weights' gradients 479, takes 101 us in one launch
+// and 59 in two. Only for a clear gain: one launch reads weights while it writes gradients
+// (20 x 4096 x 11264 63 us against 68 in two).
+uint32_t two_launches(const Product& x, const Clusters& clusters, double one) {
+  auto depth = [&](uint32_t i) { return over(x.k[i], 128) * x.segments[i]; };
+  if (x.problems == 1 || depth(0) < 4 * depth(x.problems - 1)) return 0;
+  uint32_t best = 0;
+  one *= 0.9;
+  for (uint32_t s = 1; s < x.problems; ++s) {
+    const double two = make_plan(some_of(x, 0, s), clusters).cost +
+                       make_plan(some_of(x, s, x.problems), clusters).cost;
+    if (two < one) {
+      one = two;
+      best = s;
+    }
+  }
+  return best;
+}
+
 // Tensor map of an operand: whole 64-wide blocks as a third dimension where its
 // contiguous extent is a multiple of 64, two dimensions otherwise.
 int encode_operand(CUtensorMap* map, const Mat& x, bool mn, bool whole, uint32_t rows, uint32_t k,
@@ -1076,6 +1121,11 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
   const Clusters* clusters = clusters_of(dev);
   if (!clusters) return felix_impl::launch_error(cudaGetLastError(), "feed-forward product: device");
   const Plan r = make_plan(x, *clusters);
+  if (const uint32_t first = two_launches(x, *clusters, r.cost)) {
+    const FelixCode code = product_launch(dev, some_of(x, 0, first), workspace, stream);
+    if (code.type != FELIX_SUCCESS) return code;
+    return product_launch(dev, some_of(x, first, x.problems), workspace, stream);
+  }
   if (r.tiles > 0x3fffffffu)
     return felix_impl::api_error("feed-forward product: too many tiles");
   const bool gated = x.epilogue == kGated;

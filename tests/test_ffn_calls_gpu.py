@@ -72,6 +72,23 @@ def test_backward_shapes(S, T, K, N):
             assert torch.equal(a, again)
 
 
+@pytest.mark.parametrize("T,K,F", [(479, 128, 8192), (70, 64, 4104), (4100, 72, 184)])
+def test_backward_of_very_different_depths(S, T, K, F):
+    # gradients of tokens and of weights of which one sums over far more than the other
+    for dtype in DTYPES:
+        x, wg, wu, wd = gated_inputs(T, K, F, dtype)
+        gate, up = (rand(T, F, dtype=dtype, seed=i) for i in (6, 7))
+        dy = rand(T, K, dtype=dtype, seed=8)
+        got = S.gated_ffn_backward(dy, x, wg, wu, wd, gate, up)
+        for a, want in zip(got, R.ffn_backward(dy, x, wg, wu, wd, gate, up)):
+            R.check(a, want)
+        for a, again in zip(got, S.gated_ffn_backward(dy, x, wg, wu, wd, gate, up)):
+            assert torch.equal(a, again)
+        got = S.linear_backward(gate, x, wg, bias=True)
+        for a, want in zip(got, R.linear_backward(gate, x, wg)):
+            R.check(a, want)
+
+
 # ------------------------------------------------------------------------ layouts
 def layouts(t):
     """The same values in other layouts: rows with room behind them, an odd stride, an odd
