@@ -1121,13 +1121,13 @@ FelixCode product_launch(DeviceInfo* dev, const Product& x, void* workspace, cud
   const Clusters* clusters = clusters_of(dev);
   if (!clusters) return felix_impl::launch_error(cudaGetLastError(), "feed-forward product: device");
   const Plan r = make_plan(x, *clusters);
+  if (r.tiles > 0x3fffffffu)
+    return felix_impl::api_error("feed-forward product: too many tiles");
   if (const uint32_t first = two_launches(x, *clusters, r.cost)) {
     const FelixCode code = product_launch(dev, some_of(x, 0, first), workspace, stream);
     if (code.type != FELIX_SUCCESS) return code;
     return product_launch(dev, some_of(x, first, x.problems), workspace, stream);
   }
-  if (r.tiles > 0x3fffffffu)
-    return felix_impl::api_error("feed-forward product: too many tiles");
   const bool gated = x.epilogue == kGated;
   Params p{};
   p.fin = finish_of(x);

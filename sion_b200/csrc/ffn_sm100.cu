@@ -22,8 +22,9 @@ constexpr FelixCode kDone{FELIX_SUCCESS, cudaSuccess};
 
 // ------------------------------------------------------------ element-wise passes
 // Rows that TMA cannot address (odd sizes, addresses or strides, repeated rows) are
-// copied to rows of a multiple of 16 bytes; what lies behind a row is never read. A thread
-// writes one vector from the 4 or 5 aligned words that hold it (10 MB: 13 -> 6 us against one
+// copied to rows of a multiple of 16 bytes; what lies beside a row is never used. A thread
+// writes one vector from the 4 or 5 aligned words that hold it, each with an element of the
+// row (10 MB: 13 -> 6 us against one
 // element at a time).
 __global__ void __launch_bounds__(256)
     pack_kernel(const uint16_t* src, int64_t src_ld, uint16_t* dst, int64_t dst_ld, uint32_t rows,
@@ -237,7 +238,7 @@ Mat as_mat(const felix_matrix& m) { return {m.data, m.stride}; }
 MutMat as_mut(const felix_matrix& m) { return {m.data, m.stride}; }
 Mat as_mat(const MutMat& m) { return {m.p, m.ld}; }
 
-// The products of a backward pass, in one launch, deepest first: B always lies with n
+// The products of a backward pass, in one launch or two, deepest first: B always lies with n
 // contiguous, A with k (dx) or m (the weights' gradients).
 struct Backward {
   struct One {

@@ -451,3 +451,41 @@ def test_calls_that_follow_one_another(S):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize("T", [2, 40, 300])
+def test_captured_with_branches(S, T):
+    """Calls behind fills, copies, other kernels and joined streams, captured."""
+    dtype, K = torch.bfloat16, 512
+    x = rand(T, K, dtype=dtype, seed=1)
+    w = [rand(K, K, dtype=dtype, seed=i, scale=K ** -0.5) for i in range(3)]
+    side = torch.cuda.Stream()
+
+    def f():
+        here = torch.cuda.current_stream()
+        a = S.linear(x, w[0], activation="silu")
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = torch.zeros_like(a)
+            b = S.linear(b, w[1], residual=a)
+            c = S.linear(b, w[2])
+        d = S.gated_linear(a, w[1], w[2])
+        here.wait_stream(side)
+        e = S.linear(c, w[0], residual=d)
+        y = e.clone()
+        y.zero_()
+        y.copy_(e)
+        y = S.gated_ffn(y, w[0], w[1], w[2], residual=b)
+        for t in (a, b, c):
+            t.record_stream(here)
+        return a, b, c, d, e, y
+
+    want = f()
+    torch.cuda.synchronize()
+    graph, out = capture(f)
+    for _ in range(5):
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
