@@ -9,6 +9,9 @@
 // k, so lane t of a quad takes k 8 t .. 8 t + 7 of 32 as one 16-byte load for two
 // instructions, and x is read the same way. Not tcgen05: its smallest tile is 128 rows,
 // which would leave 32 CTAs for 4096 rows, and W would pass through shared memory.
+//
+// Measured, one token: 4096 x 4096 7.9 us (4.25 TB/s; launch, start and tail of the stream),
+// two projections of 4096 x 11264 29.9 to 31.3 us (6 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>
