@@ -34,7 +34,9 @@ struct Params {
   int act;
 };
 
-// 8 elements of a row from k on; what lies behind the row's end is 0.
+// 8 elements of a row from k on; what lies behind the row's end is 0. Not by read-only loads:
+// the launch before may still write while this kernel lives, and the compiler may move those
+// in front of the wait for it.
 template <bool VEC, bool STREAM>
 __device__ __forceinline__ uint4 load8(const uint16_t* row, uint32_t k, uint32_t K, bool there) {
   uint4 v = make_uint4(0, 0, 0, 0);
@@ -42,16 +44,16 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, uint32_t k, uint32_t
     if (there && k < K) {
       const uint4* p = reinterpret_cast<const uint4*>(row + k);
       if constexpr (STREAM)
-        asm("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-            : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-            : "l"(p));
+        asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(p));
       else
-        v = __ldg(p);
+        v = *p;
     }
   } else if (there) {
     uint32_t e[8];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) e[i] = k + i < K ? __ldg(row + k + i) : 0u;
+    for (uint32_t i = 0; i < 8; ++i) e[i] = k + i < K ? row[k + i] : 0u;
     v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
   }
   return v;

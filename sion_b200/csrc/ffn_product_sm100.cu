@@ -260,7 +260,7 @@ __device__ __forceinline__ void add_bias(const Params& p, uint32_t col, uint32_t
   if (col + 32 <= N && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(b) + j);
+      const uint4 w = reinterpret_cast<const uint4*>(b)[j];
       const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -272,7 +272,7 @@ __device__ __forceinline__ void add_bias(const Params& p, uint32_t col, uint32_t
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (col + i < N) v[i] += Pair<T>::to_float(__ldg(b + i));
+      if (col + i < N) v[i] += Pair<T>::to_float(b[i]);
   }
 }
 

@@ -149,8 +149,10 @@ __device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity,
 // In a kernel launched with programmatic stream serialization: the next such launch may be
 // set up from here on (once all CTAs have come here), and everything that was launched
 // before is complete and visible after the wait. No memory that another launch writes or
-// reads is touched before it. Not for a kernel that allocates tensor memory: a CTA of the
-// next launch on the same SM could take the columns first and hold them while it waits.
+// reads is touched before it, and none of it by read-only loads (ld.global.nc, __ldg), which
+// may be moved in front of it. launch_dependents is not for a kernel that allocates tensor
+// memory: a CTA of the next launch on the same SM could take the columns first and hold them
+// while it waits.
 __device__ __forceinline__ void launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

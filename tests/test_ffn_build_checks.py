@@ -33,3 +33,18 @@ def test_the_sources_assume_the_same_count():
     m = re.search(r"kRegsLaunch = (\d+), kRegsFirst = (\d+), kRegsEpi = (\d+)", text)
     launch, first, epi = map(int, m.groups())
     assert launch == build.FFN_REGS_LAUNCH and 128 * first + 256 * epi <= 384 * launch
+
+
+def test_kernels_that_start_early():
+    """Every kernel waits for the launches before it; none has loads that may be moved in
+    front of the wait, and none that allocates tensor memory lets the next launch in."""
+    for name in ("ffn_sm100.cu", "ffn_product_sm100.cu", "ffn_few_sm100.cu",
+                 "ffn_narrow_sm100.cu", "ffn_finish.cuh", "ffn_internal.h"):
+        with open(os.path.join(build.CSRC, name)) as f:
+            text = f.read()
+        assert not re.search(r"__ldg\(|ld\.global\.nc|__restrict__|<<<", text), name
+        for kernel in text.split("__global__")[1:]:
+            body = kernel[:kernel.index("\n}\n")]
+            assert "wait_for_earlier_launches();" in body, name
+            if "tmem_alloc" in body:
+                assert "launch_dependents" not in body, name
