@@ -1038,10 +1038,10 @@ Product some_of(const Product& x, uint32_t from, uint32_t to) {
 // (20 x 4096 x 11264 63 us against 68 in two).
 uint32_t two_launches(const Product& x, const Clusters& clusters, double one) {
   auto depth = [&](uint32_t i) { return over(x.k[i], 128) * x.segments[i]; };
-  if (x.problems == 1 || depth(0) < 4 * depth(x.problems - 1)) return 0;
   uint32_t best = 0;
   one *= 0.9;
   for (uint32_t s = 1; s < x.problems; ++s) {
+    if (depth(s - 1) < 4 * depth(s)) continue;
     const double two = make_plan(some_of(x, 0, s), clusters).cost +
                        make_plan(some_of(x, s, x.problems), clusters).cost;
     if (two < one) {
