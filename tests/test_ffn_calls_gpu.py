@@ -1,6 +1,9 @@
 """Feed-forward operators on the GPU: layouts, masks of padding, scratch, streams, graphs,
 threads, and the sizes at which the kernels change."""
 import ctypes as C
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -489,3 +492,31 @@ def test_captured_with_branches(S, T):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+FIRST_CALL = """
+import torch, sion_b200 as S
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16() / 16
+x, wg, wu, wd, dy = r({T}, 512), r(1024, 512), r(1024, 512), r(512, 1024), r({T}, 512)
+odd = r(1024, 513)[:, 1:]
+def f():
+    y, g, u = S.gated_ffn_save(x, wg, wu, wd, x)
+    z, pre = S.linear_save(y, odd, activation="gelu")
+    return (y, z, *S.gated_ffn_backward(dy, x, wg, wu, wd, g, u),
+            *S.linear_backward(z, y, odd, pre, "gelu", True))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = f()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, f()))
+"""
+
+
+@pytest.mark.parametrize("T", [1, 300])
+def test_the_first_call_of_a_process_is_captured(T):
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..")
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("{T}", str(T))], cwd=root,
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
