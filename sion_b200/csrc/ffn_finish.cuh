@@ -180,7 +180,7 @@ template <class T, int EPI, uint32_t W, uint32_t R, uint32_t MAXP>
 __device__ __forceinline__ void finish_tile(const Finish& p, const TilePlace& at, uint8_t* own,
                                             uint32_t parts, uint32_t me, uint32_t first,
                                             uint32_t step, uint32_t threads, uint64_t* received,
-                                            volatile int* abort_flag, unsigned* status) {
+                                            unsigned* status) {
   using namespace felix_sm100;
   if (parts > 1) {
     const uint32_t bytes = R / parts * W * 4;
@@ -195,7 +195,10 @@ __device__ __forceinline__ void finish_tile(const Finish& p, const TilePlace& at
       }
     }
     __syncwarp();
-    const bool ok = __all_sync(~0u, mbar_sleep_wait(received, 0, abort_flag, status,
+    // Whoever gave up before comes here too, and the others send to it all the same: their
+    // copies land before it leaves.
+    int none = 0;
+    const bool ok = __all_sync(~0u, mbar_sleep_wait(received, 0, &none, status,
                                                     kWdEpilogueTmemFull)) != 0;
     cluster_arrive();
     if (!ok) return cluster_wait();

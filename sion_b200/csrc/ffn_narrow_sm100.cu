@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
 
   const TilePlace place{0, t0, f0, min(uint32_t(BN), p.tokens - t0), min(kWide, p.features - f0)};
   finish_tile<T, EPI, 128, BN, 8>(p.fin, place, ring, p.parts, rank, 0, 1, kThreads, received,
-                               abort_flag, p.status);
+                                  p.status);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, BN);

@@ -827,8 +827,8 @@ __global__ void __launch_bounds__((Shape<CG, BN, HALVES>::kThreads), 1)
       TilePlace at{u.prob, (u.tm * CG + rank) * kRows, u.tn * wide, 0, 0};
       at.tokens = at.t0 < q.m ? min(kRows, q.m - at.t0) : 0u;
       at.features = min(wide, q.n - at.f0);
-      finish_tile<T, EPI, BN, kRows, S::kMaxParts>(p.fin, at, ring, p.parts, cta / CG, rank, CG, S::kThreads,
-                                     received, abort_flag, p.status);
+      finish_tile<T, EPI, BN, kRows, S::kMaxParts>(p.fin, at, ring, p.parts, cta / CG, rank, CG,
+                                                   S::kThreads, received, p.status);
     }
   } else if (CG == 2) {
     cluster_sync();  // no CTA exits while its peer may still use its memory

@@ -1,0 +1,23 @@
+"""Feed-forward operators without a GPU: what the sources have to hold where it is not provoked
+on a device, and calls that are neither refused for what they do not read nor end the
+process."""
+import os
+import re
+
+from sion_b200 import abi
+
+CSRC = os.path.join(os.path.dirname(abi.__file__), "csrc")
+
+
+def code(name):
+    return re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+
+
+def test_a_cta_waits_for_what_the_others_send_even_after_it_gave_up():
+    # Every CTA of a cluster sends its shares after the barrier, whatever happened before.
+    # The wait for them is bounded by its own time alone: one that ended because of a flag set
+    # earlier would let the CTA exit while copies into its memory are under way.
+    text = code("ffn_finish.cuh")
+    waits = re.findall(r"\bmbar_\w*wait\(([^;]*?)\)", text, re.S)
+    assert len(waits) == 1 and waits[0].startswith("received, 0, &none,") and "abort" not in text
+    assert "int none = 0;" in text
