@@ -11,7 +11,6 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
-#include <string>
 #include <thread>
 #include <tuple>
 #include <utility>
@@ -28,7 +27,9 @@ namespace felix_impl {
 
 namespace {
 thread_local int t_last_cuda = 0;
-thread_local std::string t_last_msg;
+// Memory of its own: errors are recorded, out of entry points that may not throw, where
+// there may be none left. Longer texts are cut off.
+thread_local char t_last_msg[512] = "";
 
 std::mutex g_mu;
 DeviceInfo g_dev[64];
@@ -68,13 +69,13 @@ void load_encode() {
 
 FelixCode api_error(const char* msg, cudaError_t e) {
   t_last_cuda = int(e);
-  t_last_msg = msg ? msg : "";
+  std::snprintf(t_last_msg, sizeof(t_last_msg), "%s", msg ? msg : "");
   return FelixCode{FELIX_API_ERROR, e};
 }
 
 FelixCode launch_error(cudaError_t e, const char* msg) {
   t_last_cuda = int(e);
-  t_last_msg = std::string(msg ? msg : "") + ": " + cudaGetErrorString(e);
+  std::snprintf(t_last_msg, sizeof(t_last_msg), "%s: %s", msg ? msg : "", cudaGetErrorString(e));
   return FelixCode{FELIX_KERNEL_LAUNCH_FAILED, e};
 }
 
@@ -361,7 +362,7 @@ FelixCode watchdog_probe_launch(uint32_t limit_us, cudaStream_t stream) {
 int finish(FelixCode c) {
   if (c.type == FELIX_SUCCESS) {
     t_last_cuda = 0;
-    t_last_msg.clear();
+    t_last_msg[0] = 0;
   }
   return c.type;
 }
@@ -440,7 +441,7 @@ static FelixCode pages_op(const Kv4PagesOp& o, uint32_t page_size, void* stream)
 extern "C" {
 
 int felix_last_cuda_error(void) { return t_last_cuda; }
-const char* felix_last_error_message(void) { return t_last_msg.c_str(); }
+const char* felix_last_error_message(void) { return t_last_msg; }
 const char* felix_version(void) { return "sion-b200 0.1 (sm_100a)"; }
 
 int felix_num_sms(int* count) {
@@ -784,7 +785,8 @@ int felix_watchdog_status(unsigned* code, int clear) {
   if (code) *code = v;
   if (v != 0) {
     t_last_cuda = 0;
-    t_last_msg = "device watchdog: a bounded wait gave up (site " + std::to_string(v) + ")";
+    std::snprintf(t_last_msg, sizeof(t_last_msg),
+                  "device watchdog: a bounded wait gave up (site %u)", v);
     return FELIX_KERNEL_RUNTIME_ERROR;
   }
   return finish(FelixCode{FELIX_SUCCESS, cudaSuccess});

@@ -3,6 +3,7 @@ on a device, and calls that are neither refused for what they do not read nor en
 process."""
 import os
 import re
+import subprocess
 
 from sion_b200 import abi
 
@@ -21,3 +22,14 @@ def test_a_cta_waits_for_what_the_others_send_even_after_it_gave_up():
     waits = re.findall(r"\bmbar_\w*wait\(([^;]*?)\)", text, re.S)
     assert len(waits) == 1 and waits[0].startswith("received, 0, &none,") and "abort" not in text
     assert "int none = 0;" in text
+
+
+def test_refusals_without_memory(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = str(tmp_path / "no_memory_test")
+    r = subprocess.run(["g++", "-std=c++20", "-O1", os.path.join(root, "tests", "cpp", "no_memory_test.cpp"),
+                        f"-I{root}/include", f"-L{root}/sion_b200", "-lfelix_b200",
+                        f"-Wl,-rpath,{root}/sion_b200", "-o", out], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([out], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "all checks passed" in r.stdout, r.stdout + r.stderr
