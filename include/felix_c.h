@@ -363,7 +363,8 @@ typedef struct felix_matrix {
  * activation), each where wanted (not NULL): dx = dz weight, dweight = dz^T x, dbias =
  * the sum of dz's rows. dz is rounded to 16 bits once, as the products read it; dbias
  * sums it in fp32 before that. (The residual's gradient is grad itself.)
- * Fields that a direction does not name are not read.
+ * Fields that a direction does not name are not read, nor what only a gradient needs that
+ * is not wanted.
  */
 typedef struct felix_linear_args {
   uint32_t tokens, in_features, out_features;
@@ -387,6 +388,8 @@ typedef struct felix_linear_args {
  *   dg = dh u act'(g), du = dh act(g), each rounded once;
  * and where wanted dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x,
  * dw_down = grad^T (act(g) u). (The residual's gradient is grad itself.)
+ * Fields are read as in felix_linear_args; felix_gated_linear and its backward pass want
+ * residual and dw_down NULL.
  */
 typedef struct felix_gated_args {
   uint32_t tokens, features, hidden;

@@ -482,7 +482,8 @@ FelixCode check_common(uint32_t tokens, uint32_t in, uint32_t out, int dtype, in
   return kDone;
 }
 
-// An input: null only where it is optional or there are no tokens; rows may repeat.
+// An input that the call reads: null only where it is optional or there are no tokens; rows
+// may repeat. (What a call does not read is not checked.)
 FelixCode check_in(const felix_matrix& m, const char* null_text, bool optional) {
   if (!m.data) return optional ? kDone : api_error(null_text);
   if (reinterpret_cast<uintptr_t>(m.data) & 1)
@@ -522,10 +523,10 @@ FelixCode check_linear(const felix_linear_args* a, bool backward) {
     return kDone;
   }
   FELIX_CHECK(check_in(a->grad, kNull, none));
-  FELIX_CHECK(check_in(a->x, kNull, none || !a->dweight.data));
-  FELIX_CHECK(check_in(a->weight, kNull, none || !a->dx.data));
-  FELIX_CHECK(check_in(a->pre, "feed-forward: the backward pass of an activation needs pre",
-                       none || a->activation == FELIX_ACT_NONE));
+  if (a->dweight.data) FELIX_CHECK(check_in(a->x, kNull, none));
+  if (a->dx.data) FELIX_CHECK(check_in(a->weight, kNull, none));
+  if (a->activation != FELIX_ACT_NONE)
+    FELIX_CHECK(check_in(a->pre, "feed-forward: the backward pass of an activation needs pre", none));
   FELIX_CHECK(check_out(a->dx, T, K, kNull, true));
   FELIX_CHECK(check_out(a->dweight, N, K, kNull, true));
   FELIX_CHECK(check_in({a->dbias, 0}, kNull, true));
@@ -541,7 +542,7 @@ FelixCode check_gated(const felix_gated_args* a, bool ffn, bool backward) {
     FELIX_CHECK(check_in(a->x, kNull, none));
     FELIX_CHECK(check_in(a->w_gate, kNull, none));
     FELIX_CHECK(check_in(a->w_up, kNull, none));
-    FELIX_CHECK(check_in(a->w_down, kNull, none || !ffn));
+    if (ffn) FELIX_CHECK(check_in(a->w_down, kNull, none));
     FELIX_CHECK(check_in(a->residual, kNull, true));
     if (!ffn && a->residual.data)
       return api_error("feed-forward: a gated projection alone has no residual");
@@ -553,10 +554,10 @@ FelixCode check_gated(const felix_gated_args* a, bool ffn, bool backward) {
   FELIX_CHECK(check_in(a->grad, kNull, none));
   FELIX_CHECK(check_in(a->gate, kNull, none));
   FELIX_CHECK(check_in(a->up, kNull, none));
-  FELIX_CHECK(check_in(a->x, kNull, none || (!a->dw_gate.data && !a->dw_up.data)));
-  FELIX_CHECK(check_in(a->w_gate, kNull, none || !a->dx.data));
-  FELIX_CHECK(check_in(a->w_up, kNull, none || !a->dx.data));
-  FELIX_CHECK(check_in(a->w_down, kNull, none || !ffn));
+  if (a->dw_gate.data || a->dw_up.data) FELIX_CHECK(check_in(a->x, kNull, none));
+  if (a->dx.data) FELIX_CHECK(check_in(a->w_gate, kNull, none));
+  if (a->dx.data) FELIX_CHECK(check_in(a->w_up, kNull, none));
+  if (ffn) FELIX_CHECK(check_in(a->w_down, kNull, none));
   FELIX_CHECK(check_out(a->dx, T, K, kNull, true));
   FELIX_CHECK(check_out(a->dw_gate, F, K, kNull, true));
   FELIX_CHECK(check_out(a->dw_up, F, K, kNull, true));
