@@ -133,7 +133,7 @@ __device__ __forceinline__ void finish_values(const Finish& p, uint32_t prob, in
     });
     store_values<T, V>(out(0), v);
     store_values<T, V>(out(1), du);
-    store_values<T, V>(out(2), h);
+    if (p.extra >> 2 & 1) store_values<T, V>(out(2), h);
   }
 }
 

@@ -23,7 +23,8 @@ struct MutMat {
 enum Epilogue {
   kLinear = 0,  // out0 = act(v + bias) + in0, out1 = v + bias
   kGated = 1,   // v = g | u: out0 = act(g) u, out1 = g, out2 = u
-  kDGated = 2   // v = dh, in0 = g, in1 = u: out0 = dh u act'(g), out1 = dh act(g), out2 = act(g) u
+  kDGated = 2   // v = dh, in0 = g, in1 = u: out0 = dh u act'(g), out1 = dh act(g), and, where it
+                // is wanted, out2 = act(g) u
 };
 
 constexpr uint32_t kMaxProblems = 4, kMaxOperands = 5;

@@ -808,7 +808,7 @@ __global__ void __launch_bounds__((Shape<CG, BN, HALVES>::kThreads), 1)
             });
             store_chunk<T>(p, 0, row0, col, M, N, box, lane, v);
             store_chunk<T>(p, 1, row0, col, M, N, box, lane, du);
-            store_chunk<T>(p, 2, row0, col, M, N, box, lane, h);
+            if (p.fin.extra >> 2 & 1) store_chunk<T>(p, 2, row0, col, M, N, box, lane, h);
           }
         }
       }

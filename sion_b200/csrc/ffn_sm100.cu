@@ -418,8 +418,13 @@ void no_tokens(Call& c, const felix_gated_args& a) {
   c.zero(a.dw_down, a.features, a.hidden);
 }
 
+bool no_gradient(const felix_gated_args& a) {
+  return !a.dx.data && !a.dw_gate.data && !a.dw_up.data && !a.dw_down.data;
+}
+
 void gated_linear_bwd(Call& c, const felix_gated_args& a) {
   if (!a.tokens) return no_tokens(c, a);
+  if (no_gradient(a)) return;
   const uint32_t T = a.tokens, F = a.hidden;
   const MutMat dg = c.matrix(T, F), du = c.matrix(T, F);
   if (!c.counting() && c.ok()) {
@@ -447,9 +452,11 @@ void gated_linear_bwd(Call& c, const felix_gated_args& a) {
 
 void gated_ffn_bwd(Call& c, const felix_gated_args& a) {
   if (!a.tokens) return no_tokens(c, a);
+  if (no_gradient(a)) return;
   const uint32_t T = a.tokens, K = a.features, F = a.hidden;
   const Mat grad = c.addressable(a.grad, T, K);
-  const MutMat dg = c.matrix(T, F), du = c.matrix(T, F), h = c.matrix(T, F);
+  const MutMat dg = c.matrix(T, F), du = c.matrix(T, F);
+  const MutMat h = a.dw_down.data ? c.matrix(T, F) : MutMat{};  // nothing else reads it
   Product p;
   p.epilogue = kDGated;
   p.bf16 = c.bf16;
