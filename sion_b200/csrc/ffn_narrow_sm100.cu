@@ -40,8 +40,8 @@ struct Shape {
 struct alignas(64) Params {
   CUtensorMap w[2], x;
   uint32_t tokens, features;
-  uint32_t parts, kb, stages, tiles_t;  // tiles_t: tiles along the tokens
-  uint32_t whole;                       // two blocks of 64 k in one request
+  uint32_t parts, kb, stages;
+  uint32_t whole;  // two blocks of 64 k in one request
   Finish fin;
   unsigned* status;
 };
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
 
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = p.parts > 1 ? cluster_ctarank() : 0u, tile = blockIdx.x / p.parts;
-  const uint32_t f0 = tile / p.tiles_t * kWide, t0 = tile % p.tiles_t * BN;
+  const uint32_t f0 = tile * kWide;
   const uint32_t kb0 = p.kb * rank / p.parts, kb1 = p.kb * (rank + 1) / p.parts;
 
   if (threadIdx.x == 0) {
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
         } else {
           load(sa, &p.w[0], &full[stage], f0, kb, kRows * 128);
         }
-        load(sa + S::kABytes, &p.x, &full[stage], t0, kb, BN * 128);
+        load(sa + S::kABytes, &p.x, &full[stage], 0, kb, BN * 128);
         if (++stage == stages) stage = 0, phase ^= 1u;
       }
     }
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) ffn_narrow_kernel(const __grid_co
     tc_fence_before();
   }
 
-  const TilePlace place{0, t0, f0, min(uint32_t(BN), p.tokens - t0), min(kWide, p.features - f0)};
+  const TilePlace place{0, 0, f0, p.tokens, min(kWide, p.features - f0)};  // all tokens
   finish_tile<T, EPI, 128, BN, 8>(p.fin, place, ring, p.parts, rank, 0, 1, kThreads, received,
                                   p.status);
   if (warp == 1) {
@@ -229,8 +229,7 @@ FelixCode narrow_launch(DeviceInfo* dev, const Product& x, cudaStream_t stream) 
   Params p{};
   p.tokens = x.m[0];
   p.features = x.n[0];
-  p.tiles_t = (p.tokens + bn - 1) / bn;
-  const uint32_t tiles = (p.features + wide - 1) / wide * p.tiles_t;
+  const uint32_t tiles = (p.features + wide - 1) / wide;
   p.kb = (x.k[0] + kDepth - 1) / kDepth;
   // Parts of 256 k at least, one CTA per SM at most. Measured, tokens x depth x features in 1,
   // 2, 4, 8 parts, us: 24 x 4096 x 4096 17.0, 12.2, 10.6, 11.1; 40 x 8192 x 1024 31.4, 19.2,
