@@ -264,15 +264,21 @@ def _ffn_functions():
     import torch
     from torch.autograd.function import once_differentiable
 
+    # What a backward pass does not read is not kept: x where no weight needs a gradient,
+    # weights where x needs none. Of these it takes the shape alone.
+    def stand_in(grad, shape):
+        return grad.new_empty(shape[-1]).expand(shape)
+
     class Linear(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, weight, bias, residual, activation):
-            pre = None
-            if activation == "none":
+            need, pre = ctx.needs_input_grad, None
+            if activation == "none" or not any(need[:3]):
                 y = linear(x, weight, bias, residual, activation)
             else:
                 y, pre = linear_save(x, weight, bias, residual, activation)
-            ctx.save_for_backward(x, weight, pre)
+            ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, pre)
+            ctx.shapes = x.shape, weight.shape
             ctx.activation = activation
             return y
 
@@ -282,32 +288,47 @@ def _ffn_functions():
             x, weight, pre = ctx.saved_tensors
             need = ctx.needs_input_grad
             dx = dw = db = None
-            if need[0] or need[1] or need[2]:
-                dx, dw, db = linear_backward(grad, x, weight, pre, ctx.activation, need[2],
-                                             need[0], need[1])
+            if any(need[:3]):
+                dx, dw, db = linear_backward(
+                    grad, stand_in(grad, ctx.shapes[0]) if x is None else x,
+                    stand_in(grad, ctx.shapes[1]) if weight is None else weight, pre,
+                    ctx.activation, need[2], need[0], need[1])
             return dx, dw, db, grad if need[3] else None, None
 
     class GatedLinear(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, w_gate, w_up, activation):
+            need = ctx.needs_input_grad
             h, gate, up = gated_linear_save(x, w_gate, w_up, activation)
-            ctx.save_for_backward(x, w_gate, w_up, gate, up)
+            ctx.save_for_backward(x if any(need[1:3]) else None,
+                                  *((w_gate, w_up) if need[0] else (None, None)), gate, up)
+            ctx.shapes = x.shape, w_gate.shape
             ctx.activation = activation
             return h
 
         @staticmethod
         @once_differentiable
         def backward(ctx, grad):
+            x, w_gate, w_up, gate, up = ctx.saved_tensors
             need = ctx.needs_input_grad
-            return *gated_linear_backward(grad, *ctx.saved_tensors, ctx.activation, need[0],
-                                          need[1] or need[2]), None
+            if x is None:
+                x = stand_in(grad, ctx.shapes[0])
+            if w_gate is None:
+                w_gate = w_up = stand_in(grad, ctx.shapes[1])
+            return *gated_linear_backward(grad, x, w_gate, w_up, gate, up, ctx.activation, need[0],
+                                          any(need[1:3])), None
 
     class GatedFfn(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, w_gate, w_up, w_down, residual, activation):
-            y, gate, up = gated_ffn_save(x, w_gate, w_up, w_down, residual, activation)
-            ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up)
+            need = ctx.needs_input_grad
             ctx.activation = activation
+            if not any(need[:4]):
+                return gated_ffn(x, w_gate, w_up, w_down, residual, activation)
+            y, gate, up = gated_ffn_save(x, w_gate, w_up, w_down, residual, activation)
+            ctx.save_for_backward(x if any(need[1:4]) else None,
+                                  *((w_gate, w_up) if need[0] else (None, None)), w_down, gate, up)
+            ctx.shapes = x.shape, w_gate.shape
             return y
 
         @staticmethod
@@ -316,8 +337,13 @@ def _ffn_functions():
             need = ctx.needs_input_grad
             d = (None,) * 4
             if any(need[:4]):
-                d = gated_ffn_backward(grad, *ctx.saved_tensors, ctx.activation, need[0],
-                                       any(need[1:4]))
+                x, w_gate, w_up, w_down, gate, up = ctx.saved_tensors
+                if x is None:
+                    x = stand_in(grad, ctx.shapes[0])
+                if w_gate is None:
+                    w_gate = w_up = stand_in(grad, ctx.shapes[1])
+                d = gated_ffn_backward(grad, x, w_gate, w_up, w_down, gate, up, ctx.activation,
+                                       need[0], any(need[1:4]))
             return *d, grad if need[4] else None, None
 
     return Linear, GatedLinear, GatedFfn
@@ -333,18 +359,32 @@ def _ffn_function(i):
     return _FFN_FNS[i]
 
 
+def _needs_gradient(*tensors):
+    import torch
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def linear_autograd(x, weight, bias=None, residual=None, activation: str = "none"):
-    """linear that torch.autograd can differentiate (first derivatives)."""
+    """linear that torch.autograd can differentiate (first derivatives); linear itself
+    where no input needs a gradient."""
+    if not _needs_gradient(x, weight, bias, residual):
+        return linear(x, weight, bias, residual, activation)
     return _ffn_function(0).apply(x, weight, bias, residual, activation)
 
 
 def gated_linear_autograd(x, w_gate, w_up, activation: str = "silu"):
-    """gated_linear that torch.autograd can differentiate (first derivatives)."""
+    """gated_linear that torch.autograd can differentiate (first derivatives); gated_linear
+    itself where no input needs a gradient."""
+    if not _needs_gradient(x, w_gate, w_up):
+        return gated_linear(x, w_gate, w_up, activation)
     return _ffn_function(1).apply(x, w_gate, w_up, activation)
 
 
 def gated_ffn_autograd(x, w_gate, w_up, w_down, residual=None, activation: str = "silu"):
-    """gated_ffn that torch.autograd can differentiate (first derivatives)."""
+    """gated_ffn that torch.autograd can differentiate (first derivatives); gated_ffn
+    itself where no input needs a gradient."""
+    if not _needs_gradient(x, w_gate, w_up, w_down, residual):
+        return gated_ffn(x, w_gate, w_up, w_down, residual, activation)
     return _ffn_function(2).apply(x, w_gate, w_up, w_down, residual, activation)
 
 
