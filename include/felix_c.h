@@ -388,8 +388,10 @@ typedef struct felix_linear_args {
  *   dg = dh u act'(g), du = dh act(g), each rounded once;
  * and where wanted dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x,
  * dw_down = grad^T (act(g) u). (The residual's gradient is grad itself.)
- * Fields are read as in felix_linear_args; felix_gated_linear and its backward pass want
- * residual and dw_down NULL.
+ * Fields are read as in felix_linear_args; felix_gated_linear wants residual, and
+ * felix_gated_linear_bwd dw_down, NULL. What is rounded in between (h, dg, du, and dz of the
+ * linear layer) is an operand of the next product and has the range of its type: past 65504
+ * it is infinite in fp16.
  */
 typedef struct felix_gated_args {
   uint32_t tokens, features, hidden;

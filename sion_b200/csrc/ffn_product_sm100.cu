@@ -16,7 +16,8 @@
 // small. An operand may be stored with k or with m / n contiguous: a training step's x W^T,
 // dz W and dz^T x need no transpose. One launch may do several products (a backward pass does
 // all of its own), deepest tiles first. Measured: 8192 x 4096 x 16384 843 us in a loop under
-// the power cap (1.3 PFLOP/s); 500 x 4096 x 11264 42 us, with two projections 82.
+// the power cap (1.3 PFLOP/s); 500 x 4096 x 11264 49 us, with two projections 92, which are
+// 176 tiles for 74 pairs: three waves for 2.4.
 //
 // Warps: 0 TMA, 1 MMA, 8 of the epilogue (two per quarter of the TMEM lanes, which take every
 // other 32 columns: activations cost 10 to 50 instructions a value).
