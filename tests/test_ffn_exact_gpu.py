@@ -133,3 +133,15 @@ def test_gated_backward(S, T, K, F, dtype):
         for got, ref, what in zip(S.gated_ffn_backward(dy, x, wg, wu, wd, gate, up, name), want,
                                   ("dx", "dwg", "dwu", "dwd")):
             same(got, ref, f"{name} ffn {what}")
+
+
+# more columns than there are counters for the bias gradient's sums (33 rows of 1.2 million, in
+# vectors or not), and more rows than 32 a block can hold (2.2 million)
+@pytest.mark.parametrize("T,K,N", [(33, 8, 1200000), (40, 3, 140001), (2200001, 8, 8), (2200001, 7, 9)])
+def test_very_many_rows_or_columns(S, T, K, N):
+    for dtype in DTYPES:
+        test_linear(S, T, K, N, dtype)
+        test_linear_backward(S, T, K, N, dtype)
+        if N < 100:
+            test_gated(S, T, K, N, dtype)
+            test_gated_backward(S, T, K, N, dtype)

@@ -62,11 +62,12 @@ def test_no_gradient_needs_no_launch(S):
     x, wg, wu, wd = gated_inputs(300, 128, 256, torch.bfloat16)
     h, gate, up = S.gated_linear_save(x, wg, wu)
     torch.cuda.synchronize()
-    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
-        for _ in range(3):
+    graph = torch.cuda.CUDAGraph()
+    with pytest.warns(UserWarning, match="empty"):  # nothing was recorded
+        with torch.cuda.graph(graph):
             assert S.gated_ffn_backward(x, x, wg, wu, wd, gate, up, need_x=False,
                                         need_weights=False) == (None,) * 4
             assert S.gated_linear_backward(h, x, wg, wu, gate, up, need_x=False,
                                            need_weights=False) == (None,) * 3
-        torch.cuda.synchronize()
-    assert not [e.key for e in p.key_averages() if "felix_ffn" in e.key]
+            assert S.linear_backward(h, x, wg, gate, "silu", need_x=False,
+                                     need_weight=False) == (None,) * 3
